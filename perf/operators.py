@@ -245,11 +245,13 @@ def _loss_plain(s):
 
 
 def _random16(index, key):
-    """Sixteen random bits per element, as a number between 0 and 1: a 32-bit hash of a counter."""
-    h = (index * 0x9E3779B1 + key) & 0xFFFFFFFF
+    """Sixteen random bits per element, as a number between 0 and 1: the low and the high half of a 32-bit hash of a counter of
+    pairs."""
+    h = ((index >> 1) * 0x9E3779B1 + key) & 0xFFFFFFFF
     h = ((h ^ (h >> 16)) * 0x85EBCA6B) & 0xFFFFFFFF
     h = ((h ^ (h >> 13)) * 0xC2B2AE35) & 0xFFFFFFFF
-    return ((h >> 16).float() + 0.5) * (1.0 / 65536.0)
+    h = h ^ (h >> 16)
+    return (((h >> 16 * (index & 1)) & 0xFFFF).float() + 0.5) * (1.0 / 65536.0)
 
 
 def _block_exponent(x):
@@ -466,10 +468,11 @@ def _adamw_exact(s, case):
             index = torch.cat([torch.arange(int(n), device=x.device) for n in s["room"].tolist()])
             step = (s["steps"].long() + 1).repeat_interleave(s["room"])
             key = (step * 0x85EBCA77 + s["seed"] * 0xC2B2AE3D) % 2 ** 32
-            h = (index * 0x9E3779B1 + key) % 2 ** 32
+            h = (index // 2 * 0x9E3779B1 + key) % 2 ** 32
             h = (h ^ (h // 2 ** 16)) * 0x85EBCA6B % 2 ** 32
             h = (h ^ (h // 2 ** 13)) * 0xC2B2AE35 % 2 ** 32
-            u = ((h // 2 ** 16).double() + 0.5) / 2 ** 16
+            h = h ^ (h // 2 ** 16)
+            u = (torch.where(index % 2 == 1, h // 2 ** 16, h % 2 ** 16).double() + 0.5) / 2 ** 16
             x = torch.where(x > 0, (torch.floor(x / grid + u.view_as(x)) * grid).clamp(min=2.0 ** -9), x)
         out[name], out[name + "_scale"] = x.reshape(-1), None  # a power of two has no rounding to speak of
     return out
