@@ -94,11 +94,21 @@ SIGNATURES = {
                              c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "ffm_p2p_signal_wait_dev": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, ctypes.c_longlong, c_void_p]),
     "ffm_p2p_signal_wait": (c_int, [c_void_p, c_int, c_int, ctypes.c_uint32, c_void_p, ctypes.c_longlong, c_void_p]),
+    "ffm_layer_norm_forward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_int, c_float,
+                                       c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ffm_layer_norm_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "ffm_layer_norm_backward": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "ffm_adamw_step": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
     "ffm_route_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "ffm_route_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                    c_void_p, c_size_t, c_void_p, c_void_p]),
 }
+
+# called by the torch extension itself (csrc/ffm_torch_ops.cpp)
+NATIVE_OPS = ("ffm_error_string", "ffm_layer_norm_forward", "ffm_layer_norm_workspace_bytes", "ffm_layer_norm_backward",
+              "ffm_adamw_step")
 
 _lib = None
 _native = None
@@ -144,6 +154,7 @@ def native():
         module.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
             "ffm_layer_forward", "ffm_layer_backward", "ffm_rows_capacity", "ffm_route_workspace_bytes",
             "ffm_route_backward_workspace_bytes", "ffm_cast_many")))
+        module.bind_ops({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in NATIVE_OPS})
         _native = module
     return _native
 

@@ -1,0 +1,374 @@
+// AdamW step over many tensors in one launch, with the two moments in 32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g        v = b2 v + (1 - b2) g^2        (t: steps taken, this one included)
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Eight bits: blocks of 128 values of a tensor share a power of two; m / 2^k and sqrt(v) / 2^k are e4m3 numbers, k being the
+// least for which the block's largest magnitude fits (448 * 2^k). With a power of two the scaling rounds nothing, so that a state
+// that is read and written back unchanged stays. The root of v, because its e4m3 numbers then span 2^34 in v. m is rounded to nearest.
+// sqrt(v) is rounded up or down at random, in proportion: v moves by 1 - b2 of itself a step at most when gradients fall, its
+// root by 2.5 % at b2 = 0.95, and two e4m3 numbers are 6-12 % apart: to nearest it would never leave its number. A positive v
+// does not become zero (its least is 2^-18 of the block's scale squared): the quotient would explode. The update itself uses
+// the new m and v before they are rounded.
+//
+// HBM-bound: bf16 parameters, gradients and 8-bit states move 10 bytes a value, with fp32 states 22, with an fp32 master 28.
+// A block walks chunks of 2048 values, eight neighbours a thread, over all tensors as one list. Steps are counted on the
+// device, so that a captured step can be replayed: every block reads them, and the last block to finish raises them.
+#include "ffm_types.cuh"
+
+#include "ffm_gemm_common.cuh"
+#include "ffm_internal.h"
+
+namespace ffm {
+
+namespace {
+
+constexpr int ADAMW_THREADS = 256;
+constexpr int ADAMW_CHUNK = ADAMW_THREADS * 8;
+constexpr int ADAMW_BLOCK = 128;  // values that share a scale: 16 threads
+
+struct AdamWTensor {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* master;
+  uint8_t* m_scale;
+  uint8_t* v_scale;
+  int32_t* step;
+  long long n;
+  long long chunks_end;  // chunks of this tensor and all before it
+  int p_type, g_type;
+  int wide;  // every pointer allows 16-byte accesses (8-byte ones to 8-bit states)
+};
+
+template <int MAX>
+struct AdamWJob {
+  AdamWTensor tensor[MAX];
+  int count;
+  float lr, beta1, one_minus_beta1, beta2, one_minus_beta2, eps, weight_decay;
+  double beta1_wide, beta2_wide;
+  const float* lr_device;   // instead of lr
+  const float* grad_scale;  // device scalar or null
+  uint32_t seed;
+  unsigned int* ticket;  // zero before and after
+};
+
+// b^t by squaring
+__device__ __forceinline__ double power(double b, int t) {
+  double r = 1.0;
+  for (unsigned int e = t > 0 ? t : 0; e != 0; e >>= 1) {
+    if (e & 1) r *= b;
+    b *= b;
+  }
+  return r;
+}
+
+__device__ __forceinline__ float exponent_of_two(int k) { return __int_as_float((k + 127) << 23); }
+
+// The least k for which top <= 448 * 2^k (448 = 1.75 * 2^8), within what the scale's byte and fp32 can say.
+__device__ __forceinline__ int block_exponent(float top) {
+  const uint32_t bits = __float_as_uint(top);
+  const int k = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(k, -126), 120);
+}
+
+__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<unsigned short>(two)));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+
+// Two values to e4m3, to nearest; what is over 448 (infinities, NaN: the scale sees to the rest) becomes NaN.
+__device__ __forceinline__ uint32_t e4m3x2_nearest(float lo, float hi) {
+  lo = fabsf(lo) <= 448.0f ? lo : __int_as_float(0x7fc00000);
+  hi = fabsf(hi) <= 448.0f ? hi : __int_as_float(0x7fc00000);
+  unsigned short r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// x >= 0 to e4m3, up with probability (distance from the lower neighbour) / (distance of the neighbours): the lower code plus
+// 16 random bits, as a fraction, in place of the bits that are cut off. Above 2^-6 that is integer arithmetic on the fp32
+// number; below, codes are multiples of 2^-9. Never zero for a positive x.
+__device__ __forceinline__ uint32_t e4m3_random(float x, uint32_t random16) {
+  const uint32_t bits = __float_as_uint(x);
+  uint32_t code = ((bits + (random16 << 4) + 8u) >> 20) - ((127 - 7) << 3);
+  if (x < 0.015625f) {
+    code = static_cast<uint32_t>(floorf(x * 512.0f + (static_cast<float>(random16) + 0.5f) * (1.0f / 65536.0f)));
+    code = x > 0.0f ? max(code, 1u) : 0u;
+  }
+  return x <= 448.0f ? code : 0x7fu;
+}
+
+// Random bits of a pair of neighbouring values (16 each): two rounds of multiply and fold over a counter.
+__device__ __forceinline__ uint32_t random_pair(uint32_t pair, uint32_t key) {
+  uint32_t h = pair * 0x9E3779B1u + key;
+  h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
+  h = (h ^ (h >> 13)) * 0xC2B2AE35u;
+  return h ^ (h >> 16);
+}
+
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+template <int MAX, bool EIGHT>
+__global__ void __launch_bounds__(ADAMW_THREADS)
+adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
+  __shared__ float rate[MAX], inverse[MAX];  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  __shared__ uint32_t keys[MAX];
+  __shared__ bool last;
+  const float lr = job.lr_device != nullptr ? *job.lr_device : job.lr;
+  const float grad_scale = job.grad_scale != nullptr ? *job.grad_scale : 1.0f;
+  for (int i = threadIdx.x; i < job.count; i += ADAMW_THREADS) {
+    const int t = *job.tensor[i].step + 1;
+    rate[i] = static_cast<float>(lr / (1.0 - power(job.beta1_wide, t)));
+    inverse[i] = static_cast<float>(1.0 / sqrt(1.0 - power(job.beta2_wide, t)));
+    keys[i] = static_cast<uint32_t>(t) * 0x85EBCA77u + job.seed * 0xC2B2AE3Du;
+  }
+  __syncthreads();
+  const float keep = 1.0f - lr * job.weight_decay;
+  const long long chunks = job.tensor[job.count - 1].chunks_end;
+  int i = 0;
+  for (long long chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    // the chunk's tensor, for the whole block alike
+    int top = job.count - 1;
+    while (i < top) {
+      const int mid = (i + top) >> 1;
+      if (chunk < job.tensor[mid].chunks_end) {
+        top = mid;
+      } else {
+        i = mid + 1;
+      }
+    }
+    const AdamWTensor& a = job.tensor[i];
+    const long long e0 = (chunk - (i > 0 ? job.tensor[i - 1].chunks_end : 0)) * ADAMW_CHUNK + threadIdx.x * 8;
+    const int left = static_cast<int>(min(a.n - e0, 8ll));  // values of this thread, none where <= 0
+    const bool whole = left == 8 && a.wide != 0;
+    float p[8], g[8], m[8], v[8];
+    if (whole) {
+      load8_as(a.g, a.g_type, e0, g);
+      if (a.master != nullptr) {
+        load8(a.master + e0, p);
+      } else {
+        load8_as(a.p, a.p_type, e0, p);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g[j] = j < left ? load1_as(a.g, a.g_type, e0 + j) : 0.0f;
+        p[j] = j < left ? (a.master != nullptr ? a.master[e0 + j] : load1_as(a.p, a.p_type, e0 + j)) : 0.0f;
+      }
+    }
+    if (EIGHT) {
+      const long long block = e0 / ADAMW_BLOCK;
+      uint2 cm = make_uint2(0, 0), cv = make_uint2(0, 0);
+      float sm = 0.0f, sv = 0.0f;
+      if (left > 0) {
+        sm = exponent_of_two(static_cast<int>(a.m_scale[block]) - 127);
+        sv = exponent_of_two(static_cast<int>(a.v_scale[block]) - 127);
+      }
+      if (whole) {
+        cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + e0);
+        cv = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + e0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j < left) {
+            const uint32_t x = static_cast<const uint8_t*>(a.m)[e0 + j], y = static_cast<const uint8_t*>(a.v)[e0 + j];
+            if (j < 4) {
+              cm.x |= x << (8 * j), cv.x |= y << (8 * j);
+            } else {
+              cm.y |= x << (8 * j - 32), cv.y |= y << (8 * j - 32);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 x = e4m3x2_to_float2((q < 2 ? cm.x : cm.y) >> (16 * (q & 1)) & 0xffffu);
+        const float2 y = e4m3x2_to_float2((q < 2 ? cv.x : cv.y) >> (16 * (q & 1)) & 0xffffu);
+        m[2 * q] = x.x * sm, m[2 * q + 1] = x.y * sm;
+        v[2 * q] = (y.x * sv) * (y.x * sv), v[2 * q + 1] = (y.y * sv) * (y.y * sv);
+      }
+    } else if (whole) {
+      load8(static_cast<const float*>(a.m) + e0, m);
+      load8(static_cast<const float*>(a.v) + e0, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        m[j] = j < left ? static_cast<const float*>(a.m)[e0 + j] : 0.0f;
+        v[j] = j < left ? static_cast<const float*>(a.v)[e0 + j] : 0.0f;
+      }
+    }
+
+    float root[8], top_m = 0.0f, top_v = 0.0f;
+    const float r = rate[i], inv = inverse[i];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // each product and sum is rounded on its own: in 8 bits the largest of a block decides its scale, and two evaluations
+      // that differ in the last place would now and then differ in it
+      const float gj = __fmul_rn(g[j], grad_scale);
+      m[j] = __fadd_rn(__fmul_rn(m[j], job.beta1), __fmul_rn(gj, job.one_minus_beta1));
+      v[j] = __fadd_rn(__fmul_rn(v[j], job.beta2), __fmul_rn(__fmul_rn(gj, job.one_minus_beta2), gj));
+      root[j] = __fsqrt_rn(v[j]);
+      p[j] = fmaf(-r, __fdividef(m[j], fmaf(root[j], inv, job.eps)), p[j] * keep);
+      top_m = fmaxf(top_m, fabsf(m[j]));
+      top_v = fmaxf(top_v, root[j]);
+    }
+
+    if (a.master != nullptr) {
+      if (whole) {
+        store8(a.master + e0, p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j < left) a.master[e0 + j] = p[j];
+        }
+      }
+    }
+    if (whole) {
+      store8_as(a.p, a.p_type, e0, p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j < left) store1_as(a.p, a.p_type, e0 + j, p[j]);
+      }
+    }
+    if (EIGHT) {
+      const int km = block_exponent(max16(top_m)), kv = block_exponent(max16(top_v));
+      const float fm = exponent_of_two(-km), fv = exponent_of_two(-kv);
+      uint32_t cm[2] = {0, 0}, cv[2] = {0, 0};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t random = random_pair(static_cast<uint32_t>((e0 >> 1) + q), keys[i]);
+        cm[q >> 1] |= e4m3x2_nearest(m[2 * q] * fm, m[2 * q + 1] * fm) << (16 * (q & 1));
+        cv[q >> 1] |= (e4m3_random(root[2 * q] * fv, random & 0xffffu) | e4m3_random(root[2 * q + 1] * fv, random >> 16) << 8)
+                      << (16 * (q & 1));
+      }
+      if (whole) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + e0) = make_uint2(cm[0], cm[1]);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + e0) = make_uint2(cv[0], cv[1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j < left) {
+            static_cast<uint8_t*>(a.m)[e0 + j] = static_cast<uint8_t>(cm[j >> 2] >> (8 * (j & 3)));
+            static_cast<uint8_t*>(a.v)[e0 + j] = static_cast<uint8_t>(cv[j >> 2] >> (8 * (j & 3)));
+          }
+        }
+      }
+      if (left > 0 && e0 % ADAMW_BLOCK == 0) {
+        a.m_scale[e0 / ADAMW_BLOCK] = static_cast<uint8_t>(km + 127);
+        a.v_scale[e0 / ADAMW_BLOCK] = static_cast<uint8_t>(kv + 127);
+      }
+    } else if (whole) {
+      store8(static_cast<float*>(a.m) + e0, m);
+      store8(static_cast<float*>(a.v) + e0, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j < left) {
+          static_cast<float*>(a.m)[e0 + j] = m[j];
+          static_cast<float*>(a.v)[e0 + j] = v[j];
+        }
+      }
+    }
+  }
+  // every block has read the steps before it takes a ticket; the last one raises them
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(job.ticket, 1u) == gridDim.x - 1;
+    if (last) *job.ticket = 0;
+  }
+  __syncthreads();
+  if (last) {
+    for (int k = threadIdx.x; k < job.count; k += ADAMW_THREADS) *job.tensor[k].step += 1;
+  }
+}
+
+template <int MAX, bool EIGHT>
+int launch_adamw(const ffm_adamw_tensor* t, int count, const ffm_adamw_args& h, cudaStream_t stream) {
+  AdamWJob<MAX> job;
+  long long chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    AdamWTensor& a = job.tensor[i];
+    a.p = t[i].param;
+    a.g = t[i].grad;
+    a.m = t[i].exp_avg;
+    a.v = t[i].exp_avg_sq;
+    a.master = static_cast<float*>(t[i].master);
+    a.m_scale = static_cast<uint8_t*>(t[i].exp_avg_scale);
+    a.v_scale = static_cast<uint8_t*>(t[i].exp_avg_sq_scale);
+    a.step = t[i].step;
+    a.n = t[i].elements;
+    a.p_type = static_cast<int>(t[i].param_type);
+    a.g_type = static_cast<int>(t[i].grad_type);
+    const uintptr_t states = reinterpret_cast<uintptr_t>(a.m) | reinterpret_cast<uintptr_t>(a.v);
+    a.wide = !off_16_bytes(a.p, a.g, a.master) && states % (EIGHT ? 8 : 16) == 0;
+    chunks += (a.n + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
+    a.chunks_end = chunks;
+  }
+  job.count = count;
+  job.lr = static_cast<float>(h.lr);
+  job.beta1 = static_cast<float>(h.beta1);
+  job.one_minus_beta1 = static_cast<float>(1.0 - h.beta1);
+  job.beta2 = static_cast<float>(h.beta2);
+  job.one_minus_beta2 = static_cast<float>(1.0 - h.beta2);
+  job.eps = static_cast<float>(h.eps);
+  job.weight_decay = static_cast<float>(h.weight_decay);
+  job.beta1_wide = h.beta1;
+  job.beta2_wide = h.beta2;
+  job.lr_device = h.lr_device;
+  job.grad_scale = h.grad_scale;
+  job.seed = static_cast<uint32_t>(h.seed);
+  job.ticket = static_cast<unsigned int*>(h.ticket);
+  auto kernel = adamw_kernel<MAX, EIGHT>;
+  static PerDevice resident;
+  const int most = resident.get([&] {
+    int blocks = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, ADAMW_THREADS, 0) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    return blocks * num_sms();
+  });
+  if (most <= 0) return FFM_ERR_LAUNCH;
+  kernel<<<static_cast<unsigned>(chunks < most ? (chunks > 0 ? chunks : 1) : most), ADAMW_THREADS, 0, stream>>>(job);
+  return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
+}  // namespace
+
+}  // namespace ffm
+
+using namespace ffm;
+
+extern "C" int ffm_adamw_step(const ffm_adamw_tensor* tensors, int count, const ffm_adamw_args* args, ffm_stream_t stream) {
+  if (count < 0 || !args || (count > 0 && !tensors)) return FFM_ERR_BAD_ARG;
+  if (count == 0) return FFM_OK;
+  const ffm_adamw_args& h = *args;
+  if (!h.ticket || (h.bits != 8 && h.bits != 32)) return FFM_ERR_BAD_ARG;
+  if (!(h.beta1 >= 0.0 && h.beta1 < 1.0 && h.beta2 >= 0.0 && h.beta2 < 1.0 && h.eps >= 0.0)) return FFM_ERR_BAD_ARG;
+  const bool eight = h.bits == 8;
+  for (int i = 0; i < count; ++i) {
+    const ffm_adamw_tensor& t = tensors[i];
+    if (t.elements < 0 || !t.step || !is_type(static_cast<int>(t.param_type)) || !is_type(static_cast<int>(t.grad_type))) return FFM_ERR_BAD_ARG;
+    if (t.elements == 0) continue;
+    if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return FFM_ERR_BAD_ARG;
+    if (eight && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return FFM_ERR_BAD_ARG;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (int first = 0; first < count; first += FFM_ADAMW_MAX) {
+    const int n = count - first < FFM_ADAMW_MAX ? count - first : FFM_ADAMW_MAX;
+    const ffm_adamw_tensor* t = tensors + first;
+    const int rc = n <= FFM_ADAMW_FEW ? (eight ? launch_adamw<FFM_ADAMW_FEW, true>(t, n, h, s) : launch_adamw<FFM_ADAMW_FEW, false>(t, n, h, s))
+                                      : (eight ? launch_adamw<FFM_ADAMW_MAX, true>(t, n, h, s) : launch_adamw<FFM_ADAMW_MAX, false>(t, n, h, s));
+    if (rc != FFM_OK) return rc;
+  }
+  return FFM_OK;
+}

@@ -490,8 +490,11 @@ py::tuple layer_backward(const OptTensor& grad_out, const OptTensor& grad_aux, c
 
 }  // namespace
 
+void define_ops(py::module_& m);  // ffm_torch_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
   m.def("layer_forward", &layer_forward);
   m.def("layer_backward", &layer_backward);
+  define_ops(m);
 }

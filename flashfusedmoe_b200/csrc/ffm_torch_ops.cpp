@@ -1,0 +1,343 @@
+// The operators beside the layer for torch tensors: argument checks, outputs, scratch and the call into libffmoe. A call from
+// Python costs these few checks; the torch operations that they would be there (views, contiguity, empty) take longer than
+// the kernels of a small call.
+#include <torch/extension.h>
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+
+#include <mutex>
+#include <optional>
+#include <stdexcept>
+#include <string>
+#include <unordered_map>
+#include <unordered_set>
+#include <utility>
+#include <vector>
+
+#include "../../include/ffmoe.h"
+
+namespace {
+
+namespace py = pybind11;
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+decltype(&ffm_error_string) error_string = nullptr;
+decltype(&ffm_layer_norm_forward) norm_forward = nullptr;
+decltype(&ffm_layer_norm_workspace_bytes) norm_workspace = nullptr;
+decltype(&ffm_layer_norm_backward) norm_backward = nullptr;
+decltype(&ffm_adamw_step) adamw = nullptr;
+
+void bind_ops(const std::unordered_map<std::string, uintptr_t>& at) {
+  auto take = [&](const char* name, auto& f) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(at.at(name)); };
+  take("ffm_error_string", error_string);
+  take("ffm_layer_norm_forward", norm_forward);
+  take("ffm_layer_norm_workspace_bytes", norm_workspace);
+  take("ffm_layer_norm_backward", norm_backward);
+  take("ffm_adamw_step", adamw);
+}
+
+void check(int rc, const char* what) {
+  if (rc != FFM_OK) {
+    throw std::runtime_error(std::string("libffmoe ") + what + " failed: " + std::to_string(rc) + " (" + error_string(rc) + ")");
+  }
+}
+
+// The device of `t` is current and its current stream is the call's.
+class On {
+ public:
+  explicit On(const Tensor& t) : guard_(t.device()), device_(t.device()) {}
+  ffm_stream_t stream() const {
+    return c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getStream(device_).native_handle();
+  }
+
+ private:
+  c10::DeviceGuard guard_;
+  c10::Device device_;
+};
+
+void on_gpu(const Tensor& t, const char* name) {
+  if (!t.is_cuda()) {
+    throw std::runtime_error(std::string(name) + " must be a CUDA tensor: flashfusedmoe_b200 has no CPU path");
+  }
+  if (t.layout() != at::kStrided) throw py::value_error(std::string(name) + " must be a dense tensor");
+}
+
+void same_device(const Tensor& t, const Tensor& other, const char* name) {
+  on_gpu(t, name);
+  if (t.device() != other.device()) throw py::value_error("All tensors must be on same device");
+}
+
+int element_type(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return FFM_TYPE_BF16;
+    case at::kHalf: return FFM_TYPE_FP16;
+    case at::kFloat: return FFM_TYPE_FP32;
+    default:
+      throw py::type_error(std::string(name) + " must be bfloat16, float16 or float32, got " + c10::toString(t.scalar_type()));
+  }
+}
+
+// values in memory, one after the other, with no negation pending
+Tensor plain(const Tensor& t) { return t.contiguous().resolve_neg(); }
+
+// ---- layer norm ---------------------------------------------------------------------------------------------
+
+struct Rows {
+  Tensor x;  // keeps the memory
+  int64_t rows, stride;
+};
+
+// x as rows of its last dimension: as it lies where its rows are one distance apart, else a copy
+Rows as_rows(const Tensor& t) {
+  Tensor x = t.is_neg() ? t.resolve_neg() : t;
+  const int64_t D = x.size(-1), rows = D > 0 ? x.numel() / D : 0;
+  bool fits = x.stride(-1) == 1 || D == 1;
+  int64_t stride = 0, expected = 0;  // distance of two rows; of two neighbours in the dimension looked at
+  for (int64_t d = x.dim() - 2; d >= 0 && fits; --d) {
+    if (x.size(d) == 1) continue;
+    if (stride == 0) {
+      stride = x.stride(d);
+      fits = stride >= D;
+    } else {
+      fits = x.stride(d) == expected;
+    }
+    expected = x.stride(d) * x.size(d);
+  }
+  if (!fits) {
+    x = x.contiguous();
+    stride = D;
+  }
+  return {x, rows, stride == 0 ? D : stride};
+}
+
+void check_vector(const OptTensor& v, const Tensor& x, const char* name) {
+  if (!v.has_value()) return;
+  same_device(*v, x, name);
+  if (v->dim() != 1 || v->size(0) != x.size(-1)) {
+    throw py::value_error(std::string(name) + " must be [" + std::to_string(x.size(-1)) + "], got " + c10::str(v->sizes()));
+  }
+  element_type(*v, name);
+}
+
+// (y, mean, rstd); without `stats` the last two are None
+py::tuple layer_norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, bool stats) {
+  on_gpu(x, "x");
+  if (x.dim() < 1 || x.size(-1) < 1) throw py::value_error("x must have a last dimension to normalise, got " + c10::str(x.sizes()));
+  if (!(eps >= 0.0)) throw py::value_error("eps must not be negative, got " + std::to_string(eps));
+  const int type = element_type(x, "x");
+  check_vector(weight, x, "weight");
+  check_vector(bias, x, "bias");
+  const On device(x);
+  const Rows r = as_rows(x);
+  const Tensor w = weight.has_value() ? plain(*weight) : Tensor(), b = bias.has_value() ? plain(*bias) : Tensor();
+  const Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor mean, rstd;
+  if (stats) {
+    mean = at::empty({r.rows}, x.options().dtype(at::kFloat));
+    rstd = at::empty({r.rows}, x.options().dtype(at::kFloat));
+  }
+  check(norm_forward(r.x.data_ptr(), type, r.rows, r.stride, static_cast<int>(x.size(-1)), w.defined() ? w.data_ptr() : nullptr,
+                     w.defined() ? element_type(w, "weight") : 0, b.defined() ? b.data_ptr() : nullptr,
+                     b.defined() ? element_type(b, "bias") : 0, static_cast<float>(eps), y.data_ptr(),
+                     stats ? mean.data_ptr<float>() : nullptr, stats ? rstd.data_ptr<float>() : nullptr, device.stream()),
+        "ffm_layer_norm_forward");
+  if (!stats) return py::make_tuple(y, py::none(), py::none());
+  return py::make_tuple(y, mean, rstd);
+}
+
+// (dx, dweight, dbias), None where not wanted
+py::tuple layer_norm_backward(const Tensor& dy, const Tensor& x, const OptTensor& weight, const Tensor& mean, const Tensor& rstd,
+                              bool want_x, bool want_weight, bool want_bias, const py::object& bias_type) {
+  const On device(x);
+  const int type = element_type(x, "x");
+  const int64_t D = x.size(-1);
+  const Rows r = as_rows(x);
+  if (mean.numel() != r.rows || rstd.numel() != r.rows || mean.scalar_type() != at::kFloat || rstd.scalar_type() != at::kFloat) {
+    throw py::value_error("saved statistics do not belong to x");
+  }
+  const Tensor m = plain(mean), s = plain(rstd);
+  const Tensor g = plain(dy.scalar_type() == x.scalar_type() ? dy : dy.to(x.scalar_type()));
+  if (g.sizes() != x.sizes()) throw py::value_error("the gradient of y has another shape than x");
+  const Tensor w = weight.has_value() ? plain(*weight) : Tensor();
+  Tensor dx, dw, db, workspace;
+  if (want_x) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  if (want_weight) dw = at::empty({D}, w.options());
+  if (want_bias) db = at::empty({D}, x.options().dtype(bias_type.is_none() ? x.scalar_type() : bias_type.cast<at::ScalarType>()));
+  size_t bytes = 0;
+  if (want_weight || want_bias) {
+    bytes = norm_workspace(r.rows, static_cast<int>(D), type);
+    workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+  }
+  auto address = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  check(norm_backward(g.data_ptr(), r.x.data_ptr(), type, r.rows, r.stride, static_cast<int>(D), address(w),
+                      w.defined() ? element_type(w, "weight") : 0, m.data_ptr<float>(), s.data_ptr<float>(), address(dx),
+                      address(dw), address(db), db.defined() ? element_type(db, "bias") : 0, address(workspace), bytes,
+                      device.stream()),
+        "ffm_layer_norm_backward");
+  auto handed = [](const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); };
+  return py::make_tuple(handed(dx), handed(dw), handed(db));
+}
+
+// ---- AdamW --------------------------------------------------------------------------------------------------
+
+// A zero word per device and stream that the kernel leaves zero: calls on one stream follow one another. A captured call gets
+// one of its own, zeroed in the graph: replays of two graphs may overlap.
+Tensor ticket_for(const Tensor& like, const void* stream, bool capturing) {
+  const auto options = like.options().dtype(at::kInt).requires_grad(false);
+  if (capturing) return at::zeros({1}, options);
+  static std::mutex mutex;
+  static std::unordered_map<std::string, Tensor>* kept = new std::unordered_map<std::string, Tensor>();  // never destroyed: outlives CUDA
+  const std::string key = std::to_string(like.device().index()) + ":" + std::to_string(reinterpret_cast<uintptr_t>(stream));
+  const std::lock_guard<std::mutex> lock(mutex);
+  Tensor& t = (*kept)[key];
+  if (!t.defined()) t = at::zeros({1}, options);
+  return t;
+}
+
+using Tensors = std::vector<Tensor>;
+
+// Launches.
+int64_t adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
+                   const Tensors& steps, const std::optional<Tensors>& masters, const std::optional<Tensors>& exp_avg_scales,
+                   const std::optional<Tensors>& exp_avg_sq_scales, const py::object& lr, double beta1, double beta2, double eps,
+                   double weight_decay, const OptTensor& grad_scale, int64_t seed, bool capturing) {
+  const size_t n = params.size();
+  const bool eight = exp_avg_scales.has_value();
+  auto length = [n](size_t other, const char* name) {
+    if (other != n) throw py::value_error(std::string(name) + " must have one tensor for each parameter: " + std::to_string(other) + " for " + std::to_string(n));
+  };
+  length(grads.size(), "grads");
+  length(exp_avgs.size(), "exp_avgs");
+  length(exp_avg_sqs.size(), "exp_avg_sqs");
+  length(steps.size(), "steps");
+  if (masters.has_value()) length(masters->size(), "masters");
+  if (eight != exp_avg_sq_scales.has_value()) throw py::value_error("8-bit states have scales for both moments");
+  if (eight) {
+    length(exp_avg_scales->size(), "exp_avg_scales");
+    length(exp_avg_sq_scales->size(), "exp_avg_sq_scales");
+  }
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) throw py::value_error("betas must be in [0, 1)");
+  if (!(eps >= 0.0)) throw py::value_error("eps must not be negative");
+  if (!(weight_decay >= 0.0)) throw py::value_error("weight_decay must not be negative");
+  if (n == 0) return 0;
+
+  const Tensor& first = params[0];
+  on_gpu(first, "param");
+  ffm_adamw_args h = {};
+  Tensor lr_device;
+  if (THPVariable_Check(lr.ptr())) {
+    const Tensor t = lr.cast<Tensor>();
+    if (t.numel() != 1) throw py::value_error("lr must be a number or a tensor of one element");
+    if (t.is_cuda()) {
+      same_device(t, first, "lr");
+      if (t.scalar_type() != at::kFloat) throw py::type_error("lr on the device must be float32");
+      lr_device = t.resolve_neg();
+      h.lr_device = lr_device.data_ptr<float>();
+    } else {
+      h.lr = t.item<double>();
+    }
+  } else {
+    h.lr = lr.cast<double>();
+  }
+  if (h.lr_device == nullptr && !(h.lr >= 0.0)) throw py::value_error("lr must not be negative");
+  h.beta1 = beta1;
+  h.beta2 = beta2;
+  h.eps = eps;
+  h.weight_decay = weight_decay;
+  h.bits = eight ? 8 : 32;
+  h.seed = seed;
+  Tensor scale;
+  if (grad_scale.has_value()) {
+    same_device(*grad_scale, first, "grad_scale");
+    if (grad_scale->numel() != 1 || grad_scale->scalar_type() != at::kFloat) throw py::type_error("grad_scale must be one float32 value");
+    scale = grad_scale->resolve_neg();
+    h.grad_scale = scale.data_ptr<float>();
+  }
+
+  // written in place: one after the other in memory, no negation pending, and no two entries on the same memory
+  std::unordered_set<const void*> written;
+  auto state = [&](const Tensor& t, int64_t elements, const char* name) {
+    same_device(t, first, name);
+    if (!t.is_contiguous() || t.is_neg()) throw py::value_error(std::string(name) + " must be contiguous");
+    if (t.numel() != elements) throw py::value_error(std::string(name) + " must have " + std::to_string(elements) + " elements, got " + std::to_string(t.numel()));
+    if (elements > 0 && !written.insert(t.data_ptr()).second) throw py::value_error(std::string(name) + " appears twice in one call");
+    return t.data_ptr();
+  };
+  std::vector<ffm_adamw_tensor> table(n);
+  std::vector<Tensor> held;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& p = params[i];
+    ffm_adamw_tensor& a = table[i];
+    const int64_t elements = p.numel();
+    a.elements = elements;
+    a.param = state(p, elements, "param");
+    a.param_type = element_type(p, "param");
+    Tensor g = grads[i];
+    same_device(g, first, "grad");
+    if (g.sizes() != p.sizes()) throw py::value_error("grad must have its parameter's shape: " + c10::str(g.sizes()) + " for " + c10::str(p.sizes()));
+    a.grad_type = element_type(g, "grad");
+    if (!g.is_contiguous() || g.is_neg()) {
+      g = plain(g);
+      held.push_back(g);
+    }
+    a.grad = g.data_ptr();
+    if (eight) {
+      for (const Tensor* t : {&exp_avgs[i], &exp_avg_sqs[i]}) {
+        if (t->scalar_type() != at::kFloat8_e4m3fn) throw py::type_error("8-bit states must be float8_e4m3fn, got " + std::string(c10::toString(t->scalar_type())));
+      }
+      const int64_t blocks = (elements + 127) / 128;
+      for (const Tensor* t : {&(*exp_avg_scales)[i], &(*exp_avg_sq_scales)[i]}) {
+        if (t->scalar_type() != at::kByte) throw py::type_error("scales of 8-bit states must be uint8, got " + std::string(c10::toString(t->scalar_type())));
+      }
+      a.exp_avg_scale = state((*exp_avg_scales)[i], blocks, "exp_avg_scale");
+      a.exp_avg_sq_scale = state((*exp_avg_sq_scales)[i], blocks, "exp_avg_sq_scale");
+    } else {
+      for (const Tensor* t : {&exp_avgs[i], &exp_avg_sqs[i]}) {
+        if (t->scalar_type() != at::kFloat) throw py::type_error("states must be float32 (or float8_e4m3fn with scales), got " + std::string(c10::toString(t->scalar_type())));
+      }
+    }
+    a.exp_avg = state(exp_avgs[i], elements, "exp_avg");
+    a.exp_avg_sq = state(exp_avg_sqs[i], elements, "exp_avg_sq");
+    if (masters.has_value()) {
+      if ((*masters)[i].scalar_type() != at::kFloat) throw py::type_error("masters must be float32");
+      a.master = state((*masters)[i], elements, "master");
+    }
+    if (steps[i].scalar_type() != at::kInt) throw py::type_error("steps must be int32, got " + std::string(c10::toString(steps[i].scalar_type())));
+    a.step = static_cast<int32_t*>(state(steps[i], 1, "step"));
+  }
+
+  const On device(first);
+  const ffm_stream_t stream = device.stream();
+  const Tensor ticket = ticket_for(first, stream, capturing);
+  h.ticket = ticket.data_ptr();
+  int rc;
+  {
+    py::gil_scoped_release released;
+    rc = adamw(table.data(), static_cast<int>(n), &h, stream);
+  }
+  check(rc, "ffm_adamw_step");
+  // what was read before (a saved operand, a cast or quantised copy) is not current any more
+  auto changed = [](const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  for (const Tensors* list : {&params, &exp_avgs, &exp_avg_sqs, &steps}) {
+    for (const Tensor& t : *list) changed(t);
+  }
+  for (const std::optional<Tensors>* list : {&masters, &exp_avg_scales, &exp_avg_sq_scales}) {
+    if (list->has_value()) {
+      for (const Tensor& t : **list) changed(t);
+    }
+  }
+  return (static_cast<int64_t>(n) + FFM_ADAMW_MAX - 1) / FFM_ADAMW_MAX;
+}
+
+}  // namespace
+
+void define_ops(py::module_& m) {
+  m.def("bind_ops", &bind_ops);
+  m.def("layer_norm_forward", &layer_norm_forward);
+  m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("adamw_step", &adamw_step);
+}

@@ -11,6 +11,7 @@ import torch
 import torch.nn as nn
 
 from .fused_moe import fused_moe, glu_ffn, set_ep_group
+from .norm import LayerNorm
 
 
 class _GLUFFN(nn.Module):
@@ -41,12 +42,14 @@ class MoELayer(nn.Module):
     the single shared GLU FFN, e.g. num_shared_experts * ffn_dim for models whose shared experts are merged.
     `ep_full_input_grad` (extension, default False = the reference's contract) adds the expert input gradient to
     the expert-parallel backward through a reverse dispatch exchange.
+    `pre_norm` (extension, default False) puts a layer norm in front of the layer, with its parameters as norm.weight and
+    norm.bias and `norm_eps`: forward(x) is then the layer of norm(x), the branch of a pre-norm residual block.
     """
 
     def __init__(self, d_model, ffn_dim, num_experts, top_k=2, activation="swiglu", gating="softmax",
                  num_shared_experts=0, latent_dim=None, capacity_factor=None, max_tokens_per_expert=None,
                  allow_dropped_tokens=True, aux_loss_coeff=0.0, z_loss_coeff=0.0, recompute_activations=False,
-                 shared_ffn_dim=None, ep_full_input_grad=False):
+                 shared_ffn_dim=None, ep_full_input_grad=False, pre_norm=False, norm_eps=1e-5):
         super().__init__()
         self.d_model = d_model
         self.ffn_dim = ffn_dim
@@ -65,6 +68,7 @@ class MoELayer(nn.Module):
         self._ep_group = None
         self._ep_size = 1
 
+        self.norm = LayerNorm(d_model, eps=norm_eps) if pre_norm else None
         self.gate = nn.Linear(d_model, num_experts, bias=False)
         nn.init.kaiming_uniform_(self.gate.weight, a=math.sqrt(5))
         self.gate.weight.data *= 0.01
@@ -90,6 +94,8 @@ class MoELayer(nn.Module):
         leading = x.shape[:-1]
         D = x.shape[-1]
         x_flat = x.reshape(-1, D)
+        if self.norm is not None:
+            x_flat = self.norm(x_flat)
 
         shared_weights = None
         shared_local = None

@@ -1,0 +1,109 @@
+"""AdamW over all parameters of a model in a launch per group, with its two moments in 32 or in 8 bits."""
+
+import torch
+
+from . import _lib, ops
+
+BLOCK = 128   # values of a tensor that share a scale in an 8-bit state
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, masters=None,
+               exp_avg_scales=None, exp_avg_sq_scales=None, grad_scale=None, seed=0):
+    """One AdamW step of the tensors in `params`, in place: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+    p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+
+    Lists of CUDA tensors of one device, one entry a parameter: params (bfloat16, float16 or float32, contiguous) and grads
+    (any of these types); steps, int32 tensors of one element, raised by one (t is the raised value); exp_avgs and
+    exp_avg_sqs, float32. With exp_avg_scales and exp_avg_sq_scales (uint8, one for every 128 values) the moments are held in
+    8 bits: exp_avgs[i] are float8_e4m3fn numbers of m over 2^(scale - 127), exp_avg_sqs[i] those of sqrt(v). m is rounded to
+    nearest, sqrt(v) at random by `seed`, step and place (the average moves by less than the distance of two such
+    numbers), a positive v never to zero; what is not finite becomes NaN.
+
+    masters (float32): the parameters that are updated, of which `params` then are the rounded copies. grad_scale: one
+    float32 on the device that multiplies every gradient (a clipping coefficient). lr: a number, or one float32 on the
+    device, which a captured step reads at every replay. Everything runs on the current stream without a host wait and can be
+    captured."""
+    with ops._Launch("adamw_step", 0):
+        launches = _lib.native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, masters, exp_avg_scales, exp_avg_sq_scales,
+                                            lr, betas[0], betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF,
+                                            torch.cuda.is_current_stream_capturing())
+    ops.launch_count += launches
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with a launch per parameter group. state_bits = 8 holds both moments of tensors of at least `min_8bit_size`
+    values in 8 bits (2 bytes a parameter instead of 8; adamw_step() says how), those of smaller ones, where nothing is to
+    be saved, in 32. master_weights keeps a float32 copy of parameters of fewer bits, which the updates go to: without it an
+    update of less than half a unit of a bfloat16 parameter's last place is lost.
+
+    lr may be a float32 tensor on the device: a step that was captured in a graph then reads it at every replay. State
+    dicts load and save as torch's do; `step` counts on the device."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, master_weights=True,
+                 min_8bit_size=4096, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not torch.is_tensor(lr) and not lr >= 0.0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"betas must be in [0, 1), got {betas}")
+        if not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"eps and weight_decay must not be negative, got {eps} and {weight_decay}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights, min_8bit_size=min_8bit_size, seed=seed))
+
+    def _state_of(self, p, group):
+        state = self.state[p]
+        if not state:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a parameter's first AdamW step makes its state and cannot be captured: take one step before")
+            state["step"] = torch.zeros((), dtype=torch.int32, device=p.device)
+            if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]:
+                for name in ("exp_avg", "exp_avg_sq"):
+                    state[name] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+                    state[name + "_scale"] = torch.zeros((p.numel() + BLOCK - 1) // BLOCK, dtype=torch.uint8, device=p.device)
+            else:
+                for name in ("exp_avg", "exp_avg_sq"):
+                    state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            if group["master_weights"] and p.dtype != torch.float32:
+                state["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format)
+        return state
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but every state keeps its own type: there, floating states take their parameter's."""
+        saved = {i: {k: v for k, v in s.items() if torch.is_tensor(v)} for i, s in state_dict["state"].items()}
+        super().load_state_dict(state_dict)
+        order = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(order, params):
+            for name, value in saved.get(i, {}).items():
+                self.state[p][name] = value.detach().to(p.device, copy=True)
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale=None):
+        """Updates every parameter that has a gradient. grad_scale (one float32 on the device) multiplies the gradients."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            # one launch holds one kind of state: 8 or 32 bits, with masters or without, on one device
+            kinds = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                s = self._state_of(p, group)
+                kinds.setdefault((p.device, "exp_avg_scale" in s, "master" in s), []).append((p, s))
+            for (_, eight, master), entries in kinds.items():
+                def column(name, entries=entries):
+                    return [s[name] for _, s in entries]
+
+                adamw_step([p for p, _ in entries], [p.grad for p, _ in entries], column("exp_avg"), column("exp_avg_sq"),
+                           column("step"), lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                           weight_decay=group["weight_decay"], masters=column("master") if master else None,
+                           exp_avg_scales=column("exp_avg_scale") if eight else None,
+                           exp_avg_sq_scales=column("exp_avg_sq_scale") if eight else None, grad_scale=grad_scale,
+                           seed=group["seed"])
+        return loss

@@ -55,6 +55,11 @@ extern "C" {
 #define FFM_STATUS_WAIT_PEER 105     /* a peer GPU's flag did not arrive within the wait budget */
 #define FFM_STATUS_EP_OVERFLOW 106   /* a rank would receive more rows than its declared bound: the call moved nothing */
 
+/* Element types of the operators that take several (layer norm, AdamW) */
+#define FFM_TYPE_BF16 0
+#define FFM_TYPE_FP16 1
+#define FFM_TYPE_FP32 2
+
 /* Gating */
 #define FFM_GATING_SOFTMAX 0
 #define FFM_GATING_SIGMOID 1
@@ -492,6 +497,65 @@ int ffm_p2p_signal_wait_dev(void* const* flag_arrays, int my_rank, int world, ui
                             int32_t* status, long long wait_cycles, ffm_stream_t stream);
 int ffm_p2p_signal_wait(void* const* flag_arrays, int my_rank, int world, uint32_t epoch, int32_t* status,
                         long long wait_cycles, ffm_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------------
+ * Layer norm over rows of D <= 32768 values (x_type: FFM_TYPE_*; fp32: 16384), the norm in front of the layer. `row_stride` is the
+ * distance of two rows of x in elements; y, dy and dx are contiguous. weight and bias (null: 1 and 0) may be of another
+ * type than x. Any D and any element-aligned address; rows of 16-byte boundaries are read 16 bytes at a time.
+ *
+ * ffm_layer_norm_forward: y = (x - mean) / sqrt(var + eps) * weight + bias; mean and rstd (f32 [rows], both or neither)
+ *   are what the backward pass reads. Statistics in fp32, the variance from squared differences.
+ * ffm_layer_norm_backward: dx (null: not computed), dweight [D] in w_type and dbias [D] in b_type (null: not computed).
+ *   Sums over the rows are in fp32 and in a fixed order. workspace: ffm_layer_norm_workspace_bytes, needed with dweight or
+ *   dbias. rows == 0 gives zero sums.
+ * ------------------------------------------------------------------------------------------------- */
+int ffm_layer_norm_forward(const void* x, int x_type, int64_t rows, int64_t row_stride, int D, const void* weight, int w_type,
+                           const void* bias, int b_type, float eps, void* y, float* mean, float* rstd, ffm_stream_t stream);
+size_t ffm_layer_norm_workspace_bytes(int64_t rows, int D, int x_type);
+int ffm_layer_norm_backward(const void* dy, const void* x, int x_type, int64_t rows, int64_t row_stride, int D,
+                            const void* weight, int w_type, const float* mean, const float* rstd, void* dx, void* dweight,
+                            void* dbias, int b_type, void* workspace, size_t workspace_bytes, ffm_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------------
+ * AdamW over `count` tensors, one launch for up to FFM_ADAMW_MAX of them (weight decay decoupled, eps outside of the root):
+ *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * Every field is 8 bytes wide. Types are FFM_TYPE_*; every tensor is contiguous. With `master` (f32, as many elements) that
+ * is updated and param is its rounded copy. step (int32) counts the tensor's steps and is raised by one; no two entries of a
+ * call share one. grad_scale and lr_device are device scalars (f32) or null; lr_device replaces lr.
+ *   bits = 32: exp_avg, exp_avg_sq are m and v in f32; the scales are not read.
+ *   bits = 8:  exp_avg, exp_avg_sq are e4m3 codes of m and sqrt(v) over 2^(scale - 127), with one scale byte for every 128
+ *              elements (the last block may be shorter). m is rounded to nearest, sqrt(v) at random by seed, step and place,
+ *              and never to zero where v > 0. A value that is not finite becomes NaN.
+ * ticket: a device word, zero before the call and after it, that no other call in flight uses.
+ * ------------------------------------------------------------------------------------------------- */
+#define FFM_ADAMW_MAX 256
+#define FFM_ADAMW_FEW 32 /* up to so many, a smaller argument block is launched */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  void* master;
+  void* exp_avg_scale;
+  void* exp_avg_sq_scale;
+  int32_t* step;
+  int64_t elements;
+  int64_t param_type;
+  int64_t grad_type;
+} ffm_adamw_tensor;
+typedef struct {
+  double lr;
+  double beta1;
+  double beta2;
+  double eps;
+  double weight_decay;
+  const float* lr_device;
+  const float* grad_scale;
+  int64_t bits;
+  int64_t seed;
+  void* ticket;
+} ffm_adamw_args;
+int ffm_adamw_step(const ffm_adamw_tensor* tensors, int count, const ffm_adamw_args* args, ffm_stream_t stream);
 
 #ifdef __cplusplus
 }
