@@ -28,6 +28,13 @@ constexpr int NORM_TEAM = 512;        // threads of a row at most, with two chun
 constexpr int NORM_TEAM_LONG = 1024;  // and with four
 constexpr int NORM_THREADS = 256;     // of a block, about, unless one row takes more
 constexpr int NORM_SM_THREADS = 768;  // of the backward kernel's blocks on an SM
+// The streaming kernels (many rows of 16-byte boundaries): one block an SM, four chunks a thread, a ring of rows a team.
+constexpr int STREAM_CHUNKS = 4, STREAM_STAGES = 2;
+constexpr int STREAM_BACK_STAGES = 3;     // where they fit (up to 8192 16-bit columns), else 2
+constexpr int STREAM_THREADS = 1024;      // forward: 64 registers
+constexpr int STREAM_BACK_THREADS = 512;  // backward: 128, 64 of them sums of dw and db
+static_assert(STREAM_THREADS / 64 <= 16 && STREAM_BACK_THREADS / 64 <= 15, "a barrier for every team of more than a warp");
+constexpr int STREAM_SMEM = 226 << 10;
 
 template <typename T>
 constexpr int VALUES = 16 / static_cast<int>(sizeof(T));  // of a chunk
@@ -232,6 +239,48 @@ layer_norm_forward_kernel(const T* __restrict__ x, long long stride, const void*
   }
 }
 
+// The block's row of partial sums: first the teams of a warp, then the warps that hold the same columns, one after the other
+// (sums: 2 D values of shared memory).
+template <typename T, int CH, bool VEC>
+__device__ __forceinline__ void add_teams(const Place<T, VEC>& at, int team, float* sums, int D, float (&aw)[CH][VALUES<T>],
+                                          float (&ab)[CH][VALUES<T>], float* part_w, float* part_b) {
+  constexpr int V = VALUES<T>;
+  for (int o = team; o < 32; o <<= 1) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        aw[c][j] += __shfl_xor_sync(0xffffffffu, aw[c][j], o);
+        ab[c][j] += __shfl_xor_sync(0xffffffffu, ab[c][j], o);
+      }
+    }
+  }
+  const int wide = team < 32 ? 32 : team, turns = blockDim.x / wide;
+  const bool mine = (threadIdx.x & 31) < team || team >= 32;
+  for (int k = 0; k < turns; ++k) {
+    if (static_cast<int>(threadIdx.x) / wide == k && mine) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int col = at.column(c, j);
+          if (at.has(c, j)) {
+            const float w = aw[c][j] + (k > 0 ? sums[col] : 0.0f), b = ab[c][j] + (k > 0 ? sums[D + col] : 0.0f);
+            if (k + 1 < turns) {
+              sums[col] = w;
+              sums[D + col] = b;
+            } else {
+              if (part_w != nullptr) part_w[static_cast<long long>(blockIdx.x) * D + col] = w;
+              if (part_b != nullptr) part_b[static_cast<long long>(blockIdx.x) * D + col] = b;
+            }
+          }
+        }
+      }
+    }
+    if (k + 1 < turns) __syncthreads();
+  }
+}
+
 // dx (skipped where null), and of every block one row of partial sums of dw and db (skipped where null).
 template <typename T, int CH, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -299,40 +348,337 @@ layer_norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, lo
     }
   }
   if (part_w == nullptr && part_b == nullptr) return;
-  // first the teams of a warp, then the warps that hold the same columns, one after the other
-  for (int o = team; o < 32; o <<= 1) {
+  add_teams<T, CH, VEC>(at, team, sums, D, aw, ab, part_w, part_b);
+}
+
+// ---- many rows of 16-byte boundaries ------------------------------------------------------------------------------------
+//
+// What a block holds in registers is too little to be in flight all the time: reading a row, two exchanges and writing it
+// follow one another (32768 x 7168 bf16: 354 us forward, 563 backward). Here every thread copies its chunks of the next rows
+// to shared memory (cp.async; it reads back what it copied itself, so nothing but its own wait stands between), and teams of
+// one block go their own way with a barrier each. Weight and bias lie in shared memory in fp32.
+
+// zeros where there is nothing to copy (`valid` is any address of the tensor then)
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, bool any, const void* valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(any ? src : valid), "r"(any ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void team_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// team_sum() for teams that do not keep step with one another: a barrier for each, from BARRIER on (16 teams of more than a
+// warp at most, 14 in the backward kernel, which meets as a block at barrier 0 in the end).
+template <int BARRIER, int N>
+__device__ __forceinline__ void own_team_sum(float (&v)[N], int team, float (*part)[32]) {
+  for (int o = (team < 32 ? team : 32) >> 1; o > 0; o >>= 1) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
+    for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  }
+  if (team <= 32) return;
+  if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        aw[c][j] += __shfl_xor_sync(0xffffffffu, aw[c][j], o);
-        ab[c][j] += __shfl_xor_sync(0xffffffffu, ab[c][j], o);
-      }
+    for (int n = 0; n < N; ++n) part[n][threadIdx.x >> 5] = v[n];
+  }
+  const int index = threadIdx.x / team;
+  team_barrier(BARRIER + index, team);
+  const int first = index * (team >> 5), lane = threadIdx.x & 31;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    v[n] = lane < team >> 5 ? part[n][first + lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  }
+}
+
+__device__ __forceinline__ uint4 read_shared_16(uint32_t at) {
+  uint4 v;
+  ld_shared_v4(at, v);
+  return v;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ unsigned long long bits2(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
+__device__ __forceinline__ float2 of_bits2(unsigned long long v) { return *reinterpret_cast<float2*>(&v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return of_bits2(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return of_bits2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return of_bits2(d);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+template <typename T>
+__device__ __forceinline__ void unpack2(const uint4& u, float2 (&v)[VALUES<T> / 2]) {
+  const uint32_t word[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int q = 0; q < VALUES<T> / 2; ++q) {
+    if constexpr (sizeof(T) == 4) {
+      v[q] = make_float2(__uint_as_float(word[2 * q]), __uint_as_float(word[2 * q + 1]));
+    } else if constexpr (std::is_same<T, bf16>::value) {
+      v[q] = make_float2(__uint_as_float(word[q] << 16), __uint_as_float(word[q] & 0xffff0000u));
+    } else {
+      v[q] = __half22float2(*reinterpret_cast<const __half2*>(&word[q]));
     }
   }
-  const int wide = team < 32 ? 32 : team, turns = blockDim.x / wide;
-  const bool mine = (threadIdx.x & 31) < team || team >= 32;
-  for (int k = 0; k < turns; ++k) {
-    if (static_cast<int>(threadIdx.x) / wide == k && mine) {
+}
+
+template <typename T>
+__device__ __forceinline__ void store2(T* p, const float2 (&v)[VALUES<T> / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+  } else {
+    const float values[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+    store8(p, values);
+  }
+}
+
+// A vector of D values in shared memory in fp32, four neighbours of every thread side by side: threads then read 16 bytes each
+// without a bank in common. Filled by the whole block.
+template <typename T>
+__device__ __forceinline__ void fill_vector(float* to, const void* p, int type, float fill, int D, int team) {
+  constexpr int V = VALUES<T>, PARTS = V / 4;
+  for (int i = threadIdx.x; i < team * STREAM_CHUNKS * V; i += blockDim.x) {
+    const int j = i & 3, quad = i >> 2, t = quad % team, part = quad / team;
+    const int col = (part / PARTS * team + t) * V + part % PARTS * 4 + j;
+    to[i] = p != nullptr && col < D ? load1_as(p, type, col) : fill;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void read_vector(uint32_t thread_base, int c, int team, float2 (&v)[VALUES<T> / 2]) {
+  constexpr int PARTS = VALUES<T> / 4;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
+  for (int h = 0; h < PARTS; ++h) {
+    const uint4 u = read_shared_16(thread_base + (c * PARTS + h) * team * 16);
+    v[2 * h] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    v[2 * h + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+}
+
+// Rows of a team: its own, and how often its loop runs (teams of a warp or less go in step with their warp's first).
+struct Trips {
+  int mine, all;
+  __device__ __forceinline__ Trips(long long rows, long long first, long long step, int team) {
+    auto count = [&](long long from) { return from < rows ? static_cast<int>((rows - from + step - 1) / step) : 0; };
+    mine = count(first);
+    all = team < 32 ? count(first - (threadIdx.x & 31) / team) : mine;
+  }
+};
+
+// s / n, rounded as a division would for whole results, with inv = 1 / n
+__device__ __forceinline__ float quotient(float s, float n, float inv) {
+  const float q = s * inv;
+  return fmaf(fmaf(-q, n, s), inv, q);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(STREAM_THREADS, 1)
+layer_norm_forward_stream_kernel(const T* __restrict__ x, long long stride, const void* __restrict__ weight, int w_type,
+                                 const void* __restrict__ bias, int b_type, long long rows, int D, float eps, int team,
+                                 T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+  extern __shared__ __align__(16) float scale[];  // weight, bias, ring
+  __shared__ float part[2][1][32];
+  constexpr int V = VALUES<T>, CH = STREAM_CHUNKS, S = STREAM_STAGES;
+  const Place<T, true> at(team, D);
+  float* shift = scale + team * CH * V;
+  const uint32_t my_scale = smem_u32(scale) + at.t * 16, my_shift = smem_u32(shift) + at.t * 16;
+  const uint32_t ring = smem_u32(shift + team * CH * V) + threadIdx.x * 16, slot = blockDim.x * 16;
+  const int teams = blockDim.x / team;
+  const float width = static_cast<float>(D), inv = 1.0f / width;
+  const long long first = static_cast<long long>(blockIdx.x) * teams + threadIdx.x / team, step = static_cast<long long>(gridDim.x) * teams;
+  const Trips trips(rows, first, step, team);
+  const T* source = x + first * stride + at.t * V;  // of the next row to fetch
+  auto fetch = [&](int k, uint32_t to) {
+    const int chunks = k < trips.mine ? at.count : 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int col = at.column(c, j);
-          if (at.has(c, j)) {
-            const float w = aw[c][j] + (k > 0 ? sums[col] : 0.0f), b = ab[c][j] + (k > 0 ? sums[D + col] : 0.0f);
-            if (k + 1 < turns) {
-              sums[col] = w;
-              sums[D + col] = b;
-            } else {
-              if (part_w != nullptr) part_w[static_cast<long long>(blockIdx.x) * D + col] = w;
-              if (part_b != nullptr) part_b[static_cast<long long>(blockIdx.x) * D + col] = b;
-            }
-          }
-        }
+    for (int c = 0; c < CH; ++c) copy_async_16(to + c * slot, source + c * team * V, c < chunks, x);
+    copy_async_commit();
+    source += step * stride;
+  };
+  const uint32_t row_bytes = CH * slot;
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(s, ring + s * row_bytes);
+  fill_vector<T>(scale, weight, w_type, 1.0f, D, team);
+  fill_vector<T>(shift, bias, b_type, 0.0f, D, team);
+  __syncthreads();
+  uint32_t here = ring;  // the row's stage
+  T* out = y + first * D + at.t * V;
+  for (int k = 0; k < trips.all; ++k, out += step * D) {
+    copy_async_wait<S - 1>();
+    float2 v[CH][V / 2], s2 = both(0.0f);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      unpack2<T>(read_shared_16(here + c * slot), v[c]);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) s2 = add2(s2, v[c][j]);
+    }
+    float s[1] = {s2.x + s2.y};
+    own_team_sum<0>(s, team, part[0]);
+    fetch(k + S, here);  // this thread's chunks have been read
+    here = here == ring + (S - 1) * row_bytes ? ring : here + row_bytes;
+    const float mu = quotient(s[0], width, inv);
+    s2 = both(0.0f);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const float2 less = both(c < at.count ? -mu : 0.0f);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        v[c][j] = add2(v[c][j], less);
+        s2 = fma2(v[c][j], v[c][j], s2);
       }
     }
-    if (k + 1 < turns) __syncthreads();
+    s[0] = s2.x + s2.y;
+    own_team_sum<0>(s, team, part[1]);
+    const float r = rsqrtf(fmaf(s[0], inv, eps));
+    if (k >= trips.mine) continue;
+    if (at.t == 0 && mean != nullptr) {
+      mean[first + k * step] = mu;
+      rstd[first + k * step] = r;
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float2 w[V / 2], b[V / 2];
+      read_vector<T>(my_scale, c, team, w);
+      read_vector<T>(my_shift, c, team, b);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) w[j] = fma2(mul2(v[c][j], both(r)), w[j], b[j]);
+      if (c < at.count) store2<T>(out + c * team * V, w);
+    }
+  }
+  copy_async_wait<0>();
+}
+
+template <typename T, int S>
+__global__ void __launch_bounds__(STREAM_BACK_THREADS, 1)
+layer_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict__ x, long long stride,
+                                  const void* __restrict__ weight, int w_type, const float* __restrict__ mean,
+                                  const float* __restrict__ rstd, long long rows, int D, int team, T* __restrict__ dx,
+                                  float* __restrict__ part_w, float* __restrict__ part_b) {
+  extern __shared__ __align__(16) float scale[];  // weight, ring; the ring's place then holds sums [2][D]
+  __shared__ float part[2][2][32];
+  constexpr int V = VALUES<T>, CH = STREAM_CHUNKS;
+  const Place<T, true> at(team, D);
+  const uint32_t my_scale = smem_u32(scale) + at.t * 16;
+  const uint32_t ring = smem_u32(scale + team * CH * V) + threadIdx.x * 16, slot = blockDim.x * 16;
+  const int teams = blockDim.x / team;
+  const float inv = 1.0f / static_cast<float>(D);
+  const long long first = static_cast<long long>(blockIdx.x) * teams + threadIdx.x / team, step = static_cast<long long>(gridDim.x) * teams;
+  const Trips trips(rows, first, step, team);
+  const T *source = x + first * stride + at.t * V, *source_dy = dy + first * D + at.t * V;  // of the next row to fetch
+  auto fetch = [&](int k, uint32_t to) {
+    const int chunks = k < trips.mine ? at.count : 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      copy_async_16(to + c * slot, source + c * team * V, c < chunks, x);
+      copy_async_16(to + (CH + c) * slot, source_dy + c * team * V, c < chunks, x);
+    }
+    copy_async_commit();
+    source += step * stride;
+    source_dy += step * D;
+  };
+  const uint32_t row_bytes = 2 * CH * slot;
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(s, ring + s * row_bytes);
+  fill_vector<T>(scale, weight, w_type, 1.0f, D, team);
+  __syncthreads();
+  float2 aw[CH][V / 2], ab[CH][V / 2];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) aw[c][j] = ab[c][j] = both(0.0f);
+  }
+  int parity = 0;
+  uint32_t here = ring;  // the row's stage
+  const float *mean_next = mean + first, *rstd_next = rstd + first;
+  float mu_next = 0.0f, r_next = 0.0f;
+  if (trips.mine > 0) mu_next = *mean_next, r_next = *rstd_next;
+  T* out = dx + first * D + at.t * V;
+  for (int k = 0; k < trips.all; ++k, parity ^= 1, out += step * D) {
+    // a row past the end has r = 0 and dy = 0: nothing in any sum
+    const float r = r_next, base = -mu_next * r_next;
+    mu_next = r_next = 0.0f;
+    mean_next += step;
+    rstd_next += step;
+    if (k + 1 < trips.mine) mu_next = *mean_next, r_next = *rstd_next;
+    copy_async_wait<S - 1>();
+    float2 s0 = both(0.0f), s1 = both(0.0f);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float2 v[V / 2], g[V / 2], w[V / 2];
+      unpack2<T>(read_shared_16(here + c * slot), v);
+      unpack2<T>(read_shared_16(here + (CH + c) * slot), g);
+      read_vector<T>(my_scale, c, team, w);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        const float2 xh = fma2(v[j], both(r), both(base));
+        aw[c][j] = fma2(g[j], xh, aw[c][j]);
+        ab[c][j] = add2(ab[c][j], g[j]);
+        g[j] = mul2(g[j], w[j]);
+        s0 = add2(s0, g[j]);
+        s1 = fma2(g[j], xh, s1);
+      }
+    }
+    float s[2] = {s0.x + s0.y, s1.x + s1.y};
+    own_team_sum<1>(s, team, part[parity]);
+    const int chunks = dx != nullptr && k < trips.mine ? at.count : 0;  // to write
+    const float2 c1 = both(-r * (s[0] * inv)), c2 = both(-r * (s[1] * inv));
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float2 v[V / 2], g[V / 2], w[V / 2];
+      // read again: held from the first pass on, they would take 32 of 128 registers, and others would be spilled
+      unpack2<T>(read_shared_16(here + c * slot), v);
+      unpack2<T>(read_shared_16(here + (CH + c) * slot), g);
+      read_vector<T>(my_scale, c, team, w);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        v[j] = fma2(fma2(v[j], both(r), both(base)), c2, fma2(mul2(g[j], w[j]), both(r), c1));
+      }
+      if (c < chunks) store2<T>(out + c * team * V, v);
+    }
+    fetch(k + S, here);  // this thread's chunks have been read
+    here = here == ring + (S - 1) * row_bytes ? ring : here + row_bytes;
+  }
+  copy_async_wait<0>();
+  if (part_w == nullptr && part_b == nullptr) return;
+  __syncthreads();
+  // every thread leaves its sums in the ring's place, [team][weight, bias][chunk and quarter][thread], and the block adds up the teams
+  constexpr int PARTS = V / 4;
+  float4* sums = reinterpret_cast<float4*>(scale + team * CH * V);
+  const int quads = CH * PARTS * team;
+  float4* my_sums = sums + threadIdx.x / team * 2 * quads + at.t;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+#pragma unroll
+    for (int h = 0; h < PARTS; ++h) {
+      my_sums[(c * PARTS + h) * team] = make_float4(aw[c][2 * h].x, aw[c][2 * h].y, aw[c][2 * h + 1].x, aw[c][2 * h + 1].y);
+      my_sums[quads + (c * PARTS + h) * team] = make_float4(ab[c][2 * h].x, ab[c][2 * h].y, ab[c][2 * h + 1].x, ab[c][2 * h + 1].y);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * quads; i += blockDim.x) {
+    const int q = i < quads ? i : i - quads;
+    float* out_row = i < quads ? part_w : part_b;
+    const int col = (q / team / PARTS * team + q % team) * V + q / team % PARTS * 4;
+    if (out_row == nullptr || col >= D) continue;
+    float4 total = sums[i];
+    for (int n = 1; n < teams; ++n) {
+      const float4 f = sums[n * 2 * quads + i];
+      total.x += f.x, total.y += f.y, total.z += f.z, total.w += f.w;
+    }
+    float* to = out_row + static_cast<long long>(blockIdx.x) * D + col;
+    to[0] = total.x, to[1] = total.y, to[2] = total.z, to[3] = total.w;
   }
 }
 
@@ -387,11 +733,72 @@ NormShape norm_shape(int D, int type) {
   return s;
 }
 
-// Blocks of the backward pass: one row of partial sums each.
+// Blocks of the backward pass at most (a streaming kernel has one an SM): one row of partial sums each.
 int backward_blocks(int64_t rows, int D, int type) {
   const NormShape s = norm_shape(D, type);
   const int64_t want = (rows + s.teams - 1) / s.teams, cap = static_cast<int64_t>(num_sms()) * (s.chunks == NORM_CHUNKS ? NORM_SM_THREADS / s.threads : 1);
   return static_cast<int>(want < cap ? (want > 0 ? want : 1) : cap);
+}
+
+// The streaming kernels' team and block: as many whole teams as fit.
+NormShape stream_shape(int D, int type, int most) {
+  const int values = 16 / type_bytes(type);
+  const int pieces = (D + values - 1) / values;
+  NormShape s;
+  s.chunks = STREAM_CHUNKS;
+  s.team = 1;
+  while (s.team < 32 && s.team * s.chunks < pieces) s.team *= 2;
+  if (s.team * s.chunks < pieces) s.team = (pieces + 32 * s.chunks - 1) / (32 * s.chunks) * 32;
+  s.teams = most / s.team;
+  s.threads = s.team * s.teams;
+  return s;
+}
+
+// Shared memory: `vectors` fp32 vectors of the row's width, and the ring of `stages` times `inputs` rows a team, or at least
+// the sums that lie in its place in the end.
+int stream_smem(const NormShape& s, int type, int vectors, int inputs, int stages, int least) {
+  const int ring = stages * inputs * STREAM_CHUNKS * s.threads * 16;
+  return vectors * s.team * STREAM_CHUNKS * (16 / type_bytes(type)) * static_cast<int>(sizeof(float)) + (ring > least ? ring : least);
+}
+
+// A ring pays where a team has several rows to go through.
+bool streams(int64_t rows, const NormShape& s, int smem, bool vec) {
+  return vec && s.teams > 0 && smem <= STREAM_SMEM && rows > 2ll * num_sms() * s.teams && rows < 1ll << 31;
+}
+
+template <typename T>
+int forward_stream(const void* x, int64_t stride, const void* w, int w_type, const void* b, int b_type, int64_t rows, int D,
+                   float eps, const NormShape& s, int smem, void* y, float* mean, float* rstd, cudaStream_t stream) {
+  static PerDevice room;
+  const int allowed = room.get([&] {
+    if (cudaFuncSetAttribute(layer_norm_forward_stream_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    return STREAM_SMEM;
+  });
+  if (smem > allowed) return FFM_ERR_LAUNCH;
+  layer_norm_forward_stream_kernel<T><<<num_sms(), s.threads, smem, stream>>>(static_cast<const T*>(x), stride, w, w_type, b, b_type,
+                                                                             rows, D, eps, s.team, static_cast<T*>(y), mean, rstd);
+  return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
+template <typename T, int S>
+int backward_stream(const void* dy, const void* x, int64_t stride, const void* w, int w_type, const float* mean, const float* rstd,
+                    int64_t rows, int D, const NormShape& s, int smem, void* dx, float* part_w, float* part_b, cudaStream_t stream) {
+  static PerDevice room;
+  const int allowed = room.get([&] {
+    if (cudaFuncSetAttribute(layer_norm_backward_stream_kernel<T, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    return STREAM_SMEM;
+  });
+  if (smem > allowed) return FFM_ERR_LAUNCH;
+  layer_norm_backward_stream_kernel<T, S><<<num_sms(), s.threads, smem, stream>>>(
+      static_cast<const T*>(dy), static_cast<const T*>(x), stride, w, w_type, mean, rstd, rows, D, s.team, static_cast<T*>(dx), part_w,
+      part_b);
+  return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
 
 template <typename T, int CH, bool VEC, int THREADS>
@@ -426,6 +833,13 @@ int backward_as(const void* dy, const void* x, int64_t stride, const void* w, in
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
 
+template <typename F>
+int with_type(int type, F&& f) {
+  if (type == FFM_TYPE_BF16) return f(bf16{});
+  if (type == FFM_TYPE_FP16) return f(fp16{});
+  return f(float{});
+}
+
 // f(type tag, chunks, vector accesses, threads of an SM) for the run-time values of a call
 template <typename F>
 int dispatch_norm(int type, const NormShape& s, bool vec, F&& f) {
@@ -437,9 +851,7 @@ int dispatch_norm(int type, const NormShape& s, bool vec, F&& f) {
                                    : with_vec(tag, std::integral_constant<int, NORM_CHUNKS_LONG>{},
                                               std::integral_constant<int, NORM_TEAM_LONG>{});
   };
-  if (type == FFM_TYPE_BF16) return with_chunks(bf16{});
-  if (type == FFM_TYPE_FP16) return with_chunks(fp16{});
-  return with_chunks(float{});
+  return with_type(type, with_chunks);
 }
 
 // 16-byte accesses: every row of every operand starts on a 16-byte boundary and is a whole number of them
@@ -467,6 +879,14 @@ extern "C" int ffm_layer_norm_forward(const void* x, int x_type, int64_t rows, i
   if (rows == 0) return FFM_OK;
   if (!x || !y) return FFM_ERR_BAD_ARG;
   const NormShape s = norm_shape(D, x_type);
+  const NormShape r = stream_shape(D, x_type, STREAM_THREADS);
+  const int smem = stream_smem(r, x_type, 2, 1, STREAM_STAGES, 0);
+  if (streams(rows, r, smem, norm_vectors(x_type, row_stride, D, x, y))) {
+    return with_type(x_type, [&](auto tag) {
+      return forward_stream<decltype(tag)>(x, row_stride, weight, w_type, bias, b_type, rows, D, eps, r, smem, y, mean, rstd,
+                                           static_cast<cudaStream_t>(stream));
+    });
+  }
   return dispatch_norm(x_type, s, norm_vectors(x_type, row_stride, D, x, y, weight, bias), [&](auto tag, auto ch, auto vec, auto threads) {
     return forward_as<decltype(tag), decltype(ch)::value, decltype(vec)::value, decltype(threads)::value>(
         x, row_stride, weight, w_type, bias, b_type, rows, D, eps, s, y, mean, rstd, static_cast<cudaStream_t>(stream));
@@ -490,12 +910,20 @@ extern "C" int ffm_layer_norm_backward(const void* dy, const void* x, int x_type
   if (parts && (workspace == nullptr || workspace_bytes < ffm_layer_norm_workspace_bytes(rows, D, x_type))) return FFM_ERR_WORKSPACE;
   if (!parts && (dx == nullptr || rows == 0)) return FFM_OK;
   const NormShape s = norm_shape(D, x_type);
-  const int blocks = backward_blocks(rows, D, x_type);
+  const NormShape r = stream_shape(D, x_type, STREAM_BACK_THREADS);
+  const int sums = r.threads * STREAM_CHUNKS * (16 / type_bytes(x_type)) * 2 * static_cast<int>(sizeof(float));
+  int smem = stream_smem(r, x_type, 1, 2, STREAM_BACK_STAGES, sums);
+  const bool deep = smem <= STREAM_SMEM;
+  if (!deep) smem = stream_smem(r, x_type, 1, 2, STREAM_STAGES, sums);
+  const bool vectors = norm_vectors(x_type, row_stride, D, dy, x, dx), stream_rows = streams(rows, r, smem, vectors);
+  const int blocks = stream_rows ? num_sms() : backward_blocks(rows, D, x_type);
   float* part_w = dweight != nullptr ? static_cast<float*>(workspace) : nullptr;
   float* part_b = dbias != nullptr ? static_cast<float*>(workspace) + static_cast<size_t>(blocks) * D : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool vectors = norm_vectors(x_type, row_stride, D, dy, x, dx);
-  const int rc = dispatch_norm(x_type, s, vectors, [&](auto tag, auto ch, auto vec, auto threads) {
+  const int rc = stream_rows ? with_type(x_type, [&](auto tag) {
+    return (deep ? backward_stream<decltype(tag), STREAM_BACK_STAGES> : backward_stream<decltype(tag), STREAM_STAGES>)(
+        dy, x, row_stride, weight, w_type, mean, rstd, rows, D, r, smem, dx, part_w, part_b, st);
+  }) : dispatch_norm(x_type, s, vectors, [&](auto tag, auto ch, auto vec, auto threads) {
     return backward_as<decltype(tag), decltype(ch)::value, decltype(vec)::value, decltype(threads)::value>(
         dy, x, row_stride, weight, w_type, mean, rstd, rows, D, s, dx, part_w, part_b, blocks, st);
   });

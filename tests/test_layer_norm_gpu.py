@@ -79,6 +79,31 @@ def test_forward_and_backward(width, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [8, 64, 256, 264, 1024, 1400, 4096, 8192])
+def test_many_rows(width, dtype):
+    """More rows than the device has teams for: several of them one after the other, the last round not full."""
+    rows = 148 * 1024 // min(1024, max(1, width // 32)) * 3 + 5
+    x, w, b, dy = inputs(rows, width, dtype, width)
+    out, bound = reference(x, w, b, 1e-5, dy)
+    y, (dx, dw, db) = run(x, w, b, dy)
+    for got, name in ((y, "y"), (dx, "dx"), (dw, "dw"), (db, "db")):
+        check(got, out, bound, name)
+    again, grads = run(x, w, b, dy)
+    assert torch.equal(y, again) and all(torch.equal(p, q) for p, q in zip((dx, dw, db), grads))
+
+
+@pytest.mark.gpu
+def test_many_rows_with_a_distance():
+    base = torch.randn(9000, 1040, device="cuda").bfloat16()
+    x, (_, w, b, dy) = base[:, 8:1032], inputs(9000, 1024, torch.bfloat16, 21)
+    out, bound = reference(x, w, b, 1e-5, dy)
+    y, (dx, dw, db) = run(x, w, b, dy)
+    for got, name in ((y, "y"), (dx, "dx"), (dw, "dw"), (db, "db")):
+        check(got, out, bound, name)
+
+
+@pytest.mark.gpu
 def test_widest_rows():
     for width, dtype in ((32768, torch.bfloat16), (20001, torch.float16), (16384, torch.float32), (9000, torch.float32)):
         x, w, b, dy = inputs(5, width, dtype, 3)
