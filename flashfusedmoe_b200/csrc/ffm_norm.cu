@@ -517,45 +517,49 @@ layer_norm_forward_stream_kernel(const T* __restrict__ x, long long stride, cons
   T* out = y + first * D + at.t * V;
   for (int k = 0; k < trips.all; ++k, out += step * D) {
     copy_async_wait<S - 1>();
-    float2 v[CH][V / 2], s2 = both(0.0f);
+    float2 s2 = both(0.0f);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      unpack2<T>(read_shared_16(here + c * slot), v[c]);
+      float2 v[V / 2];
+      unpack2<T>(read_shared_16(here + c * slot), v);
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) s2 = add2(s2, v[c][j]);
+      for (int j = 0; j < V / 2; ++j) s2 = add2(s2, v[j]);
     }
     float s[1] = {s2.x + s2.y};
     own_team_sum<0>(s, team, part[0]);
-    fetch(k + S, here);  // this thread's chunks have been read
-    here = here == ring + (S - 1) * row_bytes ? ring : here + row_bytes;
     const float mu = quotient(s[0], width, inv);
     s2 = both(0.0f);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const float2 less = both(c < at.count ? -mu : 0.0f);
+      float2 v[V / 2];
+      unpack2<T>(read_shared_16(here + c * slot), v);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) {
-        v[c][j] = add2(v[c][j], less);
-        s2 = fma2(v[c][j], v[c][j], s2);
+        v[j] = add2(v[j], less);
+        s2 = fma2(v[j], v[j], s2);
       }
     }
     s[0] = s2.x + s2.y;
     own_team_sum<0>(s, team, part[1]);
     const float r = rsqrtf(fmaf(s[0], inv, eps));
-    if (k >= trips.mine) continue;
-    if (at.t == 0 && mean != nullptr) {
+    const int chunks = k < trips.mine ? at.count : 0;  // to write
+    if (at.t == 0 && chunks > 0 && mean != nullptr) {
       mean[first + k * step] = mu;
       rstd[first + k * step] = r;
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float2 w[V / 2], b[V / 2];
+      float2 v[V / 2], w[V / 2], b[V / 2];
+      unpack2<T>(read_shared_16(here + c * slot), v);
       read_vector<T>(my_scale, c, team, w);
       read_vector<T>(my_shift, c, team, b);
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) w[j] = fma2(mul2(v[c][j], both(r)), w[j], b[j]);
-      if (c < at.count) store2<T>(out + c * team * V, w);
+      for (int j = 0; j < V / 2; ++j) w[j] = fma2(mul2(add2(v[j], both(-mu)), both(r)), w[j], b[j]);
+      if (c < chunks) store2<T>(out + c * team * V, w);
     }
+    fetch(k + S, here);  // this thread's chunks have been read
+    here = here == ring + (S - 1) * row_bytes ? ring : here + row_bytes;
   }
   copy_async_wait<0>();
 }
@@ -874,10 +878,10 @@ extern "C" int ffm_layer_norm_forward(const void* x, int x_type, int64_t rows, i
                                       int w_type, const void* bias, int b_type, float eps, void* y, float* mean, float* rstd,
                                       ffm_stream_t stream) {
   if (!norm_arguments(x_type, rows, row_stride, D, weight, w_type) || (bias != nullptr && !is_type(b_type))) return FFM_ERR_BAD_ARG;
-  if (!(eps >= 0.0f) || (mean == nullptr) != (rstd == nullptr)) return FFM_ERR_BAD_ARG;
+  if (!(eps >= 0.0f)) return FFM_ERR_BAD_ARG;
   if (D > max_columns(x_type)) return FFM_ERR_UNSUPPORTED;
   if (rows == 0) return FFM_OK;
-  if (!x || !y) return FFM_ERR_BAD_ARG;
+  if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return FFM_ERR_BAD_ARG;
   const NormShape s = norm_shape(D, x_type);
   const NormShape r = stream_shape(D, x_type, STREAM_THREADS);
   const int smem = stream_smem(r, x_type, 2, 1, STREAM_STAGES, 0);

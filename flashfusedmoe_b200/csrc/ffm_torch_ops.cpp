@@ -2,10 +2,12 @@
 // Python costs these few checks; the torch operations that they would be there (views, contiguity, empty) take longer than
 // the kernels of a small call.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 
+#include <atomic>
 #include <mutex>
 #include <optional>
 #include <stdexcept>
@@ -112,17 +114,24 @@ Rows as_rows(const Tensor& t) {
   return {x, rows, stride == 0 ? D : stride};
 }
 
-void check_vector(const OptTensor& v, const Tensor& x, const char* name) {
-  if (!v.has_value()) return;
-  same_device(*v, x, name);
-  if (v->dim() != 1 || v->size(0) != x.size(-1)) {
-    throw py::value_error(std::string(name) + " must be [" + std::to_string(x.size(-1)) + "], got " + c10::str(v->sizes()));
+void check_vector(const Tensor& v, const Tensor& x, const char* name) {
+  if (!v.defined()) return;
+  same_device(v, x, name);
+  if (v.dim() != 1 || v.size(0) != x.size(-1)) {
+    throw py::value_error(std::string(name) + " must be [" + std::to_string(x.size(-1)) + "], got " + c10::str(v.sizes()));
   }
-  element_type(*v, name);
+  element_type(v, name);
 }
 
-// (y, mean, rstd); without `stats` the last two are None
-py::tuple layer_norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, bool stats) {
+void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+std::atomic<int64_t> launches{0};  // of these operators' kernels so far
+
+struct NormResult {
+  Tensor y, mean, rstd;
+};
+
+NormResult norm_forward_of(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool stats) {
   on_gpu(x, "x");
   if (x.dim() < 1 || x.size(-1) < 1) throw py::value_error("x must have a last dimension to normalise, got " + c10::str(x.sizes()));
   if (!(eps >= 0.0)) throw py::value_error("eps must not be negative, got " + std::to_string(eps));
@@ -131,53 +140,112 @@ py::tuple layer_norm_forward(const Tensor& x, const OptTensor& weight, const Opt
   check_vector(bias, x, "bias");
   const On device(x);
   const Rows r = as_rows(x);
-  const Tensor w = weight.has_value() ? plain(*weight) : Tensor(), b = bias.has_value() ? plain(*bias) : Tensor();
-  const Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-  Tensor mean, rstd;
+  const Tensor w = weight.defined() ? plain(weight) : Tensor(), b = bias.defined() ? plain(bias) : Tensor();
+  NormResult out;
+  out.y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
   if (stats) {
-    mean = at::empty({r.rows}, x.options().dtype(at::kFloat));
-    rstd = at::empty({r.rows}, x.options().dtype(at::kFloat));
+    const Tensor both = at::empty({2, r.rows}, x.options().dtype(at::kFloat));
+    out.mean = both.select(0, 0);
+    out.rstd = both.select(0, 1);
   }
-  check(norm_forward(r.x.data_ptr(), type, r.rows, r.stride, static_cast<int>(x.size(-1)), w.defined() ? w.data_ptr() : nullptr,
-                     w.defined() ? element_type(w, "weight") : 0, b.defined() ? b.data_ptr() : nullptr,
-                     b.defined() ? element_type(b, "bias") : 0, static_cast<float>(eps), y.data_ptr(),
-                     stats ? mean.data_ptr<float>() : nullptr, stats ? rstd.data_ptr<float>() : nullptr, device.stream()),
+  check(norm_forward(r.x.data_ptr(), type, r.rows, r.stride, static_cast<int>(x.size(-1)), address(w),
+                     w.defined() ? element_type(w, "weight") : 0, address(b), b.defined() ? element_type(b, "bias") : 0,
+                     static_cast<float>(eps), out.y.data_ptr(), stats ? out.mean.data_ptr<float>() : nullptr,
+                     stats ? out.rstd.data_ptr<float>() : nullptr, device.stream()),
         "ffm_layer_norm_forward");
-  if (!stats) return py::make_tuple(y, py::none(), py::none());
-  return py::make_tuple(y, mean, rstd);
+  launches += r.rows > 0;
+  return out;
 }
 
-// (dx, dweight, dbias), None where not wanted
-py::tuple layer_norm_backward(const Tensor& dy, const Tensor& x, const OptTensor& weight, const Tensor& mean, const Tensor& rstd,
-                              bool want_x, bool want_weight, bool want_bias, const py::object& bias_type) {
+struct NormGradients {
+  Tensor dx, dweight, dbias;
+};
+
+NormGradients norm_backward_of(const Tensor& dy, const Tensor& x, const Tensor& weight, const Tensor& mean, const Tensor& rstd,
+                               bool want_x, bool want_weight, bool want_bias, at::ScalarType bias_type) {
   const On device(x);
   const int type = element_type(x, "x");
   const int64_t D = x.size(-1);
   const Rows r = as_rows(x);
-  if (mean.numel() != r.rows || rstd.numel() != r.rows || mean.scalar_type() != at::kFloat || rstd.scalar_type() != at::kFloat) {
-    throw py::value_error("saved statistics do not belong to x");
+  // saved-tensor hooks may have handed back other tensors than were saved
+  for (const Tensor* t : {&mean, &rstd}) {
+    if (t->numel() != r.rows || t->scalar_type() != at::kFloat || !t->is_cuda()) throw py::value_error("saved statistics do not belong to x");
   }
   const Tensor m = plain(mean), s = plain(rstd);
   const Tensor g = plain(dy.scalar_type() == x.scalar_type() ? dy : dy.to(x.scalar_type()));
+  same_device(g, x, "the gradient of y");
   if (g.sizes() != x.sizes()) throw py::value_error("the gradient of y has another shape than x");
-  const Tensor w = weight.has_value() ? plain(*weight) : Tensor();
-  Tensor dx, dw, db, workspace;
-  if (want_x) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-  if (want_weight) dw = at::empty({D}, w.options());
-  if (want_bias) db = at::empty({D}, x.options().dtype(bias_type.is_none() ? x.scalar_type() : bias_type.cast<at::ScalarType>()));
+  const Tensor w = weight.defined() ? plain(weight) : Tensor();
+  NormGradients out;
+  Tensor workspace;
+  if (want_x) out.dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  if (want_weight) out.dweight = at::empty({D}, w.options());
+  if (want_bias) out.dbias = at::empty({D}, x.options().dtype(bias_type));
   size_t bytes = 0;
   if (want_weight || want_bias) {
     bytes = norm_workspace(r.rows, static_cast<int>(D), type);
     workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
   }
-  auto address = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
   check(norm_backward(g.data_ptr(), r.x.data_ptr(), type, r.rows, r.stride, static_cast<int>(D), address(w),
-                      w.defined() ? element_type(w, "weight") : 0, m.data_ptr<float>(), s.data_ptr<float>(), address(dx),
-                      address(dw), address(db), db.defined() ? element_type(db, "bias") : 0, address(workspace), bytes,
-                      device.stream()),
+                      w.defined() ? element_type(w, "weight") : 0, m.data_ptr<float>(), s.data_ptr<float>(), address(out.dx),
+                      address(out.dweight), address(out.dbias), want_bias ? element_type(out.dbias, "bias") : 0, address(workspace),
+                      bytes, device.stream()),
         "ffm_layer_norm_backward");
-  auto handed = [](const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); };
-  return py::make_tuple(handed(dx), handed(dw), handed(db));
+  launches += want_weight || want_bias ? 2 : want_x && r.rows > 0;
+  return out;
+}
+
+using torch::autograd::variable_list;
+
+// What a backward pass hands out when it is itself recorded (create_graph): gradients that refuse to be differentiated.
+variable_list once(variable_list gradients) {
+  if (!at::GradMode::is_enabled()) return gradients;
+  for (Tensor& g : gradients) {
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  }
+  auto refuses = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that can be differentiated once", static_cast<int64_t>(gradients.size()));
+  return (*refuses)(std::move(gradients));
+}
+
+// The graph's node in C++: from Python, the engine's thread takes the interpreter's lock and a training step of a small norm
+// took 92 us of host time.
+class LayerNorm : public torch::autograd::Function<LayerNorm> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& weight_or_none, const OptTensor& bias_or_none,
+                        double eps) {
+    const Tensor weight = weight_or_none.value_or(Tensor()), bias = bias_or_none.value_or(Tensor());
+    NormResult r = norm_forward_of(x, weight, bias, eps, true);
+    ctx->save_for_backward({x, weight, r.mean, r.rstd});
+    ctx->saved_data["bias"] = bias.defined();
+    ctx->saved_data["bias_type"] = static_cast<int64_t>(bias.defined() ? bias.scalar_type() : x.scalar_type());
+    return r.y;
+  }
+  static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list grad) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out(4);
+    {
+      const at::AutoGradMode no_grad(false);
+      // an operand that is not there has no edge, and those after it move up
+      const bool weight = saved[1].defined(), bias = ctx->saved_data["bias"].toBool();
+      NormGradients g = norm_backward_of(grad[0], saved[0], saved[1], saved[2], saved[3], ctx->needs_input_grad(0),
+                                         weight && ctx->needs_input_grad(1), bias && ctx->needs_input_grad(weight ? 2 : 1),
+                                         static_cast<at::ScalarType>(ctx->saved_data["bias_type"].toInt()));
+      out[0] = g.dx;
+      out[1] = g.dweight;
+      out[2] = g.dbias;
+    }
+    return once(std::move(out));
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  const py::gil_scoped_release released;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()))) {
+    return LayerNorm::apply(x, weight, bias, eps);
+  }
+  return norm_forward_of(x, w, b, eps, false).y;
 }
 
 // ---- AdamW --------------------------------------------------------------------------------------------------
@@ -198,8 +266,7 @@ Tensor ticket_for(const Tensor& like, const void* stream, bool capturing) {
 
 using Tensors = std::vector<Tensor>;
 
-// Launches.
-int64_t adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
+void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
                    const Tensors& steps, const std::optional<Tensors>& masters, const std::optional<Tensors>& exp_avg_scales,
                    const std::optional<Tensors>& exp_avg_sq_scales, const py::object& lr, double beta1, double beta2, double eps,
                    double weight_decay, const OptTensor& grad_scale, int64_t seed, bool capturing) {
@@ -221,7 +288,7 @@ int64_t adamw_step(const Tensors& params, const Tensors& grads, const Tensors& e
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) throw py::value_error("betas must be in [0, 1)");
   if (!(eps >= 0.0)) throw py::value_error("eps must not be negative");
   if (!(weight_decay >= 0.0)) throw py::value_error("weight_decay must not be negative");
-  if (n == 0) return 0;
+  if (n == 0) return;
 
   const Tensor& first = params[0];
   on_gpu(first, "param");
@@ -330,14 +397,14 @@ int64_t adamw_step(const Tensors& params, const Tensors& grads, const Tensors& e
       for (const Tensor& t : **list) changed(t);
     }
   }
-  return (static_cast<int64_t>(n) + FFM_ADAMW_MAX - 1) / FFM_ADAMW_MAX;
+  launches += (static_cast<int64_t>(n) + FFM_ADAMW_MAX - 1) / FFM_ADAMW_MAX;
 }
 
 }  // namespace
 
 void define_ops(py::module_& m) {
   m.def("bind_ops", &bind_ops);
-  m.def("layer_norm_forward", &layer_norm_forward);
-  m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("launches", [] { return launches.load(); });
+  m.def("layer_norm", &layer_norm);
   m.def("adamw_step", &adamw_step);
 }

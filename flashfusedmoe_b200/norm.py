@@ -4,26 +4,7 @@ the kernels of libffmoe."""
 import torch
 import torch.nn as nn
 
-from . import _lib, ops
-
-
-class _LayerNormFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        with ops._Launch("layer_norm_forward", 1 if x.numel() else 0):
-            y, mean, rstd = _lib.native().layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, weight, mean, rstd = ctx.saved_tensors
-        want = ctx.needs_input_grad[:3]
-        with ops._Launch("layer_norm_backward", 1 + (want[1] or want[2])):
-            dx, dw, db = _lib.native().layer_norm_backward(grad, x, weight, mean, rstd, *want, ctx.bias_dtype)
-        return dx, dw, db, None
+from . import _lib
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -33,12 +14,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     type and shape and is contiguous. Statistics are fp32, and so is everything in between. D is any number up to 32768
     (float32: 16384). The rows of x may be further apart than D; other strides are copied. Differentiable once, with the
     gradients of weight and bias summed in a fixed order."""
-    eps = float(eps)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
-        return _LayerNormFunction.apply(x, weight, bias, eps)
-    with ops._Launch("layer_norm_forward", 1 if x.numel() else 0):
-        return _lib.native().layer_norm_forward(x, weight, bias, eps, False)[0]
+    return _lib.native().layer_norm(x, weight, bias, eps)
 
 
 class LayerNorm(nn.Module):

@@ -85,6 +85,12 @@ class _Launch:
         return False
 
 
+def operator_launches():
+    """Kernels enqueued so far by the operators beside the layer (layer norm, AdamW), which launch from the torch extension and
+    are not in `launch_count`."""
+    return _lib.native().launches()
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 

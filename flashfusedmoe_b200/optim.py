@@ -2,7 +2,7 @@
 
 import torch
 
-from . import _lib, ops
+from . import _lib
 
 BLOCK = 128   # values of a tensor that share a scale in an 8-bit state
 
@@ -23,11 +23,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     float32 on the device that multiplies every gradient (a clipping coefficient). lr: a number, or one float32 on the
     device, which a captured step reads at every replay. Everything runs on the current stream without a host wait and can be
     captured."""
-    with ops._Launch("adamw_step", 0):
-        launches = _lib.native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, masters, exp_avg_scales, exp_avg_sq_scales,
-                                            lr, betas[0], betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF,
-                                            torch.cuda.is_current_stream_capturing())
-    ops.launch_count += launches
+    _lib.native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, masters, exp_avg_scales, exp_avg_sq_scales, lr, betas[0],
+                             betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF, torch.cuda.is_current_stream_capturing())
 
 
 class AdamW(torch.optim.Optimizer):

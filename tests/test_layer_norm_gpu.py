@@ -288,3 +288,28 @@ def test_refusals():
         layer_norm(torch.zeros(1, 32776, device="cuda", dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="last dimension"):
         layer_norm(x[0, 0])
+
+
+@pytest.mark.gpu
+def test_a_recorded_backward_pass_refuses_a_second_derivative():
+    from flashfusedmoe_b200 import layer_norm, ops
+    x, w, b, dy = inputs(4, 64, torch.float32, 1)
+    out, bound = reference(x, w, b, 1e-5, dy)
+    x = x.requires_grad_()
+    before = ops.operator_launches()
+    grad, = torch.autograd.grad(layer_norm(x, w, b), x, dy, create_graph=True)
+    assert ops.operator_launches() == before + 2
+    check(grad.detach(), out, bound, "dx")
+    with pytest.raises(RuntimeError, match="twice"):
+        grad.sum().backward()
+
+
+@pytest.mark.gpu
+def test_saved_input_may_not_change():
+    from flashfusedmoe_b200 import layer_norm
+    x, w, b, dy = inputs(4, 64, torch.float32, 1)
+    w.requires_grad_()
+    y = layer_norm(x, w, b)
+    x.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
