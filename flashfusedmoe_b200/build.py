@@ -18,13 +18,13 @@ LIB = os.path.join(HERE, "libffmoe.so")
 NATIVE_SOURCES = ["ffm_torch.cpp", "ffm_torch_ops.cpp"]
 PTXAS_LOG = os.path.join(HERE, "libffmoe.ptxas.txt")
 SOURCES = ["ffm_api.cu", "ffm_route.cu", "ffm_rows.cu", "ffm_route_bwd.cu", "ffm_gemm_sm100.cu", "ffm_gemm_tok_sm100.cu",
-           "ffm_p2p.cu", "ffm_fp8.cu", "ffm_layer.cu", "ffm_norm.cu", "ffm_adamw.cu"]
+           "ffm_p2p.cu", "ffm_fp8.cu", "ffm_layer.cu", "ffm_norm.cu", "ffm_adamw.cu", "ffm_vocab.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--use_fast_math", "-Xptxas", "-v",
 ]
 # roots, quotients and small numbers as IEEE arithmetic has them: fp32 outputs, second moments far below 2^-126
-EXACT_SOURCES = {"ffm_norm.cu", "ffm_adamw.cu"}
+EXACT_SOURCES = {"ffm_norm.cu", "ffm_adamw.cu", "ffm_vocab.cu"}
 
 
 def _newest_source_mtime():

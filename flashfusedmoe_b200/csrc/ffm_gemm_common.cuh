@@ -60,6 +60,12 @@ __device__ __forceinline__ void tma_store_3d(const void* map, uint32_t src, int 
                "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
+// the same, fp32 values added to those in memory
+__device__ __forceinline__ void tma_reduce_add_3d(const void* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
 // Ask the TMA unit to bring one box of a tensor into L2 (nothing lands in shared memory, nothing to wait for).
 __device__ __forceinline__ void tma_prefetch_l2_2d(const void* map, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1)
@@ -175,6 +181,39 @@ inline int make_map_2d(CUtensorMap* map, const void* base, long long rows, long 
   CUresult r = fn(map, elt_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                   const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
+// make_map_2d for bf16 rows that are `ld` elements apart; rows may end anywhere.
+inline int make_ld_map(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_cols, int box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return FFM_ERR_NO_DRIVER;
+  if (rows <= 0 || cols <= 0 || ld < cols) return FFM_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || ld % 8 != 0) return FFM_ERR_UNSUPPORTED;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
+// 3-D output map over [groups, rows, cols] with rows `ld` elements of 2 or 4 bytes apart (4: fp32), 128-byte swizzle, boxes of 128
+// bytes x 32 rows.
+inline int make_box_map(CUtensorMap* map, void* base, long long groups, long long rows, long long cols, long long ld, int elt_bytes) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return FFM_ERR_NO_DRIVER;
+  if (groups <= 0 || rows <= 0 || cols <= 0 || ld < cols) return FFM_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (ld * elt_bytes) % 16 != 0) return FFM_ERR_UNSUPPORTED;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(groups)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * elt_bytes, static_cast<cuuint64_t>(ld) * rows * elt_bytes};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / elt_bytes), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, elt_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box,
+                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FFM_OK : FFM_ERR_LAUNCH;
 }

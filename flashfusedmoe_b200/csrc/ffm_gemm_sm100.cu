@@ -36,6 +36,8 @@
 // tiles); the GLU epilogue fills three (activation, gate, up) per 64-column step.
 #include <stdlib.h>
 
+#include <cuda_fp16.h>
+
 #include "ffm_gemm_common.cuh"
 #include "ffm_internal.h"
 
@@ -59,14 +61,16 @@ constexpr int SMEM_CTRL_BYTES = 2048;
 constexpr int MAX_STAGES = 6;
 constexpr int SMEM_LIMIT = 232448;  // 227 KiB of dynamic shared memory per CTA
 
-enum { EPI_PLAIN = 0, EPI_GLU = 1, EPI_GLUBWD = 2 };
+enum { EPI_PLAIN = 0, EPI_GLU = 1, EPI_GLUBWD = 2, EPI_SOFTMAX = 3, EPI_F32 = 4 };
 // The GLU epilogues get a second warp per TMEM lane quarter (helper warps 6..9, each taking the upper 32 columns of
 // every 64-column step). The GLU backward does about 16 instructions and two MUFU operations per accumulator element,
 // too much for one warp per scheduler inside a tile's main loop (0.174 -> 0.164 ms at 8 x 4096 rows, D 1024, H 2048);
 // the e4m3 up-projection has half the main loop of the bf16 one under the same epilogue (1382 -> 1626 TFLOP/s); the
 // bf16 up-projection gains 1 % (and needs 105 instead of 234 registers, since its loops are rolled).
 constexpr int HELPER_THREADS = 128;
-__host__ __device__ constexpr bool epilogue_helpers(int epi) { return epi == EPI_GLUBWD || epi == EPI_GLU; }
+__host__ __device__ constexpr bool epilogue_helpers(int epi) {
+  return epi == EPI_GLUBWD || epi == EPI_GLU || epi == EPI_SOFTMAX;
+}
 __host__ __device__ constexpr int gemm_threads(int epi, int pass) {
   return GEMM_THREADS + pass * PASSENGER_THREADS + (epilogue_helpers(epi) ? HELPER_THREADS : 0);
 }
@@ -98,20 +102,24 @@ __host__ __device__ constexpr int gemm_threads(int epi, int pass) {
 //   CTA pair, plain: 6 stages x 32 KiB + 1 box      CTA pair, GLU: 5 stages x 32 KiB + 3 boxes
 //   one CTA,  plain: 4 stages x 48 KiB + 2 boxes    one CTA,  GLU: 3 stages x 48 KiB + 3 boxes
 //   GLU backward epilogue (EPI_GLUBWD): 4 stages + 2 x 2 boxes (one CTA: 3 stages + 2 x 2 boxes)
+//   softmax epilogue (EPI_SOFTMAX): 5 stages (one CTA: 3) + 2 boxes for either warp of a quarter
+//   fp32 results (EPI_F32): the plain shape with 2 boxes of 32 columns
 // A GLU step stores three boxes (activation, gate, up) as one bulk group; a plain step stores one box; a GLU backward
 // step stores two (gate gradient, up gradient).
 template <int CTA2, int EPI>
 struct Shape {
   static constexpr int STAGES = EPI == EPI_GLU      ? (CTA2 ? FFM_TUNE_PG_STAGES : 3)
                                 : EPI == EPI_GLUBWD ? (CTA2 ? 4 : 3)
+                                : EPI == EPI_SOFTMAX ? (CTA2 ? 5 : 3)
                                                     : (CTA2 ? FFM_TUNE_PP_STAGES : 4);
   static constexpr int B_STAGE_BYTES = (CTA2 ? 128 : 256) * BK * 2;
   static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
-  static constexpr int BOXES_PER_STEP = EPI == EPI_GLU ? 3 : (EPI == EPI_GLUBWD ? 2 : 1);
+  static constexpr int BOXES_PER_STEP = EPI == EPI_GLU ? 3 : (EPI == EPI_GLUBWD || EPI == EPI_SOFTMAX ? 2 : 1);
   static constexpr int STEPS_BUFFERED = EPI == EPI_GLU      ? (CTA2 ? FFM_TUNE_PG_STEPS : 1)
                                         : EPI == EPI_GLUBWD ? (CTA2 ? FFM_TUNE_GB_STEPS : 2)
-                                                            : (CTA2 ? FFM_TUNE_PP_STEPS : 2);
+                                        : EPI == EPI_PLAIN  ? (CTA2 ? FFM_TUNE_PP_STEPS : 2)
+                                                            : 2;
   static constexpr int STG_WARP_BYTES = BOXES_PER_STEP * STEPS_BUFFERED * BOX_BYTES;
   static constexpr int STG_BYTES = EPI_WARPS * STG_WARP_BYTES;
   static constexpr int SMEM_BYTES = RING_BYTES + STG_BYTES + SMEM_CTRL_BYTES + 1024;  // + 1 KiB alignment slack
@@ -157,6 +165,16 @@ __device__ __forceinline__ const float* fp8_a_scale(const GemmParams& p) {
 __device__ __forceinline__ const float* fp8_b_scale(const GemmParams& p) {
   return reinterpret_cast<const float*>(p.pz_pre);
 }
+// EPI_SOFTMAX has no passenger either and keeps what it needs in the same fields: pz_rows rows, pz_h vocabulary entries, a
+// target per row, the target's logit to be written, and a (maximum, sum) per row and 128 entries. has_c2: the exponentials are
+// stored. EPI_F32: has_c2 says whether the result is added to what is there.
+__device__ __forceinline__ const long long* softmax_targets(const GemmParams& p) {
+  return reinterpret_cast<const long long*>(p.pz_dact);
+}
+__device__ __forceinline__ float* softmax_target_logits(const GemmParams& p) {
+  return reinterpret_cast<float*>(const_cast<bf16*>(p.pz_pre));
+}
+__device__ __forceinline__ float2* softmax_stats(const GemmParams& p) { return reinterpret_cast<float2*>(p.pz_gu); }
 
 struct Ctrl {
   unsigned long long full_bar[MAX_STAGES];
@@ -429,6 +447,85 @@ __device__ __forceinline__ void glu_forward_half_step(uint32_t tcol, int act, fl
   }
 }
 
+// This warp's 32 rows x 128 vocabulary entries (from entry c0 on) of a tile of logits: lane = row, entries in TMEM columns
+// tcol .. tcol + 127. Two passes over TMEM, so that 32 values are held at a time and no exponential is taken twice: the largest
+// logit (and the target's, if it is here), then e = exp(logit - largest) and its sum. With `store` the e of 64 entries at a time
+// go to the row's piece of memory in fp16: in (0, 1] it has 11 bits, so that the gradient, which is rounded to bf16 later,
+// has seen one rounding that counts; what lies below 2^-24 of the largest of 128 is lost to it. The sum is of the unrounded e.
+__device__ __forceinline__ void softmax_half_tile(const GemmParams& p, const CUtensorMap* out, uint32_t tcol, int c0, int half,
+                                                  int row0, int lane, uint32_t stg, int& slot) {
+  const int valid = min(128, p.pz_h - c0);
+  if (valid <= 0) return;  // the whole warp
+  constexpr float LOG2E = 1.4426950408889634f;
+  const bool store = p.has_c2 != 0;
+  const long long row = static_cast<long long>(row0) + lane;
+  const long long target = row < p.pz_rows ? softmax_targets(p)[row] - c0 : -1;
+  const int at = target >= 0 && target < valid ? static_cast<int>(target) : -1;
+  float top = -INFINITY, mine = 0.0f;
+  uint32_t v[32];
+#pragma unroll 1
+  for (int c = 0; c < valid; c += 32) {
+    tmem_ld_32x32(tcol + c, v);
+    tmem_ld_wait();
+    if (valid - c < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (i >= valid - c) v[i] = 0xff800000u;  // -infinity
+      }
+    }
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(v[i]));
+    top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+    if (__any_sync(0xffffffffu, at >= c && at < c + 32)) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (at == c + i) mine = __uint_as_float(v[i]);
+      }
+    }
+  }
+  if (at >= 0) softmax_target_logits(p)[row] = mine;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int c = 0; c < valid; c += 32) {
+    const uint32_t box = stg + slot * BOX_BYTES;
+    if (store && (c & 32) == 0) {
+      if (lane == 0) bulk_wait_read<1>();  // the store before the last one has read this box
+      __syncwarp();
+    }
+    tmem_ld_32x32(tcol + c, v);
+    tmem_ld_wait();
+    const int left = valid - c;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = q * 8 + j * 2;
+        float a = exp2f((__uint_as_float(v[i]) - top) * LOG2E), b = exp2f((__uint_as_float(v[i + 1]) - top) * LOG2E);
+        if (left < 32) {
+          a = i < left ? a : 0.0f;
+          b = i + 1 < left ? b : 0.0f;
+        }
+        sum[j] += a + b;
+        __half2 h = __floats2half2_rn(a, b);
+        o[j] = *reinterpret_cast<uint32_t*>(&h);
+      }
+      if (store) st_shared_v4(box + box_offset(lane, (c >> 3 & 4) + q), o[0], o[1], o[2], o[3]);
+    }
+    if (store && ((c & 32) != 0 || left <= 32)) {
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(out, box, c0 + (c & ~63), row0, 0);  // clipped at the last entry and the last row
+        bulk_commit();
+      }
+      slot ^= 1;
+    }
+  }
+  if (row < p.pz_rows) softmax_stats(p)[half * p.pz_rows + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+}
+
 // FP8 = 1: A and B hold e4m3 bytes, K-major only; a stage row is still 128 bytes, i.e. 128 K elements per block.
 template <int A_MN, int B_MN, int EPI, int GROUPK, int CTA2, int PASS = 0, int FP8 = 0>
 __global__ void __launch_bounds__(gemm_threads(EPI, PASS), 1)
@@ -562,10 +659,11 @@ ffm_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
               tma_load_2d(a_dst + 8192, &tmA, full, m0 + 64, krow);
             }
           } else {
+            const int kcol = GROUPK ? t.k_row0 + k0 : k0;
             if (CTA2) {
-              tma_load_2d_pair(a_dst, &tmA, full, k0, m0);
+              tma_load_2d_pair(a_dst, &tmA, full, kcol, m0);
             } else {
-              tma_load_2d(a_dst, &tmA, full, k0, m0);
+              tma_load_2d(a_dst, &tmA, full, kcol, m0);
             }
           }
           // B tile: all 256 columns, or with CTA2 this CTA's 128-column half
@@ -664,13 +762,13 @@ ffm_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             phase ^= 1u;
           }
         }
-        if (GROUPK && ok && t.k_tail > 0) {
+        if (GROUPK && A_MN && ok && t.k_tail > 0) {
           // The group's last K block, up to its last valid row. It stands apart because the issuing thread has no time to
           // spare: with the test for the last step in the loop above every weight gradient was slower, also without
           // padding (8 x 4096 rows, 4096 x 1024: 180 -> 203 us; 64 x 1536 rows, 2816 x 2048: 843 -> 972), and so were
           // replayed training steps (16384 tokens, 8 experts and a shared one: 1966 -> 2037 us). (Measured before the
           // issuing thread was elected.)
-          static_assert(!GROUPK || (A_MN && B_MN && !FP8), "both operands of a grouped-K GEMM are M/N-major bf16");
+          static_assert(!GROUPK || (B_MN && !FP8), "a grouped-K GEMM has an N-major bf16 B, and valid rows only with an M-major A");
           ok = mbar_wait_bounded(smem_u32(&ctrl->full_bar[stage]), phase, abort_flag, p.status, FFM_STATUS_WAIT_MMA,
                                  p.wait_cycles);
           if (!ok) break;
@@ -878,6 +976,47 @@ ffm_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           if (++step_slot == S::STEPS_BUFFERED) step_slot = 0;
         }
         if (!ok) break;
+      } else if (EPI == EPI_SOFTMAX) {
+        // a quarter's two warps take half of the entries each, with two boxes of their own
+        const int side = helper ? 1 : 0;
+        softmax_half_tile(p, &tmC, taddr + side * 128, t.n_block * BN + side * 128, t.n_block * 2 + side, row0, lane,
+                          stg + side * (S::STG_WARP_BYTES / 2), step_slot);
+      } else if (EPI == EPI_F32) {
+        // eight steps of 32 columns (one box of fp32 each), TMEM loads one step ahead; stored, or added to what is there by the
+        // memory system (one launch adds to an element once, so that the order of launches is the order of the additions)
+        const int n0 = t.n_block * BN;
+        uint32_t v[2][32];
+        if (have_acc) tmem_ld_32x32(taddr, v[0]);
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          if (have_acc) {
+            tmem_ld_wait();
+            if (c + 1 < BN / 32) tmem_ld_32x32(taddr + (c + 1) * 32, v[(c + 1) & 1]);
+          }
+          if (n0 + c * 32 >= p.n_cols) continue;
+          const uint32_t box = stg + step_slot * STEP_BYTES;
+          if (lane == 0) bulk_wait_read<S::STEPS_BUFFERED - 1>();
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            if (have_acc) {
+              st_shared_v4(box + box_offset(lane, q), v[c & 1][4 * q], v[c & 1][4 * q + 1], v[c & 1][4 * q + 2], v[c & 1][4 * q + 3]);
+            } else {
+              st_shared_v4(box + box_offset(lane, q), 0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            if (p.has_c2) {
+              tma_reduce_add_3d(&tmC, box, n0 + c * 32, row0, zdim);
+            } else {
+              tma_store_3d(&tmC, box, n0 + c * 32, row0, zdim);
+            }
+            bulk_commit();
+          }
+          if (++step_slot == S::STEPS_BUFFERED) step_slot = 0;
+        }
       } else {
         // four steps of 64 columns (one box each), two 32-column chunks per step, TMEM loads one chunk ahead
         const int n0 = t.n_block * BN;
@@ -1390,4 +1529,87 @@ extern "C" int ffm_grouped_gemm_dact_glu_backward(const void* gY, const void* Wd
   p.pz_act = activation;
   return launch_gemm<0, 1, EPI_GLUBWD, 0>(tmA, tmB, tmL, tmC, tmP, p, (rows + BM - 1) / BM, p.n_tiles,
                                           static_cast<cudaStream_t>(stream), tile_rows);
+}
+
+// ---- the products of the linear cross entropy (ffm_vocab.cu) ----
+
+int ffm::softmax_logits(const void* hidden, const void* weight, int64_t rows, int D, int V, const int64_t* targets,
+                        float* target_logits, float* stats, void* e, int64_t ld_e, int32_t* status, ffm_stream_t stream) {
+  CUtensorMap tmA, tmB, tmC;
+  int rc;
+  if ((rc = make_map_2d(&tmA, hidden, rows, D, 64, 128)) != FFM_OK) return rc;
+  if ((rc = make_map_2d(&tmB, weight, V, D, 64, 128)) != FFM_OK) return rc;
+  if (e != nullptr) {
+    if ((rc = make_box_map(&tmC, e, 1, rows, V, ld_e, 2)) != FFM_OK) return rc;
+  } else {
+    tmC = tmA;  // never stored through
+  }
+  GemmParams p = {};
+  p.groups = 1;
+  p.dense_m_tiles = static_cast<int>((rows + BM - 1) / BM);
+  p.n_cols = V;
+  p.k_blocks = (D + BK - 1) / BK;  // what is past D reads as zero
+  p.b_group_rows = V;
+  p.b1_row_offset = 128;
+  p.has_c2 = e != nullptr ? 1 : 0;
+  p.scale = 1.0f;
+  p.n_tiles = (V + BN - 1) / BN;
+  p.status = status;
+  p.wait_cycles = g_wait_cycles;
+  p.pz_dact = reinterpret_cast<const bf16*>(targets);
+  p.pz_pre = reinterpret_cast<const bf16*>(target_logits);
+  p.pz_gu = reinterpret_cast<bf16*>(stats);
+  p.pz_rows = rows;
+  p.pz_h = V;
+  return launch_gemm<0, 0, EPI_SOFTMAX, 0>(tmA, tmB, tmB, tmC, tmC, p, p.dense_m_tiles, p.n_tiles,
+                                           static_cast<cudaStream_t>(stream), rows <= BM ? 128 : 0);
+}
+
+int ffm::dense_rows(const void* A, int64_t ld_a, int64_t rows, int K, const void* B, int Nout, int splits, void* out,
+                    int32_t* status, ffm_stream_t stream) {
+  CUtensorMap tmA, tmB, tmC;
+  int rc;
+  if ((rc = make_ld_map(&tmA, A, rows, K, ld_a, 64, 128)) != FFM_OK) return rc;
+  if ((rc = make_map_2d(&tmB, B, K, Nout, 64, 64)) != FFM_OK) return rc;
+  if ((rc = make_box_map(&tmC, out, splits, rows, Nout, Nout, splits > 1 ? 4 : 2)) != FFM_OK) return rc;
+  GemmParams p = {};
+  p.groups = splits;
+  p.n_cols = Nout;
+  p.scale = 1.0f;
+  p.n_tiles = (Nout + BN - 1) / BN;
+  p.status = status;
+  p.wait_cycles = g_wait_cycles;
+  p.b_group_rows = K;
+  const int m_tiles = static_cast<int>((rows + BM - 1) / BM);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (splits > 1) {
+    p.dense_m_tiles = (K + BM - 1) / BM;  // 128-deep pieces of the contraction
+    p.m_tiles_per_group = m_tiles;
+    return launch_gemm<0, 1, EPI_F32, 1>(tmA, tmB, tmB, tmC, tmC, p, m_tiles, static_cast<long long>(splits) * p.n_tiles, s);
+  }
+  p.dense_m_tiles = m_tiles;
+  p.k_blocks = (K + BK - 1) / BK;
+  return launch_gemm<0, 1, EPI_PLAIN, 0>(tmA, tmB, tmB, tmC, tmC, p, m_tiles, p.n_tiles, s);
+}
+
+int ffm::dense_transposed(const void* A, int64_t ld_a, const void* B, int64_t rows, int M, int Nout, int f32, int add, void* out,
+                          int32_t* status, ffm_stream_t stream) {
+  CUtensorMap tmA, tmB, tmC;
+  int rc;
+  if ((rc = make_ld_map(&tmA, A, rows, M, ld_a, 64, 64)) != FFM_OK) return rc;
+  if ((rc = make_map_2d(&tmB, B, rows, Nout, 64, 64)) != FFM_OK) return rc;
+  if ((rc = make_box_map(&tmC, out, 1, M, Nout, Nout, f32 ? 4 : 2)) != FFM_OK) return rc;
+  GemmParams p = {};
+  p.groups = 1;
+  p.dense_m_tiles = static_cast<int>((rows + BM - 1) / BM);
+  p.n_cols = Nout;
+  p.scale = 1.0f;
+  p.m_tiles_per_group = (M + BM - 1) / BM;
+  p.n_tiles = (Nout + BN - 1) / BN;
+  p.status = status;
+  p.wait_cycles = g_wait_cycles;
+  p.has_c2 = add;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (f32) return launch_gemm<1, 1, EPI_F32, 1>(tmA, tmB, tmB, tmC, tmC, p, p.m_tiles_per_group, p.n_tiles, s);
+  return launch_gemm<1, 1, EPI_PLAIN, 1>(tmA, tmB, tmB, tmC, tmC, p, p.m_tiles_per_group, p.n_tiles, s);
 }

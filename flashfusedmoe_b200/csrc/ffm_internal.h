@@ -51,4 +51,22 @@ int combine_forward_status(const void* Y, const int32_t* pos, const float* w, co
 // out = a + b, bf16 values added in fp32 (n elements, a multiple of 8)
 int add_bf16(const void* a, const void* b, int64_t n, void* out, ffm_stream_t stream);
 
+// ---- products of the linear cross entropy (ffm_gemm_sm100.cu) ----
+
+// Logits hidden [rows, D] weight [V, D]^T, a tile at a time and never stored: stats[h * rows + n] = (largest, sum of exp(logit -
+// largest)) (pairs of floats) over row n's entries 128 h .. 128 h + 127, target_logits[n] the logit of targets[n] where that is
+// an entry; with `e` the exponentials in fp16, rows ld_e apart (a multiple of 8). D % 8 == 0.
+int softmax_logits(const void* hidden, const void* weight, int64_t rows, int D, int V, const int64_t* targets,
+                   float* target_logits, float* stats, void* e, int64_t ld_e, int32_t* status, ffm_stream_t stream);
+
+// A [rows, K] (rows ld_a apart) B [K, Nout]: bf16 out [rows, Nout], or with splits > 1 fp32 out [splits, rows, Nout] of as many
+// pieces of the contraction. Nout % 8 == 0, any K.
+int dense_rows(const void* A, int64_t ld_a, int64_t rows, int K, const void* B, int Nout, int splits, void* out, int32_t* status,
+               ffm_stream_t stream);
+
+// A [rows, M]^T (rows ld_a apart) B [rows, Nout]: out [M, Nout] in bf16, or in fp32, with `add` added to what is there.
+// Nout % 8 == 0, any M.
+int dense_transposed(const void* A, int64_t ld_a, const void* B, int64_t rows, int M, int Nout, int f32, int add, void* out,
+                     int32_t* status, ffm_stream_t stream);
+
 }  // namespace ffm

@@ -557,6 +557,50 @@ typedef struct {
 } ffm_adamw_args;
 int ffm_adamw_step(const ffm_adamw_tensor* tensors, int count, const ffm_adamw_args* args, ffm_stream_t stream);
 
+/* -------------------------------------------------------------------------------------------------
+ * Linear cross entropy: l = hidden weight^T (bf16 [N, D] and [V, D], D % 8 == 0, any N and V), lse = log sum exp l,
+ * nll[n] = lse - l[target] + z lse^2; 0 where targets[n] == ignore_index. The logits are never stored. A target outside of the
+ * vocabulary sets FFM_STATUS_BAD_INDEX; its nll is NaN and its gradient zero.
+ *   mean = 1: the loss is divided by the number of rows that count (NaN without any; the gradients are zero then).
+ *   loss (null: not wanted): the sum, or the mean, of nll.
+ *   d_hidden bf16 [N, D], d_weight [V, D] in bf16 or (d_weight_f32) fp32, null where not wanted: the gradients of
+ *     loss, or with row_grad (f32 [N], mean = 0) of the sum of row_grad[n] nll[n].
+ *   piece_rows: with gradients, so many rows at a time have their V entries in the workspace (2 bytes each). With fewer than N the
+ *     gradient of the weight is summed over the pieces in fp32.
+ *   workspace: ffm_linear_cross_entropy_workspace_bytes of the same block (pointers only have to be null or not).
+ *   status_host (null, or host memory the device can write): a non-zero *status is stored there.
+ *   launched (null or host): kernels enqueued are added.
+ * Every field is 8 bytes wide.
+ *
+ * ffm_scale_in_place: x *= *factor, a device scalar (elements % 8 == 0, 16-byte aligned); x is not touched where that is 1.
+ * ------------------------------------------------------------------------------------------------- */
+typedef struct {
+  int64_t N;
+  int64_t D;
+  int64_t V;
+  int64_t ignore_index;
+  int64_t mean;
+  int64_t d_weight_f32;
+  int64_t piece_rows;
+  double z;
+  const void* hidden;
+  const void* weight;
+  const int64_t* targets;
+  const float* row_grad;
+  float* nll;
+  float* loss;
+  void* d_hidden;
+  void* d_weight;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  int32_t* status_host;
+  int64_t* launched;
+} ffm_loss_args;
+size_t ffm_linear_cross_entropy_workspace_bytes(const ffm_loss_args* args);
+int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t stream);
+int ffm_scale_in_place(void* x, int x_type, int64_t elements, const float* factor, ffm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
