@@ -166,7 +166,7 @@ __device__ __forceinline__ const float* fp8_b_scale(const GemmParams& p) {
   return reinterpret_cast<const float*>(p.pz_pre);
 }
 // EPI_SOFTMAX has no passenger either and keeps what it needs in the same fields: pz_rows rows, pz_h vocabulary entries, a
-// target per row, the target's logit to be written, and a (maximum, sum) per row and 128 entries. has_c2: the exponentials are
+// target per row, the target's logit to be written, and a (maximum, sum) for every 128 entries of a row, side by side. has_c2: the exponentials are
 // stored. EPI_F32: has_c2 says whether the result is added to what is there.
 __device__ __forceinline__ const long long* softmax_targets(const GemmParams& p) {
   return reinterpret_cast<const long long*>(p.pz_dact);
@@ -485,6 +485,7 @@ __device__ __forceinline__ void softmax_half_tile(const GemmParams& p, const CUt
     }
   }
   if (at >= 0) softmax_target_logits(p)[row] = mine;
+  const float base = top == -INFINITY ? 0.0f : top;  // nothing but -infinity: e = 0
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
   for (int c = 0; c < valid; c += 32) {
@@ -502,7 +503,7 @@ __device__ __forceinline__ void softmax_half_tile(const GemmParams& p, const CUt
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = q * 8 + j * 2;
-        float a = exp2f((__uint_as_float(v[i]) - top) * LOG2E), b = exp2f((__uint_as_float(v[i + 1]) - top) * LOG2E);
+        float a = exp2f((__uint_as_float(v[i]) - base) * LOG2E), b = exp2f((__uint_as_float(v[i + 1]) - base) * LOG2E);
         if (left < 32) {
           a = i < left ? a : 0.0f;
           b = i + 1 < left ? b : 0.0f;
@@ -523,7 +524,7 @@ __device__ __forceinline__ void softmax_half_tile(const GemmParams& p, const CUt
       slot ^= 1;
     }
   }
-  if (row < p.pz_rows) softmax_stats(p)[half * p.pz_rows + row] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (row < p.pz_rows) softmax_stats(p)[row * ((p.pz_h + 127) >> 7) + half] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
 }
 
 // FP8 = 1: A and B hold e4m3 bytes, K-major only; a stage row is still 128 bytes, i.e. 128 K elements per block.

@@ -53,8 +53,8 @@ int add_bf16(const void* a, const void* b, int64_t n, void* out, ffm_stream_t st
 
 // ---- products of the linear cross entropy (ffm_gemm_sm100.cu) ----
 
-// Logits hidden [rows, D] weight [V, D]^T, a tile at a time and never stored: stats[h * rows + n] = (largest, sum of exp(logit -
-// largest)) (pairs of floats) over row n's entries 128 h .. 128 h + 127, target_logits[n] the logit of targets[n] where that is
+// Logits hidden [rows, D] weight [V, D]^T, a tile at a time and never stored: stats[n * ceil(V / 128) + h] = (largest,
+// sum of exp(logit - largest)) (pairs of floats) over row n's entries 128 h .. 128 h + 127, target_logits[n] the logit of targets[n] where that is
 // an entry; with `e` the exponentials in fp16, rows ld_e apart (a multiple of 8). D % 8 == 0.
 int softmax_logits(const void* hidden, const void* weight, int64_t rows, int D, int V, const int64_t* targets,
                    float* target_logits, float* stats, void* e, int64_t ld_e, int32_t* status, ffm_stream_t stream);

@@ -20,7 +20,6 @@ namespace ffm {
 namespace {
 
 constexpr int HALF = 128;         // entries with one maximum
-constexpr int ROW_GROUP = 32;     // rows of a block of loss_rows_kernel
 constexpr int LOSS_THREADS = 1024;
 
 __device__ __forceinline__ double block_sum(double v, double* part) {
@@ -40,119 +39,142 @@ __device__ __forceinline__ void report(const int32_t* status, volatile int32_t* 
   }
 }
 
-// *share = 1 / number of rows that count (infinite without any: the mean is NaN then). A target outside of the vocabulary is reported.
+// *share = 1 / number of rows that count (infinite without any: the mean is NaN then)
 __global__ void __launch_bounds__(LOSS_THREADS)
-loss_count_kernel(const long long* __restrict__ targets, long long rows, long long ignore, int V, float* __restrict__ share,
-                  int32_t* status) {
+loss_count_kernel(const long long* __restrict__ targets, long long rows, long long ignore, float* __restrict__ share) {
   __shared__ double part[32];
   int n = 0;
-  bool bad = false;
-  for (long long i = threadIdx.x; i < rows; i += LOSS_THREADS) {
-    const long long t = targets[i];
-    if (t != ignore) {
-      ++n;
-      bad |= t < 0 || t >= V;
-    }
-  }
-  if (bad) atomicCAS(status, 0, FFM_STATUS_BAD_INDEX);
+  for (long long i = threadIdx.x; i < rows; i += LOSS_THREADS) n += targets[i] != ignore;
   const double count = block_sum(n, part);
   if (threadIdx.x == 0) *share = static_cast<float>(1.0 / count);
 }
 
-// 32 rows a block, one a lane; the warps share the row's pieces of 128 entries. First pass: the row's largest logit and sum
-// (warps join in shared memory). Second pass (with `factor`): exp(maximum of a piece - lse) times the row's gradient, transposed
-// to [row][piece] on the way, since the next kernel goes along rows.
-__global__ void __launch_bounds__(1024)
-loss_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ target_logits, const long long* __restrict__ targets,
-                 long long rows, int pieces, int V, long long ignore, float z, const float* __restrict__ share,
-                 const float* __restrict__ row_grad, float* __restrict__ nll, float* __restrict__ factor,
-                 float* __restrict__ target_entry, const int32_t* status, volatile int32_t* status_host) {
-  report(status, status_host);
-  __shared__ float top_part[32][33], sum_part[32][33];
-  __shared__ float row_lse[ROW_GROUP], row_scale[ROW_GROUP];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long row0 = static_cast<long long>(blockIdx.x) * ROW_GROUP, row = row0 + lane;
-  const bool active = row < rows;
-  float top = -INFINITY, sum = 0.0f;
-  for (int h = warp; h < pieces; h += 4 * 32) {
-    float2 s[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool any = active && h + 32 * u < pieces;
-      s[u] = any ? stats[(h + 32 * u) * rows + row] : make_float2(-INFINITY, 0.0f);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float m = fmaxf(top, s[u].x);
-      // nothing yet (-inf), or nothing but NaN: nothing to scale
-      sum = (top == -INFINITY ? sum : sum * expf(top - m)) + (s[u].x == -INFINITY ? s[u].y : s[u].y * expf(s[u].x - m));
-      top = m;
-    }
-  }
-  top_part[warp][lane] = top;
-  sum_part[warp][lane] = sum;
-  __syncthreads();
-  if (warp == 0) {
-    for (int w = 1; w < 32; ++w) top = fmaxf(top, top_part[w][lane]);
-    sum = 0.0f;
-    for (int w = 0; w < 32; ++w) {
-      const float m = top_part[w][lane];
-      sum += m == -INFINITY ? sum_part[w][lane] : sum_part[w][lane] * expf(m - top);
-    }
-    const float lse = logf(sum) + top;
-    float scale = 0.0f;
-    if (active) {
-      const long long t = targets[row];
-      const bool counts = t != ignore, known = t >= 0 && t < V;
-      const float logit = counts && known ? target_logits[row] : NAN;
-      nll[row] = counts ? fmaf(z * lse, lse, lse - logit) : 0.0f;
-      // a row with a target that is none has no gradient; its loss is NaN
-      if (counts && known && factor != nullptr) {
-        const float g = (share != nullptr ? *share : 1.0f) * (row_grad != nullptr ? row_grad[row] : 1.0f);
-        const float less = logit - lse;
-        scale = g * fmaf(2.0f * z, lse, 1.0f);
-        target_entry[row] = g * fmaf(expf(less), 2.0f * z * lse, expm1f(less));
-      }
-    }
-    row_lse[lane] = lse;
-    row_scale[lane] = scale;
-  }
-  if (factor == nullptr) return;
-  __syncthreads();
-  const float lse = row_lse[lane], scale = row_scale[lane];
-  for (int h0 = 0; h0 < pieces; h0 += 32) {
-    const int h = h0 + warp;
-    float f = 0.0f;
-    if (active && h < pieces && scale != 0.0f) f = expf(stats[h * rows + row].x - lse) * scale;
-    __syncthreads();  // the tile before has been written out
-    top_part[warp][lane] = f;
-    __syncthreads();
-    if (row0 + warp < rows && h0 + lane < pieces) factor[(row0 + warp) * pieces + h0 + lane] = top_part[lane][warp];
-  }
+__device__ __forceinline__ void join(float& top, float& sum, float other_top, float other_sum) {
+  const float m = fmaxf(top, other_top);
+  // nothing yet (-inf), or nothing but NaN: nothing to scale
+  sum = (top == -INFINITY ? sum : sum * expf(top - m)) + (other_top == -INFINITY ? other_sum : other_sum * expf(other_top - m));
+  top = m;
 }
 
-// e (fp16) to dl (bf16) in place: eight entries a thread, 2048 a block and row.
+// From a row's maxima and sums to its loss, and (with `factor`) to what its pieces of 128 exponentials are multiplied by for the
+// gradient, exp(maximum - lse) times the row's factor. A row has TEAM threads: a warp, or a block where there are few rows.
+//
+// The tensor core's sums lose some of their last bits over a long D (4096: 3e-6 of a logit). That hardly shows in lse, which is over
+// many entries, but in the target's logit it does; so that one is taken again here in fp32, and replaces the other in the
+// row's sum as well, where it may be nearly everything (2 N D multiply-adds and 4 bytes: 0.1 % of the products).
+template <int TEAM>
+__global__ void __launch_bounds__(256)
+loss_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ target_logits, const long long* __restrict__ targets,
+                 const bf16* __restrict__ hidden, const bf16* __restrict__ weight, int D, long long rows, int pieces, int V,
+                 long long ignore, float z, const float* __restrict__ share, const float* __restrict__ row_grad,
+                 float* __restrict__ nll, float* __restrict__ factor, float* __restrict__ target_entry, int32_t* status,
+                 volatile int32_t* status_host) {
+  report(status, status_host);
+  __shared__ float part[3][8];
+  const int t = threadIdx.x % TEAM, warp = threadIdx.x >> 5;
+  const long long row = static_cast<long long>(blockIdx.x) * (256 / TEAM) + threadIdx.x / TEAM;
+  if (row >= rows) return;  // whole teams
+  const long long target = targets[row];
+  const bool counts = target != ignore, known = target >= 0 && target < V;
+  float top = -INFINITY, sum = 0.0f, dot = 0.0f;
+  const float2* mine = stats + row * pieces;
+  for (int h = t; h < pieces; h += 4 * TEAM) {
+    float2 s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s[u] = h + u * TEAM < pieces ? mine[h + u * TEAM] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) join(top, sum, s[u].x, s[u].y);
+  }
+  if (counts && known) {
+    const bf16 *x = hidden + row * D, *w = weight + target * D;
+    for (int c = t * 8; c < D; c += TEAM * 8) {
+      float a[8], b[8];
+      load8(x + c, a);
+      load8(w + c, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot = fmaf(a[j], b[j], dot);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float other_top = __shfl_xor_sync(0xffffffffu, top, o), other_sum = __shfl_xor_sync(0xffffffffu, sum, o);
+    join(top, sum, other_top, other_sum);
+    dot += __shfl_xor_sync(0xffffffffu, dot, o);
+  }
+  if (TEAM > 32) {
+    if ((threadIdx.x & 31) == 0) {
+      part[0][warp] = top;
+      part[1][warp] = sum;
+      part[2][warp] = dot;
+    }
+    __syncthreads();
+    top = part[0][0], sum = part[1][0], dot = part[2][0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      join(top, sum, part[0][w], part[1][w]);
+      dot += part[2][w];
+    }
+  }
+  if (counts && known) sum = fmaxf(sum - expf(target_logits[row] - top), 0.0f) + expf(dot - top);
+  const float lse = logf(sum) + top;
+  float scale = 0.0f;
+  // a row with a target that is none has no gradient; its loss is NaN
+  if (counts && known && factor != nullptr) {
+    const float g = (share != nullptr ? *share : 1.0f) * (row_grad != nullptr ? row_grad[row] : 1.0f);
+    scale = g * fmaf(2.0f * z, lse, 1.0f);
+    if (t == 0) target_entry[row] = g * fmaf(expf(dot - lse), 2.0f * z * lse, expm1f(dot - lse));
+  }
+  if (t == 0) {
+    nll[row] = counts ? (known ? fmaf(z * lse, lse, lse - dot) : NAN) : 0.0f;
+    if (counts && !known) atomicCAS(status, 0, FFM_STATUS_BAD_INDEX);
+  }
+  if (factor == nullptr) return;
+  float* out = factor + row * pieces;
+  for (int h = t; h < pieces; h += TEAM) out[h] = scale != 0.0f ? expf(mine[h].x - lse) * scale : 0.0f;
+}
+
+// e (fp16) to dl (bf16) in place: eight entries a thread, 2048 a block, GRADIENT_ROWS rows of them at a time (a row a block took
+// 1.9 times as long).
+constexpr int GRADIENT_ROWS = 4;
+
 __global__ void __launch_bounds__(256)
 loss_gradient_kernel(uint16_t* __restrict__ e, long long ld, int V, int pieces, const float* __restrict__ factor,
                      const long long* __restrict__ targets, const float* __restrict__ target_entry, long long ignore, long long rows) {
   const int col = (blockIdx.x * 256 + threadIdx.x) * 8;
   if (col >= V) return;
-  for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
-    uint16_t* at = e + row * ld + col;
-    const float f = factor[row * pieces + col / HALF];
-    float v[8];
-    load8(reinterpret_cast<const fp16*>(at), v);
+  for (long long row0 = static_cast<long long>(blockIdx.y) * GRADIENT_ROWS; row0 < rows; row0 += static_cast<long long>(gridDim.y) * GRADIENT_ROWS) {
+    uint4 raw[GRADIENT_ROWS];
+    float f[GRADIENT_ROWS];
+    long long t[GRADIENT_ROWS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = f != 0.0f ? v[j] * f : 0.0f;  // rows that do not count: zero whatever e is
-    const long long t = targets[row];
-    if (t >= col && t < col + 8 && t < V && t != ignore) {
-      const float entry = target_entry[row];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (t == col + j) v[j] = entry;
-      }
+    for (int u = 0; u < GRADIENT_ROWS; ++u) {
+      const long long row = row0 + u < rows ? row0 + u : rows - 1;
+      raw[u] = *reinterpret_cast<const uint4*>(e + row * ld + col);
+      f[u] = factor[row * pieces + col / HALF];
+      t[u] = targets[row];
     }
-    store8(reinterpret_cast<bf16*>(at), v);
+#pragma unroll
+    for (int u = 0; u < GRADIENT_ROWS; ++u) {
+      const long long row = row0 + u;
+      if (row >= rows) break;
+      const __half2 h[4] = {*reinterpret_cast<__half2*>(&raw[u].x), *reinterpret_cast<__half2*>(&raw[u].y),
+                            *reinterpret_cast<__half2*>(&raw[u].z), *reinterpret_cast<__half2*>(&raw[u].w)};
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 x = __half22float2(h[q]);
+        v[2 * q] = f[u] != 0.0f ? x.x * f[u] : 0.0f;  // rows that do not count: zero whatever e is
+        v[2 * q + 1] = f[u] != 0.0f ? x.y * f[u] : 0.0f;
+      }
+      if (t[u] >= col && t[u] < col + 8 && t[u] < V && t[u] != ignore) {
+        const float entry = target_entry[row];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (t[u] == col + j) v[j] = entry;
+        }
+      }
+      store8(reinterpret_cast<bf16*>(e + row * ld + col), v);
+    }
   }
 }
 
@@ -199,6 +221,171 @@ loss_scale_kernel(T* __restrict__ x, long long n, const float* __restrict__ fact
   }
 }
 
+// ---- few rows ------------------------------------------------------------------------------------------------------
+//
+// Scoring a handful of rows is reading the weight once (V D 2 bytes). Tiles of 256 entries are too coarse for that where
+// there are a few hundred of them: 50257 entries are 197 tiles for 148 SMs, and half of those have two (1 row, D = 1024: 30 us).
+// Here a warp takes 16 entries at a time, and up to 8 warps share their contraction. The entries go straight from memory into the
+// registers of mma.sync's A operand: which k a lane's eight neighbours count as does not matter as long as the rows, in shared
+// memory as B, are read the same way, so a lane loads 16 bytes where the instruction's layout has pairs. The tensor pipe
+// idles either way; a TMA-fed tcgen05 pipeline would bring nothing but its tiles. Every warp that sums keeps a
+// running maximum and sum for its entries and leaves one pair for each row.
+constexpr int FEW_WARPS = 8;
+constexpr int FEW_BATCH = 8;           // 32-deep steps whose loads are in flight together
+constexpr int FEW_SMEM = 128 << 10;    // for the rows
+
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// NT: groups of 8 rows; `split` warps (1, 2, 4 or 8) share a group of 16 entries. stats[n][piece], one piece a group of warps.
+template <int NT>
+__global__ void __launch_bounds__(FEW_WARPS * 32, NT <= 2 ? 2 : 1)
+loss_few_kernel(const bf16* __restrict__ hidden, const bf16* __restrict__ weight, int rows, int D, int V, int split,
+                const long long* __restrict__ targets, float* __restrict__ target_logits, float2* __restrict__ stats) {
+  extern __shared__ __align__(16) uint8_t few_smem[];  // the rows, `ld` bytes apart
+  __shared__ float partial[2][FEW_WARPS][NT * 4][32];
+  __shared__ long long goal[NT * 8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int groups = FEW_WARPS / split, group = warp / split, member = warp % split;
+  const int steps = (D + 31) / 32, mine = (steps + split - 1) / split, first = member * mine;
+  const int ld = steps * 64 + 64;
+  // rows to shared memory, zero past their end and in rows that are not there
+  for (int i = threadIdx.x; i < NT * 8 * (ld / 16); i += FEW_WARPS * 32) {
+    const int n = i / (ld / 16), c = i % (ld / 16) * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (n < rows && c < D) v = *reinterpret_cast<const uint4*>(hidden + static_cast<long long>(n) * D + c);
+    *reinterpret_cast<uint4*>(few_smem + n * ld + c * 2) = v;
+  }
+  if (threadIdx.x < NT * 8) goal[threadIdx.x] = threadIdx.x < rows ? targets[threadIdx.x] : -1;
+  __syncthreads();
+  const uint32_t row_base = smem_u32(few_smem) + g * ld + q * 16;
+  float top[NT][2], sum[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
+  const int units = (V + 15) / 16, stride = gridDim.x * groups;
+  int parity = 0;
+  // every warp of a block goes round as often as its first group
+  for (int unit0 = blockIdx.x * groups; unit0 < units; unit0 += stride, parity ^= 1) {
+    const int v0 = (unit0 + group) * 16;
+    const bf16* low = weight + static_cast<long long>(min(v0 + g, V - 1)) * D + q * 8;
+    const bf16* high = weight + static_cast<long long>(min(v0 + g + 8, V - 1)) * D + q * 8;
+    float c[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
+    for (int s0 = 0; s0 < mine; s0 += FEW_BATCH) {
+      uint4 a[FEW_BATCH], b[FEW_BATCH];
+#pragma unroll
+      for (int u = 0; u < FEW_BATCH; ++u) {
+        const int k = (first + s0 + u) * 32;
+        const bool any = s0 + u < mine && k + q * 8 < D;
+        a[u] = any ? load_stream(low + k) : make_uint4(0, 0, 0, 0);
+        b[u] = any ? load_stream(high + k) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < FEW_BATCH; ++u) {
+        if (s0 + u >= mine || first + s0 + u >= steps) break;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint4 x;
+          ld_shared_v4(row_base + n * 8 * ld + (first + s0 + u) * 64, x);
+          mma_16x8x16(c[n], a[u].x, b[u].x, a[u].y, b[u].y, x.x, x.y);
+          mma_16x8x16(c[n], a[u].z, b[u].z, a[u].w, b[u].w, x.z, x.w);
+        }
+      }
+    }
+    if (split > 1) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) partial[parity][warp][n * 4 + j][lane] = c[n][j];
+      }
+      __syncthreads();  // one a round: the other buffer was read before the round's own
+      if (member != 0) continue;
+      for (int w = 1; w < split; ++w) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) c[n][j] += partial[parity][warp + w][n * 4 + j][lane];
+        }
+      }
+    }
+    // entries v0 + g (values 0, 1) and v0 + g + 8 (2, 3) of rows 8 n + 2 q (0, 2) and 8 n + 2 q + 1 (1, 3)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int v = v0 + g + (j >> 1) * 8, r = 8 * n + 2 * q + (j & 1);
+        if (v < V) {
+          if (c[n][j] != -INFINITY) join(top[n][j & 1], sum[n][j & 1], c[n][j], 1.0f);
+          if (goal[r] == v) target_logits[r] = c[n][j];
+        }
+      }
+    }
+  }
+  if (member != 0) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        const float other_top = __shfl_xor_sync(0xffffffffu, top[n][j], o), other_sum = __shfl_xor_sync(0xffffffffu, sum[n][j], o);
+        join(top[n][j], sum[n][j], other_top, other_sum);
+      }
+      const int r = 8 * n + 2 * q + j;
+      if (g == 0 && r < rows) stats[static_cast<long long>(r) * stride + blockIdx.x * groups + group] = make_float2(top[n][j], sum[n][j]);
+    }
+  }
+}
+
+struct Few {
+  int tiles, split, blocks, pieces, smem;
+};
+
+// How loss_few_kernel runs for these sizes; tiles = 0 where it does not.
+Few few_rows(long long rows, int D, int V) {
+  Few f = {};
+  const int steps = (D + 31) / 32;
+  const int tiles = rows <= 8 ? 1 : (rows <= 16 ? 2 : 4);
+  f.smem = tiles * 8 * (steps * 64 + 64);
+  if (rows > 32 || f.smem > FEW_SMEM) return f;
+  f.tiles = tiles;
+  f.split = 1;
+  while (f.split < FEW_WARPS && steps / (2 * f.split) >= FEW_BATCH) f.split *= 2;
+  const int groups = FEW_WARPS / f.split, units = (V + 15) / 16;
+  const int want = (units + groups - 1) / groups, most = num_sms() * (f.smem <= FEW_SMEM / 2 && tiles <= 2 ? 2 : 1);
+  f.blocks = want < most ? want : most;
+  f.pieces = f.blocks * groups;
+  return f;
+}
+
+template <int NT>
+int launch_few(const Few& f, const void* hidden, const void* weight, int rows, int D, int V, const long long* targets, float* target_logits,
+               float* stats, cudaStream_t stream) {
+  static PerDevice room;
+  const int allowed = room.get([&] {
+    if (cudaFuncSetAttribute(loss_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    return FEW_SMEM;
+  });
+  if (f.smem > allowed) return FFM_ERR_LAUNCH;
+  loss_few_kernel<NT><<<f.blocks, FEW_WARPS * 32, f.smem, stream>>>(static_cast<const bf16*>(hidden), static_cast<const bf16*>(weight), rows, D,
+                                                                    V, f.split, targets, target_logits, reinterpret_cast<float2*>(stats));
+  return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
 int streaming_blocks(long long n) {
   const long long want = (n + 2047) / 2048, cap = static_cast<long long>(num_sms()) * 8;
   return static_cast<int>(want < 1 ? 1 : (want < cap ? want : cap));
@@ -227,6 +414,7 @@ struct Layout {
   int64_t e, stats, factor, target_entry, target_logits, share, parts, wide, bytes;
   int64_t ld;
   int pieces, splits;
+  Few few;
 };
 
 Layout lay_out(const ffm_loss_args& a) {
@@ -234,6 +422,8 @@ Layout lay_out(const ffm_loss_args& a) {
   const int64_t n = a.piece_rows < a.N ? a.piece_rows : a.N;
   const bool grads = a.d_hidden != nullptr || a.d_weight != nullptr;
   l.pieces = static_cast<int>((a.V + HALF - 1) / HALF);
+  l.few = grads ? Few{} : few_rows(a.N, static_cast<int>(a.D), static_cast<int>(a.V));
+  if (l.few.tiles > 0) l.pieces = l.few.pieces;
   l.ld = (a.V + 63) / 64 * 64;
   l.splits = a.d_hidden != nullptr ? contraction_splits(n, static_cast<int>(a.D), static_cast<int>(a.V)) : 1;
   int64_t end = 0;
@@ -294,9 +484,8 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
   const bool grads = a.d_hidden != nullptr || a.d_weight != nullptr;
   int64_t launched = 0;
   int rc = FFM_OK;
-  if (a.N > 0) {
-    // without a mean only the targets are looked over
-    loss_count_kernel<<<1, LOSS_THREADS, 0, s>>>(targets, a.N, a.ignore_index, V, at(l.share), a.status);
+  if (a.mean) {
+    loss_count_kernel<<<1, LOSS_THREADS, 0, s>>>(targets, a.N, a.ignore_index, share);
     if ((rc = launch_ok()) != FFM_OK) return rc;
     ++launched;
   }
@@ -305,19 +494,24 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
     const int64_t n = a.N - r0 < step ? a.N - r0 : step;
     const char* hidden = static_cast<const char*>(a.hidden) + r0 * a.D * 2;
     void* e = grads ? static_cast<void*>(w + l.e) : nullptr;
-    if ((rc = softmax_logits(hidden, a.weight, n, D, V, a.targets + r0, at(l.target_logits), at(l.stats), e, l.ld, a.status, stream)) !=
-        FFM_OK) {
-      return rc;
+    if (l.few.tiles > 0) {
+      const auto few = l.few.tiles == 1 ? launch_few<1> : (l.few.tiles == 2 ? launch_few<2> : launch_few<4>);
+      rc = few(l.few, hidden, a.weight, static_cast<int>(n), D, V, targets, at(l.target_logits), at(l.stats), s);
+    } else {
+      rc = softmax_logits(hidden, a.weight, n, D, V, a.targets + r0, at(l.target_logits), at(l.stats), e, l.ld, a.status, stream);
     }
-    loss_rows_kernel<<<static_cast<unsigned>((n + ROW_GROUP - 1) / ROW_GROUP), 1024, 0, s>>>(
-        reinterpret_cast<const float2*>(at(l.stats)), at(l.target_logits), targets + r0, n, l.pieces, V, a.ignore_index, z, share,
-        a.row_grad != nullptr ? a.row_grad + r0 : nullptr, a.nll + r0, grads ? at(l.factor) : nullptr, at(l.target_entry),
-        a.status, a.status_host);
+    if (rc != FFM_OK) return rc;
+    // a block a row where that does not fill the device with warps
+    const bool wide = n <= 8ll * num_sms();
+    (wide ? loss_rows_kernel<256> : loss_rows_kernel<32>)<<<static_cast<unsigned>(wide ? n : (n + 7) / 8), 256, 0, s>>>(
+        reinterpret_cast<const float2*>(at(l.stats)), at(l.target_logits), targets + r0, reinterpret_cast<const bf16*>(hidden),
+        static_cast<const bf16*>(a.weight), D, n, l.pieces, V, a.ignore_index, z, share, a.row_grad != nullptr ? a.row_grad + r0 : nullptr,
+        a.nll + r0, grads ? at(l.factor) : nullptr, at(l.target_entry), a.status, a.status_host);
     if ((rc = launch_ok()) != FFM_OK) return rc;
     launched += 2;
     if (!grads) continue;
-    const unsigned rows_at_once = static_cast<unsigned>(n < 65535 ? n : 65535);
-    loss_gradient_kernel<<<dim3((V + 2047) / 2048, rows_at_once), 256, 0, s>>>(
+    const int64_t row_groups = (n + GRADIENT_ROWS - 1) / GRADIENT_ROWS;
+    loss_gradient_kernel<<<dim3((V + 2047) / 2048, static_cast<unsigned>(row_groups < 65535 ? row_groups : 65535)), 256, 0, s>>>(
         static_cast<uint16_t*>(e), l.ld, V, l.pieces, at(l.factor), targets + r0, at(l.target_entry), a.ignore_index, n);
     if ((rc = launch_ok()) != FFM_OK) return rc;
     ++launched;
@@ -350,10 +544,6 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
     return FFM_ERR_LAUNCH;
   }
   if (a.loss != nullptr) {
-    if (a.N == 0 && share != nullptr) {  // the mean of nothing
-      loss_count_kernel<<<1, LOSS_THREADS, 0, s>>>(targets, 0, a.ignore_index, V, share, a.status);
-      ++launched;
-    }
     loss_sum_kernel<<<1, LOSS_THREADS, 0, s>>>(a.nll, a.N, share, a.loss, a.status, a.status_host);
     if ((rc = launch_ok()) != FFM_OK) return rc;
     ++launched;
