@@ -223,15 +223,16 @@ loss_scale_kernel(T* __restrict__ x, long long n, const float* __restrict__ fact
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
 //
-// Scoring a handful of rows is reading the weight once (V D 2 bytes). Tiles of 256 entries are too coarse for that where
-// there are a few hundred of them: 50257 entries are 197 tiles for 148 SMs, and half of those have two (1 row, D = 1024: 30 us).
-// Here a warp takes 16 entries at a time, and up to 8 warps share their contraction. The entries go straight from memory into the
+// Scoring a handful of rows is reading the weight once (V D 2 bytes). The tiles of 256 entries do that at 6.0 TB/s where there are
+// many of them (33 rows, D = 2048, 100352 entries: 70 us), but a few hundred do not share out over 148 SMs: 50257 entries are 197
+// tiles, and a third of the SMs has two (D = 1024: 27 us; 2000 entries, D = 2048: 16 us).
+// Here a warp takes 16 entries at a time, and up to 8 warps share their contraction (22 us and 5.4 us; where tiles share out
+// evenly it is the slower one, 161 us for 137 at D = 4096, 100352 entries: 5.1 TB/s). The entries go straight from memory into the
 // registers of mma.sync's A operand: which k a lane's eight neighbours count as does not matter as long as the rows, in shared
 // memory as B, are read the same way, so a lane loads 16 bytes where the instruction's layout has pairs. The tensor pipe
-// idles either way; a TMA-fed tcgen05 pipeline would bring nothing but its tiles. Every warp that sums keeps a
-// running maximum and sum for its entries and leaves one pair for each row.
+// idles either way. Every warp that sums keeps a running maximum and sum for its entries and leaves one pair for each row.
 constexpr int FEW_WARPS = 8;
-constexpr int FEW_BATCH = 8;           // 32-deep steps whose loads are in flight together
+constexpr int FEW_BATCH = 4;           // 32-deep steps loaded together; two batches at a time
 constexpr int FEW_SMEM = 128 << 10;    // for the rows
 
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -249,7 +250,7 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {
 
 // NT: groups of 8 rows; `split` warps (1, 2, 4 or 8) share a group of 16 entries. stats[n][piece], one piece a group of warps.
 template <int NT>
-__global__ void __launch_bounds__(FEW_WARPS * 32, NT <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2)
 loss_few_kernel(const bf16* __restrict__ hidden, const bf16* __restrict__ weight, int rows, int D, int V, int split,
                 const long long* __restrict__ targets, float* __restrict__ target_logits, float2* __restrict__ stats) {
   extern __shared__ __align__(16) uint8_t few_smem[];  // the rows, `ld` bytes apart
@@ -273,35 +274,51 @@ loss_few_kernel(const bf16* __restrict__ hidden, const bf16* __restrict__ weight
 #pragma unroll
   for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
   const int units = (V + 15) / 16, stride = gridDim.x * groups;
+  // A warp has a batch of steps in flight while it multiplies the one before, across its entries as well.
+  struct Batch {
+    uint4 low[FEW_BATCH], high[FEW_BATCH];  // entries g and g + 8
+  };
+  auto load = [&](int unit, int s0, Batch& b) {
+    const int v0 = (unit + group) * 16;
+    const bf16* low = weight + static_cast<long long>(min(v0 + g, V - 1)) * D + q * 8;
+    const bf16* high = weight + static_cast<long long>(min(v0 + g + 8, V - 1)) * D + q * 8;
+#pragma unroll
+    for (int u = 0; u < FEW_BATCH; ++u) {
+      const int k = (first + s0 + u) * 32;
+      const bool any = unit < units && s0 + u < mine && k + q * 8 < D;
+      b.low[u] = any ? load_stream(low + k) : make_uint4(0, 0, 0, 0);
+      b.high[u] = any ? load_stream(high + k) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto multiply = [&](int s0, const Batch& b, float (&c)[NT][4]) {
+#pragma unroll
+    for (int u = 0; u < FEW_BATCH; ++u) {
+      if (s0 + u >= mine || first + s0 + u >= steps) break;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint4 x;
+        ld_shared_v4(row_base + n * 8 * ld + (first + s0 + u) * 64, x);
+        mma_16x8x16(c[n], b.low[u].x, b.high[u].x, b.low[u].y, b.high[u].y, x.x, x.y);
+        mma_16x8x16(c[n], b.low[u].z, b.high[u].z, b.low[u].w, b.high[u].w, x.z, x.w);
+      }
+    }
+  };
+  Batch early, later;
+  load(blockIdx.x * groups, 0, early);
   int parity = 0;
   // every warp of a block goes round as often as its first group
   for (int unit0 = blockIdx.x * groups; unit0 < units; unit0 += stride, parity ^= 1) {
     const int v0 = (unit0 + group) * 16;
-    const bf16* low = weight + static_cast<long long>(min(v0 + g, V - 1)) * D + q * 8;
-    const bf16* high = weight + static_cast<long long>(min(v0 + g + 8, V - 1)) * D + q * 8;
     float c[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
-    for (int s0 = 0; s0 < mine; s0 += FEW_BATCH) {
-      uint4 a[FEW_BATCH], b[FEW_BATCH];
-#pragma unroll
-      for (int u = 0; u < FEW_BATCH; ++u) {
-        const int k = (first + s0 + u) * 32;
-        const bool any = s0 + u < mine && k + q * 8 < D;
-        a[u] = any ? load_stream(low + k) : make_uint4(0, 0, 0, 0);
-        b[u] = any ? load_stream(high + k) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int u = 0; u < FEW_BATCH; ++u) {
-        if (s0 + u >= mine || first + s0 + u >= steps) break;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          uint4 x;
-          ld_shared_v4(row_base + n * 8 * ld + (first + s0 + u) * 64, x);
-          mma_16x8x16(c[n], a[u].x, b[u].x, a[u].y, b[u].y, x.x, x.y);
-          mma_16x8x16(c[n], a[u].z, b[u].z, a[u].w, b[u].w, x.z, x.w);
-        }
-      }
+    for (int s0 = 0; s0 < mine; s0 += 2 * FEW_BATCH) {
+      load(unit0, s0 + FEW_BATCH, later);
+      multiply(s0, early, c);
+      // the next steps of these entries, or the first ones of the warp's next
+      const bool more = s0 + 2 * FEW_BATCH < mine;
+      load(more ? unit0 : unit0 + stride, more ? s0 + 2 * FEW_BATCH : 0, early);
+      multiply(s0 + FEW_BATCH, later, c);
     }
     if (split > 1) {
 #pragma unroll
@@ -352,18 +369,20 @@ struct Few {
   int tiles, split, blocks, pieces, smem;
 };
 
-// How loss_few_kernel runs for these sizes; tiles = 0 where it does not.
+// How loss_few_kernel runs for these sizes; tiles = 0 where it does not: for more than 16 rows (32: 52 us for 27), or where the
+// product's tiles keep three quarters of the SMs busy.
 Few few_rows(long long rows, int D, int V) {
   Few f = {};
-  const int steps = (D + 31) / 32;
-  const int tiles = rows <= 8 ? 1 : (rows <= 16 ? 2 : 4);
+  const int steps = (D + 31) / 32, sms = num_sms();
+  const int tiles = rows <= 8 ? 1 : 2;
+  const long long product_tiles = (static_cast<long long>(V) + 255) / 256, rounds = (product_tiles + sms - 1) / sms;
   f.smem = tiles * 8 * (steps * 64 + 64);
-  if (rows > 32 || f.smem > FEW_SMEM) return f;
+  if (rows > 16 || f.smem > FEW_SMEM || 4 * product_tiles > 3 * rounds * sms) return f;
   f.tiles = tiles;
   f.split = 1;
-  while (f.split < FEW_WARPS && steps / (2 * f.split) >= FEW_BATCH) f.split *= 2;
+  while (f.split < FEW_WARPS && steps / (2 * f.split) >= 2 * FEW_BATCH) f.split *= 2;
   const int groups = FEW_WARPS / f.split, units = (V + 15) / 16;
-  const int want = (units + groups - 1) / groups, most = num_sms() * (f.smem <= FEW_SMEM / 2 && tiles <= 2 ? 2 : 1);
+  const int want = (units + groups - 1) / groups, most = sms * (f.smem <= FEW_SMEM / 2 ? 2 : 1);
   f.blocks = want < most ? want : most;
   f.pieces = f.blocks * groups;
   return f;
@@ -495,7 +514,7 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
     const char* hidden = static_cast<const char*>(a.hidden) + r0 * a.D * 2;
     void* e = grads ? static_cast<void*>(w + l.e) : nullptr;
     if (l.few.tiles > 0) {
-      const auto few = l.few.tiles == 1 ? launch_few<1> : (l.few.tiles == 2 ? launch_few<2> : launch_few<4>);
+      const auto few = l.few.tiles == 1 ? launch_few<1> : launch_few<2>;
       rc = few(l.few, hidden, a.weight, static_cast<int>(n), D, V, targets, at(l.target_logits), at(l.stats), s);
     } else {
       rc = softmax_logits(hidden, a.weight, n, D, V, a.targets + r0, at(l.target_logits), at(l.stats), e, l.ld, a.status, stream);
