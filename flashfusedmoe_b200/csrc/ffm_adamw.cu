@@ -79,26 +79,26 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) {
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
 
-// Two values to e4m3, to nearest; what is over 448 (infinities, NaN: the scale sees to the rest) becomes NaN.
-__device__ __forceinline__ uint32_t e4m3x2_nearest(float lo, float hi) {
-  lo = fabsf(lo) <= 448.0f ? lo : __int_as_float(0x7fc00000);
-  hi = fabsf(hi) <= 448.0f ? hi : __int_as_float(0x7fc00000);
+// Two values of at most 448 (or NaN) to e4m3, to nearest.
+__device__ __forceinline__ uint32_t e4m3x2_nearest(float2 v) {
   unsigned short r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
   return r;
 }
 
-// x >= 0 to e4m3, up with probability (distance from the lower neighbour) / (distance of the neighbours): the lower code plus
-// 16 random bits, as a fraction, in place of the bits that are cut off. Above 2^-6 that is integer arithmetic on the fp32
-// number; below, codes are multiples of 2^-9. Never zero for a positive x.
-__device__ __forceinline__ uint32_t e4m3_random(float x, uint32_t random16) {
-  const uint32_t bits = __float_as_uint(x);
-  uint32_t code = ((bits + (random16 << 4) + 8u) >> 20) - ((127 - 7) << 3);
-  if (x < 0.015625f) {
-    code = static_cast<uint32_t>(floorf(x * 512.0f + (static_cast<float>(random16) + 0.5f) * (1.0f / 65536.0f)));
-    code = x > 0.0f ? max(code, 1u) : 0u;
-  }
-  return x <= 448.0f ? code : 0x7fu;
+// x from 2^-6 to 448 to e4m3, up with probability (distance from the lower neighbour) / (distance of the neighbours): 16 random
+// bits and a half, as a fraction, are added to the bits that are cut off. random: 20 bits, the last four of them 8. For a
+// smaller x the result is below 8, or not below 128.
+__device__ __forceinline__ uint32_t e4m3_random(float x, uint32_t random) {
+  return (__float_as_uint(x) + random - (120u << 23)) >> 20;
+}
+
+// The same for any x, and v (whose root it is) that may be anything. Below 2^-6 codes are multiples of 2^-9: 2^-6 more puts x into the
+// binade whose numbers lie as far apart, eight codes further up. Never zero for a positive v; NaN for one that is not finite.
+__device__ __noinline__ uint32_t e4m3_random_any(float x, float v, uint32_t random) {
+  if (!(fabsf(v) <= 3.402823466e38f)) return 0x7fu;
+  const uint32_t code = x < 0.015625f ? e4m3_random(x + 0.015625f, random) - 8u : e4m3_random(x, random);
+  return v > 0.0f ? max(code, 1u) : 0u;
 }
 
 // Random bits of a pair of neighbouring values (16 each): two rounds of multiply and fold over a counter.
@@ -109,11 +109,35 @@ __device__ __forceinline__ uint32_t random_pair(uint32_t pair, uint32_t key) {
   return h ^ (h >> 16);
 }
 
+// the larger one, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 __device__ __forceinline__ float max16(float v) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 8; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
+// One instruction each, good to 2 units of the last place; what is below 2^-126 counts as zero.
+__device__ __forceinline__ float root_fast(float v) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// eight values as four pairs
+__device__ __forceinline__ float (&values(float2 (&v)[4]))[8] { return *reinterpret_cast<float (*)[8]>(&v); }
 
 template <int MAX, bool EIGHT>
 __global__ void __launch_bounds__(ADAMW_THREADS)
@@ -130,46 +154,40 @@ adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
     keys[i] = static_cast<uint32_t>(t) * 0x85EBCA77u + job.seed * 0xC2B2AE3Du;
   }
   __syncthreads();
-  const float keep = 1.0f - lr * job.weight_decay;
+  const float2 keep = both(1.0f - lr * job.weight_decay), eps = both(job.eps);
+  const float2 beta1 = both(job.beta1), less1 = both(job.one_minus_beta1), beta2 = both(job.beta2), less2 = both(job.one_minus_beta2);
+  const bool scaled = job.grad_scale != nullptr;
+  // with eps from here on a root of a v below 2^-126 (10^-19) makes no difference to the update
+  const bool fast = job.eps >= 1e-12f;
   const long long chunks = job.tensor[job.count - 1].chunks_end;
   int i = 0;
   for (long long chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    // the chunk's tensor, for the whole block alike
-    int top = job.count - 1;
-    while (i < top) {
-      const int mid = (i + top) >> 1;
-      if (chunk < job.tensor[mid].chunks_end) {
-        top = mid;
-      } else {
-        i = mid + 1;
-      }
-    }
+    while (chunk >= job.tensor[i].chunks_end) ++i;  // the chunk's tensor, for the whole block alike
     const AdamWTensor& a = job.tensor[i];
     const long long e0 = (chunk - (i > 0 ? job.tensor[i - 1].chunks_end : 0)) * ADAMW_CHUNK + threadIdx.x * 8;
     const int left = static_cast<int>(min(a.n - e0, 8ll));  // values of this thread, none where <= 0
     const bool whole = left == 8 && a.wide != 0;
-    float p[8], g[8], m[8], v[8];
+    float2 p[4], g[4], m[4], v[4];
     if (whole) {
-      load8_as(a.g, a.g_type, e0, g);
+      load8_as(a.g, a.g_type, e0, values(g));
       if (a.master != nullptr) {
-        load8(a.master + e0, p);
+        load8(a.master + e0, values(p));
       } else {
-        load8_as(a.p, a.p_type, e0, p);
+        load8_as(a.p, a.p_type, e0, values(p));
       }
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        g[j] = j < left ? load1_as(a.g, a.g_type, e0 + j) : 0.0f;
-        p[j] = j < left ? (a.master != nullptr ? a.master[e0 + j] : load1_as(a.p, a.p_type, e0 + j)) : 0.0f;
+        values(g)[j] = j < left ? load1_as(a.g, a.g_type, e0 + j) : 0.0f;
+        values(p)[j] = j < left ? (a.master != nullptr ? a.master[e0 + j] : load1_as(a.p, a.p_type, e0 + j)) : 0.0f;
       }
     }
     if (EIGHT) {
-      const long long block = e0 / ADAMW_BLOCK;
       uint2 cm = make_uint2(0, 0), cv = make_uint2(0, 0);
-      float sm = 0.0f, sv = 0.0f;
+      uint32_t sm = 0, sv = 0;
       if (left > 0) {
-        sm = exponent_of_two(static_cast<int>(a.m_scale[block]) - 127);
-        sv = exponent_of_two(static_cast<int>(a.v_scale[block]) - 127);
+        sm = a.m_scale[e0 / ADAMW_BLOCK];
+        sv = a.v_scale[e0 / ADAMW_BLOCK];
       }
       if (whole) {
         cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + e0);
@@ -187,67 +205,120 @@ adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
           }
         }
       }
+      const float2 fm = both(__uint_as_float(sm << 23)), fv = both(__uint_as_float(sv << 23));
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float2 x = e4m3x2_to_float2((q < 2 ? cm.x : cm.y) >> (16 * (q & 1)) & 0xffffu);
-        const float2 y = e4m3x2_to_float2((q < 2 ? cv.x : cv.y) >> (16 * (q & 1)) & 0xffffu);
-        m[2 * q] = x.x * sm, m[2 * q + 1] = x.y * sm;
-        v[2 * q] = (y.x * sv) * (y.x * sv), v[2 * q + 1] = (y.y * sv) * (y.y * sv);
+        m[q] = mul2(e4m3x2_to_float2((q < 2 ? cm.x : cm.y) >> (16 * (q & 1)) & 0xffffu), fm);
+        v[q] = mul2(e4m3x2_to_float2((q < 2 ? cv.x : cv.y) >> (16 * (q & 1)) & 0xffffu), fv);
+        v[q] = mul2(v[q], v[q]);
       }
     } else if (whole) {
-      load8(static_cast<const float*>(a.m) + e0, m);
-      load8(static_cast<const float*>(a.v) + e0, v);
+      load8(static_cast<const float*>(a.m) + e0, values(m));
+      load8(static_cast<const float*>(a.v) + e0, values(v));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        m[j] = j < left ? static_cast<const float*>(a.m)[e0 + j] : 0.0f;
-        v[j] = j < left ? static_cast<const float*>(a.v)[e0 + j] : 0.0f;
+        values(m)[j] = j < left ? static_cast<const float*>(a.m)[e0 + j] : 0.0f;
+        values(v)[j] = j < left ? static_cast<const float*>(a.v)[e0 + j] : 0.0f;
       }
     }
 
-    float root[8], top_m = 0.0f, top_v = 0.0f;
-    const float r = rate[i], inv = inverse[i];
+    float2 root[4];
+    float top_m = 0.0f, top_v = 0.0f;
+    const float2 r = both(-rate[i]), inv = both(inverse[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       // each product and sum is rounded on its own: in 8 bits the largest of a block decides its scale, and two evaluations
       // that differ in the last place would now and then differ in it
-      const float gj = __fmul_rn(g[j], grad_scale);
-      m[j] = __fadd_rn(__fmul_rn(m[j], job.beta1), __fmul_rn(gj, job.one_minus_beta1));
-      v[j] = __fadd_rn(__fmul_rn(v[j], job.beta2), __fmul_rn(__fmul_rn(gj, job.one_minus_beta2), gj));
-      root[j] = __fsqrt_rn(v[j]);
-      p[j] = fmaf(-r, __fdividef(m[j], fmaf(root[j], inv, job.eps)), p[j] * keep);
-      top_m = fmaxf(top_m, fabsf(m[j]));
-      top_v = fmaxf(top_v, root[j]);
+      const float x = scaled ? __fmul_rn(values(g)[j], grad_scale) : values(g)[j];
+      values(m)[j] = __fadd_rn(__fmul_rn(values(m)[j], job.beta1), __fmul_rn(x, job.one_minus_beta1));
+      values(v)[j] = __fadd_rn(__fmul_rn(values(v)[j], job.beta2), __fmul_rn(__fmul_rn(x, job.one_minus_beta2), x));
+    }
+    if (fast) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        root[q] = make_float2(root_fast(v[q].x), root_fast(v[q].y));
+        const float2 under = fma2(root[q], inv, eps);
+        p[q] = fma2(r, mul2(m[q], make_float2(reciprocal_fast(under.x), reciprocal_fast(under.y))), mul2(p[q], keep));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        values(root)[j] = __fsqrt_rn(values(v)[j]);
+        values(p)[j] = fmaf(r.x, __fdiv_rn(values(m)[j], fmaf(values(root)[j], inv.x, eps.x)), values(p)[j] * keep.x);
+      }
+    }
+    if (EIGHT) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        top_m = max_nan(top_m, max_nan(fabsf(m[q].x), fabsf(m[q].y)));
+        top_v = max_nan(top_v, max_nan(v[q].x, v[q].y));
+      }
     }
 
     if (a.master != nullptr) {
       if (whole) {
-        store8(a.master + e0, p);
+        store8(a.master + e0, values(p));
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (j < left) a.master[e0 + j] = p[j];
+          if (j < left) a.master[e0 + j] = values(p)[j];
         }
       }
     }
     if (whole) {
-      store8_as(a.p, a.p_type, e0, p);
+      store8_as(a.p, a.p_type, e0, values(p));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (j < left) store1_as(a.p, a.p_type, e0 + j, p[j]);
+        if (j < left) store1_as(a.p, a.p_type, e0 + j, values(p)[j]);
       }
     }
     if (EIGHT) {
-      const int km = block_exponent(max16(top_m)), kv = block_exponent(max16(top_v));
-      const float fm = exponent_of_two(-km), fv = exponent_of_two(-kv);
-      uint32_t cm[2] = {0, 0}, cv[2] = {0, 0};
+      top_m = max16(top_m);
+      top_v = max16(top_v);
+      const bool odd = !finite(top_m) || !finite(top_v);  // something of the block is not finite
+      if (__any_sync(0xffffffffu, odd)) {
+        // what is infinite or NaN leaves the scale to the others, and becomes NaN
+        float other_m = 0.0f, other_v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = values(m)[j], y = values(v)[j];
+          if (finite(x)) other_m = fmaxf(other_m, fabsf(x));
+          if (finite(y)) other_v = fmaxf(other_v, y);
+          if (!finite(x)) values(m)[j] = __int_as_float(0x7fc00000);
+        }
+        other_m = max16(other_m);
+        other_v = max16(other_v);
+        if (odd) top_m = other_m, top_v = other_v;
+      }
+      const int km = block_exponent(top_m), kv = block_exponent(__fsqrt_rn(top_v));
+      const float2 fm = both(exponent_of_two(-km)), fv = both(exponent_of_two(-kv));
+      uint32_t cm[2], cv[2], code[8], random[8];
+      float2 x[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const uint32_t random = random_pair(static_cast<uint32_t>((e0 >> 1) + q), keys[i]);
-        cm[q >> 1] |= e4m3x2_nearest(m[2 * q] * fm, m[2 * q + 1] * fm) << (16 * (q & 1));
-        cv[q >> 1] |= (e4m3_random(root[2 * q] * fv, random & 0xffffu) | e4m3_random(root[2 * q + 1] * fv, random >> 16) << 8)
-                      << (16 * (q & 1));
+        const uint32_t two = random_pair(static_cast<uint32_t>((e0 >> 1) + q), keys[i]);
+        random[2 * q] = (two << 4 & 0xffff0u) | 8u;
+        random[2 * q + 1] = (two >> 12 & 0xffff0u) | 8u;
+        x[q] = mul2(root[q], fv);
+        code[2 * q] = e4m3_random(x[q].x, random[2 * q]);
+        code[2 * q + 1] = e4m3_random(x[q].y, random[2 * q + 1]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        cm[h] = e4m3x2_nearest(mul2(m[2 * h], fm)) | e4m3x2_nearest(mul2(m[2 * h + 1], fm)) << 16;
+        const uint32_t* c = code + 4 * h;
+        cv[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        // a code below 8 or above 127 stands for a number below 2^-6, or one that is none: rare
+        const uint32_t eights = cv[h] & 0x78787878u;
+        if (((c[0] | c[1] | c[2] | c[3]) & ~0x7fu) != 0 || ((eights - 0x01010101u) & ~eights & 0x80808080u) != 0 || odd) {
+          cv[h] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            cv[h] |= e4m3_random_any(values(x)[4 * h + j], values(v)[4 * h + j], random[4 * h + j]) << (8 * j);
+          }
+        }
       }
       if (whole) {
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + e0) = make_uint2(cm[0], cm[1]);
@@ -266,14 +337,14 @@ adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
         a.v_scale[e0 / ADAMW_BLOCK] = static_cast<uint8_t>(kv + 127);
       }
     } else if (whole) {
-      store8(static_cast<float*>(a.m) + e0, m);
-      store8(static_cast<float*>(a.v) + e0, v);
+      store8(static_cast<float*>(a.m) + e0, values(m));
+      store8(static_cast<float*>(a.v) + e0, values(v));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (j < left) {
-          static_cast<float*>(a.m)[e0 + j] = m[j];
-          static_cast<float*>(a.v)[e0 + j] = v[j];
+          static_cast<float*>(a.m)[e0 + j] = values(m)[j];
+          static_cast<float*>(a.v)[e0 + j] = values(v)[j];
         }
       }
     }

@@ -399,26 +399,6 @@ __device__ __forceinline__ uint4 read_shared_16(uint32_t at) {
   return v;
 }
 
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ unsigned long long bits2(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
-__device__ __forceinline__ float2 of_bits2(unsigned long long v) { return *reinterpret_cast<float2*>(&v); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
-  return of_bits2(d);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  unsigned long long d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
-  return of_bits2(d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
-  return of_bits2(d);
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-
 template <typename T>
 __device__ __forceinline__ void unpack2(const uint4& u, float2 (&v)[VALUES<T> / 2]) {
   const uint32_t word[4] = {u.x, u.y, u.z, u.w};

@@ -92,6 +92,26 @@ __device__ __forceinline__ void store8_as(void* p, int type, long long i, const 
   }
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ unsigned long long bits2(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
+__device__ __forceinline__ float2 of_bits2(unsigned long long v) { return *reinterpret_cast<float2*>(&v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return of_bits2(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return of_bits2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return of_bits2(d);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 inline bool is_type(int type) { return type == FFM_TYPE_BF16 || type == FFM_TYPE_FP16 || type == FFM_TYPE_FP32; }
 inline int type_bytes(int type) { return type == FFM_TYPE_FP32 ? 4 : 2; }
 
