@@ -12,7 +12,7 @@
 // the new m and v before they are rounded.
 //
 // HBM-bound: bf16 parameters, gradients and 8-bit states move 10 bytes a value, with fp32 states 22, with an fp32 master 28.
-// A block walks chunks of 2048 values, eight neighbours a thread, over all tensors as one list. Steps are counted on the
+// A block walks chunks of 4096 values, twice eight neighbours a thread, over all tensors as one list. Steps are counted on the
 // device, so that a captured step can be replayed: every block reads them, and the last block to finish raises them.
 #include "ffm_types.cuh"
 
@@ -24,7 +24,7 @@ namespace ffm {
 namespace {
 
 constexpr int ADAMW_THREADS = 256;
-constexpr int ADAMW_CHUNK = ADAMW_THREADS * 8;
+constexpr int ADAMW_CHUNK = ADAMW_THREADS * 16;
 constexpr int ADAMW_BLOCK = 128;  // values that share a scale: 16 threads
 
 struct AdamWTensor {
@@ -139,14 +139,287 @@ __device__ __forceinline__ float reciprocal_fast(float v) {
 // eight values as four pairs
 __device__ __forceinline__ float (&values(float2 (&v)[4]))[8] { return *reinterpret_cast<float (*)[8]>(&v); }
 
-template <int MAX, bool EIGHT>
+// What of a call is the same for all values.
+struct Step {
+  float2 keep, eps;
+  float beta1, less1, beta2, less2, eps_one, grad_scale;
+  bool scaled, fast;
+};
+
+// The update of eight values: m, v and p in place; root is sqrt(v).
+__device__ __forceinline__ void update8(const Step& h, float rate, float inverse, const float2 (&g)[4], float2 (&p)[4], float2 (&m)[4],
+                                        float2 (&v)[4], float2 (&root)[4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    // each product and sum is rounded on its own: in 8 bits the largest of a block decides its scale, and two evaluations
+    // that differ in the last place would now and then differ in it
+    float x = g[q].x, y = g[q].y;
+    if (h.scaled) x = __fmul_rn(x, h.grad_scale), y = __fmul_rn(y, h.grad_scale);
+    m[q].x = __fadd_rn(__fmul_rn(m[q].x, h.beta1), __fmul_rn(x, h.less1));
+    m[q].y = __fadd_rn(__fmul_rn(m[q].y, h.beta1), __fmul_rn(y, h.less1));
+    v[q].x = __fadd_rn(__fmul_rn(v[q].x, h.beta2), __fmul_rn(__fmul_rn(x, h.less2), x));
+    v[q].y = __fadd_rn(__fmul_rn(v[q].y, h.beta2), __fmul_rn(__fmul_rn(y, h.less2), y));
+  }
+  if (h.fast) {
+    const float2 r = both(-rate), inv = both(inverse);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      root[q] = make_float2(root_fast(v[q].x), root_fast(v[q].y));
+      const float2 under = fma2(root[q], inv, h.eps);
+      p[q] = fma2(r, mul2(m[q], make_float2(reciprocal_fast(under.x), reciprocal_fast(under.y))), mul2(p[q], h.keep));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      values(root)[j] = __fsqrt_rn(values(v)[j]);
+      values(p)[j] = fmaf(-rate, __fdiv_rn(values(m)[j], fmaf(values(root)[j], inverse, h.eps_one)), values(p)[j] * h.keep.x);
+    }
+  }
+}
+
+// Eight 8-bit values of either moment with their blocks' scales.
+__device__ __forceinline__ void unpack_states(uint2 cm, uint2 cv, uint32_t sm, uint32_t sv, float2 (&m)[4], float2 (&v)[4]) {
+  const float2 fm = both(__uint_as_float(sm << 23)), fv = both(__uint_as_float(sv << 23));
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    m[q] = mul2(e4m3x2_to_float2((q < 2 ? cm.x : cm.y) >> (16 * (q & 1)) & 0xffffu), fm);
+    v[q] = mul2(e4m3x2_to_float2((q < 2 ? cv.x : cv.y) >> (16 * (q & 1)) & 0xffffu), fv);
+    v[q] = mul2(v[q], v[q]);
+  }
+}
+
+// And back: the 16 threads of a block find its scales. pair0: the first value's place in the tensor, halved.
+__device__ __forceinline__ void pack_states(float2 (&m)[4], const float2 (&v)[4], const float2 (&root)[4], uint32_t pair0, uint32_t key,
+                                            uint32_t (&cm)[2], uint32_t (&cv)[2], int& km, int& kv) {
+  float top_m = 0.0f, top_v = 0.0f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    top_m = max_nan(top_m, max_nan(fabsf(m[q].x), fabsf(m[q].y)));
+    top_v = max_nan(top_v, max_nan(v[q].x, v[q].y));
+  }
+  top_m = max16(top_m);
+  top_v = max16(top_v);
+  const bool odd = !finite(top_m) || !finite(top_v);  // something of the block is not finite
+  if (__any_sync(0xffffffffu, odd)) {
+    // what is infinite or NaN leaves the scale to the others, and becomes NaN
+    float other_m = 0.0f, other_v = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (finite(m[q].x)) other_m = fmaxf(other_m, fabsf(m[q].x));
+      if (finite(m[q].y)) other_m = fmaxf(other_m, fabsf(m[q].y));
+      if (finite(v[q].x)) other_v = fmaxf(other_v, v[q].x);
+      if (finite(v[q].y)) other_v = fmaxf(other_v, v[q].y);
+      if (!finite(m[q].x)) m[q].x = __int_as_float(0x7fc00000);
+      if (!finite(m[q].y)) m[q].y = __int_as_float(0x7fc00000);
+    }
+    other_m = max16(other_m);
+    other_v = max16(other_v);
+    if (odd) top_m = other_m, top_v = other_v;
+  }
+  km = block_exponent(top_m);
+  kv = block_exponent(__fsqrt_rn(top_v));
+  const float2 fm = both(exponent_of_two(-km)), fv = both(exponent_of_two(-kv));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    cm[h] = e4m3x2_nearest(mul2(m[2 * h], fm)) | e4m3x2_nearest(mul2(m[2 * h + 1], fm)) << 16;
+    const uint32_t first = random_pair(pair0 + 2 * h, key), second = random_pair(pair0 + 2 * h + 1, key);
+    const uint32_t random[4] = {(first << 4 & 0xffff0u) | 8u, (first >> 12 & 0xffff0u) | 8u, (second << 4 & 0xffff0u) | 8u,
+                                (second >> 12 & 0xffff0u) | 8u};
+    const float2 a = mul2(root[2 * h], fv), b = mul2(root[2 * h + 1], fv);
+    const float x[4] = {a.x, a.y, b.x, b.y};
+    uint32_t c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = e4m3_random(x[j], random[j]);
+    cv[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    // a code below 8 or above 127 stands for a number below 2^-6, or one that is none: rare
+    const uint32_t eights = cv[h] & 0x78787878u;
+    if (((c[0] | c[1] | c[2] | c[3]) & ~0x7fu) != 0 || ((eights - 0x01010101u) & ~eights & 0x80808080u) != 0 || odd) {
+      const float y[4] = {v[2 * h].x, v[2 * h].y, v[2 * h + 1].x, v[2 * h + 1].y};
+      cv[h] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cv[h] |= e4m3_random_any(x[j], y[j], random[j]) << (8 * j);
+    }
+  }
+}
+
+// How a tensor's values lie: a launch is for one of these, so that its kernel knows the loads of a value at compile time. HALF:
+// parameter and gradient in the same 16-bit type. ANY: the two in different types.
+enum { ANY_LAYOUT = 0, HALF_LAYOUT = 1, HALF_MASTER_LAYOUT = 2, F32_LAYOUT = 3, LAYOUTS = 4 };
+
+// Eight values as they come from memory.
+template <int LAYOUT, bool EIGHT>
+struct Raw {
+  static constexpr int P = LAYOUT == HALF_LAYOUT ? 1 : 2, G = LAYOUT == F32_LAYOUT ? 2 : 1;
+  uint4 p[P], g[G], m[EIGHT ? 1 : 2], v[EIGHT ? 1 : 2];  // 8-bit states: the first half
+  uint32_t sm, sv;
+
+  template <int N>
+  __device__ __forceinline__ static void get(uint4 (&to)[N], const void* from) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = static_cast<const uint4*>(from)[i];
+  }
+  template <int N>
+  __device__ __forceinline__ static void as_pairs(const uint4 (&from)[N], bool fp16s, float2 (&to)[4]) {
+    if constexpr (N == 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        to[2 * i] = make_float2(__uint_as_float(from[i].x), __uint_as_float(from[i].y));
+        to[2 * i + 1] = make_float2(__uint_as_float(from[i].z), __uint_as_float(from[i].w));
+      }
+    } else {
+      const uint32_t word[4] = {from[0].x, from[0].y, from[0].z, from[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        to[i] = fp16s ? __half22float2(*reinterpret_cast<const __half2*>(&word[i]))
+                      : make_float2(__uint_as_float(word[i] << 16), __uint_as_float(word[i] & 0xffff0000u));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load(const AdamWTensor& a, long long e) {
+    get(g, static_cast<const char*>(a.g) + e * (G == 2 ? 4 : 2));
+    get(p, LAYOUT == HALF_MASTER_LAYOUT ? static_cast<const void*>(a.master + e) : static_cast<const char*>(a.p) + e * (P == 2 ? 4 : 2));
+    if constexpr (EIGHT) {
+      const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + e);
+      const uint2 y = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + e);
+      m[0] = make_uint4(x.x, x.y, 0, 0);
+      v[0] = make_uint4(y.x, y.y, 0, 0);
+      sm = a.m_scale[e / ADAMW_BLOCK];
+      sv = a.v_scale[e / ADAMW_BLOCK];
+    } else {
+      get(m, static_cast<const float*>(a.m) + e);
+      get(v, static_cast<const float*>(a.v) + e);
+    }
+  }
+  __device__ __forceinline__ void step(const AdamWTensor& a, long long e, const Step& h, float rate, float inverse, uint32_t key) {
+    float2 gf[4], pf[4], mf[4], vf[4], root[4];
+    const bool fp16s = a.p_type == FFM_TYPE_FP16;
+    as_pairs(g, fp16s, gf);
+    as_pairs(p, fp16s, pf);
+    if constexpr (EIGHT) {
+      unpack_states(make_uint2(m[0].x, m[0].y), make_uint2(v[0].x, v[0].y), sm, sv, mf, vf);
+    } else {
+      as_pairs(m, false, mf);
+      as_pairs(v, false, vf);
+    }
+    update8(h, rate, inverse, gf, pf, mf, vf, root);
+    if constexpr (LAYOUT == HALF_MASTER_LAYOUT) store8(a.master + e, values(pf));
+    if constexpr (LAYOUT == F32_LAYOUT) {
+      store8(static_cast<float*>(a.p) + e, values(pf));
+    } else if (fp16s) {
+      store8(static_cast<fp16*>(a.p) + e, values(pf));
+    } else {
+      store8(static_cast<bf16*>(a.p) + e, values(pf));
+    }
+    if constexpr (EIGHT) {
+      uint32_t cm[2], cv[2];
+      int km, kv;
+      pack_states(mf, vf, root, static_cast<uint32_t>(e >> 1), key, cm, cv, km, kv);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + e) = make_uint2(cm[0], cm[1]);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + e) = make_uint2(cv[0], cv[1]);
+      if ((threadIdx.x & 15) == 0) {
+        a.m_scale[e / ADAMW_BLOCK] = static_cast<uint8_t>(km + 127);
+        a.v_scale[e / ADAMW_BLOCK] = static_cast<uint8_t>(kv + 127);
+      }
+    } else {
+      store8(static_cast<float*>(a.m) + e, values(mf));
+      store8(static_cast<float*>(a.v) + e, values(vf));
+    }
+  }
+};
+
+// Up to eight values of any types at any address, from value e of the tensor on: the ends of tensors, tensors off 16 bytes, and
+// the ANY layout.
+template <bool EIGHT>
+__device__ __forceinline__ void step_any(const AdamWTensor& a, long long e, const Step& h, float rate, float inverse, uint32_t key) {
+  const int left = static_cast<int>(min(a.n - e, 8ll));  // none where <= 0
+  const bool whole = left == 8 && a.wide != 0;
+  float2 g[4], p[4], m[4], v[4], root[4];
+  if (whole) {
+    load8_as(a.g, a.g_type, e, values(g));
+    if (a.master != nullptr) {
+      load8(a.master + e, values(p));
+    } else {
+      load8_as(a.p, a.p_type, e, values(p));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (whole) break;
+    values(g)[j] = j < left ? load1_as(a.g, a.g_type, e + j) : 0.0f;
+    values(p)[j] = j < left ? (a.master != nullptr ? a.master[e + j] : load1_as(a.p, a.p_type, e + j)) : 0.0f;
+  }
+  if (EIGHT) {
+    uint2 cm = make_uint2(0, 0), cv = make_uint2(0, 0);
+    uint32_t sm = 0, sv = 0;
+    if (left > 0) {
+      sm = a.m_scale[e / ADAMW_BLOCK];
+      sv = a.v_scale[e / ADAMW_BLOCK];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j < left) {
+        const uint32_t x = static_cast<const uint8_t*>(a.m)[e + j], y = static_cast<const uint8_t*>(a.v)[e + j];
+        if (j < 4) {
+          cm.x |= x << (8 * j), cv.x |= y << (8 * j);
+        } else {
+          cm.y |= x << (8 * j - 32), cv.y |= y << (8 * j - 32);
+        }
+      }
+    }
+    unpack_states(cm, cv, sm, sv, m, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      values(m)[j] = j < left ? static_cast<const float*>(a.m)[e + j] : 0.0f;
+      values(v)[j] = j < left ? static_cast<const float*>(a.v)[e + j] : 0.0f;
+    }
+  }
+  update8(h, rate, inverse, g, p, m, v, root);
+  if (whole) {
+    if (a.master != nullptr) store8(a.master + e, values(p));
+    store8_as(a.p, a.p_type, e, values(p));
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j < left && !whole) {
+      if (a.master != nullptr) a.master[e + j] = values(p)[j];
+      store1_as(a.p, a.p_type, e + j, values(p)[j]);
+    }
+  }
+  if (EIGHT) {
+    uint32_t cm[2], cv[2];
+    int km, kv;
+    pack_states(m, v, root, static_cast<uint32_t>(e >> 1), key, cm, cv, km, kv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j < left) {
+        static_cast<uint8_t*>(a.m)[e + j] = static_cast<uint8_t>(cm[j >> 2] >> (8 * (j & 3)));
+        static_cast<uint8_t*>(a.v)[e + j] = static_cast<uint8_t>(cv[j >> 2] >> (8 * (j & 3)));
+      }
+    }
+    if (left > 0 && (threadIdx.x & 15) == 0) {
+      a.m_scale[e / ADAMW_BLOCK] = static_cast<uint8_t>(km + 127);
+      a.v_scale[e / ADAMW_BLOCK] = static_cast<uint8_t>(kv + 127);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j < left) {
+        static_cast<float*>(a.m)[e + j] = values(m)[j];
+        static_cast<float*>(a.v)[e + j] = values(v)[j];
+      }
+    }
+  }
+}
+
+template <int MAX, int LAYOUT, bool EIGHT>
 __global__ void __launch_bounds__(ADAMW_THREADS)
 adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
   __shared__ float rate[MAX], inverse[MAX];  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
   __shared__ uint32_t keys[MAX];
   __shared__ bool last;
   const float lr = job.lr_device != nullptr ? *job.lr_device : job.lr;
-  const float grad_scale = job.grad_scale != nullptr ? *job.grad_scale : 1.0f;
   for (int i = threadIdx.x; i < job.count; i += ADAMW_THREADS) {
     const int t = *job.tensor[i].step + 1;
     rate[i] = static_cast<float>(lr / (1.0 - power(job.beta1_wide, t)));
@@ -154,200 +427,34 @@ adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
     keys[i] = static_cast<uint32_t>(t) * 0x85EBCA77u + job.seed * 0xC2B2AE3Du;
   }
   __syncthreads();
-  const float2 keep = both(1.0f - lr * job.weight_decay), eps = both(job.eps);
-  const float2 beta1 = both(job.beta1), less1 = both(job.one_minus_beta1), beta2 = both(job.beta2), less2 = both(job.one_minus_beta2);
-  const bool scaled = job.grad_scale != nullptr;
+  Step h;
+  h.keep = both(1.0f - lr * job.weight_decay);
+  h.eps = both(job.eps);
+  h.eps_one = job.eps;
+  h.beta1 = job.beta1, h.less1 = job.one_minus_beta1, h.beta2 = job.beta2, h.less2 = job.one_minus_beta2;
+  h.scaled = job.grad_scale != nullptr;
+  h.grad_scale = h.scaled ? *job.grad_scale : 1.0f;
   // with eps from here on a root of a v below 2^-126 (10^-19) makes no difference to the update
-  const bool fast = job.eps >= 1e-12f;
+  h.fast = job.eps >= 1e-12f;
   const long long chunks = job.tensor[job.count - 1].chunks_end;
   int i = 0;
   for (long long chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     while (chunk >= job.tensor[i].chunks_end) ++i;  // the chunk's tensor, for the whole block alike
     const AdamWTensor& a = job.tensor[i];
-    const long long e0 = (chunk - (i > 0 ? job.tensor[i - 1].chunks_end : 0)) * ADAMW_CHUNK + threadIdx.x * 8;
-    const int left = static_cast<int>(min(a.n - e0, 8ll));  // values of this thread, none where <= 0
-    const bool whole = left == 8 && a.wide != 0;
-    float2 p[4], g[4], m[4], v[4];
-    if (whole) {
-      load8_as(a.g, a.g_type, e0, values(g));
-      if (a.master != nullptr) {
-        load8(a.master + e0, values(p));
-      } else {
-        load8_as(a.p, a.p_type, e0, values(p));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        values(g)[j] = j < left ? load1_as(a.g, a.g_type, e0 + j) : 0.0f;
-        values(p)[j] = j < left ? (a.master != nullptr ? a.master[e0 + j] : load1_as(a.p, a.p_type, e0 + j)) : 0.0f;
+    const long long c0 = (chunk - (i > 0 ? job.tensor[i - 1].chunks_end : 0)) * ADAMW_CHUNK, e0 = c0 + threadIdx.x * 8;
+    if constexpr (LAYOUT != ANY_LAYOUT) {
+      if (a.wide && c0 + ADAMW_CHUNK <= a.n) {
+        // both halves' loads first: twice as much in flight
+        Raw<LAYOUT, EIGHT> first, second;
+        first.load(a, e0);
+        second.load(a, e0 + ADAMW_CHUNK / 2);
+        first.step(a, e0, h, rate[i], inverse[i], keys[i]);
+        second.step(a, e0 + ADAMW_CHUNK / 2, h, rate[i], inverse[i], keys[i]);
+        continue;
       }
     }
-    if (EIGHT) {
-      uint2 cm = make_uint2(0, 0), cv = make_uint2(0, 0);
-      uint32_t sm = 0, sv = 0;
-      if (left > 0) {
-        sm = a.m_scale[e0 / ADAMW_BLOCK];
-        sv = a.v_scale[e0 / ADAMW_BLOCK];
-      }
-      if (whole) {
-        cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + e0);
-        cv = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + e0);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < left) {
-            const uint32_t x = static_cast<const uint8_t*>(a.m)[e0 + j], y = static_cast<const uint8_t*>(a.v)[e0 + j];
-            if (j < 4) {
-              cm.x |= x << (8 * j), cv.x |= y << (8 * j);
-            } else {
-              cm.y |= x << (8 * j - 32), cv.y |= y << (8 * j - 32);
-            }
-          }
-        }
-      }
-      const float2 fm = both(__uint_as_float(sm << 23)), fv = both(__uint_as_float(sv << 23));
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        m[q] = mul2(e4m3x2_to_float2((q < 2 ? cm.x : cm.y) >> (16 * (q & 1)) & 0xffffu), fm);
-        v[q] = mul2(e4m3x2_to_float2((q < 2 ? cv.x : cv.y) >> (16 * (q & 1)) & 0xffffu), fv);
-        v[q] = mul2(v[q], v[q]);
-      }
-    } else if (whole) {
-      load8(static_cast<const float*>(a.m) + e0, values(m));
-      load8(static_cast<const float*>(a.v) + e0, values(v));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        values(m)[j] = j < left ? static_cast<const float*>(a.m)[e0 + j] : 0.0f;
-        values(v)[j] = j < left ? static_cast<const float*>(a.v)[e0 + j] : 0.0f;
-      }
-    }
-
-    float2 root[4];
-    float top_m = 0.0f, top_v = 0.0f;
-    const float2 r = both(-rate[i]), inv = both(inverse[i]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // each product and sum is rounded on its own: in 8 bits the largest of a block decides its scale, and two evaluations
-      // that differ in the last place would now and then differ in it
-      const float x = scaled ? __fmul_rn(values(g)[j], grad_scale) : values(g)[j];
-      values(m)[j] = __fadd_rn(__fmul_rn(values(m)[j], job.beta1), __fmul_rn(x, job.one_minus_beta1));
-      values(v)[j] = __fadd_rn(__fmul_rn(values(v)[j], job.beta2), __fmul_rn(__fmul_rn(x, job.one_minus_beta2), x));
-    }
-    if (fast) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        root[q] = make_float2(root_fast(v[q].x), root_fast(v[q].y));
-        const float2 under = fma2(root[q], inv, eps);
-        p[q] = fma2(r, mul2(m[q], make_float2(reciprocal_fast(under.x), reciprocal_fast(under.y))), mul2(p[q], keep));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        values(root)[j] = __fsqrt_rn(values(v)[j]);
-        values(p)[j] = fmaf(r.x, __fdiv_rn(values(m)[j], fmaf(values(root)[j], inv.x, eps.x)), values(p)[j] * keep.x);
-      }
-    }
-    if (EIGHT) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        top_m = max_nan(top_m, max_nan(fabsf(m[q].x), fabsf(m[q].y)));
-        top_v = max_nan(top_v, max_nan(v[q].x, v[q].y));
-      }
-    }
-
-    if (a.master != nullptr) {
-      if (whole) {
-        store8(a.master + e0, values(p));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < left) a.master[e0 + j] = values(p)[j];
-        }
-      }
-    }
-    if (whole) {
-      store8_as(a.p, a.p_type, e0, values(p));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j < left) store1_as(a.p, a.p_type, e0 + j, values(p)[j]);
-      }
-    }
-    if (EIGHT) {
-      top_m = max16(top_m);
-      top_v = max16(top_v);
-      const bool odd = !finite(top_m) || !finite(top_v);  // something of the block is not finite
-      if (__any_sync(0xffffffffu, odd)) {
-        // what is infinite or NaN leaves the scale to the others, and becomes NaN
-        float other_m = 0.0f, other_v = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = values(m)[j], y = values(v)[j];
-          if (finite(x)) other_m = fmaxf(other_m, fabsf(x));
-          if (finite(y)) other_v = fmaxf(other_v, y);
-          if (!finite(x)) values(m)[j] = __int_as_float(0x7fc00000);
-        }
-        other_m = max16(other_m);
-        other_v = max16(other_v);
-        if (odd) top_m = other_m, top_v = other_v;
-      }
-      const int km = block_exponent(top_m), kv = block_exponent(__fsqrt_rn(top_v));
-      const float2 fm = both(exponent_of_two(-km)), fv = both(exponent_of_two(-kv));
-      uint32_t cm[2], cv[2], code[8], random[8];
-      float2 x[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t two = random_pair(static_cast<uint32_t>((e0 >> 1) + q), keys[i]);
-        random[2 * q] = (two << 4 & 0xffff0u) | 8u;
-        random[2 * q + 1] = (two >> 12 & 0xffff0u) | 8u;
-        x[q] = mul2(root[q], fv);
-        code[2 * q] = e4m3_random(x[q].x, random[2 * q]);
-        code[2 * q + 1] = e4m3_random(x[q].y, random[2 * q + 1]);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        cm[h] = e4m3x2_nearest(mul2(m[2 * h], fm)) | e4m3x2_nearest(mul2(m[2 * h + 1], fm)) << 16;
-        const uint32_t* c = code + 4 * h;
-        cv[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-        // a code below 8 or above 127 stands for a number below 2^-6, or one that is none: rare
-        const uint32_t eights = cv[h] & 0x78787878u;
-        if (((c[0] | c[1] | c[2] | c[3]) & ~0x7fu) != 0 || ((eights - 0x01010101u) & ~eights & 0x80808080u) != 0 || odd) {
-          cv[h] = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            cv[h] |= e4m3_random_any(values(x)[4 * h + j], values(v)[4 * h + j], random[4 * h + j]) << (8 * j);
-          }
-        }
-      }
-      if (whole) {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + e0) = make_uint2(cm[0], cm[1]);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + e0) = make_uint2(cv[0], cv[1]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < left) {
-            static_cast<uint8_t*>(a.m)[e0 + j] = static_cast<uint8_t>(cm[j >> 2] >> (8 * (j & 3)));
-            static_cast<uint8_t*>(a.v)[e0 + j] = static_cast<uint8_t>(cv[j >> 2] >> (8 * (j & 3)));
-          }
-        }
-      }
-      if (left > 0 && e0 % ADAMW_BLOCK == 0) {
-        a.m_scale[e0 / ADAMW_BLOCK] = static_cast<uint8_t>(km + 127);
-        a.v_scale[e0 / ADAMW_BLOCK] = static_cast<uint8_t>(kv + 127);
-      }
-    } else if (whole) {
-      store8(static_cast<float*>(a.m) + e0, values(m));
-      store8(static_cast<float*>(a.v) + e0, values(v));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j < left) {
-          static_cast<float*>(a.m)[e0 + j] = values(m)[j];
-          static_cast<float*>(a.v)[e0 + j] = values(v)[j];
-        }
-      }
-    }
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) step_any<EIGHT>(a, e0 + half * (ADAMW_CHUNK / 2), h, rate[i], inverse[i], keys[i]);
   }
   // every block has read the steps before it takes a ticket; the last one raises them
   __syncthreads();
@@ -362,7 +469,7 @@ adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
   }
 }
 
-template <int MAX, bool EIGHT>
+template <int MAX, int LAYOUT, bool EIGHT>
 int launch_adamw(const ffm_adamw_tensor* t, int count, const ffm_adamw_args& h, cudaStream_t stream) {
   AdamWJob<MAX> job;
   long long chunks = 0;
@@ -398,7 +505,7 @@ int launch_adamw(const ffm_adamw_tensor* t, int count, const ffm_adamw_args& h, 
   job.grad_scale = h.grad_scale;
   job.seed = static_cast<uint32_t>(h.seed);
   job.ticket = static_cast<unsigned int*>(h.ticket);
-  auto kernel = adamw_kernel<MAX, EIGHT>;
+  auto kernel = adamw_kernel<MAX, LAYOUT, EIGHT>;
   static PerDevice resident;
   const int most = resident.get([&] {
     int blocks = 0;
@@ -411,6 +518,23 @@ int launch_adamw(const ffm_adamw_tensor* t, int count, const ffm_adamw_args& h, 
   if (most <= 0) return FFM_ERR_LAUNCH;
   kernel<<<static_cast<unsigned>(chunks < most ? (chunks > 0 ? chunks : 1) : most), ADAMW_THREADS, 0, stream>>>(job);
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
+int adamw_layout(const ffm_adamw_tensor& t) {
+  if (t.param_type != t.grad_type) return ANY_LAYOUT;
+  if (t.param_type == FFM_TYPE_FP32) return t.master == nullptr ? F32_LAYOUT : ANY_LAYOUT;
+  return t.master != nullptr ? HALF_MASTER_LAYOUT : HALF_LAYOUT;
+}
+
+template <int MAX>
+int launch_adamw_as(int layout, bool eight, const ffm_adamw_tensor* t, int count, const ffm_adamw_args& h, cudaStream_t stream) {
+  switch (layout) {
+    case HALF_LAYOUT: return eight ? launch_adamw<MAX, HALF_LAYOUT, true>(t, count, h, stream) : launch_adamw<MAX, HALF_LAYOUT, false>(t, count, h, stream);
+    case HALF_MASTER_LAYOUT:
+      return eight ? launch_adamw<MAX, HALF_MASTER_LAYOUT, true>(t, count, h, stream) : launch_adamw<MAX, HALF_MASTER_LAYOUT, false>(t, count, h, stream);
+    case F32_LAYOUT: return eight ? launch_adamw<MAX, F32_LAYOUT, true>(t, count, h, stream) : launch_adamw<MAX, F32_LAYOUT, false>(t, count, h, stream);
+    default: return eight ? launch_adamw<MAX, ANY_LAYOUT, true>(t, count, h, stream) : launch_adamw<MAX, ANY_LAYOUT, false>(t, count, h, stream);
+  }
 }
 
 }  // namespace
@@ -434,12 +558,19 @@ extern "C" int ffm_adamw_step(const ffm_adamw_tensor* tensors, int count, const 
     if (eight && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return FFM_ERR_BAD_ARG;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  for (int first = 0; first < count; first += FFM_ADAMW_MAX) {
-    const int n = count - first < FFM_ADAMW_MAX ? count - first : FFM_ADAMW_MAX;
-    const ffm_adamw_tensor* t = tensors + first;
-    const int rc = n <= FFM_ADAMW_FEW ? (eight ? launch_adamw<FFM_ADAMW_FEW, true>(t, n, h, s) : launch_adamw<FFM_ADAMW_FEW, false>(t, n, h, s))
-                                      : (eight ? launch_adamw<FFM_ADAMW_MAX, true>(t, n, h, s) : launch_adamw<FFM_ADAMW_MAX, false>(t, n, h, s));
-    if (rc != FFM_OK) return rc;
+  ffm_adamw_tensor some[FFM_ADAMW_MAX];
+  for (int layout = 0; layout < LAYOUTS; ++layout) {
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+      if (adamw_layout(tensors[i]) == layout) some[n++] = tensors[i];
+      if (n == FFM_ADAMW_MAX || (i + 1 == count && n > 0)) {
+        const int rc = n <= FFM_ADAMW_FEW ? launch_adamw_as<FFM_ADAMW_FEW>(layout, eight, some, n, h, s)
+                                          : launch_adamw_as<FFM_ADAMW_MAX>(layout, eight, some, n, h, s);
+        if (rc != FFM_OK) return rc;
+        n = 0;
+        if (h.launched != nullptr) ++*h.launched;
+      }
+    }
   }
   return FFM_OK;
 }

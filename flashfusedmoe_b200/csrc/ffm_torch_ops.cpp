@@ -534,6 +534,8 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
   const ffm_stream_t stream = device.stream();
   const Tensor ticket = ticket_for(first, stream, capturing);
   h.ticket = ticket.data_ptr();
+  int64_t launched = 0;
+  h.launched = &launched;
   int rc;
   {
     py::gil_scoped_release released;
@@ -552,7 +554,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
       for (const Tensor& t : **list) changed(t);
     }
   }
-  launches += (static_cast<int64_t>(n) + FFM_ADAMW_MAX - 1) / FFM_ADAMW_MAX;
+  launches += launched;
 }
 
 }  // namespace

@@ -517,7 +517,8 @@ int ffm_layer_norm_backward(const void* dy, const void* x, int x_type, int64_t r
                             void* dbias, int b_type, void* workspace, size_t workspace_bytes, ffm_stream_t stream);
 
 /* -------------------------------------------------------------------------------------------------
- * AdamW over `count` tensors, one launch for up to FFM_ADAMW_MAX of them (weight decay decoupled, eps outside of the root):
+ * AdamW over `count` tensors, one launch for up to FFM_ADAMW_MAX of them (and one more for every other combination of types)
+ * (weight decay decoupled, eps outside of the root):
  *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * Every field is 8 bytes wide. Types are FFM_TYPE_*; every tensor is contiguous. With `master` (f32, as many elements) that
  * is updated and param is its rounded copy. step (int32) counts the tensor's steps and is raised by one; no two entries of a
@@ -526,7 +527,8 @@ int ffm_layer_norm_backward(const void* dy, const void* x, int x_type, int64_t r
  *   bits = 8:  exp_avg, exp_avg_sq are e4m3 codes of m and sqrt(v) over 2^(scale - 127), with one scale byte for every 128
  *              elements (the last block may be shorter). m is rounded to nearest, sqrt(v) at random by seed, step and place,
  *              and never to zero where v > 0. A value that is not finite becomes NaN.
- * ticket: a device word, zero before the call and after it, that no other call in flight uses.
+ * ticket: a device word, zero before the call and after it, that no other call in flight uses. launched (null or host): kernels
+ * enqueued are added.
  * ------------------------------------------------------------------------------------------------- */
 #define FFM_ADAMW_MAX 256
 #define FFM_ADAMW_FEW 32 /* up to so many, a smaller argument block is launched */
@@ -554,6 +556,7 @@ typedef struct {
   int64_t bits;
   int64_t seed;
   void* ticket;
+  int64_t* launched;
 } ffm_adamw_args;
 int ffm_adamw_step(const ffm_adamw_tensor* tensors, int count, const ffm_adamw_args* args, ffm_stream_t stream);
 

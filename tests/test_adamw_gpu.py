@@ -11,7 +11,7 @@ import torch
 U = 2.0 ** -24
 BLOCK = 128
 # around a thread's eight, a scale's block, a block's chunk of 2048; several chunks
-SIZES = [1, 7, 8, 127, 128, 129, 1000, 2047, 2048, 2049, 5003, 70001]
+SIZES = [1, 7, 8, 127, 128, 129, 1000, 2047, 2048, 2049, 4096, 4097, 5003, 8192, 70001]
 HYPER = dict(lr=3e-3, betas=(0.9, 0.97), eps=1e-6, weight_decay=0.1)
 
 
@@ -103,7 +103,8 @@ class Tensors:
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("dtype,grad_dtype,master", [(torch.bfloat16, None, False), (torch.bfloat16, None, True), (torch.float32, None, False),
-                                                     (torch.float16, torch.float32, True), (torch.float32, torch.bfloat16, False)])
+                                                     (torch.float16, None, False), (torch.float16, None, True), (torch.float16, torch.float32, True),
+                                                     (torch.float32, torch.bfloat16, False), (torch.bfloat16, torch.float16, False)])
 @pytest.mark.parametrize("shift", [0, 1])
 def test_a_step_over_tensors_of_every_size(bits, dtype, grad_dtype, master, shift):
     t = Tensors(SIZES, dtype, bits, master, grad_dtype, shift)
@@ -128,6 +129,39 @@ def test_any_number_of_tensors(count, bits):
     t.step()
     t.check([f for i, f in enumerate(found) if True] if count <= 40 else found[:37], before)
     assert [s.item() for s in t.steps] == [b + 1 for b in before]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_of_different_types_in_one_call(bits):
+    parts = [Tensors([300, 9000], dtype, bits, False, grad, seed=k) for k, (dtype, grad) in enumerate(
+        [(torch.bfloat16, None), (torch.float32, None), (torch.float16, None), (torch.float32, torch.bfloat16), (torch.bfloat16, None)])]
+    t = Tensors([], torch.float32, bits)
+    for name in ("params", "grads", "steps", "m", "v") + (("m_scale", "v_scale") if bits == 8 else ()):
+        setattr(t, name, [x for p in parts for x in getattr(p, name)])
+    before = [s.item() for s in t.steps]
+    found = t.exact()
+    t.step()
+    t.check(found, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-20])
+def test_tiny_gradients_and_eps(bits, eps):
+    """v around and below the smallest normal number; the quotient of two small numbers is still about 1. In 8 bits no positive v is
+    lost. v itself is fp32: 2^-149 off (a whole of it where nothing is left)."""
+    t = Tensors([5000], torch.float32, bits)
+    t.grads[0].copy_(torch.logspace(-24, -16, 5000, device="cuda"))
+    t.m[0].view(torch.uint8).zero_()
+    t.v[0].view(torch.uint8).zero_()
+    m, v, p, _, _, p_off = t.exact(eps=eps)[0]
+    t.step(eps=eps)
+    normal = v > 2.0 ** -126
+    assert ((t.params[0].double() - p).abs() <= p_off)[normal].all() and t.params[0].isfinite()[v > 2.0 ** -148].all()
+    if bits == 8:
+        root, got = v.sqrt(), decode(t.v[0], t.v_scale[0])
+        assert (got[normal] > 0).all()
 
 
 @pytest.mark.gpu
