@@ -11,7 +11,9 @@
 // does not become zero (its least is 2^-18 of the block's scale squared): the quotient would explode. The update itself uses
 // the new m and v before they are rounded.
 //
-// HBM-bound: bf16 parameters, gradients and 8-bit states move 10 bytes a value, with fp32 states 22, with an fp32 master 28.
+// Bytes a value: bf16 parameters, gradients and 8-bit states move 10, with fp32 states 22, with an fp32 master as well 28. With
+// 32-bit states memory is the bound (5.4-5.5 TB/s read and written); 8-bit states take some 55 instructions a value, which keep 60 %
+// of the issue slots busy (3.8 TB/s without a master, 5.1 with one).
 // A block walks chunks of 4096 values, twice eight neighbours a thread, over all tensors as one list. Steps are counted on the
 // device, so that a captured step can be replayed: every block reads them, and the last block to finish raises them.
 #include "ffm_types.cuh"
@@ -87,17 +89,17 @@ __device__ __forceinline__ uint32_t e4m3x2_nearest(float2 v) {
 }
 
 // x from 2^-6 to 448 to e4m3, up with probability (distance from the lower neighbour) / (distance of the neighbours): 16 random
-// bits and a half, as a fraction, are added to the bits that are cut off. random: 20 bits, the last four of them 8. For a
-// smaller x the result is below 8, or not below 128.
-__device__ __forceinline__ uint32_t e4m3_random(float x, uint32_t random) {
-  return (__float_as_uint(x) + random - (120u << 23)) >> 20;
-}
+// bits and a half, as a fraction, are added to the bits that are cut off, and the code is what is left of this from bit 20 on.
+// random: 20 bits, the last four of them 8. For a smaller x the code is below 8, or not below 128.
+__device__ __forceinline__ uint32_t e4m3_random(float x, uint32_t random) { return __float_as_uint(x) + random - (120u << 23); }
 
-// The same for any x, and v (whose root it is) that may be anything. Below 2^-6 codes are multiples of 2^-9: 2^-6 more puts x into the
-// binade whose numbers lie as far apart, eight codes further up. Never zero for a positive v; NaN for one that is not finite.
-__device__ __noinline__ uint32_t e4m3_random_any(float x, float v, uint32_t random) {
+// The code for any v, x being its root, correctly rounded, times 1 / the scale. Below 2^-6 codes are multiples of 2^-9: 2^-6 more puts x
+// into the binade whose numbers lie as far apart, eight codes further up. Never zero for a positive v; NaN for one that is not
+// finite.
+__device__ __noinline__ uint32_t e4m3_random_any(float v, float scale, uint32_t random) {
   if (!(fabsf(v) <= 3.402823466e38f)) return 0x7fu;
-  const uint32_t code = x < 0.015625f ? e4m3_random(x + 0.015625f, random) - 8u : e4m3_random(x, random);
+  const float x = __fsqrt_rn(v) * scale;
+  const uint32_t code = x < 0.015625f ? (e4m3_random(x + 0.015625f, random) >> 20) - 8u : e4m3_random(x, random) >> 20;
   return v > 0.0f ? max(code, 1u) : 0u;
 }
 
@@ -116,9 +118,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ float max16(float v) {
+// the larger of either half, over 16 threads
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 8; o > 0; o >>= 1) v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
@@ -147,18 +150,23 @@ struct Step {
 };
 
 // The update of eight values: m, v and p in place; root is sqrt(v).
+template <bool EIGHT>
 __device__ __forceinline__ void update8(const Step& h, float rate, float inverse, const float2 (&g)[4], float2 (&p)[4], float2 (&m)[4],
                                         float2 (&v)[4], float2 (&root)[4]) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    // each product and sum is rounded on its own: in 8 bits the largest of a block decides its scale, and two evaluations
-    // that differ in the last place would now and then differ in it
-    float x = g[q].x, y = g[q].y;
-    if (h.scaled) x = __fmul_rn(x, h.grad_scale), y = __fmul_rn(y, h.grad_scale);
-    m[q].x = __fadd_rn(__fmul_rn(m[q].x, h.beta1), __fmul_rn(x, h.less1));
-    m[q].y = __fadd_rn(__fmul_rn(m[q].y, h.beta1), __fmul_rn(y, h.less1));
-    v[q].x = __fadd_rn(__fmul_rn(v[q].x, h.beta2), __fmul_rn(__fmul_rn(x, h.less2), x));
-    v[q].y = __fadd_rn(__fmul_rn(v[q].y, h.beta2), __fmul_rn(__fmul_rn(y, h.less2), y));
+    const float2 x = h.scaled ? mul2(g[q], both(h.grad_scale)) : g[q];
+    if (EIGHT) {
+      // Each product and sum is rounded on its own: the largest of a block decides its scale, and two evaluations that differ in the
+      // last place would now and then differ in it. (Pairs of products and sums are put together by the compiler even so.)
+      m[q].x = __fadd_rn(__fmul_rn(m[q].x, h.beta1), __fmul_rn(x.x, h.less1));
+      m[q].y = __fadd_rn(__fmul_rn(m[q].y, h.beta1), __fmul_rn(x.y, h.less1));
+      v[q].x = __fadd_rn(__fmul_rn(v[q].x, h.beta2), __fmul_rn(__fmul_rn(x.x, h.less2), x.x));
+      v[q].y = __fadd_rn(__fmul_rn(v[q].y, h.beta2), __fmul_rn(__fmul_rn(x.y, h.less2), x.y));
+    } else {
+      m[q] = add2(mul2(m[q], both(h.beta1)), mul2(x, both(h.less1)));
+      v[q] = add2(mul2(v[q], both(h.beta2)), mul2(mul2(x, both(h.less2)), x));
+    }
   }
   if (h.fast) {
     const float2 r = both(-rate), inv = both(inverse);
@@ -197,9 +205,11 @@ __device__ __forceinline__ void pack_states(float2 (&m)[4], const float2 (&v)[4]
     top_m = max_nan(top_m, max_nan(fabsf(m[q].x), fabsf(m[q].y)));
     top_v = max_nan(top_v, max_nan(v[q].x, v[q].y));
   }
-  top_m = max16(top_m);
-  top_v = max16(top_v);
-  const bool odd = !finite(top_m) || !finite(top_v);  // something of the block is not finite
+  // the exponents grow with the values: both of the block in one maximum, 0x7fff for what is not finite
+  const uint32_t mine = static_cast<uint32_t>(finite(top_m) ? block_exponent(top_m) + 127 : 0x7fff) |
+                        static_cast<uint32_t>(finite(top_v) ? block_exponent(__fsqrt_rn(top_v)) + 127 : 0x7fff) << 16;
+  uint32_t both_k = max16(mine);
+  const bool odd = (both_k & 0xffffu) == 0x7fffu || both_k >> 16 == 0x7fffu;
   if (__any_sync(0xffffffffu, odd)) {
     // what is infinite or NaN leaves the scale to the others, and becomes NaN
     float other_m = 0.0f, other_v = 0.0f;
@@ -212,12 +222,12 @@ __device__ __forceinline__ void pack_states(float2 (&m)[4], const float2 (&v)[4]
       if (!finite(m[q].x)) m[q].x = __int_as_float(0x7fc00000);
       if (!finite(m[q].y)) m[q].y = __int_as_float(0x7fc00000);
     }
-    other_m = max16(other_m);
-    other_v = max16(other_v);
-    if (odd) top_m = other_m, top_v = other_v;
+    const uint32_t others = max16(static_cast<uint32_t>(block_exponent(other_m) + 127) |
+                                  static_cast<uint32_t>(block_exponent(__fsqrt_rn(other_v)) + 127) << 16);
+    if (odd) both_k = others;
   }
-  km = block_exponent(top_m);
-  kv = block_exponent(__fsqrt_rn(top_v));
+  km = static_cast<int>(both_k & 0xffffu) - 127;
+  kv = static_cast<int>(both_k >> 16) - 127;
   const float2 fm = both(exponent_of_two(-km)), fv = both(exponent_of_two(-kv));
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -227,17 +237,23 @@ __device__ __forceinline__ void pack_states(float2 (&m)[4], const float2 (&v)[4]
                                 (second >> 12 & 0xffff0u) | 8u};
     const float2 a = mul2(root[2 * h], fv), b = mul2(root[2 * h + 1], fv);
     const float x[4] = {a.x, a.y, b.x, b.y};
-    uint32_t c[4];
+    // The roots are good to a unit or two of their last place, and the code is that of the correctly rounded one: where so little
+    // could change it (8 times in 2^20), it is taken again.
+    uint32_t c[4], near = 0xffffffffu;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[j] = e4m3_random(x[j], random[j]);
+    for (int j = 0; j < 4; ++j) {
+      c[j] = e4m3_random(x[j], random[j]);
+      near = min(near, (c[j] + 4u) << 12);
+      c[j] >>= 20;
+    }
     cv[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-    // a code below 8 or above 127 stands for a number below 2^-6, or one that is none: rare
+    // a code below 8 or above 127 stands for a number below 2^-6, or one that is none: rare as well
     const uint32_t eights = cv[h] & 0x78787878u;
-    if (((c[0] | c[1] | c[2] | c[3]) & ~0x7fu) != 0 || ((eights - 0x01010101u) & ~eights & 0x80808080u) != 0 || odd) {
+    if (((c[0] | c[1] | c[2] | c[3]) & ~0x7fu) != 0 || ((eights - 0x01010101u) & ~eights & 0x80808080u) != 0 || near < 8u << 12 || odd) {
       const float y[4] = {v[2 * h].x, v[2 * h].y, v[2 * h + 1].x, v[2 * h + 1].y};
       cv[h] = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) cv[h] |= e4m3_random_any(x[j], y[j], random[j]) << (8 * j);
+      for (int j = 0; j < 4; ++j) cv[h] |= e4m3_random_any(y[j], fv.x, random[j]) << (8 * j);
     }
   }
 }
@@ -302,7 +318,7 @@ struct Raw {
       as_pairs(m, false, mf);
       as_pairs(v, false, vf);
     }
-    update8(h, rate, inverse, gf, pf, mf, vf, root);
+    update8<EIGHT>(h, rate, inverse, gf, pf, mf, vf, root);
     if constexpr (LAYOUT == HALF_MASTER_LAYOUT) store8(a.master + e, values(pf));
     if constexpr (LAYOUT == F32_LAYOUT) {
       store8(static_cast<float*>(a.p) + e, values(pf));
@@ -375,7 +391,7 @@ __device__ __forceinline__ void step_any(const AdamWTensor& a, long long e, cons
       values(v)[j] = j < left ? static_cast<const float*>(a.v)[e + j] : 0.0f;
     }
   }
-  update8(h, rate, inverse, g, p, m, v, root);
+  update8<EIGHT>(h, rate, inverse, g, p, m, v, root);
   if (whole) {
     if (a.master != nullptr) store8(a.master + e, values(p));
     store8_as(a.p, a.p_type, e, values(p));
@@ -414,7 +430,7 @@ __device__ __forceinline__ void step_any(const AdamWTensor& a, long long e, cons
 }
 
 template <int MAX, int LAYOUT, bool EIGHT>
-__global__ void __launch_bounds__(ADAMW_THREADS)
+__global__ void __launch_bounds__(ADAMW_THREADS, EIGHT ? 3 : 2)
 adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
   __shared__ float rate[MAX], inverse[MAX];  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
   __shared__ uint32_t keys[MAX];
@@ -448,8 +464,18 @@ adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
         Raw<LAYOUT, EIGHT> first, second;
         first.load(a, e0);
         second.load(a, e0 + ADAMW_CHUNK / 2);
-        first.step(a, e0, h, rate[i], inverse[i], keys[i]);
-        second.step(a, e0 + ADAMW_CHUNK / 2, h, rate[i], inverse[i], keys[i]);
+        if (EIGHT) {
+          // one copy of the code, which is bound by instructions (128 M bf16 values: 370 -> 352 us)
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            first.step(a, e0 + half * (ADAMW_CHUNK / 2), h, rate[i], inverse[i], keys[i]);
+            first = second;
+          }
+        } else {
+          // bound by memory; the stores of one half then lie beside the other's arithmetic (96 M with masters: 546 -> 511 us)
+          first.step(a, e0, h, rate[i], inverse[i], keys[i]);
+          second.step(a, e0 + ADAMW_CHUNK / 2, h, rate[i], inverse[i], keys[i]);
+        }
         continue;
       }
     }
