@@ -35,6 +35,7 @@ constexpr int STREAM_THREADS = 1024;      // forward: 64 registers
 constexpr int STREAM_BACK_THREADS = 512;  // backward: 128, 64 of them sums of dw and db
 static_assert(STREAM_THREADS / 64 <= 16 && STREAM_BACK_THREADS / 64 <= 15, "a barrier for every team of more than a warp");
 constexpr int STREAM_SMEM = 226 << 10;
+constexpr int SHIFTED_THREADS = 768, SHIFTED_STAGES = 3;  // the same for rows off 16-byte boundaries (forward; a stage is being filled)
 
 template <typename T>
 constexpr int VALUES = 16 / static_cast<int>(sizeof(T));  // of a chunk
@@ -666,6 +667,275 @@ layer_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict_
   }
 }
 
+// ---- many rows off 16-byte boundaries -----------------------------------------------------------------------------------
+//
+// Rows of odd width start anywhere. Read value by value they took ten times as long as their bytes (4093 x 2051 fp16: 48 us
+// forward, 80 backward). Here the 16-byte pieces that cover a row are copied to shared memory as they lie, and values are taken from there: a
+// thread has pairs of neighbours (fp32: single values), side by side with its neighbours' pairs, out of two words and a shift where
+// the row starts in the middle of one. What a piece has beside the row belongs to rows or allocations beside it and is not
+// looked at (a 16-byte piece never lies in two pages). A thread reads what others copied, so a team also meets before a
+// row; that it then is past the row before frees that row's place for the next fetch.
+
+// What a thread has of a row: PAIRS pairs of values, and how they lie.
+template <typename T>
+struct Shifted {
+  static constexpr int PAIRS = STREAM_CHUNKS * VALUES<T> / 2;
+  int t, team, D;
+  int firsts, seconds;  // pairs whose first, and whose second value is in the row
+
+  __device__ __forceinline__ Shifted(int t_, int team_, int D_) : t(t_), team(team_), D(D_) {
+    const int d = 2 * team;  // from a thread's pair to its next
+    const int a = first(0), b = second(0);
+    firsts = a < D ? (D - a + d - 1) / d : 0;
+    seconds = b < D ? (D - b + d - 1) / d : 0;
+  }
+  __device__ __forceinline__ int first(int k) const { return sizeof(T) == 2 ? 2 * (k * team + t) : 2 * k * team + t; }
+  __device__ __forceinline__ int second(int k) const { return sizeof(T) == 2 ? first(k) + 1 : first(k) + team; }
+
+  // row: shared address of the row's first value
+  __device__ __forceinline__ float2 read(uint32_t row, int k) const {
+    if constexpr (sizeof(T) == 4) {
+      return make_float2(read_word_as_float(row + first(k) * 4), read_word_as_float(row + second(k) * 4));
+    } else {
+      const uint32_t at = row + first(k) * 2, word = at & ~3u;
+      const uint32_t both_values = __funnelshift_r(read_word(word), read_word(word + 4), (at & 2u) * 8);
+      if constexpr (std::is_same<T, bf16>::value) {
+        return make_float2(__uint_as_float(both_values << 16), __uint_as_float(both_values & 0xffff0000u));
+      } else {
+        return __half22float2(*reinterpret_cast<const __half2*>(&both_values));
+      }
+    }
+  }
+  // of a vector in fp32
+  __device__ __forceinline__ float2 read_vector(uint32_t vector, int k) const {
+    if constexpr (sizeof(T) == 4) {
+      return make_float2(read_word_as_float(vector + first(k) * 4), read_word_as_float(vector + second(k) * 4));
+    } else {
+      float2 v;
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(vector + first(k) * 4) : "memory");
+      return v;
+    }
+  }
+  __device__ __forceinline__ void write(T* row, int k, float2 v, bool words) const {
+    const int a = first(k), b = second(k);
+    if constexpr (sizeof(T) == 2) {
+      if (words && k < seconds) {
+        const T pair[2] = {from_float<T>(v.x), from_float<T>(v.y)};
+        *reinterpret_cast<uint32_t*>(row + a) = *reinterpret_cast<const uint32_t*>(pair);
+        return;
+      }
+    }
+    if (k < firsts) row[a] = from_float<T>(v.x);
+    if (k < seconds) row[b] = from_float<T>(v.y);
+  }
+  __device__ __forceinline__ float2 inside(int k, float2 v) const {  // zero past the row's end
+    return make_float2(k < firsts ? v.x : 0.0f, k < seconds ? v.y : 0.0f);
+  }
+
+  __device__ __forceinline__ static uint32_t read_word(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+  }
+  __device__ __forceinline__ static float read_word_as_float(uint32_t at) { return __uint_as_float(read_word(at)); }
+
+  // copies the pieces that cover `row` to shared memory from `to` on; the row's first value then lies (address of row) % 16
+  // further
+  __device__ __forceinline__ void fetch(uint32_t to, const T* row, bool any) const {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(row), end = begin + D * sizeof(T), from = begin & ~static_cast<uintptr_t>(15);
+#pragma unroll
+    for (int c = 0; c < STREAM_CHUNKS; ++c) {
+      const uintptr_t piece = from + (c * team + t) * 16;
+      copy_async_16(to + (c * team + t) * 16, reinterpret_cast<const void*>(piece), any && piece < end, reinterpret_cast<const void*>(from));
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t phase(const T* row) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15);
+}
+
+// every thread of a team, for what the others wrote to shared memory
+__device__ __forceinline__ void team_meet(int barrier, int team) {
+  if (team > 32) {
+    team_barrier(barrier + threadIdx.x / team, team);
+  } else {
+    __syncwarp();
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SHIFTED_THREADS, 1)
+layer_norm_forward_shifted_kernel(const T* __restrict__ x, long long stride, const void* __restrict__ weight, int w_type,
+                                  const void* __restrict__ bias, int b_type, long long rows, int D, float eps, int team,
+                                  T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+  extern __shared__ __align__(16) float scale[];  // weight, bias, ring
+  __shared__ float part[2][1][32];
+  constexpr int S = SHIFTED_STAGES, PAIRS = Shifted<T>::PAIRS;
+  const Shifted<T> at(static_cast<int>(threadIdx.x) % team, team, D);
+  const int room = team * STREAM_CHUNKS * VALUES<T>;
+  for (int c = threadIdx.x; c < room; c += blockDim.x) {
+    scale[c] = weight != nullptr && c < D ? load1_as(weight, w_type, c) : 1.0f;
+    scale[room + c] = bias != nullptr && c < D ? load1_as(bias, b_type, c) : 0.0f;
+  }
+  const uint32_t my_scale = smem_u32(scale), my_shift = smem_u32(scale + room);
+  const int teams = blockDim.x / team;
+  const uint32_t row_bytes = team * STREAM_CHUNKS * 16, ring = smem_u32(scale + 2 * room) + threadIdx.x / team * S * row_bytes;
+  const float width = static_cast<float>(D), inv = 1.0f / width;
+  const long long first = static_cast<long long>(blockIdx.x) * teams + threadIdx.x / team, step = static_cast<long long>(gridDim.x) * teams;
+  const Trips trips(rows, first, step, team);
+  const T *source = x + first * stride, *here_source = source;
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) {
+    at.fetch(ring + s * row_bytes, s < trips.mine ? source : x, s < trips.mine);
+    copy_async_commit();
+    source += step * stride;
+  }
+  __syncthreads();
+  uint32_t here = ring, free = ring + (S - 1) * row_bytes;
+  T* out = y + first * D;
+  for (int k = 0; k < trips.all; ++k, out += step * D, here_source += step * stride) {
+    copy_async_wait<S - 2>();
+    team_meet(0, team);
+    at.fetch(free, k + S - 1 < trips.mine ? source : x, k + S - 1 < trips.mine);
+    copy_async_commit();
+    source += step * stride;
+    const uint32_t row = here + phase(here_source);
+    free = here;
+    here = here == ring + (S - 1) * row_bytes ? ring : here + row_bytes;
+    float2 v[PAIRS], s2 = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) {
+      v[j] = at.inside(j, at.read(row, j));
+      s2 = add2(s2, v[j]);
+    }
+    float s[1] = {s2.x + s2.y};
+    own_team_sum<0>(s, team, part[0]);
+    const float mu = quotient(s[0], width, inv);
+    s2 = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) {
+      v[j] = at.inside(j, add2(v[j], both(-mu)));
+      s2 = fma2(v[j], v[j], s2);
+    }
+    s[0] = s2.x + s2.y;
+    own_team_sum<0>(s, team, part[1]);
+    const float r = rsqrtf(fmaf(s[0], inv, eps));
+    if (k >= trips.mine) continue;
+    if (at.t == 0 && mean != nullptr) {
+      mean[first + k * step] = mu;
+      rstd[first + k * step] = r;
+    }
+    const bool words = phase(out) % 4 == 0;
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) {
+      at.write(out, j, fma2(mul2(v[j], both(r)), at.read_vector(my_scale, j), at.read_vector(my_shift, j)), words);
+    }
+  }
+  copy_async_wait<0>();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(STREAM_BACK_THREADS, 1)
+layer_norm_backward_shifted_kernel(const T* __restrict__ dy, const T* __restrict__ x, long long stride,
+                                   const void* __restrict__ weight, int w_type, const float* __restrict__ mean,
+                                   const float* __restrict__ rstd, long long rows, int D, int team, T* __restrict__ dx,
+                                   float* __restrict__ part_w, float* __restrict__ part_b) {
+  extern __shared__ __align__(16) float scale[];  // weight, ring; the ring's place then holds the teams' sums
+  __shared__ float part[2][2][32];
+  constexpr int S = SHIFTED_STAGES, PAIRS = Shifted<T>::PAIRS;
+  const Shifted<T> at(static_cast<int>(threadIdx.x) % team, team, D);
+  const int room = team * STREAM_CHUNKS * VALUES<T>;
+  for (int c = threadIdx.x; c < room; c += blockDim.x) scale[c] = weight != nullptr && c < D ? load1_as(weight, w_type, c) : 1.0f;
+  const uint32_t my_scale = smem_u32(scale);
+  const int teams = blockDim.x / team;
+  const uint32_t row_bytes = team * STREAM_CHUNKS * 16, ring = smem_u32(scale + room) + threadIdx.x / team * S * 2 * row_bytes;
+  const float inv = 1.0f / static_cast<float>(D);
+  const long long first = static_cast<long long>(blockIdx.x) * teams + threadIdx.x / team, step = static_cast<long long>(gridDim.x) * teams;
+  const Trips trips(rows, first, step, team);
+  const T *source = x + first * stride, *source_dy = dy + first * D, *here_source = source, *here_dy = source_dy;
+  auto fetch = [&](int k, uint32_t to) {
+    at.fetch(to, k < trips.mine ? source : x, k < trips.mine);
+    at.fetch(to + row_bytes, k < trips.mine ? source_dy : x, k < trips.mine);
+    copy_async_commit();
+    source += step * stride;
+    source_dy += step * D;
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(s, ring + s * 2 * row_bytes);
+  __syncthreads();
+  float2 aw[PAIRS], ab[PAIRS];
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) aw[j] = ab[j] = both(0.0f);
+  uint32_t here = ring, free = ring + (S - 1) * 2 * row_bytes;
+  int parity = 0;
+  const float *mean_next = mean + first, *rstd_next = rstd + first;
+  float mu_next = 0.0f, r_next = 0.0f;
+  if (trips.mine > 0) mu_next = *mean_next, r_next = *rstd_next;
+  T* out = dx + first * D;
+  for (int k = 0; k < trips.all; ++k, parity ^= 1, out += step * D, here_source += step * stride, here_dy += step * D) {
+    // a row past the end has r = 0 and dy = 0: nothing in any sum
+    const float r = r_next, base = -mu_next * r_next;
+    mu_next = r_next = 0.0f;
+    mean_next += step;
+    rstd_next += step;
+    if (k + 1 < trips.mine) mu_next = *mean_next, r_next = *rstd_next;
+    copy_async_wait<S - 2>();
+    team_meet(1, team);
+    fetch(k + S - 1, free);
+    const bool mine = k < trips.mine;
+    const uint32_t row = here + (mine ? phase(here_source) : 0), row_dy = here + row_bytes + (mine ? phase(here_dy) : 0);
+    free = here;
+    here = here == ring + (S - 1) * 2 * row_bytes ? ring : here + 2 * row_bytes;
+    float2 s0 = both(0.0f), s1 = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) {
+      const float2 xh = fma2(at.inside(j, at.read(row, j)), both(r), both(base));
+      float2 g = at.inside(j, at.read(row_dy, j));
+      aw[j] = fma2(g, xh, aw[j]);
+      ab[j] = add2(ab[j], g);
+      g = mul2(g, at.read_vector(my_scale, j));
+      s0 = add2(s0, g);
+      s1 = fma2(g, xh, s1);
+    }
+    float s[2] = {s0.x + s0.y, s1.x + s1.y};
+    own_team_sum<1>(s, team, part[parity]);
+    if (dx == nullptr || !mine) continue;
+    const float2 c1 = both(-r * (s[0] * inv)), c2 = both(-r * (s[1] * inv));
+    const bool words = phase(out) % 4 == 0;
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) {
+      const float2 xh = fma2(at.read(row, j), both(r), both(base)), g = mul2(at.read(row_dy, j), at.read_vector(my_scale, j));
+      at.write(out, j, fma2(xh, c2, fma2(g, both(r), c1)), words);
+    }
+  }
+  copy_async_wait<0>();
+  if (part_w == nullptr && part_b == nullptr) return;
+  __syncthreads();
+  // [team][weight, bias][pair][thread]
+  float2* sums = reinterpret_cast<float2*>(scale + room);
+  const int count = PAIRS * team;
+  float2* my_sums = sums + threadIdx.x / team * 2 * count + at.t;
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) {
+    my_sums[j * team] = aw[j];
+    my_sums[count + j * team] = ab[j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * count; i += blockDim.x) {
+    float* out_row = i < count ? part_w : part_b;
+    if (out_row == nullptr) continue;
+    float2 total = sums[i];
+    for (int n = 1; n < teams; ++n) total = add2(total, sums[n * 2 * count + i]);
+    const int j = (i < count ? i : i - count) / team;
+    const Shifted<T> of(i % team, team, D);
+    float* to = out_row + static_cast<long long>(blockIdx.x) * D;
+    if (j < of.firsts) to[of.first(j)] = total.x;
+    if (j < of.seconds) to[of.second(j)] = total.y;
+  }
+}
+
 // out[col] = sum over p of parts[p][col], in an order that depends on the number of parts alone: 32 columns a block, eight
 // warps that take every eighth part. blockIdx.y: weight or bias.
 __global__ void __launch_bounds__(256)
@@ -724,10 +994,10 @@ int backward_blocks(int64_t rows, int D, int type) {
   return static_cast<int>(want < cap ? (want > 0 ? want : 1) : cap);
 }
 
-// The streaming kernels' team and block: as many whole teams as fit.
-NormShape stream_shape(int D, int type, int most) {
+// The streaming kernels' team and block: as many whole teams as fit. Rows off 16-byte boundaries lie in one piece more.
+NormShape stream_shape(int D, int type, int most, bool vec) {
   const int values = 16 / type_bytes(type);
-  const int pieces = (D + values - 1) / values;
+  const int pieces = (D + values - 1 + (vec ? 0 : values - 1)) / values;
   NormShape s;
   s.chunks = STREAM_CHUNKS;
   s.team = 1;
@@ -739,49 +1009,51 @@ NormShape stream_shape(int D, int type, int most) {
 }
 
 // Shared memory: `vectors` fp32 vectors of the row's width, and the ring of `stages` times `inputs` rows a team, or at least
-// the sums that lie in its place in the end.
+// the sums that lie in its place in the end; and 16 bytes, for the word past a value in the ring's last row.
 int stream_smem(const NormShape& s, int type, int vectors, int inputs, int stages, int least) {
   const int ring = stages * inputs * STREAM_CHUNKS * s.threads * 16;
-  return vectors * s.team * STREAM_CHUNKS * (16 / type_bytes(type)) * static_cast<int>(sizeof(float)) + (ring > least ? ring : least);
+  return vectors * s.team * STREAM_CHUNKS * (16 / type_bytes(type)) * static_cast<int>(sizeof(float)) + (ring > least ? ring : least) + 16;
 }
 
 // A ring pays where a team has several rows to go through.
-bool streams(int64_t rows, const NormShape& s, int smem, bool vec) {
-  return vec && s.teams > 0 && smem <= STREAM_SMEM && rows > 2ll * num_sms() * s.teams && rows < 1ll << 31;
+bool streams(int64_t rows, const NormShape& s, int smem) {
+  return s.teams > 0 && smem <= STREAM_SMEM && rows > 2ll * num_sms() * s.teams && rows < 1ll << 31;
+}
+
+// `kernel` with STREAM_SMEM allowed, once for a device
+template <typename K>
+bool allow_stream_smem(K kernel, PerDevice& room) {
+  return room.get([&] {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    return 1;
+  }) > 0;
 }
 
 template <typename T>
-int forward_stream(const void* x, int64_t stride, const void* w, int w_type, const void* b, int b_type, int64_t rows, int D,
+int forward_stream(bool vec, const void* x, int64_t stride, const void* w, int w_type, const void* b, int b_type, int64_t rows, int D,
                    float eps, const NormShape& s, int smem, void* y, float* mean, float* rstd, cudaStream_t stream) {
-  static PerDevice room;
-  const int allowed = room.get([&] {
-    if (cudaFuncSetAttribute(layer_norm_forward_stream_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SMEM) != cudaSuccess) {
-      cudaGetLastError();
-      return 0;
-    }
-    return STREAM_SMEM;
-  });
-  if (smem > allowed) return FFM_ERR_LAUNCH;
-  layer_norm_forward_stream_kernel<T><<<num_sms(), s.threads, smem, stream>>>(static_cast<const T*>(x), stride, w, w_type, b, b_type,
-                                                                             rows, D, eps, s.team, static_cast<T*>(y), mean, rstd);
+  static PerDevice room[2];
+  auto kernel = vec ? layer_norm_forward_stream_kernel<T> : layer_norm_forward_shifted_kernel<T>;
+  if (!allow_stream_smem(kernel, room[vec])) return FFM_ERR_LAUNCH;
+  kernel<<<num_sms(), s.threads, smem, stream>>>(static_cast<const T*>(x), stride, w, w_type, b, b_type, rows, D, eps, s.team,
+                                                 static_cast<T*>(y), mean, rstd);
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
 
-template <typename T, int S>
-int backward_stream(const void* dy, const void* x, int64_t stride, const void* w, int w_type, const float* mean, const float* rstd,
+// stages: 0 for rows off 16-byte boundaries
+template <typename T>
+int backward_stream(int stages, const void* dy, const void* x, int64_t stride, const void* w, int w_type, const float* mean, const float* rstd,
                     int64_t rows, int D, const NormShape& s, int smem, void* dx, float* part_w, float* part_b, cudaStream_t stream) {
-  static PerDevice room;
-  const int allowed = room.get([&] {
-    if (cudaFuncSetAttribute(layer_norm_backward_stream_kernel<T, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SMEM) != cudaSuccess) {
-      cudaGetLastError();
-      return 0;
-    }
-    return STREAM_SMEM;
-  });
-  if (smem > allowed) return FFM_ERR_LAUNCH;
-  layer_norm_backward_stream_kernel<T, S><<<num_sms(), s.threads, smem, stream>>>(
-      static_cast<const T*>(dy), static_cast<const T*>(x), stride, w, w_type, mean, rstd, rows, D, s.team, static_cast<T*>(dx), part_w,
-      part_b);
+  static PerDevice room[3];
+  auto kernel = stages == 0                    ? layer_norm_backward_shifted_kernel<T>
+                : stages == STREAM_BACK_STAGES ? layer_norm_backward_stream_kernel<T, STREAM_BACK_STAGES>
+                                               : layer_norm_backward_stream_kernel<T, STREAM_STAGES>;
+  if (!allow_stream_smem(kernel, room[stages == 0 ? 0 : (stages == STREAM_BACK_STAGES ? 1 : 2)])) return FFM_ERR_LAUNCH;
+  kernel<<<num_sms(), s.threads, smem, stream>>>(static_cast<const T*>(dy), static_cast<const T*>(x), stride, w, w_type, mean, rstd, rows, D,
+                                                 s.team, static_cast<T*>(dx), part_w, part_b);
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
 
@@ -863,11 +1135,12 @@ extern "C" int ffm_layer_norm_forward(const void* x, int x_type, int64_t rows, i
   if (rows == 0) return FFM_OK;
   if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return FFM_ERR_BAD_ARG;
   const NormShape s = norm_shape(D, x_type);
-  const NormShape r = stream_shape(D, x_type, STREAM_THREADS);
-  const int smem = stream_smem(r, x_type, 2, 1, STREAM_STAGES, 0);
-  if (streams(rows, r, smem, norm_vectors(x_type, row_stride, D, x, y))) {
+  const bool vec = norm_vectors(x_type, row_stride, D, x, y);
+  const NormShape r = stream_shape(D, x_type, vec ? STREAM_THREADS : SHIFTED_THREADS, vec);
+  const int smem = stream_smem(r, x_type, 2, 1, vec ? STREAM_STAGES : SHIFTED_STAGES, 0);
+  if (streams(rows, r, smem)) {
     return with_type(x_type, [&](auto tag) {
-      return forward_stream<decltype(tag)>(x, row_stride, weight, w_type, bias, b_type, rows, D, eps, r, smem, y, mean, rstd,
+      return forward_stream<decltype(tag)>(vec, x, row_stride, weight, w_type, bias, b_type, rows, D, eps, r, smem, y, mean, rstd,
                                            static_cast<cudaStream_t>(stream));
     });
   }
@@ -894,19 +1167,21 @@ extern "C" int ffm_layer_norm_backward(const void* dy, const void* x, int x_type
   if (parts && (workspace == nullptr || workspace_bytes < ffm_layer_norm_workspace_bytes(rows, D, x_type))) return FFM_ERR_WORKSPACE;
   if (!parts && (dx == nullptr || rows == 0)) return FFM_OK;
   const NormShape s = norm_shape(D, x_type);
-  const NormShape r = stream_shape(D, x_type, STREAM_BACK_THREADS);
+  const bool vectors = norm_vectors(x_type, row_stride, D, dy, x, dx);
+  const NormShape r = stream_shape(D, x_type, STREAM_BACK_THREADS, vectors);
   const int sums = r.threads * STREAM_CHUNKS * (16 / type_bytes(x_type)) * 2 * static_cast<int>(sizeof(float));
-  int smem = stream_smem(r, x_type, 1, 2, STREAM_BACK_STAGES, sums);
-  const bool deep = smem <= STREAM_SMEM;
-  if (!deep) smem = stream_smem(r, x_type, 1, 2, STREAM_STAGES, sums);
-  const bool vectors = norm_vectors(x_type, row_stride, D, dy, x, dx), stream_rows = streams(rows, r, smem, vectors);
+  int stages = vectors ? STREAM_BACK_STAGES : 0, smem = stream_smem(r, x_type, 1, 2, vectors ? STREAM_BACK_STAGES : SHIFTED_STAGES, sums);
+  if (vectors && smem > STREAM_SMEM) {
+    stages = STREAM_STAGES;
+    smem = stream_smem(r, x_type, 1, 2, STREAM_STAGES, sums);
+  }
+  const bool stream_rows = streams(rows, r, smem);
   const int blocks = stream_rows ? num_sms() : backward_blocks(rows, D, x_type);
   float* part_w = dweight != nullptr ? static_cast<float*>(workspace) : nullptr;
   float* part_b = dbias != nullptr ? static_cast<float*>(workspace) + static_cast<size_t>(blocks) * D : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = stream_rows ? with_type(x_type, [&](auto tag) {
-    return (deep ? backward_stream<decltype(tag), STREAM_BACK_STAGES> : backward_stream<decltype(tag), STREAM_STAGES>)(
-        dy, x, row_stride, weight, w_type, mean, rstd, rows, D, r, smem, dx, part_w, part_b, st);
+    return backward_stream<decltype(tag)>(stages, dy, x, row_stride, weight, w_type, mean, rstd, rows, D, r, smem, dx, part_w, part_b, st);
   }) : dispatch_norm(x_type, s, vectors, [&](auto tag, auto ch, auto vec, auto threads) {
     return backward_as<decltype(tag), decltype(ch)::value, decltype(vec)::value, decltype(threads)::value>(
         dy, x, row_stride, weight, w_type, mean, rstd, rows, D, s, dx, part_w, part_b, blocks, st);

@@ -80,7 +80,7 @@ def test_forward_and_backward(width, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("width", [8, 64, 256, 264, 1024, 1400, 4096, 8192])
+@pytest.mark.parametrize("width", [8, 64, 256, 264, 1024, 1400, 4096, 8192, 1, 2, 9, 33, 127, 255, 257, 511, 1023, 2051, 4099, 7001])
 def test_many_rows(width, dtype):
     """More rows than the device has teams for: several of them one after the other, the last round not full."""
     rows = 148 * 1024 // min(1024, max(1, width // 32)) * 3 + 5
@@ -94,9 +94,11 @@ def test_many_rows(width, dtype):
 
 
 @pytest.mark.gpu
-def test_many_rows_with_a_distance():
-    base = torch.randn(9000, 1040, device="cuda").bfloat16()
-    x, (_, w, b, dy) = base[:, 8:1032], inputs(9000, 1024, torch.bfloat16, 21)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("room,start", [(1040, 8), (1040, 1), (1037, 5), (1025, 0), (1026, 2)])
+def test_many_rows_with_a_distance(room, start, dtype):
+    base = torch.randn(9000, room, device="cuda").to(dtype)
+    x, (_, w, b, dy) = base[:, start:start + 1024], inputs(9000, 1024, dtype, 21)
     out, bound = reference(x, w, b, 1e-5, dy)
     y, (dx, dw, db) = run(x, w, b, dy)
     for got, name in ((y, "y"), (dx, "dx"), (dw, "dw"), (db, "db")):
