@@ -292,7 +292,8 @@ LossResult loss_pass(const Tensor& hidden, const Tensor& weight, const Tensor& t
   a.z = call.z;
   a.piece_rows = call.piece_rows;
   if (a.piece_rows <= 0) {
-    const int64_t row_bytes = (a.V + 63) / 64 * 128, most = std::max<int64_t>(PIECE_BYTES / row_bytes / 256 * 256, 256);
+    // two bytes an entry, or without gradients (8 bytes for 128 entries) as many rows as would take a quarter of it
+    const int64_t row_bytes = want_hidden || want_weight ? (a.V + 63) / 64 * 128 : (a.V + 127) / 128 * 32, most = std::max<int64_t>(PIECE_BYTES / row_bytes / 256 * 256, 256);
     const int64_t pieces = std::max<int64_t>((a.N + most - 1) / most, 1);
     a.piece_rows = std::max<int64_t>(((a.N + pieces - 1) / pieces + 255) / 256 * 256, 256);
   }

@@ -441,7 +441,7 @@ Layout lay_out(const ffm_loss_args& a) {
   const int64_t n = a.piece_rows < a.N ? a.piece_rows : a.N;
   const bool grads = a.d_hidden != nullptr || a.d_weight != nullptr;
   l.pieces = static_cast<int>((a.V + HALF - 1) / HALF);
-  l.few = grads ? Few{} : few_rows(a.N, static_cast<int>(a.D), static_cast<int>(a.V));
+  l.few = grads || n < a.N ? Few{} : few_rows(n, static_cast<int>(a.D), static_cast<int>(a.V));
   if (l.few.tiles > 0) l.pieces = l.few.pieces;
   l.ld = (a.V + 63) / 64 * 64;
   l.splits = a.d_hidden != nullptr ? contraction_splits(n, static_cast<int>(a.D), static_cast<int>(a.V)) : 1;
@@ -451,7 +451,7 @@ Layout lay_out(const ffm_loss_args& a) {
     end += (bytes + 255) / 256 * 256;
     return here;
   };
-  const int64_t rows = grads ? n : a.N;
+  const int64_t rows = n;
   l.share = next(4);
   l.target_logits = next(rows * 4);
   l.stats = next(rows * l.pieces * 8);
@@ -508,7 +508,7 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
     if ((rc = launch_ok()) != FFM_OK) return rc;
     ++launched;
   }
-  const int64_t step = grads ? (a.piece_rows < a.N ? a.piece_rows : a.N) : a.N;
+  const int64_t step = a.piece_rows < a.N ? a.piece_rows : a.N;
   for (int64_t r0 = 0; r0 < a.N; r0 += step) {
     const int64_t n = a.N - r0 < step ? a.N - r0 : step;
     const char* hidden = static_cast<const char*>(a.hidden) + r0 * a.D * 2;

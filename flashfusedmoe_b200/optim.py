@@ -7,6 +7,10 @@ from . import _lib
 BLOCK = 128   # values of a tensor that share a scale in an 8-bit state
 
 
+def _capturing(tensors):
+    return bool(tensors) and tensors[0].is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, masters=None,
                exp_avg_scales=None, exp_avg_sq_scales=None, grad_scale=None, seed=0):
     """One AdamW step of the tensors in `params`, in place: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
@@ -24,7 +28,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     device, which a captured step reads at every replay. Everything runs on the current stream without a host wait and can be
     captured."""
     _lib.native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, masters, exp_avg_scales, exp_avg_sq_scales, lr, betas[0],
-                             betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF, torch.cuda.is_current_stream_capturing())
+                             betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF, _capturing(params))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -52,7 +56,7 @@ class AdamW(torch.optim.Optimizer):
     def _state_of(self, p, group):
         state = self.state[p]
         if not state:
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing([p]):
                 raise RuntimeError("a parameter's first AdamW step makes its state and cannot be captured: take one step before")
             state["step"] = torch.zeros((), dtype=torch.int32, device=p.device)
             if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]:

@@ -568,8 +568,8 @@ int ffm_adamw_step(const ffm_adamw_tensor* tensors, int count, const ffm_adamw_a
  *   loss (null: not wanted): the sum, or the mean, of nll.
  *   d_hidden bf16 [N, D], d_weight [V, D] in bf16 or (d_weight_f32) fp32, null where not wanted: the gradients of
  *     loss, or with row_grad (f32 [N], mean = 0) of the sum of row_grad[n] nll[n].
- *   piece_rows: with gradients, so many rows at a time have their V entries in the workspace (2 bytes each). With fewer than N the
- *     gradient of the weight is summed over the pieces in fp32.
+ *   piece_rows: so many rows at a time are worked on. The workspace has 8 bytes for 128 entries of each, and with gradients 2 bytes
+ *     an entry. With fewer than N the gradient of the weight is summed over the pieces in fp32.
  *   workspace: ffm_linear_cross_entropy_workspace_bytes of the same block (pointers only have to be null or not).
  *   status_host (null, or host memory the device can write): a non-zero *status is stored there.
  *   launched (null or host): kernels enqueued are added.

@@ -134,6 +134,11 @@ def test_pieces_of_rows(dtype):
     check(dw, out, bound, "dw")
     whole = run(h, w, t)
     assert torch.equal(loss, whole[0]) and torch.equal(dh.bfloat16(), whole[1])
+    from flashfusedmoe_b200 import linear_cross_entropy
+    with torch.no_grad():
+        nll = linear_cross_entropy(h, w, t, reduction="none")
+        assert torch.equal(linear_cross_entropy(h, w, t, reduction="none", _piece_rows=256), nll)
+        check(nll, out, bound, "nll")
 
 
 @pytest.mark.gpu
