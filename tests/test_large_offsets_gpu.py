@@ -66,7 +66,11 @@ def test_a_weight_of_the_vocabulary():
     h, w, t = entropy.inputs(8192, 64, 300000, seed=1)
     loss, dh, dw = entropy.run(h, w, t, _piece_rows=8192)
     other = entropy.run(h, w, t, _piece_rows=256)
-    assert torch.equal(loss, other[0]) and torch.equal(dh, other[1])
+    assert torch.equal(loss, other[0])
+    # the contraction over the vocabulary is split differently: each sum is off by (V / 16 + 20) 2^-22 of the terms' magnitudes,
+    # which are at most 2 / 8192 in all times the largest weight, and half a unit of bf16
+    off = (dh.double() - other[1].double()).abs()
+    assert (off <= 2.0 ** -7 * dh.double().abs() + 2 * (300000 / 16 + 20) * 2.0 ** -22 * 2 / 8192 * w.double().abs().max()).all()
     # one sum in fp32 of 8192 terms against 32 sums of 256: each off by less than 2^-13 of the terms' magnitudes, which here is a
     # few times the result; then half a unit of bf16 each
     off = (dw.double() - other[2].double()).abs()
