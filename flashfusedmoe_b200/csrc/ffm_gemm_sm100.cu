@@ -61,7 +61,7 @@ constexpr int SMEM_CTRL_BYTES = 2048;
 constexpr int MAX_STAGES = 6;
 constexpr int SMEM_LIMIT = 232448;  // 227 KiB of dynamic shared memory per CTA
 
-enum { EPI_PLAIN = 0, EPI_GLU = 1, EPI_GLUBWD = 2, EPI_SOFTMAX = 3, EPI_F32 = 4 };
+enum { EPI_PLAIN = 0, EPI_GLU = 1, EPI_GLUBWD = 2, EPI_SOFTMAX = 3, EPI_F32 = 4, EPI_SCALED = 5 };
 // The GLU epilogues get a second warp per TMEM lane quarter (helper warps 6..9, each taking the upper 32 columns of
 // every 64-column step). The GLU backward does about 16 instructions and two MUFU operations per accumulator element,
 // too much for one warp per scheduler inside a tile's main loop (0.174 -> 0.164 ms at 8 x 4096 rows, D 1024, H 2048);
@@ -118,7 +118,7 @@ struct Shape {
   static constexpr int BOXES_PER_STEP = EPI == EPI_GLU ? 3 : (EPI == EPI_GLUBWD || EPI == EPI_SOFTMAX ? 2 : 1);
   static constexpr int STEPS_BUFFERED = EPI == EPI_GLU      ? (CTA2 ? FFM_TUNE_PG_STEPS : 1)
                                         : EPI == EPI_GLUBWD ? (CTA2 ? FFM_TUNE_GB_STEPS : 2)
-                                        : EPI == EPI_PLAIN  ? (CTA2 ? FFM_TUNE_PP_STEPS : 2)
+                                        : EPI == EPI_PLAIN || EPI == EPI_SCALED ? (CTA2 ? FFM_TUNE_PP_STEPS : 2)
                                                             : 2;
   static constexpr int STG_WARP_BYTES = BOXES_PER_STEP * STEPS_BUFFERED * BOX_BYTES;
   static constexpr int STG_BYTES = EPI_WARPS * STG_WARP_BYTES;
@@ -167,13 +167,15 @@ __device__ __forceinline__ const float* fp8_b_scale(const GemmParams& p) {
 }
 // EPI_SOFTMAX has no passenger either and keeps what it needs in the same fields: pz_rows rows, pz_h vocabulary entries, a
 // target per row, the target's logit to be written, and a (maximum, sum) for every 128 entries of a row, side by side. has_c2: the exponentials are
-// stored. EPI_F32: has_c2 says whether the result is added to what is there.
+// stored. EPI_SCALED is EPI_PLAIN with a factor on the device, in pz_dact; EPI_F32 has one there or none, and has_c2 says whether
+// the result is added to what is there.
 __device__ __forceinline__ const long long* softmax_targets(const GemmParams& p) {
   return reinterpret_cast<const long long*>(p.pz_dact);
 }
 __device__ __forceinline__ float* softmax_target_logits(const GemmParams& p) {
   return reinterpret_cast<float*>(const_cast<bf16*>(p.pz_pre));
 }
+__device__ __forceinline__ const float* device_scale(const GemmParams& p) { return reinterpret_cast<const float*>(p.pz_dact); }
 __device__ __forceinline__ float2* softmax_stats(const GemmParams& p) { return reinterpret_cast<float2*>(p.pz_gu); }
 
 struct Ctrl {
@@ -986,6 +988,7 @@ ffm_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // eight steps of 32 columns (one box of fp32 each), TMEM loads one step ahead; stored, or added to what is there by the
         // memory system (one launch adds to an element once, so that the order of launches is the order of the additions)
         const int n0 = t.n_block * BN;
+        const float scale = device_scale(p) != nullptr ? __ldg(device_scale(p)) : 1.0f;
         uint32_t v[2][32];
         if (have_acc) tmem_ld_32x32(taddr, v[0]);
 #pragma unroll
@@ -995,6 +998,8 @@ ffm_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             if (c + 1 < BN / 32) tmem_ld_32x32(taddr + (c + 1) * 32, v[(c + 1) & 1]);
           }
           if (n0 + c * 32 >= p.n_cols) continue;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[c & 1][i] = __float_as_uint(__uint_as_float(v[c & 1][i]) * scale);
           const uint32_t box = stg + step_slot * STEP_BYTES;
           if (lane == 0) bulk_wait_read<S::STEPS_BUFFERED - 1>();
           __syncwarp();
@@ -1021,7 +1026,7 @@ ffm_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       } else {
         // four steps of 64 columns (one box each), two 32-column chunks per step, TMEM loads one chunk ahead
         const int n0 = t.n_block * BN;
-        const float scale = FP8 ? p.scale * fp8_scale : p.scale;
+        const float scale = FP8 ? p.scale * fp8_scale : (EPI == EPI_SCALED ? __ldg(device_scale(p)) : p.scale);
         uint32_t v[2][32];
         if (have_acc) tmem_ld_32x32(taddr, v[0]);
 #pragma unroll
@@ -1566,8 +1571,8 @@ int ffm::softmax_logits(const void* hidden, const void* weight, int64_t rows, in
                                            static_cast<cudaStream_t>(stream), rows <= BM ? 128 : 0);
 }
 
-int ffm::dense_rows(const void* A, int64_t ld_a, int64_t rows, int K, const void* B, int Nout, int splits, void* out,
-                    int32_t* status, ffm_stream_t stream) {
+int ffm::dense_rows(const void* A, int64_t ld_a, int64_t rows, int K, const void* B, int Nout, int splits, const float* scale,
+                    void* out, int32_t* status, ffm_stream_t stream) {
   CUtensorMap tmA, tmB, tmC;
   int rc;
   if ((rc = make_ld_map(&tmA, A, rows, K, ld_a, 64, 128)) != FFM_OK) return rc;
@@ -1581,6 +1586,7 @@ int ffm::dense_rows(const void* A, int64_t ld_a, int64_t rows, int K, const void
   p.status = status;
   p.wait_cycles = g_wait_cycles;
   p.b_group_rows = K;
+  p.pz_dact = reinterpret_cast<const bf16*>(scale);
   const int m_tiles = static_cast<int>((rows + BM - 1) / BM);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (splits > 1) {
@@ -1590,11 +1596,12 @@ int ffm::dense_rows(const void* A, int64_t ld_a, int64_t rows, int K, const void
   }
   p.dense_m_tiles = m_tiles;
   p.k_blocks = (K + BK - 1) / BK;
+  if (scale != nullptr) return launch_gemm<0, 1, EPI_SCALED, 0>(tmA, tmB, tmB, tmC, tmC, p, m_tiles, p.n_tiles, s);
   return launch_gemm<0, 1, EPI_PLAIN, 0>(tmA, tmB, tmB, tmC, tmC, p, m_tiles, p.n_tiles, s);
 }
 
-int ffm::dense_transposed(const void* A, int64_t ld_a, const void* B, int64_t rows, int M, int Nout, int f32, int add, void* out,
-                          int32_t* status, ffm_stream_t stream) {
+int ffm::dense_transposed(const void* A, int64_t ld_a, const void* B, int64_t rows, int M, int Nout, int f32, int add,
+                          const float* scale, void* out, int32_t* status, ffm_stream_t stream) {
   CUtensorMap tmA, tmB, tmC;
   int rc;
   if ((rc = make_ld_map(&tmA, A, rows, M, ld_a, 64, 64)) != FFM_OK) return rc;
@@ -1610,7 +1617,9 @@ int ffm::dense_transposed(const void* A, int64_t ld_a, const void* B, int64_t ro
   p.status = status;
   p.wait_cycles = g_wait_cycles;
   p.has_c2 = add;
+  p.pz_dact = reinterpret_cast<const bf16*>(scale);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (f32) return launch_gemm<1, 1, EPI_F32, 1>(tmA, tmB, tmB, tmC, tmC, p, p.m_tiles_per_group, p.n_tiles, s);
+  if (scale != nullptr) return launch_gemm<1, 1, EPI_SCALED, 1>(tmA, tmB, tmB, tmC, tmC, p, p.m_tiles_per_group, p.n_tiles, s);
   return launch_gemm<1, 1, EPI_PLAIN, 1>(tmA, tmB, tmB, tmC, tmC, p, p.m_tiles_per_group, p.n_tiles, s);
 }

@@ -60,13 +60,13 @@ int softmax_logits(const void* hidden, const void* weight, int64_t rows, int D, 
                    float* target_logits, float* stats, void* e, int64_t ld_e, int32_t* status, ffm_stream_t stream);
 
 // A [rows, K] (rows ld_a apart) B [K, Nout]: bf16 out [rows, Nout], or with splits > 1 fp32 out [splits, rows, Nout] of as many
-// pieces of the contraction. Nout % 8 == 0, any K.
-int dense_rows(const void* A, int64_t ld_a, int64_t rows, int K, const void* B, int Nout, int splits, void* out, int32_t* status,
-               ffm_stream_t stream);
+// pieces of the contraction. Nout % 8 == 0, any K. scale: device scalar that multiplies the result before it is rounded, or null.
+int dense_rows(const void* A, int64_t ld_a, int64_t rows, int K, const void* B, int Nout, int splits, const float* scale, void* out,
+               int32_t* status, ffm_stream_t stream);
 
 // A [rows, M]^T (rows ld_a apart) B [rows, Nout]: out [M, Nout] in bf16, or in fp32, with `add` added to what is there.
-// Nout % 8 == 0, any M.
-int dense_transposed(const void* A, int64_t ld_a, const void* B, int64_t rows, int M, int Nout, int f32, int add, void* out,
-                     int32_t* status, ffm_stream_t stream);
+// Nout % 8 == 0, any M. scale as above.
+int dense_transposed(const void* A, int64_t ld_a, const void* B, int64_t rows, int M, int Nout, int f32, int add, const float* scale,
+                     void* out, int32_t* status, ffm_stream_t stream);
 
 }  // namespace ffm

@@ -34,7 +34,7 @@ decltype(&ffm_layer_norm_backward) norm_backward = nullptr;
 decltype(&ffm_adamw_step) adamw = nullptr;
 decltype(&ffm_linear_cross_entropy) cross_entropy = nullptr;
 decltype(&ffm_linear_cross_entropy_workspace_bytes) cross_entropy_workspace = nullptr;
-decltype(&ffm_scale_in_place) scale_in_place = nullptr;
+decltype(&ffm_scale_many) scale_many = nullptr;
 
 void bind_ops(const std::unordered_map<std::string, uintptr_t>& at) {
   auto take = [&](const char* name, auto& f) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(at.at(name)); };
@@ -45,7 +45,7 @@ void bind_ops(const std::unordered_map<std::string, uintptr_t>& at) {
   take("ffm_adamw_step", adamw);
   take("ffm_linear_cross_entropy", cross_entropy);
   take("ffm_linear_cross_entropy_workspace_bytes", cross_entropy_workspace);
-  take("ffm_scale_in_place", scale_in_place);
+  take("ffm_scale_many", scale_many);
 }
 
 void check(int rc, const char* what) {
@@ -326,10 +326,19 @@ LossResult loss_pass(const Tensor& hidden, const Tensor& weight, const Tensor& t
   return out;
 }
 
-void scale_gradient(const Tensor& t, const Tensor& factor) {
-  if (!t.defined() || t.numel() == 0) return;
-  const On device(t);
-  check(scale_in_place(t.data_ptr(), element_type(t, "gradient"), t.numel(), factor.data_ptr<float>(), device.stream()), "ffm_scale_in_place");
+void scale_gradients(const Tensor& a, const Tensor& b, const Tensor& factor) {
+  void* x[2];
+  int64_t types[2], elements[2];
+  int n = 0;
+  for (const Tensor* t : {&a, &b}) {
+    if (!t->defined() || t->numel() == 0) continue;
+    x[n] = t->data_ptr();
+    types[n] = element_type(*t, "gradient");
+    elements[n++] = t->numel();
+  }
+  if (n == 0) return;
+  const On device(factor);
+  check(scale_many(n, x, types, elements, factor.data_ptr<float>(), device.stream()), "ffm_scale_many");
   ++launches;
 }
 
@@ -381,10 +390,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         dh = r.d_hidden;
         dw = r.d_weight;
       }
-      if (call.reduction != REDUCE_NONE) {
-        scale_gradient(dh, factor);
-        scale_gradient(dw, factor);
-      }
+      if (call.reduction != REDUCE_NONE) scale_gradients(dh, dw, factor);
       if (dh.defined()) out[0] = dh.view(hidden.sizes()).to(hidden.scalar_type());
       if (dw.defined()) out[1] = dw.to(weight.scalar_type());
     }

@@ -39,14 +39,17 @@ __device__ __forceinline__ void report(const int32_t* status, volatile int32_t* 
   }
 }
 
-// *share = 1 / number of rows that count (infinite without any: the mean is NaN then)
+// share[0] = 1 / number of rows that count (infinite without any: the mean is NaN then), share[1] the same for the gradients (0 then)
 __global__ void __launch_bounds__(LOSS_THREADS)
 loss_count_kernel(const long long* __restrict__ targets, long long rows, long long ignore, float* __restrict__ share) {
   __shared__ double part[32];
   int n = 0;
   for (long long i = threadIdx.x; i < rows; i += LOSS_THREADS) n += targets[i] != ignore;
   const double count = block_sum(n, part);
-  if (threadIdx.x == 0) *share = static_cast<float>(1.0 / count);
+  if (threadIdx.x == 0) {
+    share[0] = static_cast<float>(1.0 / count);
+    share[1] = count > 0.0 ? share[0] : 0.0f;
+  }
 }
 
 __device__ __forceinline__ void join(float& top, float& sum, float other_top, float other_sum) {
@@ -66,8 +69,7 @@ template <int TEAM>
 __global__ void __launch_bounds__(256)
 loss_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ target_logits, const long long* __restrict__ targets,
                  const bf16* __restrict__ hidden, const bf16* __restrict__ weight, int D, long long rows, int pieces, int V,
-                 long long ignore, float z, const float* __restrict__ share, const float* __restrict__ row_grad,
-                 float* __restrict__ nll, float* __restrict__ factor, float* __restrict__ target_entry, int32_t* status,
+                 long long ignore, float z, const float* __restrict__ row_grad, float* __restrict__ nll, float* __restrict__ factor, float* __restrict__ target_entry, int32_t* status,
                  volatile int32_t* status_host) {
   report(status, status_host);
   __shared__ float part[3][8];
@@ -120,7 +122,9 @@ loss_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ tar
   float scale = 0.0f;
   // a row with a target that is none has no gradient; its loss is NaN
   if (counts && known && factor != nullptr) {
-    const float g = (share != nullptr ? *share : 1.0f) * (row_grad != nullptr ? row_grad[row] : 1.0f);
+    // One over the number of rows is not in dl but multiplies its products: as a factor of every target's entry (-1, where the model
+    // has no idea) its rounding would be the same in all of them, up to 2^-8 of the whole gradient.
+    const float g = row_grad != nullptr ? row_grad[row] : 1.0f;
     scale = g * fmaf(2.0f * z, lse, 1.0f);
     if (t == 0) target_entry[row] = g * fmaf(expf(dot - lse), 2.0f * z * lse, expm1f(dot - lse));
   }
@@ -206,18 +210,28 @@ loss_join_kernel(const float* __restrict__ in, int parts, long long n, bf16* __r
   }
 }
 
-// x *= *factor in place (n a multiple of 8), nothing at all where that is 1
-template <typename T>
+struct ScaleJob {
+  void* x[FFM_CAST_MAX];
+  long long chunks_end[FFM_CAST_MAX];  // 8-value chunks of this tensor and all before it
+  int type[FFM_CAST_MAX];
+  int count;
+};
+
+// x *= *factor in place, nothing at all where that is 1
 __global__ void __launch_bounds__(256)
-loss_scale_kernel(T* __restrict__ x, long long n, const float* __restrict__ factor) {
+loss_scale_kernel(const __grid_constant__ ScaleJob job, const float* __restrict__ factor) {
   const float f = *factor;
   if (f == 1.0f) return;
-  for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += static_cast<long long>(gridDim.x) * 2048) {
+  const long long total = job.chunks_end[job.count - 1];
+  for (long long c = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; c < total; c += static_cast<long long>(gridDim.x) * 256) {
+    int i = 0;
+    while (c >= job.chunks_end[i]) ++i;
+    const long long e = (c - (i > 0 ? job.chunks_end[i - 1] : 0)) * 8;
     float v[8];
-    load8(x + i, v);
+    load8_as(job.x[i], job.type[i], e, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= f;
-    store8(x + i, v);
+    store8_as(job.x[i], job.type[i], e, v);
   }
 }
 
@@ -452,7 +466,7 @@ Layout lay_out(const ffm_loss_args& a) {
     return here;
   };
   const int64_t rows = n;
-  l.share = next(4);
+  l.share = next(8);
   l.target_logits = next(rows * 4);
   l.stats = next(rows * l.pieces * 8);
   l.target_entry = next(grads ? rows * 4 : 0);
@@ -500,6 +514,7 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
   auto at = [&](int64_t offset) { return reinterpret_cast<float*>(w + offset); };
   const long long* targets = reinterpret_cast<const long long*>(a.targets);
   float* share = a.mean ? at(l.share) : nullptr;
+  const float* factor = a.mean ? share + 1 : nullptr;
   const bool grads = a.d_hidden != nullptr || a.d_weight != nullptr;
   int64_t launched = 0;
   int rc = FFM_OK;
@@ -524,7 +539,7 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
     const bool wide = n <= 8ll * num_sms();
     (wide ? loss_rows_kernel<256> : loss_rows_kernel<32>)<<<static_cast<unsigned>(wide ? n : (n + 7) / 8), 256, 0, s>>>(
         reinterpret_cast<const float2*>(at(l.stats)), at(l.target_logits), targets + r0, reinterpret_cast<const bf16*>(hidden),
-        static_cast<const bf16*>(a.weight), D, n, l.pieces, V, a.ignore_index, z, share, a.row_grad != nullptr ? a.row_grad + r0 : nullptr,
+        static_cast<const bf16*>(a.weight), D, n, l.pieces, V, a.ignore_index, z, a.row_grad != nullptr ? a.row_grad + r0 : nullptr,
         a.nll + r0, grads ? at(l.factor) : nullptr, at(l.target_entry), a.status, a.status_host);
     if ((rc = launch_ok()) != FFM_OK) return rc;
     launched += 2;
@@ -537,7 +552,7 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
     if (a.d_hidden != nullptr) {
       char* dh = static_cast<char*>(a.d_hidden) + r0 * a.D * 2;
       const int splits = l.splits;
-      if ((rc = dense_rows(e, l.ld, n, V, a.weight, D, splits, splits > 1 ? static_cast<void*>(at(l.parts)) : dh, a.status, stream)) != FFM_OK) return rc;
+      if ((rc = dense_rows(e, l.ld, n, V, a.weight, D, splits, factor, splits > 1 ? static_cast<void*>(at(l.parts)) : dh, a.status, stream)) != FFM_OK) return rc;
       ++launched;
       if (splits > 1) {
         loss_join_kernel<<<streaming_blocks(n * a.D), 256, 0, s>>>(at(l.parts), splits, n * a.D, reinterpret_cast<bf16*>(dh));
@@ -548,7 +563,7 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
     if (a.d_weight != nullptr) {
       const bool wide = a.d_weight_f32 || step < a.N;
       void* to = a.d_weight_f32 || !wide ? a.d_weight : static_cast<void*>(at(l.wide));
-      if ((rc = dense_transposed(e, l.ld, hidden, n, V, D, wide, r0 > 0, to, a.status, stream)) != FFM_OK) return rc;
+      if ((rc = dense_transposed(e, l.ld, hidden, n, V, D, wide, r0 > 0, factor, to, a.status, stream)) != FFM_OK) return rc;
       ++launched;
     }
   }
@@ -571,19 +586,21 @@ extern "C" int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t 
   return FFM_OK;
 }
 
-extern "C" int ffm_scale_in_place(void* x, int x_type, int64_t elements, const float* factor, ffm_stream_t stream) {
-  if (!is_type(x_type) || elements < 0 || !factor) return FFM_ERR_BAD_ARG;
-  if (elements == 0) return FFM_OK;
-  if (!x) return FFM_ERR_BAD_ARG;
-  if (elements % 8 != 0 || off_16_bytes(static_cast<const char*>(x))) return FFM_ERR_UNSUPPORTED;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int blocks = streaming_blocks(elements);
-  if (x_type == FFM_TYPE_BF16) {
-    loss_scale_kernel<<<blocks, 256, 0, s>>>(static_cast<bf16*>(x), elements, factor);
-  } else if (x_type == FFM_TYPE_FP16) {
-    loss_scale_kernel<<<blocks, 256, 0, s>>>(static_cast<fp16*>(x), elements, factor);
-  } else {
-    loss_scale_kernel<<<blocks, 256, 0, s>>>(static_cast<float*>(x), elements, factor);
+extern "C" int ffm_scale_many(int count, void* const* x, const int64_t* types, const int64_t* elements, const float* factor, ffm_stream_t stream) {
+  if (count < 0 || count > FFM_CAST_MAX || !factor || (count > 0 && (!x || !types || !elements))) return FFM_ERR_BAD_ARG;
+  ScaleJob job = {};
+  long long chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (elements[i] < 0 || !is_type(static_cast<int>(types[i]))) return FFM_ERR_BAD_ARG;
+    if (elements[i] == 0) continue;
+    if (!x[i]) return FFM_ERR_BAD_ARG;
+    if (elements[i] % 8 != 0 || off_16_bytes(static_cast<const char*>(x[i]))) return FFM_ERR_UNSUPPORTED;
+    chunks += elements[i] / 8;
+    job.x[job.count] = x[i];
+    job.type[job.count] = static_cast<int>(types[i]);
+    job.chunks_end[job.count++] = chunks;
   }
+  if (job.count == 0) return FFM_OK;
+  loss_scale_kernel<<<streaming_blocks(chunks * 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(job, factor);
   return launch_ok();
 }

@@ -575,7 +575,8 @@ int ffm_adamw_step(const ffm_adamw_tensor* tensors, int count, const ffm_adamw_a
  *   launched (null or host): kernels enqueued are added.
  * Every field is 8 bytes wide.
  *
- * ffm_scale_in_place: x *= *factor, a device scalar (elements % 8 == 0, 16-byte aligned); x is not touched where that is 1.
+ * ffm_scale_many: x[i] *= *factor, a device scalar, for up to FFM_CAST_MAX tensors (types: FFM_TYPE_*; elements % 8 == 0, 16-byte
+ *   aligned) in one launch; nothing is touched where it is 1.
  * ------------------------------------------------------------------------------------------------- */
 typedef struct {
   int64_t N;
@@ -602,7 +603,7 @@ typedef struct {
 } ffm_loss_args;
 size_t ffm_linear_cross_entropy_workspace_bytes(const ffm_loss_args* args);
 int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t stream);
-int ffm_scale_in_place(void* x, int x_type, int64_t elements, const float* factor, ffm_stream_t stream);
+int ffm_scale_many(int count, void* const* x, const int64_t* types, const int64_t* elements, const float* factor, ffm_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -156,9 +156,15 @@ def test_linear_cross_entropy_entry_points():
     assert size(d_hidden=0, d_weight=0) < 100000 * 50257 // 8
     assert lib.ffm_linear_cross_entropy_workspace_bytes(0) == 0
 
-    assert lib.ffm_scale_in_place(0, BF16, 8, 256, 0) == BAD and lib.ffm_scale_in_place(256, BF16, 8, 0, 0) == BAD
-    assert lib.ffm_scale_in_place(256, 4, 8, 256, 0) == BAD and lib.ffm_scale_in_place(256, BF16, 7, 256, 0) == UNSUPPORTED
-    assert lib.ffm_scale_in_place(0, BF16, 0, 256, 0) == 0
+    assert _scale(lib, [(256, BF16, 8)], factor=0) == BAD and _scale(lib, [(0, BF16, 8)]) == BAD and _scale(lib, [(256, 4, 8)]) == BAD
+    assert _scale(lib, [(256, BF16, -8)]) == BAD and _scale(lib, [(256, BF16, 8)] * 9) == BAD and lib.ffm_scale_many(1, 0, 0, 0, 256, 0) == BAD
+    assert _scale(lib, [(256, BF16, 7)]) == UNSUPPORTED and _scale(lib, [(256, BF16, 8), (260, BF16, 8)]) == UNSUPPORTED
+    assert _scale(lib, []) == 0 and _scale(lib, [(0, BF16, 0)]) == 0
+
+
+def _scale(lib, tensors, factor=256):
+    columns = [(ctypes.c_int64 * max(1, len(tensors)))(*[t[i] for t in tensors]) for i in range(3)]
+    return lib.ffm_scale_many(len(tensors), *[ctypes.addressof(c) for c in columns], factor, 0)
 
 
 def _without_a_device():
@@ -170,7 +176,7 @@ def _without_a_device():
     assert lib.ffm_adamw_step(ctypes.addressof(t), 1, ctypes.addressof(h), 0) < 0
     for values in ({}, dict(d_hidden=0, d_weight=0), dict(mean=0, loss=0), dict(N=5, d_hidden=0, d_weight=0)):
         assert _run_loss(lib, **values) < 0
-    assert lib.ffm_scale_in_place(a, FP32, 8, a, 0) < 0
+    assert _scale(lib, [(a, FP32, 8)]) < 0
 
 
 def test_calls_without_a_device_return_an_error(monkeypatch):
