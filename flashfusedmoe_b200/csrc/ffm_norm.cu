@@ -35,7 +35,9 @@ constexpr int STREAM_THREADS = 1024;      // forward: 64 registers
 constexpr int STREAM_BACK_THREADS = 512;  // backward: 128, 64 of them sums of dw and db
 static_assert(STREAM_THREADS / 64 <= 16 && STREAM_BACK_THREADS / 64 <= 15, "a barrier for every team of more than a warp");
 constexpr int STREAM_SMEM = 226 << 10;
-constexpr int SHIFTED_THREADS = 768, SHIFTED_STAGES = 3;  // the same for rows off 16-byte boundaries (forward; a stage is being filled)
+// The same for rows off 16-byte boundaries. A stage is being filled while a row is worked on; the backward kernel needs 140
+// registers (with 512 threads it spilled, and took 98 us for 16384 x 1025 bf16).
+constexpr int SHIFTED_THREADS = 768, SHIFTED_BACK_THREADS = 384, SHIFTED_STAGES = 3;
 
 template <typename T>
 constexpr int VALUES = 16 / static_cast<int>(sizeof(T));  // of a chunk
@@ -355,7 +357,7 @@ layer_norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, lo
 // ---- many rows of 16-byte boundaries ------------------------------------------------------------------------------------
 //
 // What a block holds in registers is too little to be in flight all the time: reading a row, two exchanges and writing it
-// follow one another (32768 x 7168 bf16: 354 us forward, 563 backward). Here every thread copies its chunks of the next rows
+// follow one another (32768 x 7168 bf16: 354 us forward, 563 backward; here 167 and 225, 5.6 and 6.3 TB/s). Here every thread copies its chunks of the next rows
 // to shared memory (cp.async; it reads back what it copied itself, so nothing but its own wait stands between), and teams of
 // one block go their own way with a barrier each. Weight and bias lie in shared memory in fp32.
 
@@ -670,66 +672,74 @@ layer_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict_
 // ---- many rows off 16-byte boundaries -----------------------------------------------------------------------------------
 //
 // Rows of odd width start anywhere. Read value by value they took ten times as long as their bytes (4093 x 2051 fp16: 48 us
-// forward, 80 backward). Here the 16-byte pieces that cover a row are copied to shared memory as they lie, and values are taken from there: a
+// forward, 80 backward; here 20 and 27, bound by instructions: two to four times the time of rows on 16 bytes). Here the 16-byte pieces that cover a row are copied to shared memory as they lie, and values are taken from there: a
 // thread has pairs of neighbours (fp32: single values), side by side with its neighbours' pairs, out of two words and a shift where
 // the row starts in the middle of one. What a piece has beside the row belongs to rows or allocations beside it and is not
 // looked at (a 16-byte piece never lies in two pages). A thread reads what others copied, so a team also meets before a
 // row; that it then is past the row before frees that row's place for the next fetch.
 
-// What a thread has of a row: PAIRS pairs of values, and how they lie.
-template <typename T>
+// What a thread has of a row: PAIRS pairs of values, and how they lie. WORDS (16-bit types): a pair is a word of memory, for all of a
+// team's rows alike; where they start in the middle of one, pairs begin a value before the row (`before` = 1).
+template <typename T, bool WORDS>
 struct Shifted {
   static constexpr int PAIRS = STREAM_CHUNKS * VALUES<T> / 2;
-  int t, team, D;
-  int firsts, seconds;  // pairs whose first, and whose second value is in the row
+  int t, team, D, before;
+  int firsts, seconds;  // pairs whose first, and whose second value is in the row (the first pair's first: has_first)
 
-  __device__ __forceinline__ Shifted(int t_, int team_, int D_) : t(t_), team(team_), D(D_) {
+  __device__ __forceinline__ Shifted(int t_, int team_, int D_, int before_) : t(t_), team(team_), D(D_), before(WORDS ? before_ : 0) {
     const int d = 2 * team;  // from a thread's pair to its next
     const int a = first(0), b = second(0);
     firsts = a < D ? (D - a + d - 1) / d : 0;
     seconds = b < D ? (D - b + d - 1) / d : 0;
   }
-  __device__ __forceinline__ int first(int k) const { return sizeof(T) == 2 ? 2 * (k * team + t) : 2 * k * team + t; }
+  __device__ __forceinline__ int first(int k) const { return sizeof(T) == 2 ? 2 * (k * team + t) - before : 2 * k * team + t; }
   __device__ __forceinline__ int second(int k) const { return sizeof(T) == 2 ? first(k) + 1 : first(k) + team; }
+  __device__ __forceinline__ bool has_first(int k) const { return k < firsts && !(WORDS && k == 0 && t < before); }
 
+  __device__ __forceinline__ static float2 of_word(uint32_t word) {
+    if constexpr (std::is_same<T, bf16>::value) {
+      return make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u));
+    } else {
+      return __half22float2(*reinterpret_cast<const __half2*>(&word));
+    }
+  }
   // row: shared address of the row's first value
   __device__ __forceinline__ float2 read(uint32_t row, int k) const {
     if constexpr (sizeof(T) == 4) {
       return make_float2(read_word_as_float(row + first(k) * 4), read_word_as_float(row + second(k) * 4));
+    } else if constexpr (WORDS) {
+      return of_word(read_word(row + first(k) * 2));
     } else {
       const uint32_t at = row + first(k) * 2, word = at & ~3u;
-      const uint32_t both_values = __funnelshift_r(read_word(word), read_word(word + 4), (at & 2u) * 8);
-      if constexpr (std::is_same<T, bf16>::value) {
-        return make_float2(__uint_as_float(both_values << 16), __uint_as_float(both_values & 0xffff0000u));
-      } else {
-        return __half22float2(*reinterpret_cast<const __half2*>(&both_values));
-      }
+      return of_word(__funnelshift_r(read_word(word), read_word(word + 4), (at & 2u) * 8));
     }
   }
-  // of a vector in fp32
+  // of a vector in fp32, which is there `before` places further on for WORDS
   __device__ __forceinline__ float2 read_vector(uint32_t vector, int k) const {
     if constexpr (sizeof(T) == 4) {
       return make_float2(read_word_as_float(vector + first(k) * 4), read_word_as_float(vector + second(k) * 4));
     } else {
       float2 v;
-      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(vector + first(k) * 4) : "memory");
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(vector + 8 * (k * team + t)) : "memory");
       return v;
     }
   }
+  // words: the row starts at a word (WORDS: pairs do)
   __device__ __forceinline__ void write(T* row, int k, float2 v, bool words) const {
-    const int a = first(k), b = second(k);
     if constexpr (sizeof(T) == 2) {
-      if (words && k < seconds) {
+      if ((WORDS || words) && k < seconds && has_first(k)) {
         const T pair[2] = {from_float<T>(v.x), from_float<T>(v.y)};
-        *reinterpret_cast<uint32_t*>(row + a) = *reinterpret_cast<const uint32_t*>(pair);
+        *reinterpret_cast<uint32_t*>(row + first(k)) = *reinterpret_cast<const uint32_t*>(pair);
         return;
       }
     }
-    if (k < firsts) row[a] = from_float<T>(v.x);
-    if (k < seconds) row[b] = from_float<T>(v.y);
+    if (has_first(k)) row[first(k)] = from_float<T>(v.x);
+    if (k < seconds) row[second(k)] = from_float<T>(v.y);
   }
-  __device__ __forceinline__ float2 inside(int k, float2 v) const {  // zero past the row's end
-    return make_float2(k < firsts ? v.x : 0.0f, k < seconds ? v.y : 0.0f);
+  // zero beside the row. (Leaving the loops where no thread of a team has a pair any more breaks them into pieces: 8192 x 4097 bf16
+  // took 84 us forward for 56, 121 backward for 90.)
+  __device__ __forceinline__ float2 inside(int k, float2 v) const {
+    return make_float2(has_first(k) ? v.x : 0.0f, k < seconds ? v.y : 0.0f);
   }
 
   __device__ __forceinline__ static uint32_t read_word(uint32_t at) {
@@ -765,27 +775,35 @@ __device__ __forceinline__ void team_meet(int barrier, int team) {
   }
 }
 
-template <typename T>
+// A vector of D values in shared memory in fp32, `fill` past its end; with WORDS twice, the second time a place further on, for teams whose
+// pairs begin before the row. Filled by the whole block.
+template <bool WORDS>
+__device__ __forceinline__ void fill_shifted(float* to, const void* p, int type, float fill, int D, int room) {
+  for (int c = threadIdx.x; c < room; c += blockDim.x) {
+    to[c] = p != nullptr && c < D ? load1_as(p, type, c) : fill;
+    if (WORDS) to[room + c] = p != nullptr && c > 0 && c <= D ? load1_as(p, type, c - 1) : fill;
+  }
+}
+
+template <typename T, bool WORDS>
 __global__ void __launch_bounds__(SHIFTED_THREADS, 1)
 layer_norm_forward_shifted_kernel(const T* __restrict__ x, long long stride, const void* __restrict__ weight, int w_type,
                                   const void* __restrict__ bias, int b_type, long long rows, int D, float eps, int team,
                                   T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
   extern __shared__ __align__(16) float scale[];  // weight, bias, ring
   __shared__ float part[2][1][32];
-  constexpr int S = SHIFTED_STAGES, PAIRS = Shifted<T>::PAIRS;
-  const Shifted<T> at(static_cast<int>(threadIdx.x) % team, team, D);
+  constexpr int S = SHIFTED_STAGES, PAIRS = Shifted<T, WORDS>::PAIRS, COPIES = WORDS ? 2 : 1;
   const int room = team * STREAM_CHUNKS * VALUES<T>;
-  for (int c = threadIdx.x; c < room; c += blockDim.x) {
-    scale[c] = weight != nullptr && c < D ? load1_as(weight, w_type, c) : 1.0f;
-    scale[room + c] = bias != nullptr && c < D ? load1_as(bias, b_type, c) : 0.0f;
-  }
-  const uint32_t my_scale = smem_u32(scale), my_shift = smem_u32(scale + room);
+  fill_shifted<WORDS>(scale, weight, w_type, 1.0f, D, room);
+  fill_shifted<WORDS>(scale + COPIES * room, bias, b_type, 0.0f, D, room);
   const int teams = blockDim.x / team;
-  const uint32_t row_bytes = team * STREAM_CHUNKS * 16, ring = smem_u32(scale + 2 * room) + threadIdx.x / team * S * row_bytes;
+  const uint32_t row_bytes = team * STREAM_CHUNKS * 16, ring = smem_u32(scale + 2 * COPIES * room) + threadIdx.x / team * S * row_bytes;
   const float width = static_cast<float>(D), inv = 1.0f / width;
   const long long first = static_cast<long long>(blockIdx.x) * teams + threadIdx.x / team, step = static_cast<long long>(gridDim.x) * teams;
   const Trips trips(rows, first, step, team);
   const T *source = x + first * stride, *here_source = source;
+  const Shifted<T, WORDS> at(static_cast<int>(threadIdx.x) % team, team, D, static_cast<int>(phase(source) >> 1 & 1));
+  const uint32_t my_scale = smem_u32(scale + at.before * room), my_shift = smem_u32(scale + (COPIES + at.before) * room);
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
     at.fetch(ring + s * row_bytes, s < trips.mine ? source : x, s < trips.mine);
@@ -836,25 +854,25 @@ layer_norm_forward_shifted_kernel(const T* __restrict__ x, long long stride, con
   copy_async_wait<0>();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(STREAM_BACK_THREADS, 1)
+template <typename T, bool WORDS>
+__global__ void __launch_bounds__(SHIFTED_BACK_THREADS, 1)
 layer_norm_backward_shifted_kernel(const T* __restrict__ dy, const T* __restrict__ x, long long stride,
                                    const void* __restrict__ weight, int w_type, const float* __restrict__ mean,
                                    const float* __restrict__ rstd, long long rows, int D, int team, T* __restrict__ dx,
                                    float* __restrict__ part_w, float* __restrict__ part_b) {
   extern __shared__ __align__(16) float scale[];  // weight, ring; the ring's place then holds the teams' sums
   __shared__ float part[2][2][32];
-  constexpr int S = SHIFTED_STAGES, PAIRS = Shifted<T>::PAIRS;
-  const Shifted<T> at(static_cast<int>(threadIdx.x) % team, team, D);
+  constexpr int S = SHIFTED_STAGES, PAIRS = Shifted<T, WORDS>::PAIRS, COPIES = WORDS ? 2 : 1;
   const int room = team * STREAM_CHUNKS * VALUES<T>;
-  for (int c = threadIdx.x; c < room; c += blockDim.x) scale[c] = weight != nullptr && c < D ? load1_as(weight, w_type, c) : 1.0f;
-  const uint32_t my_scale = smem_u32(scale);
+  fill_shifted<WORDS>(scale, weight, w_type, 1.0f, D, room);
   const int teams = blockDim.x / team;
-  const uint32_t row_bytes = team * STREAM_CHUNKS * 16, ring = smem_u32(scale + room) + threadIdx.x / team * S * 2 * row_bytes;
+  const uint32_t row_bytes = team * STREAM_CHUNKS * 16, ring = smem_u32(scale + COPIES * room) + threadIdx.x / team * S * 2 * row_bytes;
   const float inv = 1.0f / static_cast<float>(D);
   const long long first = static_cast<long long>(blockIdx.x) * teams + threadIdx.x / team, step = static_cast<long long>(gridDim.x) * teams;
   const Trips trips(rows, first, step, team);
   const T *source = x + first * stride, *source_dy = dy + first * D, *here_source = source, *here_dy = source_dy;
+  const Shifted<T, WORDS> at(static_cast<int>(threadIdx.x) % team, team, D, static_cast<int>(phase(source) >> 1 & 1));
+  const uint32_t my_scale = smem_u32(scale + at.before * room);
   auto fetch = [&](int k, uint32_t to) {
     at.fetch(to, k < trips.mine ? source : x, k < trips.mine);
     at.fetch(to + row_bytes, k < trips.mine ? source_dy : x, k < trips.mine);
@@ -885,7 +903,7 @@ layer_norm_backward_shifted_kernel(const T* __restrict__ dy, const T* __restrict
     team_meet(1, team);
     fetch(k + S - 1, free);
     const bool mine = k < trips.mine;
-    const uint32_t row = here + (mine ? phase(here_source) : 0), row_dy = here + row_bytes + (mine ? phase(here_dy) : 0);
+    const uint32_t row = here + phase(here_source), row_dy = here + row_bytes + phase(here_dy);
     free = here;
     here = here == ring + (S - 1) * 2 * row_bytes ? ring : here + 2 * row_bytes;
     float2 s0 = both(0.0f), s1 = both(0.0f);
@@ -913,26 +931,21 @@ layer_norm_backward_shifted_kernel(const T* __restrict__ dy, const T* __restrict
   copy_async_wait<0>();
   if (part_w == nullptr && part_b == nullptr) return;
   __syncthreads();
-  // [team][weight, bias][pair][thread]
-  float2* sums = reinterpret_cast<float2*>(scale + room);
-  const int count = PAIRS * team;
-  float2* my_sums = sums + threadIdx.x / team * 2 * count + at.t;
+  // [team][weight, bias], and there a value at its column
+  float* sums = scale + COPIES * room;
+  float* my_sums = sums + threadIdx.x / team * 2 * D;
 #pragma unroll
   for (int j = 0; j < PAIRS; ++j) {
-    my_sums[j * team] = aw[j];
-    my_sums[count + j * team] = ab[j];
+    if (at.has_first(j)) my_sums[at.first(j)] = aw[j].x, my_sums[D + at.first(j)] = ab[j].x;
+    if (j < at.seconds) my_sums[at.second(j)] = aw[j].y, my_sums[D + at.second(j)] = ab[j].y;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * count; i += blockDim.x) {
-    float* out_row = i < count ? part_w : part_b;
+  for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
+    float* out_row = c < D ? part_w : part_b;
     if (out_row == nullptr) continue;
-    float2 total = sums[i];
-    for (int n = 1; n < teams; ++n) total = add2(total, sums[n * 2 * count + i]);
-    const int j = (i < count ? i : i - count) / team;
-    const Shifted<T> of(i % team, team, D);
-    float* to = out_row + static_cast<long long>(blockIdx.x) * D;
-    if (j < of.firsts) to[of.first(j)] = total.x;
-    if (j < of.seconds) to[of.second(j)] = total.y;
+    float total = sums[c];
+    for (int n = 1; n < teams; ++n) total += sums[n * 2 * D + c];
+    out_row[static_cast<long long>(blockIdx.x) * D + (c < D ? c : c - D)] = total;
   }
 }
 
@@ -1032,26 +1045,33 @@ bool allow_stream_smem(K kernel, PerDevice& room) {
   }) > 0;
 }
 
+// How the streaming kernels read a row: as 16-byte pieces, as words (16-bit values, two a word, where every operand's rows start alike in a word),
+// as single values.
+enum { STREAM_PIECES = 0, STREAM_WORDS = 1, STREAM_VALUES = 2 };
+
 template <typename T>
-int forward_stream(bool vec, const void* x, int64_t stride, const void* w, int w_type, const void* b, int b_type, int64_t rows, int D,
+int forward_stream(int how, const void* x, int64_t stride, const void* w, int w_type, const void* b, int b_type, int64_t rows, int D,
                    float eps, const NormShape& s, int smem, void* y, float* mean, float* rstd, cudaStream_t stream) {
-  static PerDevice room[2];
-  auto kernel = vec ? layer_norm_forward_stream_kernel<T> : layer_norm_forward_shifted_kernel<T>;
-  if (!allow_stream_smem(kernel, room[vec])) return FFM_ERR_LAUNCH;
+  static PerDevice room[3];
+  auto kernel = how == STREAM_PIECES  ? layer_norm_forward_stream_kernel<T>
+                : how == STREAM_WORDS ? layer_norm_forward_shifted_kernel<T, sizeof(T) == 2>
+                                      : layer_norm_forward_shifted_kernel<T, false>;
+  if (!allow_stream_smem(kernel, room[how])) return FFM_ERR_LAUNCH;
   kernel<<<num_sms(), s.threads, smem, stream>>>(static_cast<const T*>(x), stride, w, w_type, b, b_type, rows, D, eps, s.team,
                                                  static_cast<T*>(y), mean, rstd);
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
 
-// stages: 0 for rows off 16-byte boundaries
+// stages: of STREAM_PIECES
 template <typename T>
-int backward_stream(int stages, const void* dy, const void* x, int64_t stride, const void* w, int w_type, const float* mean, const float* rstd,
+int backward_stream(int how, int stages, const void* dy, const void* x, int64_t stride, const void* w, int w_type, const float* mean, const float* rstd,
                     int64_t rows, int D, const NormShape& s, int smem, void* dx, float* part_w, float* part_b, cudaStream_t stream) {
-  static PerDevice room[3];
-  auto kernel = stages == 0                    ? layer_norm_backward_shifted_kernel<T>
+  static PerDevice room[4];
+  auto kernel = how == STREAM_WORDS              ? layer_norm_backward_shifted_kernel<T, sizeof(T) == 2>
+                : how == STREAM_VALUES           ? layer_norm_backward_shifted_kernel<T, false>
                 : stages == STREAM_BACK_STAGES ? layer_norm_backward_stream_kernel<T, STREAM_BACK_STAGES>
                                                : layer_norm_backward_stream_kernel<T, STREAM_STAGES>;
-  if (!allow_stream_smem(kernel, room[stages == 0 ? 0 : (stages == STREAM_BACK_STAGES ? 1 : 2)])) return FFM_ERR_LAUNCH;
+  if (!allow_stream_smem(kernel, room[how == STREAM_PIECES && stages == STREAM_BACK_STAGES ? 3 : how])) return FFM_ERR_LAUNCH;
   kernel<<<num_sms(), s.threads, smem, stream>>>(static_cast<const T*>(dy), static_cast<const T*>(x), stride, w, w_type, mean, rstd, rows, D,
                                                  s.team, static_cast<T*>(dx), part_w, part_b);
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
@@ -1116,6 +1136,14 @@ bool norm_vectors(int type, int64_t stride, int D, const P*... p) {
   return static_cast<int64_t>(D) * type_bytes(type) % 16 == 0 && (stride * type_bytes(type)) % 16 == 0 && !off_16_bytes(p...);
 }
 
+// 16-bit rows of all operands start alike in a word, and so do all rows of a team (an even number of rows apart).
+template <typename... P>
+bool norm_words(int type, int64_t stride, int D, const NormShape& s, const void* x, const P*... p) {
+  const uintptr_t base = reinterpret_cast<uintptr_t>(x);
+  return type != FFM_TYPE_FP32 && (stride - D) % 2 == 0 && (D % 2 == 0 || num_sms() * s.teams % 2 == 0) &&
+         ((p == nullptr || (reinterpret_cast<uintptr_t>(p) - base) % 4 == 0) && ...);
+}
+
 bool norm_arguments(int x_type, int64_t rows, int64_t stride, int D, const void* w, int w_type) {
   return is_type(x_type) && rows >= 0 && D > 0 && (stride >= D || rows <= 1) && (w == nullptr || is_type(w_type));
 }
@@ -1137,10 +1165,15 @@ extern "C" int ffm_layer_norm_forward(const void* x, int x_type, int64_t rows, i
   const NormShape s = norm_shape(D, x_type);
   const bool vec = norm_vectors(x_type, row_stride, D, x, y);
   const NormShape r = stream_shape(D, x_type, vec ? STREAM_THREADS : SHIFTED_THREADS, vec);
-  const int smem = stream_smem(r, x_type, 2, 1, vec ? STREAM_STAGES : SHIFTED_STAGES, 0);
+  int how = vec ? STREAM_PIECES : (norm_words(x_type, row_stride, D, r, x, y) ? STREAM_WORDS : STREAM_VALUES);
+  int smem = stream_smem(r, x_type, how == STREAM_WORDS ? 4 : 2, 1, vec ? STREAM_STAGES : SHIFTED_STAGES, 0);
+  if (how == STREAM_WORDS && smem > STREAM_SMEM) {
+    how = STREAM_VALUES;
+    smem = stream_smem(r, x_type, 2, 1, SHIFTED_STAGES, 0);
+  }
   if (streams(rows, r, smem)) {
     return with_type(x_type, [&](auto tag) {
-      return forward_stream<decltype(tag)>(vec, x, row_stride, weight, w_type, bias, b_type, rows, D, eps, r, smem, y, mean, rstd,
+      return forward_stream<decltype(tag)>(how, x, row_stride, weight, w_type, bias, b_type, rows, D, eps, r, smem, y, mean, rstd,
                                            static_cast<cudaStream_t>(stream));
     });
   }
@@ -1168,9 +1201,15 @@ extern "C" int ffm_layer_norm_backward(const void* dy, const void* x, int x_type
   if (!parts && (dx == nullptr || rows == 0)) return FFM_OK;
   const NormShape s = norm_shape(D, x_type);
   const bool vectors = norm_vectors(x_type, row_stride, D, dy, x, dx);
-  const NormShape r = stream_shape(D, x_type, STREAM_BACK_THREADS, vectors);
+  const NormShape r = stream_shape(D, x_type, vectors ? STREAM_BACK_THREADS : SHIFTED_BACK_THREADS, vectors);
   const int sums = r.threads * STREAM_CHUNKS * (16 / type_bytes(x_type)) * 2 * static_cast<int>(sizeof(float));
-  int stages = vectors ? STREAM_BACK_STAGES : 0, smem = stream_smem(r, x_type, 1, 2, vectors ? STREAM_BACK_STAGES : SHIFTED_STAGES, sums);
+  int how = vectors ? STREAM_PIECES : (norm_words(x_type, row_stride, D, r, x, dy, dx) ? STREAM_WORDS : STREAM_VALUES);
+  int stages = STREAM_BACK_STAGES;
+  int smem = stream_smem(r, x_type, how == STREAM_WORDS ? 2 : 1, 2, vectors ? STREAM_BACK_STAGES : SHIFTED_STAGES, sums);
+  if (how == STREAM_WORDS && smem > STREAM_SMEM) {
+    how = STREAM_VALUES;
+    smem = stream_smem(r, x_type, 1, 2, SHIFTED_STAGES, sums);
+  }
   if (vectors && smem > STREAM_SMEM) {
     stages = STREAM_STAGES;
     smem = stream_smem(r, x_type, 1, 2, STREAM_STAGES, sums);
@@ -1181,7 +1220,7 @@ extern "C" int ffm_layer_norm_backward(const void* dy, const void* x, int x_type
   float* part_b = dbias != nullptr ? static_cast<float*>(workspace) + static_cast<size_t>(blocks) * D : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = stream_rows ? with_type(x_type, [&](auto tag) {
-    return backward_stream<decltype(tag)>(stages, dy, x, row_stride, weight, w_type, mean, rstd, rows, D, r, smem, dx, part_w, part_b, st);
+    return backward_stream<decltype(tag)>(how, stages, dy, x, row_stride, weight, w_type, mean, rstd, rows, D, r, smem, dx, part_w, part_b, st);
   }) : dispatch_norm(x_type, s, vectors, [&](auto tag, auto ch, auto vec, auto threads) {
     return backward_as<decltype(tag), decltype(ch)::value, decltype(vec)::value, decltype(threads)::value>(
         dy, x, row_stride, weight, w_type, mean, rstd, rows, D, s, dx, part_w, part_b, blocks, st);
