@@ -9,6 +9,7 @@ from .fused_moe import _get_compute_dtype, _require_bf16
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
+@torch.compiler.disable
 def linear_cross_entropy(hidden, weight, target, *, ignore_index=-100, reduction="mean", z_loss_coeff=0.0, _piece_rows=0):
     """Softmax cross entropy of the logits hidden weight^T, which are never stored: with lse = log sum exp of a row's logits,
     lse - logit[target] + z_loss_coeff * lse^2 for every row, 0 where the target is ignore_index.

@@ -7,6 +7,7 @@ import torch.nn as nn
 from . import _lib
 
 
+@torch.compiler.disable
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x [*, D].
 

@@ -11,6 +11,7 @@ def _capturing(tensors):
     return bool(tensors) and tensors[0].is_cuda and torch.cuda.is_current_stream_capturing()
 
 
+@torch.compiler.disable
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, masters=None,
                exp_avg_scales=None, exp_avg_sq_scales=None, grad_scale=None, seed=0):
     """One AdamW step of the tensors in `params`, in place: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
@@ -37,8 +38,9 @@ class AdamW(torch.optim.Optimizer):
     be saved, in 32. master_weights keeps a float32 copy of parameters of fewer bits, which the updates go to: without it an
     update of less than half a unit of a bfloat16 parameter's last place is lost.
 
-    lr may be a float32 tensor on the device: a step that was captured in a graph then reads it at every replay. State
-    dicts load and save as torch's do; `step` counts on the device."""
+    Parameters are contiguous CUDA tensors. lr may be a float32 tensor on the device: a step that was captured in a graph then
+    reads it at every replay. State dicts load and save as torch's do, and one of torch.optim.AdamW can be loaded; `step` counts
+    on the device."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, master_weights=True,
                  min_8bit_size=4096, seed=0):
@@ -71,14 +73,25 @@ class AdamW(torch.optim.Optimizer):
         return state
 
     def load_state_dict(self, state_dict):
-        """As torch's, but every state keeps its own type: there, floating states take their parameter's."""
+        """As torch's, but every state keeps its own type: there, floating states take their parameter's. Steps and unscaled
+        moments of another optimizer become int32 and float32."""
         saved = {i: {k: v for k, v in s.items() if torch.is_tensor(v)} for i, s in state_dict["state"].items()}
+        own = [dict(g) for g in self.param_groups]
         super().load_state_dict(state_dict)
+        for group, mine in zip(self.param_groups, own):   # options that another optimizer's groups do not have
+            for name, value in mine.items():
+                group.setdefault(name, value)
         order = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(order, params):
-            for name, value in saved.get(i, {}).items():
-                self.state[p][name] = value.detach().to(p.device, copy=True)
+            old = saved.get(i, {})
+            for name, value in old.items():
+                kind = value.dtype
+                if name == "step":
+                    kind = torch.int32
+                elif name in ("exp_avg", "exp_avg_sq") and name + "_scale" not in old:
+                    kind = torch.float32
+                self.state[p][name] = value.detach().to(p.device, kind, copy=True).contiguous()
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale=None):

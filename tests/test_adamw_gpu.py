@@ -312,6 +312,36 @@ def test_state_dict_resumes_bit_for_bit(dtype, options):
 
 
 @pytest.mark.gpu
+def test_a_state_dict_of_torchs_optimizer_goes_on():
+    """Five steps with torch.optim.AdamW, then ten with either; the bound is that of twenty steps above."""
+    params, opt = _models(torch.float32)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = torch.optim.AdamW([{"params": twins[:2], "weight_decay": 0.1}, {"params": twins[2:], "lr": 2e-3}], lr=1e-3,
+                              betas=(0.9, 0.95), weight_decay=0.0)
+
+    def gradients(k):
+        gen = torch.Generator(device="cuda").manual_seed(k)
+        for p, q in zip(params, twins):
+            q.grad = torch.randn(q.shape, device="cuda", generator=gen)
+            p.grad = q.grad.clone()
+
+    for k in range(5):
+        gradients(k)
+        other.step()
+    with torch.no_grad():
+        for p, q in zip(params, twins):
+            p.copy_(q)
+    opt.load_state_dict(other.state_dict())
+    assert all(opt.state[p]["step"].dtype == torch.int32 and opt.state[p]["step"].item() == 5 for p in params)
+    for k in range(5, 15):
+        gradients(k)
+        opt.step()
+        other.step()
+    for p, q in zip(params, twins):
+        assert ((p - q).abs() <= 2 * 20 * (40 * U * 2e-3 * 5 + 4 * U * (q.detach().abs() + 0.1))).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_steps_replay_to_the_eager_bits(bits):
     """Two graphs of one optimizer, replayed in turn, with the rate read from the device."""

@@ -169,3 +169,19 @@ def test_scoring_after_training():
         one = linear_cross_entropy(hidden[1, 5:6], model.head, target[1, 5:6], reduction="none", z_loss_coeff=1e-4)
         row = tokens.shape[1] + 5
         entropy.check(one, {"nll": out["nll"][row:row + 1]}, {"nll": bound["nll"][row:row + 1]}, "nll")
+
+
+@pytest.mark.gpu
+def test_a_compiled_model_breaks_its_graph_around_them():
+    model, _ = make(32)
+    tokens, target = batch(11)
+
+    def run(m):
+        model.zero_grad(set_to_none=True)
+        loss, extra = m(tokens, target)
+        (loss + extra).backward()
+        return loss.detach(), [p.grad.clone() for p in model.parameters()]
+
+    loss, grads = run(model)
+    other, others = run(torch.compile(model, backend="aot_eager"))
+    assert torch.equal(loss, other) and all(torch.equal(a, b) for a, b in zip(grads, others))
