@@ -199,6 +199,24 @@ def test_rounding_of_the_second_moment_is_even_handed():
 
 
 @pytest.mark.gpu
+def test_codes_do_not_depend_on_how_the_root_was_taken():
+    """The states do not depend on eps, so a call whose eps wants exact roots and quotients stores the codes of one whose eps does
+    not. One value in 2^20 lies where a root one unit off gives another code: 32 or so of these 2^25 at either step."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    n = 1 << 25
+    grad = torch.randn(n, device="cuda", generator=gen).mul_(1e-3)
+    one, other = ([torch.zeros(n, device="cuda")] + [torch.zeros(n, device="cuda", dtype=torch.float8_e4m3fn) for _ in range(2)]
+                  + [torch.full((n // BLOCK,), 1, dtype=torch.uint8, device="cuda") for _ in range(2)]
+                  + [torch.zeros((), dtype=torch.int32, device="cuda")] for _ in range(2))
+    from flashfusedmoe_b200 import adamw_step
+    for _ in range(2):
+        for (p, m, v, ms, vs, step), eps in ((one, 1e-6), (other, 1e-30)):
+            adamw_step([p], [grad], [m], [v], [step], exp_avg_scales=[ms], exp_avg_sq_scales=[vs], **{**HYPER, "eps": eps})
+        for x, y in zip(one[1:5], other[1:5]):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.gpu
 def test_a_small_average_keeps_moving_in_8_bits():
     """Gradients fall to nothing: v = b2^t v then, 2 % of sqrt(v) a step, far less than the distance of two e4m3 numbers."""
     from flashfusedmoe_b200 import adamw_step
