@@ -9,13 +9,13 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 #include <limits>
 #include <mutex>
 #include <optional>
 #include <stdexcept>
 #include <string>
 #include <unordered_map>
-#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -89,6 +89,23 @@ int element_type(const Tensor& t, const char* name) {
   }
 }
 
+// A leaf's gradient is added to it on the stream where the oldest graph that still lives first took the leaf. Where that is the
+// default stream, which takes no part in a capture, a captured backward pass ends the process: refused while nothing has happened.
+void capturable(std::initializer_list<const Tensor*> operands) {
+  for (const Tensor* t : operands) {
+    if (!t->defined() || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
+    const c10::impl::VirtualGuardImpl cuda(c10::DeviceType::CUDA);
+    if (cuda.getStream(t->device()) == cuda.getDefaultStream(t->device())) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (node == nullptr || node->stream() != cuda.getDefaultStream(t->device())) continue;
+    const py::gil_scoped_acquire held;
+    if (py::module_::import("torch.cuda").attr("is_current_stream_capturing")().cast<bool>()) {
+      throw std::runtime_error("an autograd graph that was made on the default stream before the capture still holds an operand: let go of what "
+                               "came from it (a loss, an output) before the capture");
+    }
+  }
+}
+
 // values in memory, one after the other, with no negation pending
 Tensor plain(const Tensor& t) { return t.contiguous().resolve_neg(); }
 
@@ -142,6 +159,7 @@ struct NormResult {
 NormResult norm_forward_of(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool stats) {
   on_gpu(x, "x");
   if (x.dim() < 1 || x.size(-1) < 1) throw py::value_error("x must have a last dimension to normalise, got " + c10::str(x.sizes()));
+  if (x.size(-1) > std::numeric_limits<int>::max()) throw py::value_error("x has rows of " + std::to_string(x.size(-1)) + " values");
   if (!(eps >= 0.0)) throw py::value_error("eps must not be negative, got " + std::to_string(eps));
   const int type = element_type(x, "x");
   check_vector(weight, x, "weight");
@@ -251,6 +269,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   const py::gil_scoped_release released;
   if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()))) {
+    capturable({&x, &w, &b});
     return LayerNorm::apply(x, weight, bias, eps);
   }
   return norm_forward_of(x, w, b, eps, false).y;
@@ -403,6 +422,7 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
   const py::gil_scoped_release released;
   const Tensor t = plain(target);
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
+    capturable({&hidden, &weight});
     return LinearCrossEntropy::apply(hidden, weight, t, ignore_index, reduction, z, piece_rows, status, status_host);
   }
   const LossCall call{ignore_index, reduction, z, piece_rows, status, status_host};
@@ -485,13 +505,23 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
     h.grad_scale = scale.data_ptr<float>();
   }
 
-  // written in place: one after the other in memory, no negation pending, and no two entries on the same memory
-  std::unordered_set<const void*> written;
+  // written in place: one after the other in memory, no negation pending, and no two on the same memory, nor on a gradient's
+  struct Range {
+    const char *from, *to;
+    const char* name;
+    bool written;
+  };
+  std::vector<Range> ranges;
+  ranges.reserve(n * 8 + 2);
+  auto range = [&](const Tensor& t, const char* name, bool written) {
+    const char* from = static_cast<const char*>(t.data_ptr());
+    if (t.numel() > 0) ranges.push_back({from, from + t.numel() * t.element_size(), name, written});
+  };
   auto state = [&](const Tensor& t, int64_t elements, const char* name) {
     same_device(t, first, name);
     if (!t.is_contiguous() || t.is_neg()) throw py::value_error(std::string(name) + " must be contiguous");
     if (t.numel() != elements) throw py::value_error(std::string(name) + " must have " + std::to_string(elements) + " elements, got " + std::to_string(t.numel()));
-    if (elements > 0 && !written.insert(t.data_ptr()).second) throw py::value_error(std::string(name) + " appears twice in one call");
+    range(t, name, true);
     return t.data_ptr();
   };
   std::vector<ffm_adamw_tensor> table(n);
@@ -512,6 +542,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
       held.push_back(g);
     }
     a.grad = g.data_ptr();
+    range(g, "grad", false);
     if (eight) {
       for (const Tensor* t : {&exp_avgs[i], &exp_avg_sqs[i]}) {
         if (t->scalar_type() != at::kFloat8_e4m3fn) throw py::type_error("8-bit states must be float8_e4m3fn, got " + std::string(c10::toString(t->scalar_type())));
@@ -535,6 +566,18 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
     }
     if (steps[i].scalar_type() != at::kInt) throw py::type_error("steps must be int32, got " + std::string(c10::toString(steps[i].scalar_type())));
     a.step = static_cast<int32_t*>(state(steps[i], 1, "step"));
+  }
+
+  if (lr_device.defined()) range(lr_device, "lr", false);
+  if (scale.defined()) range(scale, "grad_scale", false);
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+  // what was written or read so far, up to its furthest end
+  const char *written_to = nullptr, *read_to = nullptr;
+  for (const Range& r : ranges) {
+    if (r.from < written_to || (r.written && r.from < read_to)) {
+      throw py::value_error(std::string(r.name) + " appears twice in one call, or lies on another of its tensors");
+    }
+    (r.written ? written_to : read_to) = std::max(r.written ? written_to : read_to, r.to);
   }
 
   const On device(first);

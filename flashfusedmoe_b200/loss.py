@@ -14,7 +14,8 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index=-100, reduction
     """Softmax cross entropy of the logits hidden weight^T, which are never stored: with lse = log sum exp of a row's logits,
     lse - logit[target] + z_loss_coeff * lse^2 for every row, 0 where the target is ignore_index.
 
-    hidden [*, D] and weight [V, D] are CUDA tensors, D a multiple of 8, V any number; target [*] is int64. As in fused_moe()
+    hidden [*, D] and weight [V, D] are CUDA tensors, D a multiple of 8, V any number, both on 16 bytes
+    (as allocated; rows that are not contiguous are copied); target [*] is int64. As in fused_moe()
     the compute type is the autocast type if autocast is on, else hidden's, and has to be bfloat16; gradients come in the
     tensors' own types (the weight's, where that is float32, without a rounding in between). reduction: "mean" over the rows that
     are not ignored (NaN without any, with zero gradients), "sum", or "none" (float32 [*]). The result is float32.

@@ -26,8 +26,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
 
     masters (float32): the parameters that are updated, of which `params` then are the rounded copies. grad_scale: one
     float32 on the device that multiplies every gradient (a clipping coefficient). lr: a number, or one float32 on the
-    device, which a captured step reads at every replay. Everything runs on the current stream without a host wait and can be
-    captured."""
+    device, which a captured step reads at every replay. What is written lies on nothing else of the call. Everything runs on the
+    current stream without a host wait and can be captured."""
     _lib.native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, masters, exp_avg_scales, exp_avg_sq_scales, lr, betas[0],
                              betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF, _capturing(params))
 

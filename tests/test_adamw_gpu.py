@@ -467,3 +467,25 @@ def test_refusals():
     with pytest.raises(ValueError, match="8-bit"):
         t = Tensors([100], torch.float32, 8)
         adamw_step(t.params, t.grads, t.m, t.v, t.steps, lr=0.1, exp_avg_scales=t.m_scale)
+
+
+@pytest.mark.gpu
+def test_tensors_that_share_memory_are_refused():
+    from flashfusedmoe_b200 import adamw_step
+
+    def call(p, g, m, v, step, **h):
+        adamw_step([*p], [*g], [*m], [*v], [*step], lr=1e-3, **h)
+
+    room = torch.zeros(100000, device="cuda")
+    step = torch.zeros(4, dtype=torch.int32, device="cuda")
+    piece = [room[1000 * k:1000 * k + 1000] for k in range(9)]
+    call(piece[:2], piece[2:4], piece[4:6], piece[6:8], (step[0], step[1]))   # side by side is not on another
+    call(piece[:2], [piece[2]] * 2, piece[4:6], piece[6:8], (step[0], step[1]))   # gradients are only read
+    shifted = room[999:1999]
+    for p, g, m in (((piece[0], shifted), piece[2:4], piece[4:6]), (piece[:2], (shifted, piece[3]), piece[4:6]),
+                    ((piece[0], piece[5]), piece[2:4], (piece[4], shifted)), (piece[:2], (piece[2], piece[0]), piece[4:6])):
+        with pytest.raises(ValueError, match="lies on another"):
+            call(p, g, m, piece[6:8], (step[0], step[1]))
+    with pytest.raises(ValueError, match="lies on another"):
+        call(piece[:1], piece[1:2], piece[2:3], piece[3:4], (step[0],), grad_scale=room[500:501])
+    assert step.tolist() == [2, 2, 0, 0] and not room.any()

@@ -33,6 +33,12 @@ def test_layer_norm_rows(width):
     assert torch.equal(y[0], b) and torch.equal(y[rows - 65], b) and not dx[:64].any() and not dx[-128:-64].any()
 
 
+def test_a_row_longer_than_32_bits_say_is_refused():
+    from flashfusedmoe_b200 import layer_norm
+    with pytest.raises(ValueError, match="4294967304 values"):
+        layer_norm(torch.empty(1, (1 << 32) + 8, dtype=torch.bfloat16, device="cuda"))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_values(bits):
     from flashfusedmoe_b200 import adamw_step

@@ -315,3 +315,31 @@ def test_saved_input_may_not_change():
     x.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward(dy)
+
+
+@pytest.mark.gpu
+def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    """The gradients of such leaves would be added on the default stream, which takes no part in the capture."""
+    from flashfusedmoe_b200 import layer_norm, linear_cross_entropy
+    x = torch.randn(40, 64, device="cuda").bfloat16()
+    w = torch.randn(64, device="cuda", requires_grad=True)
+    head = torch.randn(100, 64, device="cuda").bfloat16().requires_grad_()
+    t = torch.randint(0, 100, (40,), device="cuda")
+    side = torch.cuda.Stream()
+    for call, leaf in ((lambda: layer_norm(x, w).float().sum(), w), (lambda: linear_cross_entropy(x, head, t), head)):
+        eager = call()
+        want, = torch.autograd.grad(eager, leaf, retain_graph=True)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            with pytest.raises(RuntimeError, match="before the capture"):
+                call()
+            with torch.no_grad():
+                call()
+        del eager
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got, = torch.autograd.grad(call(), leaf)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
