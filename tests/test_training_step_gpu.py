@@ -185,3 +185,32 @@ def test_a_compiled_model_breaks_its_graph_around_them():
     loss, grads = run(model)
     other, others = run(torch.compile(model, backend="aot_eager"))
     assert torch.equal(loss, other) and all(torch.equal(a, b) for a, b in zip(grads, others))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_recomputed_and_moved_operands_give_the_same_bits(reentrant):
+    """Checkpointing runs the forward calls again in the backward pass (and leaves them at the last saved tensor); hooks that move
+    saved tensors to the host hand back others."""
+    from torch.utils.checkpoint import checkpoint
+    from flashfusedmoe_b200 import layer_norm, linear_cross_entropy
+    torch.manual_seed(3)
+    x = torch.randn(40, WIDTH, device="cuda").bfloat16().requires_grad_()
+    w, b = (torch.randn(WIDTH, device="cuda", requires_grad=True) for _ in range(2))
+    head = torch.randn(VOCAB, WIDTH, device="cuda").bfloat16().requires_grad_()
+    target = torch.randint(0, VOCAB, (40,), device="cuda")
+
+    def normed(x):
+        return layer_norm(x, w, b)
+
+    def scored(x):
+        return linear_cross_entropy(normed(x), head, target)
+
+    for call, leaves in ((normed, (x, w, b)), (scored, (x, w, b, head))):
+        want = torch.autograd.grad(call(x).float().sum(), leaves)
+        x.grad = w.grad = b.grad = head.grad = None
+        checkpoint(call, x, use_reentrant=reentrant).float().sum().backward()
+        assert all(torch.equal(leaf.grad, g) for leaf, g in zip(leaves, want))
+        with torch.autograd.graph.save_on_cpu():
+            out = call(x)
+        assert all(torch.equal(p, g) for p, g in zip(torch.autograd.grad(out.float().sum(), leaves), want))
