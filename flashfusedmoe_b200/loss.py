@@ -22,7 +22,8 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index=-100, reduction
 
     With "mean" and "sum" the gradients are computed together with the loss, wherever hidden or weight requires one: under
     torch.no_grad() the call takes a third of the time. Scratch: 2 bytes an entry for as many rows as 2 GiB hold.
-    Differentiable once. A target outside of the vocabulary gives NaN, and raises from a later call as other device failures do."""
+    Differentiable once; a device's first call cannot be captured. A target outside of the vocabulary gives NaN, and raises from a
+    later call as other device failures do."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"Unknown reduction: {reduction}")
     for t, name in ((hidden, "hidden"), (weight, "weight"), (target, "target")):
@@ -43,6 +44,8 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index=-100, reduction
         raise TypeError(f"target must be int64, got {target.dtype}")
     if not z_loss_coeff >= 0.0:
         raise ValueError(f"z_loss_coeff must not be negative, got {z_loss_coeff}")
+    if not ops.has_status(hidden.device) and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the first call on a device cannot be captured: make one before")
     ops.raise_reported(hidden.device)
     return _lib.native().linear_cross_entropy(hidden, weight, target, ignore_index, _REDUCTIONS[reduction], z_loss_coeff, _piece_rows,
                                               ops.status_tensor(hidden.device).data_ptr(), ops.reported_word(hidden.device))

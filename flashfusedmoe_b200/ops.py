@@ -7,6 +7,7 @@ or without the built library every call raises.
 
 import ctypes
 import struct
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -14,6 +15,7 @@ import torch
 from . import _lib
 
 _status = {}
+_status_lock = threading.Lock()
 _workspaces = {}
 
 # Instrumentation used by bench.py: a launch counter (kernels of this library enqueued so far) and an
@@ -122,8 +124,18 @@ def status_tensor(device):
     if key is None:
         key = torch.cuda.current_device()
     if key not in _status:
-        _status[key] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+        with _status_lock:
+            if key not in _status:
+                word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.synchronize(key)   # calls on other streams use the word from here on
+                _status[key] = word
     return _status[key]
+
+
+def has_status(device):
+    """Whether a call on `device` has made its status word, which a captured call cannot: the word would be zeroed at replay."""
+    return device.index in _status
 
 
 def check_status(device=None):
@@ -162,8 +174,11 @@ def reported_word(device):
     if entry is None:
         if torch.cuda.is_current_stream_capturing():
             return 0
-        word = torch.zeros(1, dtype=torch.int32).pin_memory().numpy()
-        entry = _reported[device.index] = (word, word.ctypes.data)
+        with _status_lock:
+            entry = _reported.get(device.index)
+            if entry is None:
+                word = torch.zeros(1, dtype=torch.int32).pin_memory().numpy()
+                entry = _reported[device.index] = (word, word.ctypes.data)
     return entry[1]
 
 

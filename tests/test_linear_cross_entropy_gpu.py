@@ -351,3 +351,16 @@ def test_refusals():
     room = torch.zeros(10 * 64 + 1, device="cuda").bfloat16()
     with pytest.raises(RuntimeError, match="16 bytes|not supported"):
         linear_cross_entropy(room[1:].view(10, 64), w, t)
+
+
+@pytest.mark.gpu
+def test_the_first_call_on_a_device_is_not_captured(monkeypatch):
+    from flashfusedmoe_b200 import linear_cross_entropy, ops
+    monkeypatch.setattr(ops, "_status", {})
+    h, w, t = inputs(10, 64, 30)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            linear_cross_entropy(h, w, t)
+    linear_cross_entropy(h, w, t)
+    ops.check_status()

@@ -214,3 +214,41 @@ def test_recomputed_and_moved_operands_give_the_same_bits(reentrant):
         with torch.autograd.graph.save_on_cpu():
             out = call(x)
         assert all(torch.equal(p, g) for p, g in zip(torch.autograd.grad(out.float().sum(), leaves), want))
+
+
+@pytest.mark.gpu
+def test_steps_of_several_threads_at_once(monkeypatch):
+    """Each thread on a stream of its own, against the same steps one after the other; the first calls of all."""
+    import threading
+    from flashfusedmoe_b200 import adamw_step, layer_norm, linear_cross_entropy, ops
+    monkeypatch.setattr(ops, "_status", {})
+    monkeypatch.setattr(ops, "_reported", {})
+
+    def steps(seed, found):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            x = torch.randn(700, WIDTH, device="cuda", generator=g).bfloat16().requires_grad_()
+            w = torch.randn(WIDTH, device="cuda", generator=g).requires_grad_()
+            head = torch.randn(VOCAB, WIDTH, device="cuda", generator=g).bfloat16().requires_grad_()
+            target = torch.randint(0, VOCAB, (700,), device="cuda", generator=g)
+            moments = [torch.zeros(VOCAB, WIDTH, device="cuda") for _ in range(2)]
+            count = torch.zeros((), dtype=torch.int32, device="cuda")
+            for _ in range(40):
+                x.grad = w.grad = head.grad = None
+                linear_cross_entropy(layer_norm(x, w), head, target).backward()
+                adamw_step([head.detach()], [head.grad], moments[:1], moments[1:], [count], lr=1e-3)
+            torch.cuda.current_stream().synchronize()
+            found[seed] = [t.clone() for t in (x.grad, w.grad, head.detach(), *moments, count)]
+            torch.cuda.current_stream().synchronize()
+
+    at_once, alone = {}, {}
+    threads = [threading.Thread(target=steps, args=(seed, at_once)) for seed in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for seed in range(3):
+        steps(seed, alone)
+    assert len(at_once) == 3
+    for seed in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(at_once[seed], alone[seed]))
