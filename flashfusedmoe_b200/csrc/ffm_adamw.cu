@@ -12,7 +12,7 @@
 // the new m and v before they are rounded.
 //
 // Bytes a value: bf16 parameters, gradients and 8-bit states move 10, with fp32 states 22, with an fp32 master as well 28. With
-// 32-bit states memory is the bound (5.4-5.5 TB/s read and written); 8-bit states take some 55 instructions a value, which keep 60 %
+// 32-bit states memory is the bound (5.4-5.9 TB/s read and written); 8-bit states take 55-64 instructions a value, which keep 60-69 %
 // of the issue slots busy (3.8 TB/s without a master, 5.1 with one).
 // A block walks chunks of 4096 values, twice eight neighbours a thread, over all tensors as one list. Steps are counted on the
 // device, so that a captured step can be replayed: every block reads them, and the last block to finish raises them.
@@ -474,7 +474,7 @@ adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
             first = second;
           }
         } else {
-          // bound by memory; the stores of one half then lie beside the other's arithmetic (96 M with masters: 546 -> 511 us)
+          // bound by memory; the stores of one half then lie beside the other's arithmetic (96 M with masters, roots not yet exact: 546 -> 511 us)
           first.step(a, e0, h, rate[i], inverse[i], keys[i]);
           second.step(a, e0 + ADAMW_CHUNK / 2, h, rate[i], inverse[i], keys[i]);
         }
