@@ -74,7 +74,13 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but every state keeps its own type: there, floating states take their parameter's. Steps and unscaled
-        moments of another optimizer become int32 and float32."""
+        moments of another optimizer become int32 and float32; one whose step is another is refused."""
+        for group in state_dict["param_groups"]:
+            for name in ("amsgrad", "maximize"):
+                if group.get(name):
+                    raise ValueError(f"a state dict with {name} is of another step than AdamW's here")
+            if group["weight_decay"] != 0 and not group.get("decoupled_weight_decay", True):
+                raise ValueError("a state dict whose weight decay is part of the gradient is of another step than AdamW's here")
         saved = {i: {k: v for k, v in s.items() if torch.is_tensor(v)} for i, s in state_dict["state"].items()}
         own = [dict(g) for g in self.param_groups]
         super().load_state_dict(state_dict)

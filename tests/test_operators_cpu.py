@@ -52,6 +52,17 @@ def test_optimizer_arguments():
     assert AdamW(p).step(closure=lambda: 3.0) == 3.0   # nothing has a gradient
 
 
+def test_state_dicts_of_other_steps_are_refused():
+    p = [torch.nn.Parameter(torch.ones(2))]
+    for other in (torch.optim.AdamW(p, amsgrad=True), torch.optim.AdamW(p, maximize=True), torch.optim.Adam(p, weight_decay=0.1)):
+        with pytest.raises(ValueError, match="another step"):
+            AdamW(p).load_state_dict(other.state_dict())
+    for same in (torch.optim.AdamW(p, lr=0.5), torch.optim.Adam(p, lr=0.5)):
+        mine = AdamW(p)
+        mine.load_state_dict(same.state_dict())
+        assert mine.param_groups[0]["lr"] == 0.5 and mine.param_groups[0]["state_bits"] == 32
+
+
 def test_layer_norm_entry_points():
     lib, a = _lib.load(), 256
 
