@@ -87,6 +87,7 @@ class AdamW(torch.optim.Optimizer):
         for group, mine in zip(self.param_groups, own):   # options that another optimizer's groups do not have
             for name, value in mine.items():
                 group.setdefault(name, value)
+            group.pop("decoupled_weight_decay", None)   # it always is here
         order = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(order, params):
