@@ -117,7 +117,10 @@ loss_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ tar
       dot += part[2][w];
     }
   }
-  if (counts && known) sum = fmaxf(sum - expf(target_logits[row] - top), 0.0f) + expf(dot - top);
+  if (counts && known) {
+    const float rest = sum - expf(target_logits[row] - top);
+    sum = (rest < 0.0f ? 0.0f : rest) + expf(dot - top);  // (a maximum with zero would lose a NaN that some other logit brought)
+  }
   const float lse = logf(sum) + top;
   float scale = 0.0f;
   // a row with a target that is none has no gradient; its loss is NaN
