@@ -121,7 +121,9 @@ loss_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ tar
     const float rest = sum - expf(target_logits[row] - top);
     sum = (rest < 0.0f ? 0.0f : rest) + expf(dot - top);  // (a maximum with zero would lose a NaN that some other logit brought)
   }
-  const float lse = logf(sum) + top;
+  // The loss and p - 1 come from the margin: lse itself is rounded at the size of the logits, which may be far above their
+  // differences.
+  const float log_sum = logf(sum), lse = log_sum + top, margin = log_sum + (top - dot);
   float scale = 0.0f;
   // a row with a target that is none has no gradient; its loss is NaN
   if (counts && known && factor != nullptr) {
@@ -129,15 +131,15 @@ loss_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ tar
     // has no idea) its rounding would be the same in all of them, up to 2^-8 of the whole gradient.
     const float g = row_grad != nullptr ? row_grad[row] : 1.0f;
     scale = g * fmaf(2.0f * z, lse, 1.0f);
-    if (t == 0) target_entry[row] = g * fmaf(expf(dot - lse), 2.0f * z * lse, expm1f(dot - lse));
+    if (t == 0) target_entry[row] = g * fmaf(expf(-margin), 2.0f * z * lse, expm1f(-margin));
   }
   if (t == 0) {
-    nll[row] = counts ? (known ? fmaf(z * lse, lse, lse - dot) : NAN) : 0.0f;
+    nll[row] = counts ? (known ? fmaf(z * lse, lse, margin) : NAN) : 0.0f;
     if (counts && !known) atomicCAS(status, 0, FFM_STATUS_BAD_INDEX);
   }
   if (factor == nullptr) return;
   float* out = factor + row * pieces;
-  for (int h = t; h < pieces; h += TEAM) out[h] = scale != 0.0f ? expf(mine[h].x - lse) * scale : 0.0f;
+  for (int h = t; h < pieces; h += TEAM) out[h] = scale != 0.0f ? expf((mine[h].x - top) - log_sum) * scale : 0.0f;
 }
 
 // e (fp16) to dl (bf16) in place: eight entries a thread, 2048 a block, GRADIENT_ROWS rows of them at a time (a row a block took

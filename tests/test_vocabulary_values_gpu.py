@@ -50,3 +50,30 @@ def test_an_infinity_in_the_vocabulary(n):
     low = h[:, 2] < 0
     check(nll[low], {"nll": out["nll"][low]}, {"nll": bound["nll"][low]}, "nll")
     assert not nll[~low].isfinite().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 100, 1500])
+@pytest.mark.parametrize("size", [0.0, 28.0, 500.0, -500.0])
+def test_certain_rows_of_large_logits(rows, size):
+    """Two entries, size and size - 10: the loss log(1 + e^-10), and 1 - p, do not depend on size, which fp32 holds in steps of 2^-15 at
+    500. The sum is about 1 and is off by its roundings: three additions, the exponentials' and the logarithm's are less than 16 u in all."""
+    from flashfusedmoe_b200 import linear_cross_entropy
+    h = torch.zeros(rows, 8, device="cuda").bfloat16()
+    h[:, 0] = 1.0
+    h[:, 1] = 1.0
+    w = torch.zeros(2, 8, device="cuda").bfloat16()
+    w[:, 0] = size
+    w[1, 1] = -10.0
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    q = torch.exp(torch.tensor(-10.0, dtype=torch.float64, device="cuda"))
+    with torch.no_grad():
+        nll = linear_cross_entropy(h, w, t, reduction="none")
+    assert ((nll.double() - torch.log1p(q)).abs() <= 16 * U).all()
+    loss, dh, dw = run(h, w, t)
+    assert (loss.double() - torch.log1p(q)).abs() <= 16 * U
+    # dl = -(1 - p), 1 - p, each rounded to bf16, and so is their product with the rows' mean of 1 (times 1 / rows and rows times)
+    share = q / (1 + q)
+    for entry, sign in ((0, -1.0), (1, 1.0)):
+        got = dw[entry, 0].double() * sign
+        assert (got - share).abs() <= share * (2 * 2.0 ** -8 + 2.0 ** -10) + 16 * U
