@@ -452,8 +452,9 @@ __device__ __forceinline__ void glu_forward_half_step(uint32_t tcol, int act, fl
 // This warp's 32 rows x 128 vocabulary entries (from entry c0 on) of a tile of logits: lane = row, entries in TMEM columns
 // tcol .. tcol + 127. Two passes over TMEM, so that 32 values are held at a time and no exponential is taken twice: the largest
 // logit (and the target's, if it is here), then e = exp(logit - largest) and its sum. With `store` the e of 64 entries at a time
-// go to the row's piece of memory in fp16: in (0, 1] it has 11 bits, so that the gradient, which is rounded to bf16 later,
-// has seen one rounding that counts; what lies below 2^-24 of the largest of 128 is lost to it. The sum is of the unrounded e.
+// go to the row's piece of memory in fp16, times 2^15: down to 2^-29 of the largest of 128 (20 nats) they have 11 bits there, so that the
+// gradient, which is rounded to bf16 later, has seen one rounding that counts; what lies below 2^-40 of it (27 nats) is lost. The sum is of the
+// unrounded e.
 __device__ __forceinline__ void softmax_half_tile(const GemmParams& p, const CUtensorMap* out, uint32_t tcol, int c0, int half,
                                                   int row0, int lane, uint32_t stg, int& slot) {
   const int valid = min(128, p.pz_h - c0);
@@ -511,7 +512,7 @@ __device__ __forceinline__ void softmax_half_tile(const GemmParams& p, const CUt
           b = i + 1 < left ? b : 0.0f;
         }
         sum[j] += a + b;
-        __half2 h = __floats2half2_rn(a, b);
+        __half2 h = __floats2half2_rn(a * SOFTMAX_STORED_SCALE, b * SOFTMAX_STORED_SCALE);
         o[j] = *reinterpret_cast<uint32_t*>(&h);
       }
       if (store) st_shared_v4(box + box_offset(lane, (c >> 3 & 4) + q), o[0], o[1], o[2], o[3]);

@@ -53,9 +53,13 @@ int add_bf16(const void* a, const void* b, int64_t n, void* out, ffm_stream_t st
 
 // ---- products of the linear cross entropy (ffm_gemm_sm100.cu) ----
 
+// What softmax_logits' exponentials are stored times of: the largest of 128 is 2^15 then, and fp16 holds all of its 11 bits down to 2^-29 of
+// that one in place of 2^-14 (and something down to 2^-40 in place of 2^-25).
+constexpr float SOFTMAX_STORED_SCALE = 32768.0f;
+
 // Logits hidden [rows, D] weight [V, D]^T, a tile at a time and never stored: stats[n * ceil(V / 128) + h] = (largest,
 // sum of exp(logit - largest)) (pairs of floats) over row n's entries 128 h .. 128 h + 127, target_logits[n] the logit of targets[n] where that is
-// an entry; with `e` the exponentials in fp16, rows ld_e apart (a multiple of 8). D % 8 == 0.
+// an entry; with `e` the exponentials times SOFTMAX_STORED_SCALE in fp16, rows ld_e apart (a multiple of 8). D % 8 == 0.
 int softmax_logits(const void* hidden, const void* weight, int64_t rows, int D, int V, const int64_t* targets,
                    float* target_logits, float* stats, void* e, int64_t ld_e, int32_t* status, ffm_stream_t stream);
 

@@ -5,7 +5,7 @@
 //
 // The logits never exist: the product's epilogue (EPI_SOFTMAX, ffm_gemm_sm100.cu) leaves the maximum and the sum of exponentials of
 // every 128 entries of a row, 8 bytes in place of 512, and the target's logit. For the gradients it also leaves the exponentials
-// against those maxima in fp16, for one piece of the rows at a time. They become dl in bf16 in the same place once the row's lse is known: a
+// against those maxima in fp16, times 2^15, for one piece of the rows at a time. They become dl in bf16 in the same place once the row's lse is known: a
 // multiplication by exp(maximum - lse), which costs 4 bytes an entry; taking the product again instead would cost 2 D
 // operations an entry, more from D = 650 on (at 1.45 PFLOP/s and 6.4 TB/s). Every logit is computed once, and the three
 // products are all that is left: 6 N V D operations. Statistics, sums and the target's entry (p - 1, from expm1, since
@@ -60,7 +60,7 @@ __device__ __forceinline__ void join(float& top, float& sum, float other_top, fl
 }
 
 // From a row's maxima and sums to its loss, and (with `factor`) to what its pieces of 128 exponentials are multiplied by for the
-// gradient, exp(maximum - lse) times the row's factor. A row has TEAM threads: a warp, or a block where there are few rows.
+// gradient, exp(maximum - lse) times the row's factor, over what they are stored times of. A row has TEAM threads: a warp, or a block where there are few rows.
 //
 // The tensor core's sums lose some of their last bits over a long D (4096: 3e-6 of a logit). That hardly shows in lse, which is over
 // many entries, but in the target's logit it does; so that one is taken again here in fp32, and replaces the other in the
@@ -139,7 +139,9 @@ loss_rows_kernel(const float2* __restrict__ stats, const float* __restrict__ tar
   }
   if (factor == nullptr) return;
   float* out = factor + row * pieces;
-  for (int h = t; h < pieces; h += TEAM) out[h] = scale != 0.0f ? expf((mine[h].x - top) - log_sum) * scale : 0.0f;
+  for (int h = t; h < pieces; h += TEAM) {
+    out[h] = scale != 0.0f ? expf((mine[h].x - top) - log_sum) * scale * (1.0f / SOFTMAX_STORED_SCALE) : 0.0f;
+  }
 }
 
 // e (fp16) to dl (bf16) in place: eight entries a thread, 2048 a block, GRADIENT_ROWS rows of them at a time (a row a block took

@@ -77,3 +77,25 @@ def test_certain_rows_of_large_logits(rows, size):
     for entry, sign in ((0, -1.0), (1, 1.0)):
         got = dw[entry, 0].double() * sign
         assert (got - share).abs() <= share * (2 * 2.0 ** -8 + 2.0 ** -10) + 16 * U
+
+
+@pytest.mark.gpu
+def test_gradients_of_entries_far_below_the_largest():
+    """One entry dominates its piece of 128, others lie 1 to 26 nats below it, exactly. An exponential is held in fp16 as 2^15 of itself: 11 bits down to
+    2^-29 (20 nats), steps of 2^-39 below. Beside that, dl is rounded once, to bf16 (2^-8), and everything in fp32 adds less than 2^-16:
+    arguments of up to 38 in the exponential's base 2, rounded, are 38 u ln 2 of it. The products are with one row of ones."""
+    below = torch.arange(1, 27, dtype=torch.float64, device="cuda")
+    h = torch.zeros(1, 8, device="cuda").bfloat16()
+    h[0, 0] = 1.0
+    w = torch.zeros(300, 8, device="cuda").bfloat16()
+    w[:, 0] = -100.0
+    w[7, 0] = 0.0
+    w[20:46, 0] = -below.bfloat16()
+    t = torch.tensor([7], device="cuda")
+    lse = torch.log1p(torch.exp(-below).sum())
+    p = torch.exp(-below - lse)
+    _, dh, dw = run(h, w, t)
+    got = dw[20:46, 0].double()
+    limit = p * (2.0 ** -11 + 2.0 ** -8 + 2.0 ** -16) + torch.where(below > 20, 2.0 ** -40, 0.0)
+    assert ((got - p).abs() <= limit).all(), ((got - p).abs() / limit).tolist()
+    assert (got > 0).all()
