@@ -68,8 +68,11 @@ class AdamW(torch.optim.Optimizer):
             else:
                 for name in ("exp_avg", "exp_avg_sq"):
                     state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-            if group["master_weights"] and p.dtype != torch.float32:
-                state["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format)
+        # (also where a loaded state had none: made as late as this, since the parameters may be loaded after it)
+        if group["master_weights"] and p.dtype != torch.float32 and "master" not in state:
+            if _capturing([p]):
+                raise RuntimeError("a parameter's first AdamW step after loading makes its master and cannot be captured: take one step before")
+            state["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format)
         return state
 
     def load_state_dict(self, state_dict):
