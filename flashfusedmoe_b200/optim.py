@@ -32,6 +32,20 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
                              betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF, _capturing(params))
 
 
+def _in_8_bits(moment, root):
+    """A moment in 32 bits as codes and scales of adamw_step() (of its root). Rounded to nearest, the root too: this is done once, on loading."""
+    x = (moment.sqrt() if root else moment).reshape(-1)
+    blocks = torch.cat([x, x.new_zeros(-x.numel() % BLOCK)]).view(-1, BLOCK)
+    finite = blocks.isfinite()
+    top = torch.where(finite, blocks.abs(), 0.0).amax(1)
+    mantissa, exponent = torch.frexp(top)   # 448, the largest number, is 0.875 * 2^9
+    k = torch.where(top > 0, exponent - 9 + (mantissa > 0.875).int(), -126).clamp(-126, 120)
+    codes = torch.where(finite, torch.ldexp(blocks, -k[:, None]), torch.nan).to(torch.float8_e4m3fn).view(torch.uint8)
+    if root:
+        codes = torch.where(blocks > 0, codes.clamp(min=1), codes)
+    return codes.view(-1)[:x.numel()].clone().view(torch.float8_e4m3fn).view(moment.shape), (k + 127).to(torch.uint8)
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with a launch per parameter group. state_bits = 8 holds both moments of tensors of at least `min_8bit_size`
     values in 8 bits (2 bytes a parameter instead of 8; adamw_step() says how), those of smaller ones, where nothing is to
@@ -77,7 +91,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but every state keeps its own type: there, floating states take their parameter's. Steps and unscaled
-        moments of another optimizer become int32 and float32; one whose step is another is refused."""
+        moments of another optimizer become int32 and float32, or 8 bits where the group's state_bits says so; one whose step is another
+        is refused."""
         for group in state_dict["param_groups"]:
             for name in ("amsgrad", "maximize"):
                 if group.get(name):
@@ -92,8 +107,8 @@ class AdamW(torch.optim.Optimizer):
                 group.setdefault(name, value)
             group.pop("decoupled_weight_decay", None)   # it always is here
         order = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(order, params):
+        params = [(p, g) for g in self.param_groups for p in g["params"]]
+        for i, (p, group) in zip(order, params):
             old = saved.get(i, {})
             for name, value in old.items():
                 kind = value.dtype
@@ -102,6 +117,9 @@ class AdamW(torch.optim.Optimizer):
                 elif name in ("exp_avg", "exp_avg_sq") and name + "_scale" not in old:
                     kind = torch.float32
                 self.state[p][name] = value.detach().to(p.device, kind, copy=True).contiguous()
+            if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"] and "exp_avg" in old and "exp_avg_scale" not in old:
+                for name in ("exp_avg", "exp_avg_sq"):
+                    self.state[p][name], self.state[p][name + "_scale"] = _in_8_bits(self.state[p][name], root=name == "exp_avg_sq")
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale=None):

@@ -71,3 +71,76 @@ def test_a_step_that_makes_a_master_is_not_captured():
             opt.step()
     opt.step()
     assert "master" in opt.state[p]
+
+
+def _decoded(codes, scale, root=False):
+    x = codes.reshape(-1).double() * torch.pow(2.0, scale.double() - 127).repeat_interleave(128)[:codes.numel()]
+    return (x * x if root else x).view(codes.shape)
+
+
+@pytest.mark.parametrize("shape", [(5000,), (33, 129), (4096,)])
+def test_loaded_moments_are_held_in_8_bits_where_the_group_says_so(shape):
+    """To nearest: half a step, 2^-4 of a value or 2^-10 of its block's scale, of the root for the second moment (twice that of the
+    moment itself, and its square); the root itself is off by 2^-24."""
+    from flashfusedmoe_b200 import AdamW
+    n = torch.Size(shape).numel()
+    p, state = _torchs(torch.float32, "cpu", size=n)
+    with torch.no_grad():
+        s = state["state"][0]
+        s["exp_avg"].mul_(torch.logspace(-12, 3, n))
+        s["exp_avg_sq"].mul_(torch.logspace(-40, 3, n))
+        s["exp_avg"][:300] = s["exp_avg_sq"][:300] = 0.0
+        s["exp_avg"][200], s["exp_avg_sq"][201], s["exp_avg"][202] = float("nan"), float("inf"), 3.0
+    p = torch.nn.Parameter(p.detach().view(shape))
+    s["exp_avg"], s["exp_avg_sq"] = s["exp_avg"].view(shape), s["exp_avg_sq"].view(shape)
+    opt = AdamW([p], state_bits=8)
+    opt.load_state_dict(state)
+    mine = opt.state[p]
+    for name, root in (("exp_avg", False), ("exp_avg_sq", True)):
+        codes, scale = mine[name], mine[name + "_scale"]
+        assert codes.dtype == torch.float8_e4m3fn and codes.shape == torch.Size(shape) and codes.is_contiguous()
+        assert scale.dtype == torch.uint8 and scale.numel() == (n + 127) // 128
+        want = s[name].view(-1).double()
+        want = want.sqrt() if root else want
+        got = _decoded(codes, scale).view(-1)
+        finite = want.isfinite()
+        assert got[~finite].isnan().all() and got[finite].isfinite().all()
+        unit = torch.pow(2.0, scale.double() - 127).repeat_interleave(128)[:n]
+        limit = torch.maximum(want.abs() * (2.0 ** -4 + 2.0 ** -23), unit * 2.0 ** -10)
+        if root:
+            assert ((got > 0) == (want > 0))[finite].all()
+            limit = torch.where(got == unit * 2.0 ** -9, unit * 2.0 ** -9, limit)   # what would be zero is the least number
+        assert ((got - want).abs() <= limit)[finite].all()
+        # the least power of two that holds the block's largest
+        top = torch.where(finite, want.abs(), 0.0)
+        top = torch.cat([top, top.new_zeros(-n % 128)]).view(-1, 128).amax(1)
+        k = torch.pow(2.0, scale.double() - 127)
+        assert (top <= 448 * k * (1 + 2.0 ** -23)).all() and ((top > 224 * k * (1 - 2.0 ** -23)) | (scale == 1)).all()
+    assert mine["step"].item() == 3
+    # what is smaller than the group's bound stays in 32 bits, as do groups of 32
+    for options in ({"state_bits": 8, "min_8bit_size": n + 1}, {}):
+        other = AdamW([p], **options)
+        other.load_state_dict(state)
+        assert other.state[p]["exp_avg"].dtype == torch.float32 and "exp_avg_scale" not in other.state[p]
+
+
+@pytest.mark.gpu
+def test_a_step_after_moments_were_loaded_into_8_bits():
+    """The kernel reads the loaded moments as they were written: without gradients they fall by their factors, and the parameter moves by their quotient."""
+    from flashfusedmoe_b200 import AdamW
+    p, state = _torchs(torch.float32, "cuda", size=5003)
+    opt = AdamW([p], state_bits=8, weight_decay=0.0)
+    opt.load_state_dict(state)
+    s = opt.state[p]
+    m = _decoded(s["exp_avg"], s["exp_avg_scale"])
+    v = _decoded(s["exp_avg_sq"], s["exp_avg_sq_scale"], root=True)
+    group = opt.param_groups[0]
+    (b1, b2), lr, eps, decay = group["betas"], group["lr"], group["eps"], group["weight_decay"]
+    old = p.detach().double()
+    p.grad = torch.zeros_like(p)
+    opt.step()
+    update = lr / (1 - b1 ** 4) * (b1 * m) / ((b2 * v / (1 - b2 ** 4)).sqrt() + eps)
+    want = old * (1 - lr * decay) - update
+    # as in test_adamw_gpu: 32 u of the update, 4 u of the parameter, and 4 u of either moment
+    assert ((p.detach().double() - want).abs() <= 2.0 ** -24 * (40 * update.abs() + 8 * old.abs())).all()
+    assert s["step"].item() == 4
