@@ -93,15 +93,28 @@ class AdamW(torch.optim.Optimizer):
         """As torch's, but every state keeps its own type: there, floating states take their parameter's. Steps and unscaled
         moments of another optimizer become int32 and float32, or 8 bits where the group's state_bits says so; one whose step is another
         is refused."""
-        for group in state_dict["param_groups"]:
-            for name in ("amsgrad", "maximize"):
-                if group.get(name):
-                    raise ValueError(f"a state dict with {name} is of another step than AdamW's here")
-            if group["weight_decay"] != 0 and not group.get("decoupled_weight_decay", True):
-                raise ValueError("a state dict whose weight decay is part of the gradient is of another step than AdamW's here")
-        saved = {i: {k: v for k, v in s.items() if torch.is_tensor(v)} for i, s in state_dict["state"].items()}
         own = [dict(g) for g in self.param_groups]
-        super().load_state_dict(state_dict)
+        given = {}
+
+        def look(_, state_dict):   # what the hooks before made of it
+            for group in state_dict["param_groups"]:
+                for name in ("amsgrad", "maximize"):
+                    if group.get(name):
+                        raise ValueError(f"a state dict with {name} is of another step than AdamW's here")
+                if group["weight_decay"] != 0 and not group.get("decoupled_weight_decay", True):
+                    raise ValueError("a state dict whose weight decay is part of the gradient is of another step than AdamW's here")
+            given.update(state_dict)
+
+        # last of the hooks before loading, first of those after it
+        hooks = [self.register_load_state_dict_pre_hook(look),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_states(given, own), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_states(self, state_dict, own):
         for group, mine in zip(self.param_groups, own):   # options that another optimizer's groups do not have
             for name, value in mine.items():
                 group.setdefault(name, value)
@@ -109,7 +122,7 @@ class AdamW(torch.optim.Optimizer):
         order = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [(p, g) for g in self.param_groups for p in g["params"]]
         for i, (p, group) in zip(order, params):
-            old = saved.get(i, {})
+            old = {k: v for k, v in state_dict["state"].get(i, {}).items() if torch.is_tensor(v)}
             for name, value in old.items():
                 kind = value.dtype
                 if name == "step":

@@ -144,3 +144,42 @@ def test_a_step_after_moments_were_loaded_into_8_bits():
     # as in test_adamw_gpu: 32 u of the update, 4 u of the parameter, and 4 u of either moment
     assert ((p.detach().double() - want).abs() <= 2.0 ** -24 * (40 * update.abs() + 8 * old.abs())).all()
     assert s["step"].item() == 4
+
+
+def test_hooks_see_and_change_what_is_loaded():
+    """A hook may hand back another state dict (fewer states, other values, other options); hooks after loading see it as it stays."""
+    from flashfusedmoe_b200 import AdamW
+    p, state = _torchs(torch.bfloat16, "cpu")
+    q = torch.nn.Parameter(torch.ones(7))
+    theirs = torch.optim.AdamW([p, q], lr=1e-3)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    theirs.step()
+    opt = AdamW([p, q])
+    seen = []
+
+    def other(_, state_dict):
+        first = dict(state_dict["state"][0])
+        first["exp_avg"] = first["exp_avg"] * 0.5
+        return {"state": {0: first}, "param_groups": [dict(g, lr=0.25) for g in state_dict["param_groups"]]}
+
+    handles = [opt.register_load_state_dict_pre_hook(other),
+               opt.register_load_state_dict_post_hook(lambda o: seen.append({k: v.dtype for k, v in o.state[p].items()}))]
+    state = theirs.state_dict()
+    opt.load_state_dict(state)
+    assert torch.equal(opt.state[p]["exp_avg"], state["state"][0]["exp_avg"].float() * 0.5) and not opt.state[q]
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["state_bits"] == 32
+    assert seen == [{"step": torch.int32, "exp_avg": torch.float32, "exp_avg_sq": torch.float32}]
+    # a hook that turns a state dict into one that can be loaded, or into one that cannot
+    handles[0].remove()
+    turn = opt.register_load_state_dict_pre_hook(
+        lambda _, s: {**s, "param_groups": [dict(g, amsgrad=not g["amsgrad"]) for g in s["param_groups"]]})
+    odd = {**state, "param_groups": [dict(g, amsgrad=True) for g in state["param_groups"]]}
+    opt.load_state_dict(odd)
+    assert torch.equal(opt.state[p]["exp_avg"], state["state"][0]["exp_avg"].float())
+    before = {k: v.clone() for k, v in opt.state[p].items()}
+    with pytest.raises(ValueError, match="another step"):
+        opt.load_state_dict(state)
+    assert all(torch.equal(v, before[k]) for k, v in opt.state[p].items())
+    # the hooks that loading itself uses are gone again
+    turn.remove()
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == 0 and len(opt._optimizer_load_state_dict_post_hooks) == 1
