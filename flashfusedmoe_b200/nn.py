@@ -68,7 +68,10 @@ class MoELayer(nn.Module):
         self._ep_group = None
         self._ep_size = 1
 
-        self.norm = LayerNorm(d_model, eps=norm_eps) if pre_norm else None
+        # only where asked for: a subclass may have a `norm` or `pre_norm` of its own
+        self._pre_norm = pre_norm
+        if pre_norm:
+            self.norm = LayerNorm(d_model, eps=norm_eps)
         self.gate = nn.Linear(d_model, num_experts, bias=False)
         nn.init.kaiming_uniform_(self.gate.weight, a=math.sqrt(5))
         self.gate.weight.data *= 0.01
@@ -89,12 +92,17 @@ class MoELayer(nn.Module):
             self.proj_down = nn.Linear(d_model, latent_dim, bias=False)
             self.proj_up = nn.Linear(latent_dim, d_model, bias=False)
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "_pre_norm" not in state:   # pickled before there was the option, or before there was this attribute
+            self._pre_norm = isinstance(self._modules.get("norm"), LayerNorm)
+
     def forward(self, x):
         """x [*, D] -> ([*, D], dict)."""
         leading = x.shape[:-1]
         D = x.shape[-1]
         x_flat = x.reshape(-1, D)
-        if self.norm is not None:
+        if self._pre_norm:
             x_flat = self.norm(x_flat)
 
         shared_weights = None
