@@ -5,7 +5,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <atomic>
@@ -67,7 +69,20 @@ class On {
   c10::Device device_;
 };
 
+// What goes past torch's dispatcher: a tangent would be dropped, and a trace would record an output that nothing fills.
+void no_tangent(const Tensor& t, const char* name) {
+  if (t.defined() && t._fw_grad(0).defined()) {
+    throw std::runtime_error(std::string(name) + " carries a forward-mode tangent: there are no forward-mode derivatives here");
+  }
+}
+void not_traced(const char* what) {
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value()) {
+    throw std::runtime_error(std::string(what) + " cannot be traced");
+  }
+}
+
 void on_gpu(const Tensor& t, const char* name) {
+  no_tangent(t, name);
   if (!t.is_cuda()) {
     throw std::runtime_error(std::string(name) + " must be a CUDA tensor: flashfusedmoe_b200 has no CPU path");
   }
@@ -266,7 +281,11 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  not_traced("layer_norm");
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  no_tangent(x, "x");
+  no_tangent(w, "weight");
+  no_tangent(b, "bias");
   const py::gil_scoped_release released;
   if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()))) {
     capturable({&x, &w, &b});
@@ -392,6 +411,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     {
       const at::AutoGradMode no_grad(false);
       const bool want_hidden = ctx->needs_input_grad(0), want_weight = ctx->needs_input_grad(1);
+      no_tangent(grad[0], "the gradient of the loss");
       const Tensor factor = plain(grad[0].to(at::kFloat));
       Tensor dh, dw;
       auto take = [&](const char* name, bool want, Tensor& to) {
@@ -419,6 +439,9 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
 
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& target, int64_t ignore_index, int64_t reduction, double z,
                             int64_t piece_rows, int64_t status, int64_t status_host) {
+  not_traced("linear_cross_entropy");
+  no_tangent(hidden, "hidden");
+  no_tangent(weight, "weight");
   const py::gil_scoped_release released;
   const Tensor t = plain(target);
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
@@ -452,6 +475,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
                    const Tensors& steps, const std::optional<Tensors>& masters, const std::optional<Tensors>& exp_avg_scales,
                    const std::optional<Tensors>& exp_avg_sq_scales, const py::object& lr, double beta1, double beta2, double eps,
                    double weight_decay, const OptTensor& grad_scale, int64_t seed, bool capturing) {
+  not_traced("adamw_step");
   const size_t n = params.size();
   const bool eight = exp_avg_scales.has_value();
   auto length = [n](size_t other, const char* name) {
