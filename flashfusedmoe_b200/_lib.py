@@ -102,6 +102,7 @@ SIGNATURES = {
     "ffm_adamw_step": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
     "ffm_linear_cross_entropy_workspace_bytes": (c_size_t, [c_void_p]),
     "ffm_linear_cross_entropy": (c_int, [c_void_p, c_void_p]),
+    "ffm_capture_id": (ctypes.c_uint64, [c_void_p]),
     "ffm_scale_many": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "ffm_route_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "ffm_route_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -111,7 +112,8 @@ SIGNATURES = {
 
 # called by the torch extension itself (csrc/ffm_torch_ops.cpp)
 NATIVE_OPS = ("ffm_error_string", "ffm_layer_norm_forward", "ffm_layer_norm_workspace_bytes", "ffm_layer_norm_backward",
-              "ffm_adamw_step", "ffm_linear_cross_entropy", "ffm_linear_cross_entropy_workspace_bytes", "ffm_scale_many")
+              "ffm_adamw_step", "ffm_linear_cross_entropy", "ffm_linear_cross_entropy_workspace_bytes", "ffm_scale_many",
+              "ffm_capture_id")
 
 _lib = None
 _native = None

@@ -22,3 +22,13 @@ extern "C" const char* ffm_error_string(int code) {
     default: return "unknown code";
   }
 }
+
+extern "C" uint64_t ffm_capture_id(ffm_stream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();  // the default stream beside another's capture: not part of it
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}

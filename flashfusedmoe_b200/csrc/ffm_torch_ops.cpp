@@ -37,6 +37,7 @@ decltype(&ffm_adamw_step) adamw = nullptr;
 decltype(&ffm_linear_cross_entropy) cross_entropy = nullptr;
 decltype(&ffm_linear_cross_entropy_workspace_bytes) cross_entropy_workspace = nullptr;
 decltype(&ffm_scale_many) scale_many = nullptr;
+decltype(&ffm_capture_id) capture_id = nullptr;
 
 void bind_ops(const std::unordered_map<std::string, uintptr_t>& at) {
   auto take = [&](const char* name, auto& f) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(at.at(name)); };
@@ -48,6 +49,7 @@ void bind_ops(const std::unordered_map<std::string, uintptr_t>& at) {
   take("ffm_linear_cross_entropy", cross_entropy);
   take("ffm_linear_cross_entropy_workspace_bytes", cross_entropy_workspace);
   take("ffm_scale_many", scale_many);
+  take("ffm_capture_id", capture_id);
 }
 
 void check(int rc, const char* what) {
@@ -385,7 +387,9 @@ Tensor as_bf16(const Tensor& t) { return plain(t.scalar_type() == at::kBFloat16 
 // Where the loss is one number, its gradients are computed with it, while the exponentials of a piece of rows are there: with them
 // taken again in the backward pass a step would have four large products instead of three. The backward pass multiplies them by
 // its factor, in place, which does nothing where that is 1. It hands them out once; a second backward pass over the same graph
-// computes them again. With a value for each row the factors come with the backward pass, and so do the products.
+// computes them again. A backward pass that is not in the loss's own capture may run more often than the loss (a graph of its own,
+// replayed): it takes a copy, or computes the gradients again where the loss was not captured and is not there to be read by replays. With a value
+// for each row the factors come with the backward pass, and so do the products.
 class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
  public:
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& target,
@@ -398,6 +402,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     ctx->save_for_backward({hidden, weight, target});
     ctx->saved_data["call"] = std::vector<int64_t>{ignore_index, reduction, piece_rows, status, status_host};
     ctx->saved_data["z"] = z;
+    if (now) ctx->saved_data["capture"] = static_cast<int64_t>(capture_id(On(hidden).stream()));
     if (r.d_hidden.defined()) ctx->saved_data["d_hidden"] = r.d_hidden;
     if (r.d_weight.defined()) ctx->saved_data["d_weight"] = r.d_weight;
     return now ? r.loss : r.nll.view(target.sizes());
@@ -414,11 +419,14 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
       no_tangent(grad[0], "the gradient of the loss");
       const Tensor factor = plain(grad[0].to(at::kFloat));
       Tensor dh, dw;
+      const int64_t now = static_cast<int64_t>(capture_id(On(hidden).stream()));
+      const auto made = ctx->saved_data.find("capture");
+      const int64_t then = made == ctx->saved_data.end() ? 0 : made->second.toInt();
       auto take = [&](const char* name, bool want, Tensor& to) {
         auto it = ctx->saved_data.find(name);
-        if (it == ctx->saved_data.end()) return;
-        if (want) to = it->second.toTensor();
-        ctx->saved_data.erase(it);
+        if (it == ctx->saved_data.end() || (then == 0 && now != 0)) return;
+        if (want) to = now == then ? it->second.toTensor() : it->second.toTensor().clone();
+        if (now == then) ctx->saved_data.erase(it);
       };
       take("d_hidden", want_hidden, dh);
       take("d_weight", want_weight, dw);

@@ -79,6 +79,9 @@ typedef void* ffm_stream_t; /* cudaStream_t */
 int ffm_version(void);
 const char* ffm_error_string(int code);
 
+/* The id of the capture that `stream` is part of, 0 where it is not captured. Different captures have different ids. */
+uint64_t ffm_capture_id(ffm_stream_t stream);
+
 /* Rows a grouped buffer must hold for T routed rows over E experts: 256 * floor((T + 255 E) / 256). */
 int64_t ffm_rows_capacity(int64_t T, int E);
 
