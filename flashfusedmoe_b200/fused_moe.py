@@ -23,6 +23,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.multiprocessing.reductions import StorageWeakRef
 
 from . import _lib, ops
 import os
@@ -66,6 +67,7 @@ _EP_DIRECT = os.environ.get("FFM_EP_DIRECT", "1") != "0"
 # backward pass always runs in bf16 on the saved bf16 tensors.
 _EXPERT_GEMM = "bf16"
 _fp8_weight_cache = {}
+_replayed = {}   # address -> weak reference to a storage that captured calls write
 
 
 def set_expert_gemm_precision(mode):
@@ -78,12 +80,31 @@ def set_expert_gemm_precision(mode):
     return old
 
 
+def written_by_replays(tensors):
+    """A captured call writes `tensors`: its replays do so without raising their versions, so no copy of them is kept from now on."""
+    for t in tensors:
+        storage = t.untyped_storage()
+        _replayed[storage.data_ptr()] = StorageWeakRef(storage)
+
+
+def _is_written_by_replays(t):
+    at = t.untyped_storage().data_ptr()
+    ref = _replayed.get(at)
+    if ref is not None and ref.expired():   # the address is another tensor's now
+        del _replayed[at]
+        ref = None
+    return ref is not None
+
+
 def _quantized_weight(owner, w):
     """e4m3 copy of the weight tensor `w` [E, N, K] (bf16, possibly a cast copy of `owner`) with one scale per expert.
     Cached per owner, the caller's own weight tensor (normally an nn.Parameter): the entry is reused while that very
     object is alive, unmodified (same version counter) and still where it was; a weak reference drops the entry
-    when the owner dies, so an address reused by another tensor can never hit a stale entry."""
+    when the owner dies, so an address reused by another tensor can never hit a stale entry. Weights that a captured optimizer step writes
+    change without a new version: theirs are made at every call."""
     import weakref
+    if _replayed and _is_written_by_replays(owner):
+        return ops.quantize_weight_e4m3(w)
     key = id(owner)
     hit = _fp8_weight_cache.get(key)
     if hit is not None and hit[0]() is owner and hit[1] == (owner._version, owner.data_ptr(), tuple(owner.shape)):

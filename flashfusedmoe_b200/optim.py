@@ -3,6 +3,7 @@
 import torch
 
 from . import _lib
+from .fused_moe import written_by_replays
 
 BLOCK = 128   # values of a tensor that share a scale in an 8-bit state
 
@@ -28,8 +29,11 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     float32 on the device that multiplies every gradient (a clipping coefficient). lr: a number, or one float32 on the
     device, which a captured step reads at every replay. What is written lies on nothing else of the call. Everything runs on the
     current stream without a host wait and can be captured."""
+    capturing = _capturing(params)
     _lib.native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, masters, exp_avg_scales, exp_avg_sq_scales, lr, betas[0],
-                             betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF, _capturing(params))
+                             betas[1], eps, weight_decay, grad_scale, seed & 0xFFFFFFFF, capturing)
+    if capturing:
+        written_by_replays(params)
 
 
 def _in_8_bits(moment, root):

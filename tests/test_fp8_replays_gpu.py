@@ -1,0 +1,48 @@
+"""GPU: the e4m3 copies of expert weights beside captured optimizer steps."""
+
+import gc
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import flashfusedmoe_b200 as ffm  # noqa: E402
+
+DEV = "cuda"
+layer_module = sys.modules["flashfusedmoe_b200.fused_moe"]   # the package has the function under this name
+
+
+def test_fp8_copies_of_weights_that_replays_update():
+    """A replayed step changes weights without raising their version: the e4m3 copy of an earlier call is not theirs."""
+    torch.manual_seed(2)
+    layer = ffm.MoELayer(256, 512, 4, top_k=2).to(DEV).bfloat16()
+    opt = ffm.AdamW([layer.w_up, layer.w_down], lr=0.05)
+    x = torch.randn(2048, 256, device=DEV).bfloat16()
+    for p in (layer.w_up, layer.w_down):
+        p.grad = torch.randn_like(p)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    old = ffm.set_expert_gemm_precision("fp8")
+    try:
+        with torch.no_grad():
+            for _ in range(3):
+                out, _ = layer(x)
+                fresh = ffm.MoELayer(256, 512, 4, top_k=2).to(DEV).bfloat16()
+                fresh.load_state_dict(layer.state_dict())
+                assert torch.equal(out, fresh(x)[0])
+                graph.replay()
+    finally:
+        ffm.set_expert_gemm_precision(old)
+    # once the weights are gone their address may be another tensor's
+    assert layer_module._is_written_by_replays(layer.w_up)
+    at = layer.w_up.untyped_storage().data_ptr()
+    opt.state.clear()
+    del layer, opt, graph, p
+    gc.collect()
+    ref = layer_module._replayed.get(at)
+    assert ref is None or ref.expired()
