@@ -110,6 +110,8 @@ def _quantized_weight(owner, w):
     if hit is not None and hit[0]() is owner and hit[1] == (owner._version, owner.data_ptr(), tuple(owner.shape)):
         return hit[2], hit[3]
     q, sc = ops.quantize_weight_e4m3(w)
+    if torch.cuda.is_current_stream_capturing():
+        return q, sc   # the graph's: nothing fills them before a replay
     try:
         ref = weakref.ref(owner, lambda _r, k=key: _fp8_weight_cache.pop(k, None))
     except TypeError:

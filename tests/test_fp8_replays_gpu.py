@@ -46,3 +46,27 @@ def test_fp8_copies_of_weights_that_replays_update():
     gc.collect()
     ref = layer_module._replayed.get(at)
     assert ref is None or ref.expired()
+
+
+def test_fp8_copies_made_in_a_capture_are_not_kept():
+    """They are not filled before a replay."""
+    torch.manual_seed(4)
+    layer = ffm.MoELayer(256, 512, 4, top_k=2).to(DEV).bfloat16()
+    x = torch.randn(2048, 256, device=DEV).bfloat16()
+    with torch.no_grad():
+        layer(x)
+        torch.cuda.synchronize()
+        old = ffm.set_expert_gemm_precision("fp8")
+        try:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                captured, _ = layer(x)
+            eager, _ = layer(x)
+            twin = ffm.MoELayer(256, 512, 4, top_k=2).to(DEV).bfloat16()
+            twin.load_state_dict(layer.state_dict())
+            want, _ = twin(x)
+            assert torch.equal(eager, want)
+            graph.replay()
+            assert torch.equal(captured, want)
+        finally:
+            ffm.set_expert_gemm_precision(old)
