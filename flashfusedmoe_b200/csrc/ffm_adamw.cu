@@ -12,8 +12,10 @@
 // the new m and v before they are rounded.
 //
 // Bytes a value: bf16 parameters, gradients and 8-bit states move 10, with fp32 states 22, with an fp32 master as well 28. With
-// 32-bit states memory is the bound (5.4-5.9 TB/s read and written); 8-bit states take 55-64 instructions a value, which keep 60-69 %
-// of the issue slots busy (3.8 TB/s without a master, 5.1 with one).
+// 32-bit states memory is the bound (5.4-5.9 TB/s read and written). 8-bit states take 55-64 instructions a value: 60-69 % of the issue
+// slots at 59 % of the memory's rate (3.8 TB/s without a master, 5.1 with one), neither of them full, so that waiting for loads, of which 24
+// warps an SM have two halves of a chunk in flight, is what is left. Tensors of mixed types (bf16 parameters with fp32 gradients) go value
+// by value where their states are: 96 M in 1.88 ms with 32-bit states, 0.81 with 8-bit ones.
 // A block walks chunks of 4096 values, twice eight neighbours a thread, over all tensors as one list. Steps are counted on the
 // device, so that a captured step can be replayed: every block reads them, and the last block to finish raises them.
 #include "ffm_types.cuh"
@@ -102,7 +104,7 @@ __device__ __noinline__ uint32_t e4m3_random_any(float v, float scale, uint32_t 
   return v > 0.0f ? max(code, 1u) : 0u;
 }
 
-// Random bits of a pair of neighbouring values (16 each): two rounds of multiply and fold over a counter.
+// Random bits of a pair of neighbouring values (16 each): the finaliser of MurmurHash3 (two rounds of multiply and fold) over a counter.
 __device__ __forceinline__ uint32_t random_pair(uint32_t pair, uint32_t key) {
   uint32_t h = pair * 0x9E3779B1u + key;
   h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
@@ -467,14 +469,15 @@ adamw_kernel(const __grid_constant__ AdamWJob<MAX> job) {
         first.load(a, e0);
         second.load(a, e0 + ADAMW_CHUNK / 2);
         if (EIGHT) {
-          // one copy of the code, which is bound by instructions (128 M bf16 values: 370 -> 352 us)
+          // one copy of the code (128 M bf16 values with masters: 408 us, with two copies 428; without masters 350 and 352)
 #pragma unroll 1
           for (int half = 0; half < 2; ++half) {
             first.step(a, e0 + half * (ADAMW_CHUNK / 2), h, rate[i], inverse[i], keys[i]);
             first = second;
           }
         } else {
-          // bound by memory; the stores of one half then lie beside the other's arithmetic (96 M with masters, roots not yet exact: 546 -> 511 us)
+          // bound by memory; the stores of one half then lie beside the other's arithmetic (96 M bf16 values with masters: 475 us, with one copy
+          // of the code 536; fp32 values 514 and 519)
           first.step(a, e0, h, rate[i], inverse[i], keys[i]);
           second.step(a, e0 + ADAMW_CHUNK / 2, h, rate[i], inverse[i], keys[i]);
         }

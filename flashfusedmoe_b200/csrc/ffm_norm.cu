@@ -35,8 +35,8 @@ constexpr int STREAM_THREADS = 1024;      // forward: 64 registers
 constexpr int STREAM_BACK_THREADS = 512;  // backward: 128, 64 of them sums of dw and db
 static_assert(STREAM_THREADS / 64 <= 16 && STREAM_BACK_THREADS / 64 <= 15, "a barrier for every team of more than a warp");
 constexpr int STREAM_SMEM = 226 << 10;
-// The same for rows off 16-byte boundaries. A stage is being filled while a row is worked on; the backward kernel needs 140
-// registers (with 512 threads it spilled, and took 98 us for 16384 x 1025 bf16).
+// The same for rows off 16-byte boundaries. A stage is being filled while a row is worked on; the backward kernel needs 168
+// registers (at 512 threads there are 128: it spilled, and took 98 us for 16384 x 1025 bf16, where it takes 55).
 constexpr int SHIFTED_THREADS = 768, SHIFTED_BACK_THREADS = 384, SHIFTED_STAGES = 3;
 
 template <typename T>
@@ -460,7 +460,7 @@ struct Trips {
   }
 };
 
-// s / n, rounded as a division would for whole results, with inv = 1 / n
+// s / n, rounded as a division would for whole results, with inv = 1 / n: one step of correction by the residual, Markstein's method
 __device__ __forceinline__ float quotient(float s, float n, float inv) {
   const float q = s * inv;
   return fmaf(fmaf(-q, n, s), inv, q);
@@ -674,8 +674,9 @@ layer_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict_
 // Rows of odd width start anywhere. Read value by value they took ten times as long as their bytes (4093 x 2051 fp16: 48 us
 // forward, 80 backward; here 20 and 27, bound by instructions: two to four times the time of rows on 16 bytes). Here the 16-byte pieces that cover a row are copied to shared memory as they lie, and values are taken from there: a
 // thread has pairs of neighbours (fp32: single values), side by side with its neighbours' pairs, out of two words and a shift where
-// the row starts in the middle of one. What a piece has beside the row belongs to rows or allocations beside it and is not
-// looked at (a 16-byte piece never lies in two pages). A thread reads what others copied, so a team also meets before a
+// the row starts in the middle of one. What a piece has beside the row, up to 14 bytes in front of and behind a
+// tensor's memory, belongs to rows or allocations beside it, may be written by others meanwhile, and is not looked at. This is intended, and cannot
+// fault: a 16-byte piece never lies in two pages. A thread reads what others copied, so a team also meets before a
 // row; that it then is past the row before frees that row's place for the next fetch.
 
 // What a thread has of a row: PAIRS pairs of values, and how they lie. WORDS (16-bit types): a pair is a word of memory, for all of a

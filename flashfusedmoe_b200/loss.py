@@ -21,8 +21,13 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index=-100, reduction
     are not ignored (NaN without any, with zero gradients), "sum", or "none" (float32 [*]). The result is float32.
 
     With "mean" and "sum" the gradients are computed together with the loss, wherever hidden or weight requires one: under
-    torch.no_grad() the call takes a third of the time. Scratch: 2 bytes an entry for as many rows as 2 GiB hold.
-    Differentiable once; a device's first call cannot be captured. A target outside of the vocabulary gives NaN, and raises from a
+    torch.no_grad() the call takes a third of the time. With "none" they are computed in the backward pass, which takes the logits a second
+    time. Scratch: without gradients 8 bytes for 128 entries; with them 2 bytes an entry (a probability, then its gradient) for as many rows as
+    2 GiB hold, 4 V D bytes where that is not all of them and the weight's gradient is not float32, and up to 64 N D bytes for few rows.
+    Precision: logits, sums and losses are fp32. Probabilities are fp16 numbers over the largest of 128 neighbouring entries: 11 bits
+    down to e^-20 of that one, nothing below e^-27. The gradients of the logits are bf16, as the products' operands; so are gradients of bf16
+    operands before the backward pass's factor, where that is not 1, multiplies them.
+    Differentiable once, in reverse mode; a device's first call cannot be captured. A target outside of the vocabulary gives NaN, and raises from a
     later call as other device failures do."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"Unknown reduction: {reduction}")

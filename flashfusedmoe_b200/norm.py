@@ -13,7 +13,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
     x, weight [D] and bias [D] (None: 1 and 0) are CUDA tensors in bfloat16, float16 or float32, each in its own; y has x's
     type and shape and is contiguous. Statistics are fp32, and so is everything in between. D is any number up to 32768
-    (float32: 16384). The rows of x may be further apart than D; other strides are copied. Differentiable once, with the
+    (float32: 16384). The rows of x may be further apart than D; other strides are copied. Differentiable once, in reverse mode, with the
     gradients of weight and bias summed in a fixed order."""
     return _lib.native().layer_norm(x, weight, bias, eps)
 

@@ -88,7 +88,7 @@ class _Launch:
 
 
 def operator_launches():
-    """Kernels enqueued so far by the operators beside the layer (layer norm, AdamW), which launch from the torch extension and
+    """Kernels enqueued so far by the operators beside the layer (layer norm, linear cross entropy, AdamW), which launch from the torch extension and
     are not in `launch_count`."""
     return _lib.native().launches()
 

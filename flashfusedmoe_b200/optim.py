@@ -57,7 +57,8 @@ class AdamW(torch.optim.Optimizer):
     update of less than half a unit of a bfloat16 parameter's last place is lost.
 
     Parameters are contiguous CUDA tensors. lr may be a float32 tensor on the device: a step that was captured in a graph then
-    reads it at every replay. State dicts load and save as torch's do, and one of torch.optim.AdamW can be loaded; `step` counts
+    reads it at every replay. State dicts load and save as torch's do, and one of torch.optim.AdamW can be loaded: its moments go to 8 bits
+    where state_bits says so, and the first step makes masters that it does not have (from the parameters as they are then); `step` counts
     on the device."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, master_weights=True,
