@@ -96,14 +96,15 @@ def _is_written_by_replays(t):
     return ref is not None
 
 
-def _quantized_weight(owner, w):
+def _quantized_weight(owner, w, learns):
     """e4m3 copy of the weight tensor `w` [E, N, K] (bf16, possibly a cast copy of `owner`) with one scale per expert.
     Cached per owner, the caller's own weight tensor (normally an nn.Parameter): the entry is reused while that very
     object is alive, unmodified (same version counter) and still where it was; a weak reference drops the entry
     when the owner dies, so an address reused by another tensor can never hit a stale entry. Weights that a captured optimizer step writes
-    change without a new version: theirs are made at every call."""
+    change without a new version: theirs are made at every call. So are those of a captured call whose weights learn, which are to be what an
+    optimizer made of them before each replay."""
     import weakref
-    if _replayed and _is_written_by_replays(owner):
+    if (_replayed and _is_written_by_replays(owner)) or (learns and torch.cuda.is_current_stream_capturing()):
         return ops.quantize_weight_e4m3(w)
     key = id(owner)
     hit = _fp8_weight_cache.get(key)
@@ -481,7 +482,8 @@ class _FusedMoEFunction(torch.autograd.Function):
             few = _few_rows(N, D, E, k, H, cfg.capacity is not None, weights[2], weights[3])
         if _EXPERT_GEMM == "fp8" and D % 128 == 0 and H % 128 == 0 and not few & _FEW_TILES:
             weights = (_to(w_up, dtype), _to(w_down, dtype), *weights[2:])
-            quantized = _quantized_weight(w_up, weights[0]) + _quantized_weight(w_down, weights[1])
+            learns = [need_grad and ctx.needs_input_grad[i] for i in (2, 3)]
+            quantized = _quantized_weight(w_up, weights[0], learns[0]) + _quantized_weight(w_down, weights[1], learns[1])
         dev = hidden_states.device
         pairs, timer = ops.timed(ops.FORWARD_SITES)
         done, out, aux, z, counts, dropped, saved = _lib.native().layer_forward(

@@ -70,3 +70,36 @@ def test_fp8_copies_made_in_a_capture_are_not_kept():
             assert torch.equal(captured, want)
         finally:
             ffm.set_expert_gemm_precision(old)
+
+
+def test_fp8_training_steps_that_are_replayed_see_new_weights():
+    """The weights of a captured forward and backward pass are updated between replays; the e4m3 copies kept from before the capture
+    are not its."""
+    torch.manual_seed(6)
+    layer = ffm.MoELayer(256, 512, 4, top_k=2).to(DEV).bfloat16()
+    x = torch.randn(2048, 256, device=DEV).bfloat16().requires_grad_()
+    go = torch.randn_like(x)
+    leaves = [x, *layer.parameters()]
+    old = ffm.set_expert_gemm_precision("fp8")
+    try:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                torch.autograd.grad(layer(x)[0], leaves, go)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out, _ = layer(x)
+            grads = torch.autograd.grad(out, leaves, go)
+        for _ in range(2):
+            with torch.no_grad():
+                layer.w_up.mul_(0.5)
+                layer.w_down.add_(0.01)
+            graph.replay()
+            torch.cuda.synchronize()
+            want, _ = layer(x)
+            assert torch.equal(out, want)
+            assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(want, leaves, go)))
+    finally:
+        ffm.set_expert_gemm_precision(old)
