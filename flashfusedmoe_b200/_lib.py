@@ -99,6 +99,14 @@ SIGNATURES = {
     "ffm_layer_norm_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "ffm_layer_norm_backward": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "ffm_rms_norm_forward": (c_int, [c_void_p, c_void_p]),
+    "ffm_rms_norm_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "ffm_rms_norm_backward": (c_int, [c_void_p, c_void_p]),
+    "ffm_quantize_blocks_e4m3": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "ffm_linear_blocks_e4m3": (c_int, [c_void_p, c_void_p]),
+    "ffm_grad_norm_workspace_bytes": (c_size_t, [c_int]),
+    "ffm_grad_norm": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
+    "ffm_scale_tensors": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "ffm_adamw_step": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
     "ffm_linear_cross_entropy_workspace_bytes": (c_size_t, [c_void_p]),
     "ffm_linear_cross_entropy": (c_int, [c_void_p, c_void_p]),
@@ -111,7 +119,9 @@ SIGNATURES = {
 }
 
 # called by the torch extension itself (csrc/ffm_torch_ops.cpp)
-NATIVE_OPS = ("ffm_error_string", "ffm_layer_norm_forward", "ffm_layer_norm_workspace_bytes", "ffm_layer_norm_backward",
+NATIVE_OPS = ("ffm_rms_norm_forward", "ffm_rms_norm_workspace_bytes", "ffm_rms_norm_backward", "ffm_quantize_blocks_e4m3",
+              "ffm_linear_blocks_e4m3", "ffm_grad_norm", "ffm_grad_norm_workspace_bytes", "ffm_scale_tensors",
+              "ffm_error_string", "ffm_layer_norm_forward", "ffm_layer_norm_workspace_bytes", "ffm_layer_norm_backward",
               "ffm_adamw_step", "ffm_linear_cross_entropy", "ffm_linear_cross_entropy_workspace_bytes", "ffm_scale_many",
               "ffm_capture_id")
 

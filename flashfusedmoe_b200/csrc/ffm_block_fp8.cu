@@ -1,0 +1,824 @@
+// 8-bit operands (e4m3) with a scale for every 128 values: quantising rows and weights, and products of them, dense or grouped by expert.
+//
+//   x [rows, K] with x_scale [rows, ceil(K / 128)], w [experts, N, K] with w_scale [experts, ceil(N / 128), ceil(K / 128)]:
+//   out[m, n] = sum over blocks b of 128 k's of x_scale[m, b] w_scale[e, n / 128, b] sum over the k's of block b of x[m, k] w[e, n, k]
+//   for the expert e with ends[e - 1] <= m < ends[e]; 0 for rows from the last end on.
+//
+// The sum over a block is what the tensor core accumulates in TMEM (exactly enough: 128 products of 8 bits in fp32). The scales change from block
+// to block, so eight warps take each block's sums out of TMEM while the tensor core is at the next one (two accumulators in turn) and add them,
+// scaled, to fp32 sums in registers.
+#include "ffm_e4m3.cuh"
+#include "ffm_gemm_common.cuh"
+#include "ffm_internal.h"
+#include "ffm_norm_common.cuh"
+
+namespace ffm {
+
+namespace {
+
+// ---- quantising -------------------------------------------------------------------------------------------------
+
+constexpr int QB_THREADS = 256;
+constexpr int QB_GROUPS = 4;  // blocks of a row that a thread works on at once
+
+template <typename T>
+__device__ __forceinline__ void store_e4m3(uint8_t* to, const uint4& raw, float inverse) {
+  float v[VALUES<T>];
+  unpack<T>(raw, v);
+  const uint32_t low = pack_e4m3x4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
+  if constexpr (VALUES<T> == 8) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(low, pack_e4m3x4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
+  } else {
+    *reinterpret_cast<uint32_t*>(to) = low;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float largest(const uint4& raw) {
+  float v[VALUES<T>], top = 0.0f;
+  unpack<T>(raw, v);
+#pragma unroll
+  for (int j = 0; j < VALUES<T>; ++j) top = fmaxf(top, fabsf(v[j]));
+  return top;
+}
+
+// A scale for 128 values of a row: 16 (fp32: 32) neighbouring lanes hold a block, 16 bytes each.
+template <typename T>
+__global__ void __launch_bounds__(QB_THREADS)
+quantize_row_blocks_kernel(const T* __restrict__ x, long long stride, long long blocks, int across, int K, uint8_t* __restrict__ q,
+                           float* __restrict__ scale) {
+  constexpr int V = VALUES<T>, LANES = E4M3_BLOCK / V, TEAMS = QB_THREADS / LANES;
+  const int t = threadIdx.x % LANES;
+  const long long first = static_cast<long long>(blockIdx.x) * (TEAMS * QB_GROUPS) + threadIdx.x / LANES;
+  uint4 raw[QB_GROUPS];
+  long long row[QB_GROUPS];
+  int col[QB_GROUPS];
+#pragma unroll
+  for (int i = 0; i < QB_GROUPS; ++i) {
+    const long long b = first + i * TEAMS;
+    row[i] = (b >> 32) == 0 ? static_cast<uint32_t>(b) / static_cast<uint32_t>(across) : b / across;
+    col[i] = static_cast<int>(b - row[i] * across) * E4M3_BLOCK + t * V;
+    const bool has = b < blocks && col[i] < K;
+    raw[i] = has ? *reinterpret_cast<const uint4*>(x + row[i] * stride + col[i]) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < QB_GROUPS; ++i) {
+    float top = largest<T>(raw[i]);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float s = e4m3_scale(top);
+    const long long b = first + i * TEAMS;
+    if (b < blocks && col[i] < K) {
+      store_e4m3<T>(q + row[i] * K + col[i], raw[i], 1.0f / s);
+      if (t == 0) scale[b] = s;
+    }
+  }
+}
+
+// A scale for 128 x 128 values of a matrix: one thread block for each, its values in registers in between. blockIdx.y: the matrix.
+template <typename T>
+__global__ void __launch_bounds__(QB_THREADS)
+quantize_tiles_kernel(const T* __restrict__ x, int N, int K, int down, int across, uint8_t* __restrict__ q, float* __restrict__ scale) {
+  constexpr int V = VALUES<T>, LANES = E4M3_BLOCK / V, TEAMS = QB_THREADS / LANES, STEPS = E4M3_BLOCK / TEAMS;
+  __shared__ float part[QB_THREADS / 32];
+  const long long tile = blockIdx.x;
+  const int bn = static_cast<int>(tile / across % down), bk = static_cast<int>(tile % across);
+  const long long base = tile / (static_cast<long long>(down) * across) * N * K;
+  const int col = bk * E4M3_BLOCK + threadIdx.x % LANES * V, n0 = bn * E4M3_BLOCK + threadIdx.x / LANES;
+  uint4 raw[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int n = n0 + i * TEAMS;
+    raw[i] = n < N && col < K ? *reinterpret_cast<const uint4*>(x + base + static_cast<long long>(n) * K + col) : make_uint4(0, 0, 0, 0);
+  }
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) top = fmaxf(top, largest<T>(raw[i]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < QB_THREADS / 32; ++w) top = fmaxf(top, part[w]);
+  const float s = e4m3_scale(top), inverse = 1.0f / s;
+  if (threadIdx.x == 0) scale[tile] = s;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int n = n0 + i * TEAMS;
+    if (n < N && col < K) store_e4m3<T>(q + base + static_cast<long long>(n) * K + col, raw[i], inverse);
+  }
+}
+
+// ---- products ---------------------------------------------------------------------------------------------------
+
+constexpr int BLOCK_THREADS = 320;
+constexpr int MAX_EXPERTS = 1024;
+constexpr int A_ROWS = 128;
+constexpr int UMMA_K8 = 32;  // e4m3 values of the contraction in an instruction
+
+struct BlockParams {
+  const float* x_scale;
+  const float* w_scale;
+  const int32_t* ends;  // null: one expert takes all rows
+  int experts;
+  int rows;
+  int N;
+  int k_blocks;
+  int out_type;
+  int out_wide;  // rows of out lie on 16 bytes
+  void* out;
+  int32_t* status;
+  volatile int32_t* status_host;
+  long long wait_cycles;
+};
+
+// Row ranges of the experts, and behind them as one more group the rows that belong to none; tiles before each. Read by the whole block.
+struct Groups {
+  int begin[MAX_EXPERTS + 2];
+  int items[MAX_EXPERTS + 2];
+};
+
+// Filled by one warp. An end below the one before it or past the rows would have tiles read and written out of place: such ends are
+// moved into place, and reported.
+__device__ __forceinline__ void fill_groups(Groups& g, const BlockParams& p, int tile_rows, int tiles_across) {
+  const int lane = threadIdx.x & 31;
+  int last = 0, run = 0;
+  bool bad = false;
+  for (int base = 0; base < p.experts; base += 32) {
+    const int e = base + lane;
+    int end = p.rows;
+    if (p.ends != nullptr && e < p.experts) {
+      end = __ldg(p.ends + e);
+      bad |= end < 0 || end > p.rows;
+      end = min(max(end, 0), p.rows);
+    }
+    int reach = e < p.experts ? max(end, last) : last;  // the largest end so far
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, reach, d);
+      if (lane >= d) reach = max(reach, before);
+    }
+    int begin = __shfl_up_sync(0xffffffffu, reach, 1);
+    if (lane == 0) begin = last;
+    bad |= e < p.experts && end < begin;
+    const int mine = e < p.experts ? (reach - begin + tile_rows - 1) / tile_rows * tiles_across : 0;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += before;
+    }
+    if (e < p.experts) {
+      g.begin[e] = begin;
+      g.items[e] = run + sum - mine;
+    }
+    last = __shfl_sync(0xffffffffu, reach, 31);
+    run += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane == 0) {
+    g.begin[p.experts] = last;
+    g.items[p.experts] = run;
+    g.begin[p.experts + 1] = p.rows;
+    g.items[p.experts + 1] = run + (p.rows - last + tile_rows - 1) / tile_rows * tiles_across;
+  }
+  if (__any_sync(0xffffffffu, bad) && lane == 0) {
+    atomicCAS(p.status, 0, FFM_STATUS_BAD_INDEX);
+    if (p.status_host != nullptr) *p.status_host = FFM_STATUS_BAD_INDEX;
+  }
+}
+
+struct BlockTile {
+  int group;     // p.experts: rows of no expert
+  int across;    // tile of output features
+  int row0;      // first row
+  int rows;      // valid rows, 1..tile_rows
+  int k_blocks;  // 0 for rows of no expert
+};
+
+// Tiles by expert and feature tile, row tile fastest: the row tiles of an expert share its weights through L2.
+struct BlockWalker {
+  const Groups* groups;
+  int experts, tile_rows, k_blocks, cur, step, g;
+
+  __device__ BlockWalker(const Groups* groups_, const BlockParams& p, int tile_rows_, int first, int step_)
+      : groups(groups_), experts(p.experts), tile_rows(tile_rows_), k_blocks(p.k_blocks), cur(first), step(step_), g(0) {}
+  __device__ bool next(BlockTile& t) {
+    if (cur >= groups->items[experts + 1]) return false;
+    while (cur >= groups->items[g + 1]) ++g;
+    const int begin = groups->begin[g], count = groups->begin[g + 1] - begin, down = (count + tile_rows - 1) / tile_rows;
+    const int r = cur - groups->items[g], first = r % down * tile_rows;
+    t.group = g;
+    t.across = r / down;
+    t.row0 = begin + first;
+    t.rows = min(tile_rows, count - first);
+    t.k_blocks = g < experts ? k_blocks : 0;
+    cur += step;
+    return true;
+  }
+};
+
+__device__ __forceinline__ uint32_t pack_out(int type, float a, float b) {
+  if (type == FFM_TYPE_BF16) return pack_bf16x2(a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---- many rows: 128 rows x BN features, rows on the M side -------------------------------------------------------
+
+template <int BN>
+struct ManyRows {
+  static constexpr int COLS = BN / 2;  // features of a warp: the eight warps are two halves of a tile by four lane quarters
+  static constexpr int STAGE_BYTES = (A_ROWS + BN) * 128;
+  static constexpr int STAGES = 196608 / STAGE_BYTES;
+  static constexpr int STAGING = 8 * 32 * 64;  // 32 rows x 64 bytes a warp
+  struct Ctrl {
+    unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[2], acc_empty_bar[2], drain_bar;
+    uint32_t tmem_base;
+    int abort_flag;
+    int filled;
+    Groups groups;
+  };
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING + static_cast<int>(sizeof(Ctrl)) + 1024;
+  static_assert(SMEM_BYTES <= 232448, "tile shape does not fit in shared memory");
+};
+
+// 16 bytes q (0..3) of row r in 32 rows of 64 bytes: eight neighbouring rows meet no bank twice
+__device__ __forceinline__ uint32_t staged(int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); }
+
+//   warp 0      TMA producer          warp 1   MMA issuer, TMEM owner
+//   warps 2..9  take a block's sums out of TMEM, scale and add them, store the tile
+template <int BN, int OUT_BYTES>
+__global__ void __launch_bounds__(BLOCK_THREADS, 1)
+block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ BlockParams p) {
+  using S = ManyRows<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw), pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t smem_base = raw_addr + pad, staging = smem_base + S::STAGES * S::STAGE_BYTES;
+  auto* ctrl = reinterpret_cast<typename S::Ctrl*>(smem_raw + pad + S::STAGES * S::STAGE_BYTES + S::STAGING);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(smem_u32(&ctrl->full_bar[s]), 1);
+      mbar_init(smem_u32(&ctrl->empty_bar[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&ctrl->acc_full_bar[a]), 1);
+      mbar_init(smem_u32(&ctrl->acc_empty_bar[a]), 8);
+    }
+    mbar_init(smem_u32(&ctrl->drain_bar), 1);
+    ctrl->abort_flag = 0;
+    ctrl->filled = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  if (warp == 2) fill_groups(ctrl->groups, p, A_ROWS, (p.N + BN - 1) / BN);
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ctrl->tmem_base), 2 * BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  const uint32_t tmem_base = ctrl->tmem_base;
+  volatile int* abort_flag = &ctrl->abort_flag;
+  bool issuer = false;
+  BlockWalker walker(&ctrl->groups, p, A_ROWS, blockIdx.x, gridDim.x);
+  BlockTile t;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0, filled = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      while (ok && walker.next(t)) {
+        for (int kb = 0; kb < t.k_blocks; ++kb) {
+          ok = mbar_wait_bounded(smem_u32(&ctrl->empty_bar[stage]), phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_PRODUCER, p.wait_cycles);
+          if (!ok) break;
+          const uint32_t full = smem_u32(&ctrl->full_bar[stage]), a_dst = smem_base + stage * S::STAGE_BYTES;
+          mbar_expect_tx(full, S::STAGE_BYTES);
+          tma_load_2d(a_dst, &tm_x, full, kb * E4M3_BLOCK, t.row0);
+          tma_load_3d(a_dst + A_ROWS * 128, &tm_w, full, kb * E4M3_BLOCK, t.across * BN, t.group);
+          ++filled;
+          if (++stage == S::STAGES) stage = 0, phase ^= 1u;
+        }
+      }
+      ctrl->filled = filled;
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      issuer = true;
+      constexpr uint32_t idesc = make_idesc_e4m3(A_ROWS, BN);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      while (ok && walker.next(t)) {
+        for (int kb = 0; kb < t.k_blocks; ++kb) {
+          ok = mbar_wait_bounded(smem_u32(&ctrl->acc_empty_bar[acc]), acc_phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_MMA, p.wait_cycles) &&
+               mbar_wait_bounded(smem_u32(&ctrl->full_bar[stage]), phase, abort_flag, p.status, FFM_STATUS_WAIT_MMA, p.wait_cycles);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_src = smem_base + stage * S::STAGE_BYTES, b_src = a_src + A_ROWS * 128;
+#pragma unroll
+          for (int kk = 0; kk < E4M3_BLOCK / UMMA_K8; ++kk) {
+            umma_f8(tmem_base + acc * BN, make_smem_desc_sw128(a_src + kk * UMMA_K8, 16, 1024), make_smem_desc_sw128(b_src + kk * UMMA_K8, 16, 1024),
+                    idesc, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(smem_u32(&ctrl->empty_bar[stage]));
+          umma_commit(smem_u32(&ctrl->acc_full_bar[acc]));
+          if (++stage == S::STAGES) stage = 0, phase ^= 1u;
+          if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * S::COLS, mine = staging + (warp - 2) * 2048;
+    const int scale_rows = (p.N + E4M3_BLOCK - 1) / E4M3_BLOCK;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    while (ok && walker.next(t)) {
+      const int f0 = t.across * BN + half * S::COLS;  // this warp's first feature
+      const bool in_tile = quarter * 32 + lane < t.rows;
+      const float* xs = p.x_scale + static_cast<long long>(t.row0 + (in_tile ? quarter * 32 + lane : 0)) * p.k_blocks;
+      const float* ws = p.w_scale + (static_cast<long long>(t.group) * scale_rows + min(f0 / E4M3_BLOCK, scale_rows - 1)) * p.k_blocks;
+      float2 sum[S::COLS / 2];
+#pragma unroll
+      for (int j = 0; j < S::COLS / 2; ++j) sum[j] = both(0.0f);
+      // the scales of the next two blocks are on their way
+      float s0 = t.k_blocks > 0 ? __ldg(xs) * __ldg(ws) : 0.0f, s1 = t.k_blocks > 1 ? __ldg(xs + 1) * __ldg(ws + 1) : 0.0f;
+      for (int kb = 0; kb < t.k_blocks; ++kb) {
+        const float x2 = kb + 2 < t.k_blocks ? __ldg(xs + kb + 2) : 0.0f, w2 = kb + 2 < t.k_blocks ? __ldg(ws + kb + 2) : 0.0f;
+        ok = mbar_wait_bounded(smem_u32(&ctrl->acc_full_bar[acc]), acc_phase, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float2 s = both(s0);
+        uint32_t v[2][16];
+        tmem_ld_32x16(taddr + acc * BN, v[0]);
+#pragma unroll
+        for (int c = 0; c < S::COLS / 16; ++c) {
+          tmem_ld_wait();
+          if (c + 1 < S::COLS / 16) {
+            tmem_ld_32x16(taddr + acc * BN + (c + 1) * 16, v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(smem_u32(&ctrl->acc_empty_bar[acc]));
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sum[c * 8 + j] = fma2(make_float2(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1])), s, sum[c * 8 + j]);
+          }
+        }
+        if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        s0 = s1;
+        s1 = x2 * w2;
+      }
+      if (!ok) break;
+      // 64 bytes of every row at a time through shared memory, so that neighbouring lanes store neighbouring 16 bytes
+      constexpr int STEP = 64 / OUT_BYTES;
+      const int limit = t.rows - quarter * 32;  // of this warp's rows
+#pragma unroll
+      for (int c = 0; c < S::COLS / STEP; ++c) {
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (OUT_BYTES == 2) {
+            const float2* f = sum + c * 16 + q * 4;
+            st_shared_v4(mine + staged(lane, q), pack_out(p.out_type, f[0].x, f[0].y), pack_out(p.out_type, f[1].x, f[1].y),
+                         pack_out(p.out_type, f[2].x, f[2].y), pack_out(p.out_type, f[3].x, f[3].y));
+          } else {
+            const float2* f = sum + c * 8 + q * 2;
+            st_shared_v4(mine + staged(lane, q), __float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+          }
+        }
+        __syncwarp();
+        const int first = f0 + c * STEP;
+        uint8_t* out = static_cast<uint8_t*>(p.out) + (static_cast<long long>(t.row0 + quarter * 32) * p.N + first) * OUT_BYTES;
+        if (p.out_wide) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2), q = lane & 3;
+            uint4 u;
+            ld_shared_v4(mine + staged(r, q), u);
+            if (r < limit && first + q * (16 / OUT_BYTES) < p.N) *reinterpret_cast<uint4*>(out + static_cast<long long>(r) * p.N * OUT_BYTES + q * 16) = u;
+          }
+        } else {
+          constexpr int AT_ONCE = 32 / STEP;  // rows of an instruction
+          const int col = lane % STEP, r0 = lane / STEP;
+          const uint32_t from = (col * OUT_BYTES) & 15, piece = (col * OUT_BYTES) >> 4;
+#pragma unroll 4
+          for (int i = 0; i < 32 / AT_ONCE; ++i) {
+            const int r = i * AT_ONCE + r0;
+            uint32_t bits;
+            if constexpr (OUT_BYTES == 2) {
+              uint16_t b;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(mine + staged(r, piece) + from) : "memory");
+              bits = b;
+            } else {
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bits) : "r"(mine + staged(r, piece) + from) : "memory");
+            }
+            if (r < limit && first + col < p.N) {
+              uint8_t* to = out + (static_cast<long long>(r) * p.N + col) * OUT_BYTES;
+              if constexpr (OUT_BYTES == 2) {
+                *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(bits);
+              } else {
+                *reinterpret_cast<uint32_t*>(to) = bits;
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---- common exit: every role reaches this point, also after an abort
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    // loads and MMAs that nobody waited for must not land in shared memory or TMEM that the CTA has given back
+    if (threadIdx.x == 0) {
+      for (int f = max(ctrl->filled - S::STAGES, 0); f < ctrl->filled; ++f) mbar_drain(smem_u32(&ctrl->full_bar[f % S::STAGES]), (f / S::STAGES) & 1);
+      if (p.status_host != nullptr) *p.status_host = *p.status;
+    } else if (issuer) {
+      umma_commit(smem_u32(&ctrl->drain_bar));
+      mbar_drain(smem_u32(&ctrl->drain_bar), 0);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * BN);
+  }
+}
+
+// ---- few rows an expert: 128 features x up to 64 rows, features on the M side -------------------------------------
+
+// The weights are streamed once and everything else should cost nothing: a tile loads and computes the 16-row boxes that hold rows.
+struct FewRows {
+  static constexpr int ROWS = 64;
+  static constexpr int STAGE_BYTES = (A_ROWS + ROWS) * 128;
+  static constexpr int STAGES = 7;
+  static constexpr int PART = ROWS * A_ROWS * 4;  // a split contraction's sums
+  struct Ctrl {
+    unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[2], acc_empty_bar[2], drain_bar;
+    uint32_t tmem_base;
+    int abort_flag;
+    int filled;
+    alignas(16) float scale[4][2][ROWS];  // of a warp's block and the next
+    Groups groups;
+  };
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PART + static_cast<int>(sizeof(Ctrl)) + 1024;
+  static_assert(SMEM_BYTES <= 232448, "tile shape does not fit in shared memory");
+};
+constexpr int FEW_THREADS = 192;  // producer, MMA issuer, and a warp for each lane quarter
+constexpr int MAX_SPLIT = 8;
+
+__device__ __forceinline__ float ld_shared_cluster(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+// SPLIT: a cluster's CTAs share a tile's contraction, one tile a cluster; their sums meet in shared memory and are added in the order of the ranks.
+template <bool SPLIT>
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ BlockParams p,
+                      int split) {
+  using S = FewRows;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw), pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t smem_base = raw_addr + pad, part = smem_base + S::STAGES * S::STAGE_BYTES;
+  auto* ctrl = reinterpret_cast<S::Ctrl*>(smem_raw + pad + S::STAGES * S::STAGE_BYTES + S::PART);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(smem_u32(&ctrl->full_bar[s]), 1);
+      mbar_init(smem_u32(&ctrl->empty_bar[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&ctrl->acc_full_bar[a]), 1);
+      mbar_init(smem_u32(&ctrl->acc_empty_bar[a]), 4);
+    }
+    mbar_init(smem_u32(&ctrl->drain_bar), 1);
+    ctrl->abort_flag = 0;
+    ctrl->filled = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  if (warp == 2) fill_groups(ctrl->groups, p, S::ROWS, (p.N + A_ROWS - 1) / A_ROWS);
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ctrl->tmem_base), 2 * S::ROWS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  const uint32_t tmem_base = ctrl->tmem_base;
+  volatile int* abort_flag = &ctrl->abort_flag;
+  bool issuer = false;
+  const int total = ctrl->groups.items[p.experts + 1];
+  // a cluster has one tile: no second one to step to
+  BlockWalker walker(&ctrl->groups, p, S::ROWS, SPLIT ? blockIdx.x / split : blockIdx.x, SPLIT ? total : gridDim.x);
+  BlockTile t;
+  // this CTA's blocks of a tile's contraction
+  auto from = [&] { return SPLIT ? t.k_blocks * rank / split : 0; };
+  auto to = [&] { return SPLIT ? t.k_blocks * (rank + 1) / split : t.k_blocks; };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0, filled = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      while (ok && walker.next(t)) {
+        const int boxed = (t.rows + 15) & ~15;
+        for (int kb = from(); kb < to(); ++kb) {
+          ok = mbar_wait_bounded(smem_u32(&ctrl->empty_bar[stage]), phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_PRODUCER, p.wait_cycles);
+          if (!ok) break;
+          const uint32_t full = smem_u32(&ctrl->full_bar[stage]), w_dst = smem_base + stage * S::STAGE_BYTES;
+          mbar_expect_tx(full, (A_ROWS + boxed) * 128);
+          tma_load_3d(w_dst, &tm_w, full, kb * E4M3_BLOCK, t.across * A_ROWS, t.group);
+          for (int r = 0; r < boxed; r += 16) tma_load_2d(w_dst + (A_ROWS + r) * 128, &tm_x, full, kb * E4M3_BLOCK, t.row0 + r);
+          ++filled;
+          if (++stage == S::STAGES) stage = 0, phase ^= 1u;
+        }
+      }
+      ctrl->filled = filled;
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      issuer = true;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      while (ok && walker.next(t)) {
+        const uint32_t idesc = make_idesc_e4m3(A_ROWS, (t.rows + 15) & ~15);
+        for (int kb = from(); kb < to(); ++kb) {
+          ok = mbar_wait_bounded(smem_u32(&ctrl->acc_empty_bar[acc]), acc_phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_MMA, p.wait_cycles) &&
+               mbar_wait_bounded(smem_u32(&ctrl->full_bar[stage]), phase, abort_flag, p.status, FFM_STATUS_WAIT_MMA, p.wait_cycles);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_src = smem_base + stage * S::STAGE_BYTES, b_src = a_src + A_ROWS * 128;
+#pragma unroll
+          for (int kk = 0; kk < E4M3_BLOCK / UMMA_K8; ++kk) {
+            umma_f8(tmem_base + acc * S::ROWS, make_smem_desc_sw128(a_src + kk * UMMA_K8, 16, 1024),
+                    make_smem_desc_sw128(b_src + kk * UMMA_K8, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(smem_u32(&ctrl->empty_bar[stage]));
+          umma_commit(smem_u32(&ctrl->acc_full_bar[acc]));
+          if (++stage == S::STAGES) stage = 0, phase ^= 1u;
+          if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const int scale_rows = (p.N + E4M3_BLOCK - 1) / E4M3_BLOCK;
+    float(*scale)[S::ROWS] = ctrl->scale[quarter];
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    while (ok && walker.next(t)) {
+      const float* ws = p.w_scale + (static_cast<long long>(t.group) * scale_rows + t.across) * p.k_blocks;
+      const float* xs0 = p.x_scale + static_cast<long long>(t.row0 + min(lane, t.rows - 1)) * p.k_blocks;
+      const float* xs1 = p.x_scale + static_cast<long long>(t.row0 + min(lane + 32, t.rows - 1)) * p.k_blocks;
+      float sum[S::ROWS];
+#pragma unroll
+      for (int j = 0; j < S::ROWS; ++j) sum[j] = 0.0f;
+      const int last = to();
+      float a = 0.0f, b = 0.0f, w = 0.0f;
+      if (from() < last) a = __ldg(xs0 + from()), b = __ldg(xs1 + from()), w = __ldg(ws + from());
+      for (int kb = from(); kb < last; ++kb) {
+        // an accumulator's number serves for the scales' place too: the one before last has been read by all lanes
+        scale[acc][lane] = a * w;
+        scale[acc][lane + 32] = b * w;
+        if (kb + 1 < last) a = __ldg(xs0 + kb + 1), b = __ldg(xs1 + kb + 1), w = __ldg(ws + kb + 1);
+        __syncwarp();
+        ok = mbar_wait_bounded(smem_u32(&ctrl->acc_full_bar[acc]), acc_phase, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < S::ROWS / 16; ++c) {
+          if (c * 16 < t.rows) {
+            uint32_t v[16];
+            tmem_ld_32x16(taddr + acc * S::ROWS + c * 16, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const float4 s = *reinterpret_cast<const float4*>(&scale[acc][c * 16 + j]);
+              sum[c * 16 + j] = fmaf(__uint_as_float(v[j]), s.x, sum[c * 16 + j]);
+              sum[c * 16 + j + 1] = fmaf(__uint_as_float(v[j + 1]), s.y, sum[c * 16 + j + 1]);
+              sum[c * 16 + j + 2] = fmaf(__uint_as_float(v[j + 2]), s.z, sum[c * 16 + j + 2]);
+              sum[c * 16 + j + 3] = fmaf(__uint_as_float(v[j + 3]), s.w, sum[c * 16 + j + 3]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctrl->acc_empty_bar[acc]));
+        if (++acc == 2) acc = 0, acc_phase ^= 1u;
+      }
+      if (!ok) break;
+      const int feature = quarter * 32 + lane, n = t.across * A_ROWS + feature;
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int j = 0; j < S::ROWS; ++j) {
+          if (j < t.rows) asm volatile("st.shared.f32 [%0], %1;" ::"r"(part + (j * A_ROWS + feature) * 4), "f"(sum[j]) : "memory");
+        }
+      } else {
+        const long long out = static_cast<long long>(t.row0) * p.N + n;
+#pragma unroll
+        for (int j = 0; j < S::ROWS; ++j) {
+          if (j < t.rows && n < p.N) store1_as(p.out, p.out_type, out + static_cast<long long>(j) * p.N, sum[j]);
+        }
+      }
+    }
+  }
+
+  if constexpr (SPLIT) {
+    __syncwarp();
+    cluster_sync_all();
+    BlockWalker again(&ctrl->groups, p, S::ROWS, blockIdx.x / split, total);
+    if (warp >= 2 && again.next(t)) {
+      // every rank adds up and stores every split-th row
+      const int feature = threadIdx.x - 64, n = t.across * A_ROWS + feature;
+      for (int j = rank; j < t.rows; j += split) {
+        float v = 0.0f;
+        for (int r = 0; r < split; ++r) v += ld_shared_cluster(map_to_cta(part + (j * A_ROWS + feature) * 4, r));
+        if (n < p.N) store1_as(p.out, p.out_type, static_cast<long long>(t.row0 + j) * p.N + n, v);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // this CTA's sums have been read
+  }
+
+  // ---- common exit, as above
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    if (threadIdx.x == 0) {
+      for (int f = max(ctrl->filled - S::STAGES, 0); f < ctrl->filled; ++f) mbar_drain(smem_u32(&ctrl->full_bar[f % S::STAGES]), (f / S::STAGES) & 1);
+      if (p.status_host != nullptr) *p.status_host = *p.status;
+    } else if (issuer) {
+      umma_commit(smem_u32(&ctrl->drain_bar));
+      mbar_drain(smem_u32(&ctrl->drain_bar), 0);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * S::ROWS);
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------
+
+// bytes [groups, rows, cols], rows `ld` bytes apart, boxes of 128 bytes x box_rows, 128-byte swizzle, zeros out of bounds
+int make_byte_map(CUtensorMap* map, const void* base, long long groups, long long rows, long long cols, long long ld, int box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return FFM_ERR_NO_DRIVER;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || ld % 16 != 0) return FFM_ERR_UNSUPPORTED;
+  const bool flat = groups == 0;  // two dimensions
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(groups)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld), static_cast<cuuint64_t>(ld) * rows};
+  cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, flat ? 2 : 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
+template <typename K>
+bool allow_smem(K kernel, int bytes, PerDevice& room) {
+  return room.get([&] {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    return 1;
+  }) > 0;
+}
+
+template <int BN, int OUT_BYTES>
+int launch_many(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const BlockParams& p, long long tiles, cudaStream_t stream) {
+  static PerDevice room;
+  auto kernel = block_gemm_kernel<BN, OUT_BYTES>;
+  if (!allow_smem(kernel, ManyRows<BN>::SMEM_BYTES, room)) return FFM_ERR_LAUNCH;
+  kernel<<<static_cast<unsigned>(tiles < num_sms() ? tiles : num_sms()), BLOCK_THREADS, ManyRows<BN>::SMEM_BYTES, stream>>>(tm_x, tm_w, p);
+  return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
+template <bool SPLIT>
+int launch_few(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const BlockParams& p, long long tiles, int split, cudaStream_t stream) {
+  static PerDevice room;
+  auto kernel = block_gemm_few_kernel<SPLIT>;
+  if (!allow_smem(kernel, FewRows::SMEM_BYTES, room)) return FFM_ERR_LAUNCH;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(SPLIT ? tiles * split : (tiles < num_sms() ? tiles : num_sms())));
+  config.blockDim = dim3(FEW_THREADS);
+  config.dynamicSmemBytes = FewRows::SMEM_BYTES;
+  config.stream = stream;
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(split);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = SPLIT ? 1 : 0;
+  const cudaError_t rc = cudaLaunchKernelEx(&config, kernel, tm_x, tm_w, p, split);
+  if (rc != cudaSuccess) cudaGetLastError();
+  return rc == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
+}  // namespace
+
+}  // namespace ffm
+
+using namespace ffm;
+
+extern "C" int ffm_quantize_blocks_e4m3(const void* x, int x_type, int64_t matrices, int64_t rows, int64_t row_stride, int K, int block_rows, void* q,
+                                        float* scale, ffm_stream_t stream) {
+  if (!is_type(x_type) || matrices < 0 || rows < 0 || K <= 0 || (block_rows != 1 && block_rows != E4M3_BLOCK)) return FFM_ERR_BAD_ARG;
+  if ((row_stride < K && rows > 1) || (block_rows == 1 && matrices > 1)) return FFM_ERR_BAD_ARG;
+  if (K % 16 != 0 || rows > 0x7fffffffll || (block_rows > 1 && matrices * rows > 0 && row_stride != K)) return FFM_ERR_UNSUPPORTED;
+  if (matrices == 0 || rows == 0) return FFM_OK;
+  if (!x || !q || !scale) return FFM_ERR_BAD_ARG;
+  if (off_16_bytes(x) || (row_stride * type_bytes(x_type)) % 16 != 0 || (reinterpret_cast<uintptr_t>(q) & 7u) != 0) return FFM_ERR_UNSUPPORTED;
+  const int across = (K + E4M3_BLOCK - 1) / E4M3_BLOCK, down = static_cast<int>((rows + block_rows - 1) / block_rows);
+  const long long blocks = block_rows == 1 ? rows * across : matrices * down * across;
+  const int per = block_rows == 1 ? QB_GROUPS * QB_THREADS / (x_type == FFM_TYPE_FP32 ? 32 : 16) : 1;
+  const long long grid = (blocks + per - 1) / per;
+  if (grid > 0x7fffffffll) return FFM_ERR_UNSUPPORTED;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto launch = [&](auto tag) {
+    using T = decltype(tag);
+    if (block_rows == 1) {
+      quantize_row_blocks_kernel<T><<<static_cast<unsigned>(grid), QB_THREADS, 0, st>>>(static_cast<const T*>(x), row_stride, blocks, across, K,
+                                                                                      static_cast<uint8_t*>(q), scale);
+    } else {
+      quantize_tiles_kernel<T><<<static_cast<unsigned>(grid), QB_THREADS, 0, st>>>(static_cast<const T*>(x), static_cast<int>(rows), K, down, across,
+                                                                                 static_cast<uint8_t*>(q), scale);
+    }
+    return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
+  };
+  if (x_type == FFM_TYPE_BF16) return launch(bf16{});
+  if (x_type == FFM_TYPE_FP16) return launch(fp16{});
+  return launch(float{});
+}
+
+extern "C" int ffm_linear_blocks_e4m3(const ffm_linear_blocks_args* args, ffm_stream_t stream) {
+  if (args == nullptr) return FFM_ERR_BAD_ARG;
+  const ffm_linear_blocks_args& a = *args;
+  if (a.rows < 0 || a.N < 1 || a.K < 1 || a.experts < 1 || !is_type(static_cast<int>(a.out_type)) || (a.x_stride < a.K && a.rows > 1)) return FFM_ERR_BAD_ARG;
+  if (a.ends == nullptr && a.experts != 1) return FFM_ERR_BAD_ARG;
+  if (a.rows == 0) return FFM_OK;
+  if (!a.x || !a.x_scale || !a.w || !a.w_scale || !a.out || !a.status) return FFM_ERR_BAD_ARG;
+  if (a.K % 16 != 0 || a.x_stride % 16 != 0 || a.experts > MAX_EXPERTS || a.rows > (1ll << 30) || a.N > (1ll << 30) || a.K > (1ll << 30)) return FFM_ERR_UNSUPPORTED;
+  BlockParams p = {};
+  p.x_scale = a.x_scale;
+  p.w_scale = a.w_scale;
+  p.ends = a.ends;
+  p.experts = static_cast<int>(a.experts);
+  p.rows = static_cast<int>(a.rows);
+  p.N = static_cast<int>(a.N);
+  p.k_blocks = static_cast<int>((a.K + E4M3_BLOCK - 1) / E4M3_BLOCK);
+  p.out_type = static_cast<int>(a.out_type);
+  p.out_wide = a.N * type_bytes(p.out_type) % 16 == 0 && !off_16_bytes(a.out);
+  p.out = a.out;
+  p.status = a.status;
+  p.status_host = a.status_host;
+  p.wait_cycles = gemm_wait_cycles();
+  const int64_t average = a.rows / a.experts;
+  const bool few = average <= FewRows::ROWS;
+  // tiles at most: every expert may end inside of one, and so may the rows behind the last
+  auto tiles = [&](int64_t tile_rows, int64_t width) {
+    const int64_t parts = a.ends != nullptr ? (a.experts < a.rows ? a.experts : a.rows) + 1 : 0;
+    return (a.rows / tile_rows + (a.ends != nullptr ? parts : (a.rows % tile_rows != 0))) * ((a.N + width - 1) / width);
+  };
+  const int64_t wide = tiles(A_ROWS, 256);
+  const int box_n = few ? A_ROWS : (wide >= 2 * num_sms() ? 256 : 128), box_m = few ? 16 : A_ROWS;
+  const int64_t most = tiles(few ? FewRows::ROWS : A_ROWS, box_n);
+  if (most > 0x3fffffff) return FFM_ERR_UNSUPPORTED;
+  CUtensorMap tm_x, tm_w;
+  int rc = make_byte_map(&tm_x, a.x, 0, a.rows, a.K, a.rows > 1 ? a.x_stride : a.K, box_m);
+  if (rc == FFM_OK) rc = make_byte_map(&tm_w, a.w, a.experts, a.N, a.K, a.K, box_n);
+  if (rc != FFM_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool four = p.out_type == FFM_TYPE_FP32;
+  if (few) {
+    int split = 1;
+    while (split < MAX_SPLIT && most * split * 2 <= num_sms() && p.k_blocks >= split * 4) split *= 2;
+    return split > 1 ? launch_few<true>(tm_x, tm_w, p, most, split, st) : launch_few<false>(tm_x, tm_w, p, most, 1, st);
+  }
+  if (box_n == 256) return four ? launch_many<256, 4>(tm_x, tm_w, p, most, st) : launch_many<256, 2>(tm_x, tm_w, p, most, st);
+  return four ? launch_many<128, 4>(tm_x, tm_w, p, most, st) : launch_many<128, 2>(tm_x, tm_w, p, most, st);
+}

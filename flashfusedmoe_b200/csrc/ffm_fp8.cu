@@ -3,9 +3,8 @@
 // the row (the second one hits L1 / L2), 16-byte loads and 8-byte stores. HBM-bound: reads 2 B and writes 1 B per
 // element. The same kernel quantises activations (one scale per token row) and weights (one scale per output
 // channel: a row of [E * N, K]).
-#include <cuda_fp8.h>
-
 #include "ffm_common.cuh"
+#include "ffm_e4m3.cuh"
 #include "ffm_internal.h"
 
 namespace ffm {
@@ -14,12 +13,6 @@ namespace {
 
 constexpr int Q_THREADS = 256;
 constexpr int Q_WARPS = Q_THREADS / 32;
-
-__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
 
 __global__ void __launch_bounds__(Q_THREADS)
 quantize_rows_e4m3_kernel(const bf16* __restrict__ x, long long rows, int K, uint8_t* __restrict__ q,

@@ -38,6 +38,14 @@ decltype(&ffm_linear_cross_entropy) cross_entropy = nullptr;
 decltype(&ffm_linear_cross_entropy_workspace_bytes) cross_entropy_workspace = nullptr;
 decltype(&ffm_scale_many) scale_many = nullptr;
 decltype(&ffm_capture_id) capture_id = nullptr;
+decltype(&ffm_rms_norm_forward) rms_forward = nullptr;
+decltype(&ffm_rms_norm_workspace_bytes) rms_workspace = nullptr;
+decltype(&ffm_rms_norm_backward) rms_backward = nullptr;
+decltype(&ffm_quantize_blocks_e4m3) quantize_blocks = nullptr;
+decltype(&ffm_linear_blocks_e4m3) linear_blocks = nullptr;
+decltype(&ffm_grad_norm_workspace_bytes) grad_norm_workspace = nullptr;
+decltype(&ffm_grad_norm) grad_norm = nullptr;
+decltype(&ffm_scale_tensors) scale_tensors = nullptr;
 
 void bind_ops(const std::unordered_map<std::string, uintptr_t>& at) {
   auto take = [&](const char* name, auto& f) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(at.at(name)); };
@@ -50,6 +58,14 @@ void bind_ops(const std::unordered_map<std::string, uintptr_t>& at) {
   take("ffm_linear_cross_entropy_workspace_bytes", cross_entropy_workspace);
   take("ffm_scale_many", scale_many);
   take("ffm_capture_id", capture_id);
+  take("ffm_rms_norm_forward", rms_forward);
+  take("ffm_rms_norm_workspace_bytes", rms_workspace);
+  take("ffm_rms_norm_backward", rms_backward);
+  take("ffm_quantize_blocks_e4m3", quantize_blocks);
+  take("ffm_linear_blocks_e4m3", linear_blocks);
+  take("ffm_grad_norm_workspace_bytes", grad_norm_workspace);
+  take("ffm_grad_norm", grad_norm);
+  take("ffm_scale_tensors", scale_tensors);
 }
 
 void check(int rc, const char* what) {
@@ -462,6 +478,310 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
   return reduction != REDUCE_NONE ? r.loss : r.nll.view(t.sizes());
 }
 
+// ---- RMS norm -------------------------------------------------------------------------------------------------
+
+struct RmsCall {
+  double eps = 0.0, offset = 0.0;
+  bool e4m3 = false;
+};
+
+struct RmsResult {
+  Tensor y, y_scale, h, rstd;
+};
+
+// rows as they lie, or copied where 8-bit outputs ask for 16-byte boundaries that they are not on
+Rows as_rows_for(const Tensor& t, bool on_16) {
+  Rows r = as_rows(t);
+  if (on_16 && (reinterpret_cast<uintptr_t>(r.x.data_ptr()) % 16 != 0 || r.stride * static_cast<int64_t>(t.element_size()) % 16 != 0)) {
+    r.x = r.x.clone(at::MemoryFormat::Contiguous);
+    r.stride = t.size(-1);
+  }
+  return r;
+}
+
+RmsResult rms_forward_of(const Tensor& x, const Tensor& weight, const Tensor& residual, const RmsCall& call, bool stats) {
+  on_gpu(x, "x");
+  if (x.dim() < 1 || x.size(-1) < 1) throw py::value_error("x must have a last dimension to normalise, got " + c10::str(x.sizes()));
+  if (x.size(-1) > std::numeric_limits<int>::max()) throw py::value_error("x has rows of " + std::to_string(x.size(-1)) + " values");
+  if (!(call.eps >= 0.0)) throw py::value_error("eps must not be negative, got " + std::to_string(call.eps));
+  if (!(std::abs(call.offset) <= std::numeric_limits<float>::max())) throw py::value_error("weight_offset must be finite, got " + std::to_string(call.offset));
+  ffm_rms_norm_args a = {};
+  a.x_type = element_type(x, "x");
+  check_vector(weight, x, "weight");
+  if (residual.defined()) {
+    same_device(residual, x, "residual");
+    if (residual.sizes() != x.sizes()) throw py::value_error("residual must be " + c10::str(x.sizes()) + ", got " + c10::str(residual.sizes()));
+    if (residual.scalar_type() != x.scalar_type()) {
+      throw py::type_error(std::string("residual must be of x's type, got ") + c10::toString(residual.scalar_type()) + " and " + c10::toString(x.scalar_type()));
+    }
+  }
+  const int64_t D = x.size(-1);
+  if (call.e4m3 && D % 16 != 0) throw py::value_error("an 8-bit output has rows of a multiple of 16 values, got " + std::to_string(D));
+  const On device(x);
+  const Rows r = as_rows_for(x, call.e4m3);
+  Rows more;
+  Tensor w = weight.defined() ? plain(weight) : Tensor();
+  if (call.e4m3 && w.defined() && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 != 0) w = w.clone();
+  const auto contiguous = x.options().memory_format(at::MemoryFormat::Contiguous);
+  RmsResult out;
+  if (residual.defined()) {
+    more = as_rows_for(residual, call.e4m3);
+    out.h = at::empty(x.sizes(), contiguous);
+  }
+  if (call.e4m3) {
+    std::vector<int64_t> sizes = x.sizes().vec();
+    out.y = at::empty(sizes, contiguous.dtype(at::kFloat8_e4m3fn));
+    sizes.back() = (D + 127) / 128;
+    out.y_scale = at::empty(sizes, contiguous.dtype(at::kFloat));
+  } else {
+    out.y = at::empty(x.sizes(), contiguous);
+  }
+  if (stats) out.rstd = at::empty({r.rows}, contiguous.dtype(at::kFloat));
+  a.rows = r.rows;
+  a.D = D;
+  a.x_stride = r.stride;
+  a.eps = call.eps;
+  a.offset = call.offset;
+  a.x = r.x.data_ptr();
+  if (residual.defined()) {
+    a.residual = more.x.data_ptr();
+    a.residual_stride = more.stride;
+    a.h = out.h.data_ptr();
+  }
+  a.weight = address(w);
+  a.w_type = w.defined() ? element_type(w, "weight") : 0;
+  a.y = out.y.data_ptr();
+  a.y_scale = static_cast<float*>(address(out.y_scale));
+  a.rstd = static_cast<float*>(address(out.rstd));
+  check(rms_forward(&a, device.stream()), "ffm_rms_norm_forward");
+  launches += r.rows > 0;
+  return out;
+}
+
+struct RmsGradients {
+  Tensor dx, dweight;
+};
+
+RmsGradients rms_backward_of(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& weight, const Tensor& rstd, const RmsCall& call,
+                             bool want_x, bool want_weight) {
+  const On device(h);
+  ffm_rms_norm_args a = {};
+  a.x_type = element_type(h, "x");
+  const int64_t D = h.size(-1);
+  const Rows r = as_rows(h);
+  // saved-tensor hooks may have handed back other tensors than were saved
+  if (rstd.numel() != r.rows || rstd.scalar_type() != at::kFloat || !rstd.is_cuda()) throw py::value_error("saved statistics do not belong to x");
+  const Tensor s = plain(rstd), w = weight.defined() ? plain(weight) : Tensor();
+  auto gradient = [&](const Tensor& t, const char* name) {
+    if (!t.defined()) return Tensor();
+    const Tensor g = plain(t.scalar_type() == h.scalar_type() ? t : t.to(h.scalar_type()));
+    same_device(g, h, name);
+    if (g.sizes() != h.sizes()) throw py::value_error(std::string(name) + " has another shape than x");
+    return g;
+  };
+  Tensor g = gradient(dy, "the gradient of y");
+  const Tensor m = gradient(dh, "the gradient of the sum");
+  RmsGradients out;
+  if (!g.defined()) {  // only the sum was used
+    if (want_x && m.defined()) out.dx = m;
+    if (want_weight) out.dweight = at::zeros_like(w);
+    return out;
+  }
+  Tensor workspace;
+  if (want_x) out.dx = at::empty(h.sizes(), h.options().memory_format(at::MemoryFormat::Contiguous));
+  if (want_weight) {
+    out.dweight = at::empty({D}, w.options());
+    a.workspace_bytes = static_cast<int64_t>(rms_workspace(r.rows, static_cast<int>(D), static_cast<int>(a.x_type)));
+    workspace = at::empty({a.workspace_bytes}, h.options().dtype(at::kByte));
+    a.workspace = workspace.data_ptr();
+  }
+  a.rows = r.rows;
+  a.D = D;
+  a.x_stride = r.stride;
+  a.eps = call.eps;
+  a.offset = call.offset;
+  a.x = r.x.data_ptr();
+  a.weight = address(w);
+  a.w_type = w.defined() ? element_type(w, "weight") : 0;
+  a.rstd = s.data_ptr<float>();
+  a.dy = g.data_ptr();
+  a.dh = address(m);
+  a.dx = address(out.dx);
+  a.dweight = address(out.dweight);
+  check(rms_backward(&a, device.stream()), "ffm_rms_norm_backward");
+  launches += want_weight ? 2 : want_x && r.rows > 0;
+  return out;
+}
+
+class RmsNorm : public torch::autograd::Function<RmsNorm> {
+ public:
+  static variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& weight_or_none, const OptTensor& residual_or_none,
+                               double eps, double offset) {
+    const Tensor weight = weight_or_none.value_or(Tensor()), residual = residual_or_none.value_or(Tensor());
+    RmsResult r = rms_forward_of(x, weight, residual, {eps, offset, false}, true);
+    ctx->save_for_backward({residual.defined() ? r.h : x, weight, r.rstd});
+    ctx->saved_data["residual"] = residual.defined();
+    ctx->saved_data["call"] = std::vector<double>{eps, offset};
+    ctx->set_materialize_grads(false);
+    return residual.defined() ? variable_list{r.y, r.h} : variable_list{r.y};
+  }
+  static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list grad) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out(5);
+    {
+      const at::AutoGradMode no_grad(false);
+      // an operand that is not there has no edge, and those after it move up
+      const bool weight = saved[1].defined(), residual = ctx->saved_data["residual"].toBool();
+      const std::vector<double> call = ctx->saved_data["call"].toDoubleVector();
+      const bool want_x = ctx->needs_input_grad(0), want_residual = residual && ctx->needs_input_grad(weight ? 2 : 1);
+      RmsGradients g = rms_backward_of(grad[0], residual ? grad[1] : Tensor(), saved[0], saved[1], saved[2], {call[0], call[1], false},
+                                       want_x || want_residual, weight && ctx->needs_input_grad(1));
+      if (want_x) out[0] = g.dx;
+      out[1] = g.dweight;
+      if (want_residual) out[2] = g.dx;
+    }
+    return once(std::move(out));
+  }
+};
+
+py::object rms_norm(const Tensor& x, const OptTensor& weight, double eps, const OptTensor& residual, double offset, bool e4m3) {
+  not_traced("rms_norm");
+  const Tensor w = weight.value_or(Tensor()), more = residual.value_or(Tensor());
+  no_tangent(x, "x");
+  no_tangent(w, "weight");
+  no_tangent(more, "residual");
+  const bool grads = at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (more.defined() && more.requires_grad()));
+  if (grads && e4m3) throw std::runtime_error("an 8-bit output is not differentiable: call under torch.no_grad()");
+  RmsResult r;
+  {
+    const py::gil_scoped_release released;
+    if (grads) {
+      capturable({&x, &w, &more});
+      const variable_list out = RmsNorm::apply(x, weight, residual, eps, offset);
+      r.y = out[0];
+      if (more.defined()) r.h = out[1];
+    } else {
+      r = rms_forward_of(x, w, more, {eps, offset, e4m3}, false);
+    }
+  }
+  if (e4m3) return more.defined() ? py::object(py::make_tuple(r.y, r.y_scale, r.h)) : py::object(py::make_tuple(r.y, r.y_scale));
+  return more.defined() ? py::object(py::make_tuple(r.y, r.h)) : py::cast(r.y);
+}
+
+// ---- 8-bit operands with a scale for every 128 values -----------------------------------------------------------
+
+void no_gradient(const Tensor& t, const char* name, const char* what) {
+  no_tangent(t, name);
+  if (at::GradMode::is_enabled() && t.requires_grad()) {
+    throw std::runtime_error(std::string(what) + " is not differentiable, and " + name + " requires a gradient: call under torch.no_grad()");
+  }
+}
+
+py::tuple quantize_e4m3(const Tensor& x, int64_t block_rows) {
+  not_traced("quantize_e4m3");
+  no_gradient(x, "x", "quantize_e4m3");
+  on_gpu(x, "x");
+  if (block_rows != 1 && block_rows != 128) throw py::value_error("block_rows must be 1 or 128, got " + std::to_string(block_rows));
+  if (x.dim() < (block_rows == 1 ? 1 : 2)) throw py::value_error("x must have rows" + std::string(block_rows == 1 ? "" : " and columns") + ", got " + c10::str(x.sizes()));
+  const int type = element_type(x, "x");
+  const int64_t K = x.size(-1);
+  if (K < 1 || K % 16 != 0 || K > std::numeric_limits<int>::max()) throw py::value_error("rows must have a multiple of 16 values, got " + std::to_string(K));
+  const int64_t rows = block_rows == 1 ? x.numel() / K : x.size(-2), matrices = block_rows == 1 ? 1 : (rows > 0 ? x.numel() / K / rows : 0);
+  Tensor q, scale;
+  {
+    const py::gil_scoped_release released;
+    const On device(x);
+    Rows r;
+    if (block_rows == 1) {
+      r = as_rows_for(x, true);
+    } else {
+      r.x = plain(x);
+      if (reinterpret_cast<uintptr_t>(r.x.data_ptr()) % 16 != 0) r.x = r.x.clone();
+      r.stride = K;
+    }
+    const auto contiguous = x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+    std::vector<int64_t> sizes = x.sizes().vec();
+    q = at::empty(sizes, contiguous.dtype(at::kFloat8_e4m3fn));
+    sizes.back() = (K + 127) / 128;
+    if (block_rows > 1) sizes[sizes.size() - 2] = (rows + 127) / 128;
+    scale = at::empty(sizes, contiguous.dtype(at::kFloat));
+    check(quantize_blocks(r.x.data_ptr(), type, matrices, rows, r.stride, static_cast<int>(K), static_cast<int>(block_rows), q.data_ptr(),
+                          scale.data_ptr<float>(), device.stream()),
+          "ffm_quantize_blocks_e4m3");
+    launches += matrices > 0 && rows > 0;
+  }
+  return py::make_tuple(q, scale);
+}
+
+void check_scale(const Tensor& scale, const Tensor& of, std::vector<int64_t> sizes, const char* name) {
+  same_device(scale, of, name);
+  no_gradient(scale, name, "linear_e4m3");
+  if (scale.scalar_type() != at::kFloat) throw py::type_error(std::string(name) + " must be float32, got " + c10::toString(scale.scalar_type()));
+  if (scale.sizes() != at::IntArrayRef(sizes)) throw py::value_error(std::string(name) + " must be " + c10::str(at::IntArrayRef(sizes)) + ", got " + c10::str(scale.sizes()));
+}
+
+Tensor linear_e4m3(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& weight_scale, const OptTensor& ends_or_none,
+                   at::ScalarType out_type, int64_t status, int64_t status_host) {
+  not_traced("linear_e4m3");
+  on_gpu(x, "x");
+  same_device(weight, x, "weight");
+  for (const auto& [t, name] : {std::pair<const Tensor*, const char*>{&x, "x"}, {&weight, "weight"}}) {
+    no_gradient(*t, name, "linear_e4m3");
+    if (t->scalar_type() != at::kFloat8_e4m3fn) throw py::type_error(std::string(name) + " must be float8_e4m3fn, got " + c10::toString(t->scalar_type()));
+  }
+  const bool grouped = ends_or_none.has_value();
+  if (weight.dim() != (grouped ? 3 : 2)) throw py::value_error(std::string("weight must be ") + (grouped ? "[experts, N, K]" : "[N, K]") + ", got " + c10::str(weight.sizes()));
+  const int64_t K = weight.size(-1), N = weight.size(-2), experts = grouped ? weight.size(0) : 1;
+  if (x.dim() < 1 || x.size(-1) != K) throw py::value_error("x must end in " + std::to_string(K) + ", got " + c10::str(x.sizes()));
+  if (grouped && x.dim() != 2) throw py::value_error("x must be [rows, K] where rows belong to experts, got " + c10::str(x.sizes()));
+  if (K < 1 || K % 16 != 0 || N < 1) throw py::value_error("K must be a multiple of 16 and N positive, got " + c10::str(weight.sizes()));
+  if (experts < 1 || experts > 1024) throw py::value_error("there are 1 to 1024 experts, got " + std::to_string(experts));
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = (K + 127) / 128;
+  check_scale(x_scale, x, sizes, "x_scale");
+  std::vector<int64_t> w_sizes = weight.sizes().vec();
+  w_sizes.back() = (K + 127) / 128;
+  w_sizes[w_sizes.size() - 2] = (N + 127) / 128;
+  check_scale(weight_scale, x, w_sizes, "weight_scale");
+  Tensor ends;
+  if (grouped) {
+    ends = *ends_or_none;
+    same_device(ends, x, "ends");
+    if (ends.scalar_type() != at::kInt) throw py::type_error(std::string("ends must be int32, got ") + c10::toString(ends.scalar_type()));
+    if (ends.dim() != 1 || ends.size(0) != experts) throw py::value_error("ends must be [" + std::to_string(experts) + "], got " + c10::str(ends.sizes()));
+  }
+  if (out_type != at::kBFloat16 && out_type != at::kHalf && out_type != at::kFloat) {
+    throw py::type_error(std::string("out_dtype must be bfloat16, float16 or float32, got ") + c10::toString(out_type));
+  }
+  const py::gil_scoped_release released;
+  const On device(x);
+  const Rows r = as_rows_for(x, true);
+  const Tensor xs = plain(x_scale), ws = plain(weight_scale);
+  Tensor w = plain(weight);
+  if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 != 0) w = w.clone();
+  if (grouped) ends = ends.contiguous();
+  sizes.back() = N;
+  const Tensor out = at::empty(sizes, x.options().dtype(out_type).requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+  ffm_linear_blocks_args a = {};
+  a.rows = r.rows;
+  a.N = N;
+  a.K = K;
+  a.experts = experts;
+  a.x_stride = r.stride;
+  a.out_type = element_type(out, "out");
+  a.x = r.x.data_ptr();
+  a.x_scale = xs.data_ptr<float>();
+  a.w = w.data_ptr();
+  a.w_scale = ws.data_ptr<float>();
+  a.ends = grouped ? ends.data_ptr<int32_t>() : nullptr;
+  a.out = out.data_ptr();
+  a.status = reinterpret_cast<int32_t*>(status);
+  a.status_host = reinterpret_cast<int32_t*>(status_host);
+  check(linear_blocks(&a, device.stream()), "ffm_linear_blocks_e4m3");
+  launches += r.rows > 0;
+  return out;
+}
+
 // ---- AdamW --------------------------------------------------------------------------------------------------
 
 // A zero word per device and stream that the kernel leaves zero: calls on one stream follow one another. A captured call gets
@@ -640,6 +960,109 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
   launches += launched;
 }
 
+// ---- gradient norm ----------------------------------------------------------------------------------------------
+
+// One after the other in memory in some order of the dimensions, each value once: then any pass over the memory is one over the tensor.
+bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense() && !t.is_neg(); }
+
+struct ClipTable {
+  std::vector<ffm_clip_tensor> entries;
+  std::vector<Tensor> held;
+
+  void add(const Tensor& t, const Tensor& like, const char* name) {
+    same_device(t, like, name);
+    ffm_clip_tensor e = {};
+    e.type = element_type(t, name);
+    held.push_back(dense(t) ? t : t.contiguous().resolve_neg());
+    e.x = held.back().data_ptr();
+    e.elements = t.numel();
+    if (e.elements > 0) entries.push_back(e);
+  }
+  int count() const {
+    if (entries.size() > static_cast<size_t>(std::numeric_limits<int>::max())) throw py::value_error("too many tensors");
+    return static_cast<int>(entries.size());
+  }
+};
+
+// The norm of `grads` and of what `other` (float64 [1], a sum of squares or a magnitude) stands for: (total float64 [1], norm, coefficient).
+py::tuple gradient_norm(const Tensors& grads, const Tensor& like, double max_norm, bool largest, const OptTensor& other, bool capturing) {
+  not_traced("the gradient norm");
+  on_gpu(like, "grad");
+  if (!(max_norm >= 0.0)) throw py::value_error("max_norm must not be negative, got " + std::to_string(max_norm));
+  for (const Tensor& t : grads) on_gpu(t, "grad");
+  const On device(like);
+  ClipTable table;
+  for (const Tensor& t : grads) table.add(t, like, "grad");
+  ffm_grad_norm_args a = {};
+  a.kind = largest ? 1 : 0;
+  a.max_norm = max_norm;
+  Tensor more;
+  if (other.has_value()) {
+    same_device(*other, like, "other");
+    if (other->numel() != 1 || other->scalar_type() != at::kDouble) throw py::type_error("other must be one float64 value");
+    more = other->resolve_neg();
+    a.other = more.data_ptr<double>();
+  }
+  const auto options = like.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+  const Tensor total = at::empty({1}, options.dtype(at::kDouble)), both = at::empty({2}, options.dtype(at::kFloat));
+  a.total = total.data_ptr<double>();
+  a.norm = both.data_ptr<float>();
+  a.coefficient = both.data_ptr<float>() + 1;
+  a.workspace_bytes = static_cast<int64_t>(grad_norm_workspace(table.count()));
+  const Tensor workspace = at::empty({a.workspace_bytes}, options.dtype(at::kByte));
+  a.workspace = workspace.data_ptr();
+  const Tensor ticket = ticket_for(like, device.stream(), capturing);
+  a.ticket = ticket.data_ptr();
+  int64_t launched = 0;
+  a.launched = &launched;
+  check(grad_norm(table.entries.data(), table.count(), &a, device.stream()), "ffm_grad_norm");
+  launches += launched;
+  return py::make_tuple(total, both.select(0, 0), both.select(0, 1));
+}
+
+// grads *= factor (one float32 on the device), in place
+void scale_gradients_by(const Tensors& grads, const Tensor& factor) {
+  not_traced("clipping");
+  on_gpu(factor, "factor");
+  if (factor.numel() != 1 || factor.scalar_type() != at::kFloat) throw py::type_error("factor must be one float32 value");
+  const On device(factor);
+  ClipTable table;
+  for (const Tensor& t : grads) table.add(t, factor, "grad");
+  int64_t launched = 0;
+  check(scale_tensors(table.entries.data(), table.count(), factor.data_ptr<float>(), &launched, device.stream()), "ffm_scale_tensors");
+  launches += launched;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& t = grads[i];
+    if (!table.held[i].is_same(t)) {
+      const at::NoGradGuard no_grad;
+      t.copy_(table.held[i]);  // it lies in a way that the kernel does not take
+    } else if (!t.is_inference()) {
+      t.unsafeGetTensorImpl()->bump_version();
+    }
+  }
+}
+
+// Whether two of the tensors, or two elements of one, share memory: scaling in place would multiply twice.
+void check_separate(const Tensors& grads) {
+  std::vector<std::pair<const char*, const char*>> ranges;
+  for (const Tensor& t : grads) {
+    if (t.numel() == 0) continue;
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      if (t.size(d) > 1 && t.stride(d) == 0) throw py::value_error("a gradient that was expanded cannot be scaled in place");
+      last += (t.size(d) - 1) * t.stride(d);
+    }
+    const char* from = static_cast<const char*>(t.data_ptr());
+    ranges.emplace_back(from, from + (last + 1) * t.element_size());
+  }
+  std::sort(ranges.begin(), ranges.end());
+  const char* end = nullptr;
+  for (const auto& r : ranges) {
+    if (r.first < end) throw py::value_error("a gradient appears twice in one call, or lies on another");
+    end = std::max(end, r.second);
+  }
+}
+
 }  // namespace
 
 void define_ops(py::module_& m) {
@@ -648,4 +1071,13 @@ void define_ops(py::module_& m) {
   m.def("layer_norm", &layer_norm);
   m.def("linear_cross_entropy", &linear_cross_entropy);
   m.def("adamw_step", &adamw_step);
+  m.def("rms_norm", &rms_norm);
+  m.def("quantize_e4m3", &quantize_e4m3);
+  m.def("linear_e4m3", [](const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& weight_scale, const OptTensor& ends,
+                          const py::object& out_type, int64_t status, int64_t status_host) {
+    return linear_e4m3(x, x_scale, weight, weight_scale, ends, torch::python::detail::py_object_to_dtype(out_type), status, status_host);
+  });
+  m.def("gradient_norm", &gradient_norm);
+  m.def("check_separate", &check_separate);
+  m.def("scale_gradients", &scale_gradients_by);
 }

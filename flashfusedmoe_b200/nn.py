@@ -11,7 +11,7 @@ import torch
 import torch.nn as nn
 
 from .fused_moe import fused_moe, glu_ffn, set_ep_group
-from .norm import LayerNorm
+from .norm import LayerNorm, RMSNorm
 
 
 class _GLUFFN(nn.Module):
@@ -43,7 +43,8 @@ class MoELayer(nn.Module):
     `ep_full_input_grad` (extension, default False = the reference's contract) adds the expert input gradient to
     the expert-parallel backward through a reverse dispatch exchange.
     `pre_norm` (extension, default False) puts a layer norm in front of the layer, with its parameters as norm.weight and
-    norm.bias and `norm_eps`: forward(x) is then the layer of norm(x), the branch of a pre-norm residual block.
+    norm.bias and `norm_eps`: forward(x) is then the layer of norm(x), the branch of a pre-norm residual block. "rms" puts a
+    root-mean-square norm there, with norm.weight alone.
     """
 
     def __init__(self, d_model, ffn_dim, num_experts, top_k=2, activation="swiglu", gating="softmax",
@@ -70,8 +71,10 @@ class MoELayer(nn.Module):
 
         # only where asked for: a subclass may have a `norm` or `pre_norm` of its own
         self._pre_norm = pre_norm
+        if isinstance(pre_norm, str) and pre_norm not in ("layer", "rms"):
+            raise ValueError(f"Unknown norm: {pre_norm}")
         if pre_norm:
-            self.norm = LayerNorm(d_model, eps=norm_eps)
+            self.norm = (RMSNorm if pre_norm == "rms" else LayerNorm)(d_model, eps=norm_eps)
         self.gate = nn.Linear(d_model, num_experts, bias=False)
         nn.init.kaiming_uniform_(self.gate.weight, a=math.sqrt(5))
         self.gate.weight.data *= 0.01

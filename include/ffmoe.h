@@ -608,6 +608,112 @@ size_t ffm_linear_cross_entropy_workspace_bytes(const ffm_loss_args* args);
 int ffm_linear_cross_entropy(const ffm_loss_args* args, ffm_stream_t stream);
 int ffm_scale_many(int count, void* const* x, const int64_t* types, const int64_t* elements, const float* factor, ffm_stream_t stream);
 
+/* -------------------------------------------------------------------------------------------------
+ * Root-mean-square norm over rows of D <= 32768 values (fp32: 16384), with the residual's addition in front:
+ *   h = x + residual (rounded to x's type; null residual: h is x), y = h / sqrt(mean(h^2) + eps) * (weight + offset)
+ * x_type: of x, residual, h, y, dy, dh and dx; weight (null: 1) and dweight are of w_type. x and residual have rows x_stride and
+ * residual_stride elements apart, all others are contiguous. Any D and any element-aligned address, but for the 8-bit output.
+ *
+ * ffm_rms_norm_forward reads x, residual, weight and writes h (with a residual), rstd (f32 [rows], null: not wanted: 1 / sqrt(...)) and y; with
+ *   y_scale (f32 [rows, ceil(D / 128)]) y is e4m3 [rows, D]: y over the scale of its 128 columns, which is their largest magnitude / 448,
+ *   at least 2^-126 (1 where all are zero). D % 16 == 0 and addresses and rows on 16 bytes then.
+ * ffm_rms_norm_backward reads dy, dh (null: none), x (the forward pass's h, rows x_stride apart), rstd and weight, and writes dx (null: not
+ *   wanted; the gradient of x and of residual, dh added) and dweight (null: not wanted; summed in fp32 in a fixed order).
+ *   workspace: ffm_rms_norm_workspace_bytes, needed with dweight. rows == 0 gives zero sums.
+ * Every field is 8 bytes wide.
+ * ------------------------------------------------------------------------------------------------- */
+typedef struct {
+  int64_t rows;
+  int64_t D;
+  int64_t x_type;
+  int64_t w_type;
+  int64_t x_stride;
+  int64_t residual_stride;
+  double eps;
+  double offset;
+  const void* x;
+  const void* residual;
+  const void* weight;
+  void* h;
+  void* y;
+  float* y_scale;
+  float* rstd;
+  const void* dy;
+  const void* dh;
+  void* dx;
+  void* dweight;
+  void* workspace;
+  int64_t workspace_bytes;
+} ffm_rms_norm_args;
+int ffm_rms_norm_forward(const ffm_rms_norm_args* args, ffm_stream_t stream);
+size_t ffm_rms_norm_workspace_bytes(int64_t rows, int D, int x_type);
+int ffm_rms_norm_backward(const ffm_rms_norm_args* args, ffm_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------------
+ * e4m3 operands with a scale for every 128 values, and their products. K % 16 == 0, addresses and rows on 16 bytes.
+ *
+ * ffm_quantize_blocks_e4m3: x [matrices, rows, K] (FFM_TYPE_*) to q and scale. block_rows = 1: a scale for 128 values of a row, [rows,
+ *   ceil(K / 128)], matrices = 1, rows row_stride elements apart; block_rows = 128: one for 128 x 128 values, [matrices, ceil(rows / 128),
+ *   ceil(K / 128)], x contiguous. The scale is the largest magnitude / 448, at least 2^-126 (1 where all are zero); NaN values do not count.
+ * ffm_linear_blocks_e4m3: out [rows, N] (out_type) = x [rows, K] w[e] [N, K]^T with x_scale [rows, ceil(K / 128)] and w_scale [experts,
+ *   ceil(N / 128), ceil(K / 128)]; e is the expert with ends[e - 1] <= row < ends[e], rows from the last end on are 0. ends null: experts
+ *   = 1 takes all rows. ends (int32 on the device) must not decrease nor pass rows: such ends are moved into place and set
+ *   FFM_STATUS_BAD_INDEX. At most 1024 experts. Sums are fp32. status, status_host: as in ffm_linear_cross_entropy.
+ * Every field is 8 bytes wide.
+ * ------------------------------------------------------------------------------------------------- */
+typedef struct {
+  int64_t rows;
+  int64_t N;
+  int64_t K;
+  int64_t experts;
+  int64_t x_stride;
+  int64_t out_type;
+  const void* x;
+  const float* x_scale;
+  const void* w;
+  const float* w_scale;
+  const int32_t* ends;
+  void* out;
+  int32_t* status;
+  int32_t* status_host;
+} ffm_linear_blocks_args;
+int ffm_quantize_blocks_e4m3(const void* x, int x_type, int64_t matrices, int64_t rows, int64_t row_stride, int K, int block_rows, void* q,
+                             float* scale, ffm_stream_t stream);
+int ffm_linear_blocks_e4m3(const ffm_linear_blocks_args* args, ffm_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------------
+ * The norm of all gradients together, and clipping. `count` tensors (contiguous; types: FFM_TYPE_*), FFM_CLIP_MAX a launch.
+ *
+ * ffm_grad_norm: kind 0: the root of the sum of squares; kind 1: the largest magnitude. Sums are in 64 bits and in a fixed order.
+ *   other (null, or one f64 on the device): a sum of squares (a magnitude) of tensors elsewhere, taken in.
+ *   total (null or f64): the sum of squares (the magnitude); norm, coefficient (null or f32): the norm, and min(1, max_norm / (norm + 1e-6)),
+ *   NaN where the norm is.
+ *   workspace: ffm_grad_norm_workspace_bytes(count). ticket: a device word, zero before the call and after it, that no other call in flight uses.
+ * ffm_scale_tensors: x *= *factor for every tensor; nothing is written where it is 1.
+ * launched (null or host): kernels enqueued are added. Every field is 8 bytes wide.
+ * ------------------------------------------------------------------------------------------------- */
+#define FFM_CLIP_MAX 512
+typedef struct {
+  void* x;
+  int64_t type;
+  int64_t elements;
+} ffm_clip_tensor;
+typedef struct {
+  int64_t kind;
+  double max_norm;
+  const double* other;
+  double* total;
+  float* norm;
+  float* coefficient;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* ticket;
+  int64_t* launched;
+} ffm_grad_norm_args;
+size_t ffm_grad_norm_workspace_bytes(int count);
+int ffm_grad_norm(const ffm_clip_tensor* tensors, int count, const ffm_grad_norm_args* args, ffm_stream_t stream);
+int ffm_scale_tensors(const ffm_clip_tensor* tensors, int count, const float* factor, int64_t* launched, ffm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
