@@ -111,7 +111,7 @@ quantize_tiles_kernel(const T* __restrict__ x, int N, int K, int down, int acros
 
 // ---- products ---------------------------------------------------------------------------------------------------
 
-constexpr int BLOCK_THREADS = 320;
+constexpr int BLOCK_THREADS = 384;
 constexpr int MAX_EXPERTS = 1024;
 constexpr int A_ROWS = 128;
 constexpr int UMMA_K8 = 32;  // e4m3 values of the contraction in an instruction
@@ -229,32 +229,57 @@ template <int BN>
 struct ManyRows {
   static constexpr int COLS = BN / 2;  // features of a warp: the eight warps are two halves of a tile by four lane quarters
   static constexpr int STAGE_BYTES = (A_ROWS + BN) * 128;
-  static constexpr int STAGES = 196608 / STAGE_BYTES;
-  static constexpr int STAGING = 8 * 32 * 64;  // 32 rows x 64 bytes a warp
+  static constexpr int STAGES = 147456 / STAGE_BYTES;
+  static constexpr int STORE_WARP = 2 * 32 * 128;  // two boxes of 32 rows x 128 bytes (128-byte swizzle) on their way out
+  static constexpr int STORE_BYTES = 8 * STORE_WARP;
+  static constexpr int SLOTS = 8;  // blocks whose scales are there or on their way
   struct Ctrl {
-    unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[2], acc_empty_bar[2], drain_bar;
+    unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[2], acc_empty_bar[2], scale_full_bar[SLOTS], scale_empty_bar[SLOTS], drain_bar;
     uint32_t tmem_base;
     int abort_flag;
     int filled;
+    alignas(16) float scale[SLOTS][A_ROWS + 4];  // of the rows, and of the two halves' features
     Groups groups;
   };
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING + static_cast<int>(sizeof(Ctrl)) + 1024;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STORE_BYTES + static_cast<int>(sizeof(Ctrl)) + 1024;
   static_assert(SMEM_BYTES <= 232448, "tile shape does not fit in shared memory");
 };
 
-// 16 bytes q (0..3) of row r in 32 rows of 64 bytes: eight neighbouring rows meet no bank twice
-__device__ __forceinline__ uint32_t staged(int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); }
+__device__ __forceinline__ void copy_async_4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// arrives once this thread's copies so far have landed; the barrier's count has an arrival for it
+__device__ __forceinline__ void copy_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 
-//   warp 0      TMA producer          warp 1   MMA issuer, TMEM owner
-//   warps 2..9  take a block's sums out of TMEM, scale and add them, store the tile
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// byte b of row r in a warp's boxes
+__device__ __forceinline__ uint32_t in_boxes(int r, int b) { return (b >> 7) * 4096 + box_offset(r, (b >> 4) & 7) + (b & 15); }
+
+// A value in front of the first whole word of a row of 16-bit values
+__device__ __forceinline__ int head_of(const uint8_t* row) { return (reinterpret_cast<uintptr_t>(row) >> 1) & 1; }
+
+// The launch's 168 registers a thread go from the four warps of the first group to the eight that hold sums: 128 x 56 + 256 x 224 = 384 x 168.
+constexpr int ISSUE_REGISTERS = 56, SUM_REGISTERS = 224;
+static_assert(128 * ISSUE_REGISTERS + 256 * SUM_REGISTERS <= BLOCK_THREADS * 168, "more registers than the launch has");
+
+//   warp 0      TMA producer          warp 1   MMA issuer, TMEM owner          warp 2   row ranges, scales          warp 3   nothing
+//   warps 4..11 take a block's sums out of TMEM, scale and add them, store the tile
 template <int BN, int OUT_BYTES>
 __global__ void __launch_bounds__(BLOCK_THREADS, 1)
-block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ BlockParams p) {
+block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_out,
+                  const __grid_constant__ BlockParams p) {
   using S = ManyRows<BN>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw), pad = (1024u - (raw_addr & 1023u)) & 1023u;
   const uint32_t smem_base = raw_addr + pad, staging = smem_base + S::STAGES * S::STAGE_BYTES;
-  auto* ctrl = reinterpret_cast<typename S::Ctrl*>(smem_raw + pad + S::STAGES * S::STAGE_BYTES + S::STAGING);
+  auto* ctrl = reinterpret_cast<typename S::Ctrl*>(smem_raw + pad + S::STAGES * S::STAGE_BYTES + S::STORE_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -265,6 +290,10 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&ctrl->acc_full_bar[a]), 1);
       mbar_init(smem_u32(&ctrl->acc_empty_bar[a]), 8);
+    }
+    for (int i = 0; i < S::SLOTS; ++i) {
+      mbar_init(smem_u32(&ctrl->scale_full_bar[i]), 32);
+      mbar_init(smem_u32(&ctrl->scale_empty_bar[i]), 8);
     }
     mbar_init(smem_u32(&ctrl->drain_bar), 1);
     ctrl->abort_flag = 0;
@@ -288,8 +317,9 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
   BlockWalker walker(&ctrl->groups, p, A_ROWS, blockIdx.x, gridDim.x);
   BlockTile t;
 
-  if (warp == 0) {
-    if (elect_one()) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ISSUE_REGISTERS));
+    if (warp == 0 && elect_one()) {
       int stage = 0, filled = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -307,8 +337,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
       }
       ctrl->filled = filled;
     }
-  } else if (warp == 1) {
-    if (elect_one()) {
+    if (warp == 1 && elect_one()) {
       issuer = true;
       constexpr uint32_t idesc = make_idesc_e4m3(A_ROWS, BN);
       int stage = 0, acc = 0;
@@ -333,106 +362,154 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
         }
       }
     }
+    if (warp == 2) {
+      // the scales of the tile's rows and features, block by block, ahead of the sums that they belong to
+      const int scale_rows = (p.N + E4M3_BLOCK - 1) / E4M3_BLOCK;
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      while (ok && walker.next(t)) {
+        // rows past the tile's last: any
+        const float* xs = p.x_scale + static_cast<long long>(t.row0) * p.k_blocks;
+        const int f = min(t.across * (BN / E4M3_BLOCK) + (BN > E4M3_BLOCK ? lane & 1 : 0), scale_rows - 1);
+        const float* ws = p.w_scale + (static_cast<long long>(t.group) * scale_rows + f) * p.k_blocks;
+        for (int kb = 0; kb < t.k_blocks; ++kb) {
+          ok = mbar_wait_bounded(smem_u32(&ctrl->scale_empty_bar[slot]), phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_PRODUCER, p.wait_cycles);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t to = smem_u32(ctrl->scale[slot]);
+#pragma unroll
+          for (int r = 0; r < A_ROWS; r += 32) copy_async_4(to + (r + lane) * 4, xs + static_cast<long long>(min(r + lane, t.rows - 1)) * p.k_blocks + kb);
+          if (lane < 2) copy_async_4(to + (A_ROWS + lane) * 4, ws + kb);
+          copy_async_arrive(smem_u32(&ctrl->scale_full_bar[slot]));
+          if (++slot == S::SLOTS) slot = 0, phase ^= 1u;
+        }
+      }
+      copy_async_wait<0>();
+    }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * S::COLS, mine = staging + (warp - 2) * 2048;
-    const int scale_rows = (p.N + E4M3_BLOCK - 1) / E4M3_BLOCK;
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SUM_REGISTERS));
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * S::COLS;
+    const uint32_t mine = staging + (warp - 4) * S::STORE_WARP;  // this warp's rows on their way out
+    int acc = 0, slot = 0;
+    uint32_t acc_phase = 0, slot_phase = 0;
     bool ok = true;
     while (ok && walker.next(t)) {
-      const int f0 = t.across * BN + half * S::COLS;  // this warp's first feature
-      const bool in_tile = quarter * 32 + lane < t.rows;
-      const float* xs = p.x_scale + static_cast<long long>(t.row0 + (in_tile ? quarter * 32 + lane : 0)) * p.k_blocks;
-      const float* ws = p.w_scale + (static_cast<long long>(t.group) * scale_rows + min(f0 / E4M3_BLOCK, scale_rows - 1)) * p.k_blocks;
       float2 sum[S::COLS / 2];
 #pragma unroll
       for (int j = 0; j < S::COLS / 2; ++j) sum[j] = both(0.0f);
-      // the scales of the next two blocks are on their way
-      float s0 = t.k_blocks > 0 ? __ldg(xs) * __ldg(ws) : 0.0f, s1 = t.k_blocks > 1 ? __ldg(xs + 1) * __ldg(ws + 1) : 0.0f;
+      uint32_t v[2][32];
       for (int kb = 0; kb < t.k_blocks; ++kb) {
-        const float x2 = kb + 2 < t.k_blocks ? __ldg(xs + kb + 2) : 0.0f, w2 = kb + 2 < t.k_blocks ? __ldg(ws + kb + 2) : 0.0f;
         ok = mbar_wait_bounded(smem_u32(&ctrl->acc_full_bar[acc]), acc_phase, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const float2 s = both(s0);
-        uint32_t v[2][16];
-        tmem_ld_32x16(taddr + acc * BN, v[0]);
+        // 64 columns at a time: with 32 and the next 32 on their way the two warps of a scheduler waited together (8192 x 4096 x 4096 without
+        // the stores: 137 us, so 122)
+        tmem_ld_32x32(taddr + acc * BN, v[0]);
+        tmem_ld_32x32(taddr + acc * BN + 32, v[1]);
+        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_full_bar[slot]), slot_phase, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
+        ok = __all_sync(0xffffffffu, ok);
+        const float2 s = both(ctrl->scale[slot][quarter * 32 + lane] * ctrl->scale[slot][A_ROWS + half]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctrl->scale_empty_bar[slot]));
+        if (++slot == S::SLOTS) slot = 0, slot_phase ^= 1u;
 #pragma unroll
-        for (int c = 0; c < S::COLS / 16; ++c) {
+        for (int c = 0; c < S::COLS / 64; ++c) {
           tmem_ld_wait();
-          if (c + 1 < S::COLS / 16) {
-            tmem_ld_32x16(taddr + acc * BN + (c + 1) * 16, v[(c + 1) & 1]);
-          } else {
+          if (c + 1 == S::COLS / 64) {
             tc_fence_before();
             if (lane == 0) mbar_arrive(smem_u32(&ctrl->acc_empty_bar[acc]));
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            sum[c * 8 + j] = fma2(make_float2(__uint_as_float(v[c & 1][2 * j]), __uint_as_float(v[c & 1][2 * j + 1])), s, sum[c * 8 + j]);
+          for (int j = 0; j < 32; ++j) {
+            sum[c * 32 + j] = fma2(make_float2(__uint_as_float(v[j >> 4][2 * (j & 15)]), __uint_as_float(v[j >> 4][2 * (j & 15) + 1])), s, sum[c * 32 + j]);
+          }
+          if (c + 1 < S::COLS / 64) {
+            tmem_ld_32x32(taddr + acc * BN + (c + 1) * 64, v[0]);
+            tmem_ld_32x32(taddr + acc * BN + (c + 1) * 64 + 32, v[1]);
           }
         }
+        if (!ok) break;
         if (++acc == 2) acc = 0, acc_phase ^= 1u;
-        s0 = s1;
-        s1 = x2 * w2;
       }
       if (!ok) break;
-      // 64 bytes of every row at a time through shared memory, so that neighbouring lanes store neighbouring 16 bytes
-      constexpr int STEP = 64 / OUT_BYTES;
-      const int limit = t.rows - quarter * 32;  // of this warp's rows
+      // Up to 256 bytes of every row at a time through shared memory. 32 whole rows on 16 bytes go out by themselves, while the next tile's sums
+      // begin; others are stored from here.
+      constexpr int STEP = S::COLS * OUT_BYTES > 256 ? 256 / OUT_BYTES : S::COLS;
+      const int limit = min(t.rows - quarter * 32, 32);  // of this warp's rows
 #pragma unroll
       for (int c = 0; c < S::COLS / STEP; ++c) {
+        const int first = t.across * BN + half * S::COLS + c * STEP, count = min(STEP, p.N - first);
+        if (lane == 0) bulk_wait_read<0>();  // what was sent before has been read
         __syncwarp();
+        const long long pitch = static_cast<long long>(p.N) * OUT_BYTES;
+        uint8_t* out = static_cast<uint8_t*>(p.out) + (t.row0 + quarter * 32) * pitch + first * OUT_BYTES;
+        // 16-bit rows off 16 bytes are staged as the words that memory has them in, without the value in front of the first
+        const bool shift = OUT_BYTES == 2 && !p.out_wide && head_of(out + lane * pitch);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < STEP * OUT_BYTES / 16; ++q) {
+          const uint32_t at = mine + in_boxes(lane, q * 16);
           if constexpr (OUT_BYTES == 2) {
-            const float2* f = sum + c * 16 + q * 4;
-            st_shared_v4(mine + staged(lane, q), pack_out(p.out_type, f[0].x, f[0].y), pack_out(p.out_type, f[1].x, f[1].y),
-                         pack_out(p.out_type, f[2].x, f[2].y), pack_out(p.out_type, f[3].x, f[3].y));
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = c * (STEP / 2) + q * 4 + i;
+              const float after = q * 4 + i + 1 < STEP / 2 ? sum[j + 1 < S::COLS / 2 ? j + 1 : j].x : 0.0f;
+              u[i] = pack_out(p.out_type, shift ? sum[j].y : sum[j].x, shift ? after : sum[j].y);
+            }
+            st_shared_v4(at, u[0], u[1], u[2], u[3]);
           } else {
-            const float2* f = sum + c * 8 + q * 2;
-            st_shared_v4(mine + staged(lane, q), __float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+            const float2* f = sum + c * (STEP / 2) + q * 2;
+            st_shared_v4(at, __float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
           }
         }
-        __syncwarp();
-        const int first = f0 + c * STEP;
-        uint8_t* out = static_cast<uint8_t*>(p.out) + (static_cast<long long>(t.row0 + quarter * 32) * p.N + first) * OUT_BYTES;
-        if (p.out_wide) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2), q = lane & 3;
+        if (count <= 0 || limit <= 0) continue;
+        if (p.out_wide && limit == 32) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            for (int b = 0; b < count * OUT_BYTES; b += 128) tma_store_3d(&tm_out, mine + b * 32, first + b / OUT_BYTES, t.row0 + quarter * 32, 0);
+            bulk_commit();
+          }
+        } else if (p.out_wide) {
+          __syncwarp();
+          for (int i = lane; i < limit * 16; i += 32) {  // 16 bytes each
+            const int r = i >> 4, at = (i & 15) * 16;
             uint4 u;
-            ld_shared_v4(mine + staged(r, q), u);
-            if (r < limit && first + q * (16 / OUT_BYTES) < p.N) *reinterpret_cast<uint4*>(out + static_cast<long long>(r) * p.N * OUT_BYTES + q * 16) = u;
+            ld_shared_v4(mine + in_boxes(r, at), u);
+            if (at < count * OUT_BYTES) *reinterpret_cast<uint4*>(out + r * pitch + at) = u;
           }
         } else {
-          constexpr int AT_ONCE = 32 / STEP;  // rows of an instruction
-          const int col = lane % STEP, r0 = lane / STEP;
-          const uint32_t from = (col * OUT_BYTES) & 15, piece = (col * OUT_BYTES) >> 4;
-#pragma unroll 4
-          for (int i = 0; i < 32 / AT_ONCE; ++i) {
-            const int r = i * AT_ONCE + r0;
-            uint32_t bits;
-            if constexpr (OUT_BYTES == 2) {
-              uint16_t b;
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(mine + staged(r, piece) + from) : "memory");
-              bits = b;
-            } else {
-              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bits) : "r"(mine + staged(r, piece) + from) : "memory");
+          if constexpr (OUT_BYTES == 2) {
+            // what is not in a whole word: the first value, and the last
+            uint8_t* row = out + lane * pitch;
+            const int last = (count - (shift ? 1 : 0)) & 1;
+            if (lane < limit && shift) *reinterpret_cast<uint16_t*>(row) = static_cast<uint16_t>(pack_out(p.out_type, sum[c * (STEP / 2)].x, 0.0f));
+            if (lane < limit && last) {
+              const int word = (count - (shift ? 1 : 0)) >> 1;
+              reinterpret_cast<uint16_t*>(row)[count - 1] = static_cast<uint16_t>(ld_shared_u32(mine + in_boxes(lane, word * 4)));
             }
-            if (r < limit && first + col < p.N) {
-              uint8_t* to = out + (static_cast<long long>(r) * p.N + col) * OUT_BYTES;
-              if constexpr (OUT_BYTES == 2) {
-                *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(bits);
-              } else {
-                *reinterpret_cast<uint32_t*>(to) = bits;
-              }
+          }
+          __syncwarp();
+          // words of a row: a warp's 32 at a time
+          for (int r0 = 0; r0 < limit; r0 += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = r0 + i;
+              uint8_t* row = out + r * pitch;
+              const int head = OUT_BYTES == 2 ? head_of(row) : 0, words = r < limit ? (OUT_BYTES == 2 ? (count - head) >> 1 : count) : 0;
+              const uint32_t from = mine + r * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4;
+              uint32_t* to = reinterpret_cast<uint32_t*>(row + head * 2) + lane;
+              if (lane < words) to[0] = ld_shared_u32(from);
+              if (STEP * OUT_BYTES > 128 && lane + 32 < words) to[32] = ld_shared_u32(from + 4096);
             }
           }
         }
       }
     }
+    bulk_wait0();  // its stores have landed before the CTA's shared memory goes away
   }
 
   // ---- common exit: every role reaches this point, also after an abort
@@ -710,11 +787,11 @@ bool allow_smem(K kernel, int bytes, PerDevice& room) {
 }
 
 template <int BN, int OUT_BYTES>
-int launch_many(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const BlockParams& p, long long tiles, cudaStream_t stream) {
+int launch_many(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const CUtensorMap& tm_out, const BlockParams& p, long long tiles, cudaStream_t stream) {
   static PerDevice room;
   auto kernel = block_gemm_kernel<BN, OUT_BYTES>;
   if (!allow_smem(kernel, ManyRows<BN>::SMEM_BYTES, room)) return FFM_ERR_LAUNCH;
-  kernel<<<static_cast<unsigned>(tiles < num_sms() ? tiles : num_sms()), BLOCK_THREADS, ManyRows<BN>::SMEM_BYTES, stream>>>(tm_x, tm_w, p);
+  kernel<<<static_cast<unsigned>(tiles < num_sms() ? tiles : num_sms()), BLOCK_THREADS, ManyRows<BN>::SMEM_BYTES, stream>>>(tm_x, tm_w, tm_out, p);
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
 
@@ -819,6 +896,11 @@ extern "C" int ffm_linear_blocks_e4m3(const ffm_linear_blocks_args* args, ffm_st
     while (split < MAX_SPLIT && most * split * 2 <= num_sms() && p.k_blocks >= split * 4) split *= 2;
     return split > 1 ? launch_few<true>(tm_x, tm_w, p, most, split, st) : launch_few<false>(tm_x, tm_w, p, most, 1, st);
   }
-  if (box_n == 256) return four ? launch_many<256, 4>(tm_x, tm_w, p, most, st) : launch_many<256, 2>(tm_x, tm_w, p, most, st);
-  return four ? launch_many<128, 4>(tm_x, tm_w, p, most, st) : launch_many<128, 2>(tm_x, tm_w, p, most, st);
+  CUtensorMap tm_out = {};  // read only where rows lie on 16 bytes
+  if (p.out_wide) {
+    rc = make_box_map(&tm_out, a.out, 1, a.rows, a.N, a.N, type_bytes(p.out_type));
+    if (rc != FFM_OK) return rc;
+  }
+  if (box_n == 256) return four ? launch_many<256, 4>(tm_x, tm_w, tm_out, p, most, st) : launch_many<256, 2>(tm_x, tm_w, tm_out, p, most, st);
+  return four ? launch_many<128, 4>(tm_x, tm_w, tm_out, p, most, st) : launch_many<128, 2>(tm_x, tm_w, tm_out, p, most, st);
 }
