@@ -126,6 +126,7 @@ struct BlockParams {
   int k_blocks;
   int out_type;
   int out_wide;  // rows of out lie on 16 bytes
+  int box_rows;  // few rows: of x in a load
   void* out;
   int32_t* status;
   volatile int32_t* status_host;
@@ -534,53 +535,95 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
 
 // ---- few rows an expert: 128 features x up to 64 rows, features on the M side -------------------------------------
 
-// The weights are streamed once and everything else should cost nothing: a tile loads and computes the 16-row boxes that hold rows.
+// The weights are streamed once and everything else should cost nothing: a tile loads and computes the boxes (of 16, 32 or 64 rows) that hold rows.
+constexpr int FEW_ROWS = 64;
+
+// ONE: a cluster's CTAs share one tile's contraction, and so do the two groups of warps of each; else a CTA goes through tiles.
+template <bool ONE>
 struct FewRows {
-  static constexpr int ROWS = 64;
+  static constexpr int ROWS = FEW_ROWS;
   static constexpr int STAGE_BYTES = (A_ROWS + ROWS) * 128;
-  static constexpr int STAGES = 7;
-  static constexpr int PART = ROWS * A_ROWS * 4;  // a split contraction's sums
+  static constexpr int STAGES = ONE ? 6 : 8;
+  static constexpr int PART = ONE ? 2 * ROWS * A_ROWS * 4 : 0;  // the two groups' sums
+  static constexpr int SLOTS = 8;                 // blocks whose scales are there or on their way
   struct Ctrl {
-    unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[2], acc_empty_bar[2], drain_bar;
+    unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[4], acc_empty_bar[4], scale_full_bar[SLOTS], scale_empty_bar[SLOTS], drain_bar;
     uint32_t tmem_base;
     int abort_flag;
     int filled;
-    alignas(16) float scale[4][2][ROWS];  // of a warp's block and the next
+    alignas(16) float scale[SLOTS][ROWS + 4];  // of the rows, and of the features
     Groups groups;
   };
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PART + static_cast<int>(sizeof(Ctrl)) + 1024;
   static_assert(SMEM_BYTES <= 232448, "tile shape does not fit in shared memory");
 };
-constexpr int FEW_THREADS = 192;  // producer, MMA issuer, and a warp for each lane quarter
+constexpr int FEW_THREADS = 384;  // four warps as above, and two groups of a warp for each lane quarter, which take tiles in turn
 constexpr int MAX_SPLIT = 8;
 
-__device__ __forceinline__ float ld_shared_cluster(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ float4 ld_shared_cluster(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
   return v;
 }
 
-// SPLIT: a cluster's CTAs share a tile's contraction, one tile a cluster; their sums meet in shared memory and are added in the order of the ranks.
-template <bool SPLIT>
+// a feature's sums, rows `pitch` apart
+template <typename T>
+__device__ __forceinline__ void store_rows(T* out, long long pitch, int rows, const float (&sum)[FEW_ROWS]) {
+#pragma unroll
+  for (int j = 0; j < FEW_ROWS; ++j) {
+    if (j < rows) out[j * pitch] = from_float<T>(sum[j]);
+  }
+}
+
+// Sums of COLS rows from TMEM, scaled, added to those in registers
+template <int COLS>
+__device__ __forceinline__ void add_rows(uint32_t taddr, const float* scale, float w, float (&sum)[FEW_ROWS]) {
+  uint32_t v[COLS];
+  if constexpr (COLS == 16) {
+    tmem_ld_32x16(taddr, v);
+  } else {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32) tmem_ld_32x32(taddr + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
+  }
+  tmem_ld_wait();
+#pragma unroll
+  for (int j = 0; j < COLS; j += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(scale + j);
+    sum[j] = fmaf(__uint_as_float(v[j]), s.x * w, sum[j]);
+    sum[j + 1] = fmaf(__uint_as_float(v[j + 1]), s.y * w, sum[j + 1]);
+    sum[j + 2] = fmaf(__uint_as_float(v[j + 2]), s.z * w, sum[j + 2]);
+    sum[j + 3] = fmaf(__uint_as_float(v[j + 3]), s.w * w, sum[j + 3]);
+  }
+}
+
+//   warp 0      TMA producer          warp 1   MMA issuer, TMEM owner          warp 2   row ranges, scales          warp 3   nothing
+//   warps 4..7, 8..11   take every other tile: while one group stores, the other has the next tile's sums
+// ONE: they take every other block of the one tile. The groups' and the CTAs' sums meet in shared memory and are added in their order, row j by
+// rank j % split. What runs once has little code: unrolled over the rows, with divisions and every output type, it cost 3 us of instruction fetches.
+template <bool ONE>
 __global__ void __launch_bounds__(FEW_THREADS, 1)
 block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ BlockParams p,
                       int split) {
-  using S = FewRows;
+  using S = FewRows<ONE>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw), pad = (1024u - (raw_addr & 1023u)) & 1023u;
   const uint32_t smem_base = raw_addr + pad, part = smem_base + S::STAGES * S::STAGE_BYTES;
-  auto* ctrl = reinterpret_cast<S::Ctrl*>(smem_raw + pad + S::STAGES * S::STAGE_BYTES + S::PART);
+  auto* ctrl = reinterpret_cast<typename S::Ctrl*>(smem_raw + pad + S::STAGES * S::STAGE_BYTES + S::PART);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+  const int rank = ONE ? static_cast<int>(cluster_ctarank()) : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(smem_u32(&ctrl->full_bar[s]), 1);
       mbar_init(smem_u32(&ctrl->empty_bar[s]), 1);
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < 4; ++a) {
       mbar_init(smem_u32(&ctrl->acc_full_bar[a]), 1);
       mbar_init(smem_u32(&ctrl->acc_empty_bar[a]), 4);
+    }
+    for (int i = 0; i < S::SLOTS; ++i) {
+      mbar_init(smem_u32(&ctrl->scale_full_bar[i]), 32);
+      mbar_init(smem_u32(&ctrl->scale_empty_bar[i]), 4);
     }
     mbar_init(smem_u32(&ctrl->drain_bar), 1);
     ctrl->abort_flag = 0;
@@ -591,7 +634,7 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
   }
   if (warp == 2) fill_groups(ctrl->groups, p, S::ROWS, (p.N + A_ROWS - 1) / A_ROWS);
   if (warp == 1) {
-    tmem_alloc(smem_u32(&ctrl->tmem_base), 2 * S::ROWS);
+    tmem_alloc(smem_u32(&ctrl->tmem_base), 4 * S::ROWS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -601,13 +644,13 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
   const uint32_t tmem_base = ctrl->tmem_base;
   volatile int* abort_flag = &ctrl->abort_flag;
   bool issuer = false;
-  const int total = ctrl->groups.items[p.experts + 1];
+  const int total = ctrl->groups.items[p.experts + 1], scale_rows = (p.N + E4M3_BLOCK - 1) / E4M3_BLOCK;
   // a cluster has one tile: no second one to step to
-  BlockWalker walker(&ctrl->groups, p, S::ROWS, SPLIT ? blockIdx.x / split : blockIdx.x, SPLIT ? total : gridDim.x);
+  BlockWalker walker(&ctrl->groups, p, S::ROWS, ONE ? blockIdx.x / split : blockIdx.x, ONE ? total : gridDim.x);
   BlockTile t;
   // this CTA's blocks of a tile's contraction
-  auto from = [&] { return SPLIT ? t.k_blocks * rank / split : 0; };
-  auto to = [&] { return SPLIT ? t.k_blocks * (rank + 1) / split : t.k_blocks; };
+  auto from = [&] { return ONE ? t.k_blocks * rank / split : 0; };
+  auto to = [&] { return ONE ? t.k_blocks * (rank + 1) / split : t.k_blocks; };
 
   if (warp == 0) {
     if (elect_one()) {
@@ -615,14 +658,14 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
       uint32_t phase = 0;
       bool ok = true;
       while (ok && walker.next(t)) {
-        const int boxed = (t.rows + 15) & ~15;
+        const int boxed = (t.rows + p.box_rows - 1) / p.box_rows * p.box_rows;
         for (int kb = from(); kb < to(); ++kb) {
           ok = mbar_wait_bounded(smem_u32(&ctrl->empty_bar[stage]), phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_PRODUCER, p.wait_cycles);
           if (!ok) break;
           const uint32_t full = smem_u32(&ctrl->full_bar[stage]), w_dst = smem_base + stage * S::STAGE_BYTES;
           mbar_expect_tx(full, (A_ROWS + boxed) * 128);
           tma_load_3d(w_dst, &tm_w, full, kb * E4M3_BLOCK, t.across * A_ROWS, t.group);
-          for (int r = 0; r < boxed; r += 16) tma_load_2d(w_dst + (A_ROWS + r) * 128, &tm_x, full, kb * E4M3_BLOCK, t.row0 + r);
+          for (int r = 0; r < boxed; r += p.box_rows) tma_load_2d(w_dst + (A_ROWS + r) * 128, &tm_x, full, kb * E4M3_BLOCK, t.row0 + r);
           ++filled;
           if (++stage == S::STAGES) stage = 0, phase ^= 1u;
         }
@@ -632,13 +675,16 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
   } else if (warp == 1) {
     if (elect_one()) {
       issuer = true;
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      int stage = 0, group = 0;
+      uint32_t phase = 0, count[2] = {0, 0};  // accumulators that a group was given so far
       bool ok = true;
-      while (ok && walker.next(t)) {
+      for (; ok && walker.next(t); group ^= 1) {
         const uint32_t idesc = make_idesc_e4m3(A_ROWS, (t.rows + 15) & ~15);
         for (int kb = from(); kb < to(); ++kb) {
-          ok = mbar_wait_bounded(smem_u32(&ctrl->acc_empty_bar[acc]), acc_phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_MMA, p.wait_cycles) &&
+          if (ONE) group = (kb - from()) & 1;
+          const int acc = group * 2 + (count[group] & 1);
+          ok = mbar_wait_bounded(smem_u32(&ctrl->acc_empty_bar[acc]), ((count[group] >> 1) & 1) ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_MMA,
+                                 p.wait_cycles) &&
                mbar_wait_bounded(smem_u32(&ctrl->full_bar[stage]), phase, abort_flag, p.status, FFM_STATUS_WAIT_MMA, p.wait_cycles);
           if (!ok) break;
           tc_fence_after();
@@ -650,88 +696,120 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
           }
           umma_commit(smem_u32(&ctrl->empty_bar[stage]));
           umma_commit(smem_u32(&ctrl->acc_full_bar[acc]));
+          ++count[group];
           if (++stage == S::STAGES) stage = 0, phase ^= 1u;
-          if (++acc == 2) acc = 0, acc_phase ^= 1u;
         }
       }
     }
-  } else {
-    const int quarter = warp & 3;
-    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const int scale_rows = (p.N + E4M3_BLOCK - 1) / E4M3_BLOCK;
-    float(*scale)[S::ROWS] = ctrl->scale[quarter];
-    int acc = 0;
-    uint32_t acc_phase = 0;
+  } else if (warp == 2) {
+    // the scales of the tile's rows and features, block by block, ahead of the sums that they belong to
+    int slot = 0;
+    uint32_t phase = 0;
     bool ok = true;
     while (ok && walker.next(t)) {
       const float* ws = p.w_scale + (static_cast<long long>(t.group) * scale_rows + t.across) * p.k_blocks;
       const float* xs0 = p.x_scale + static_cast<long long>(t.row0 + min(lane, t.rows - 1)) * p.k_blocks;
       const float* xs1 = p.x_scale + static_cast<long long>(t.row0 + min(lane + 32, t.rows - 1)) * p.k_blocks;
+      for (int kb = from(); kb < to(); ++kb) {
+        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_empty_bar[slot]), phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_PRODUCER, p.wait_cycles);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t dst = smem_u32(ctrl->scale[slot]);
+        copy_async_4(dst + lane * 4, xs0 + kb);
+        if (t.rows > 32) copy_async_4(dst + (lane + 32) * 4, xs1 + kb);
+        if (lane == 0) copy_async_4(dst + S::ROWS * 4, ws + kb);
+        copy_async_arrive(smem_u32(&ctrl->scale_full_bar[slot]));
+        if (++slot == S::SLOTS) slot = 0, phase ^= 1u;
+      }
+    }
+    copy_async_wait<0>();
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + group * 2 * S::ROWS;
+    uint32_t count = 0, blocks = 0;  // accumulators that this group was given so far, and blocks of all tiles so far
+    bool ok = true;
+    for (int turn = 0; ok && walker.next(t); turn ^= 1) {
+      if (!ONE && turn != group) {
+        blocks += to() - from();
+        continue;
+      }
       float sum[S::ROWS];
 #pragma unroll
       for (int j = 0; j < S::ROWS; ++j) sum[j] = 0.0f;
-      const int last = to();
-      float a = 0.0f, b = 0.0f, w = 0.0f;
-      if (from() < last) a = __ldg(xs0 + from()), b = __ldg(xs1 + from()), w = __ldg(ws + from());
-      for (int kb = from(); kb < last; ++kb) {
-        // an accumulator's number serves for the scales' place too: the one before last has been read by all lanes
-        scale[acc][lane] = a * w;
-        scale[acc][lane + 32] = b * w;
-        if (kb + 1 < last) a = __ldg(xs0 + kb + 1), b = __ldg(xs1 + kb + 1), w = __ldg(ws + kb + 1);
-        __syncwarp();
-        ok = mbar_wait_bounded(smem_u32(&ctrl->acc_full_bar[acc]), acc_phase, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
+      for (int kb = from() + (ONE ? group : 0); kb < to(); kb += ONE ? 2 : 1, ++count, ++blocks) {
+        if (ONE) blocks = kb - from();
+        const uint32_t acc = count & 1, slot = blocks % S::SLOTS;
+        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_full_bar[slot]), (blocks / S::SLOTS) & 1, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE,
+                               p.wait_cycles) &&
+             mbar_wait_bounded(smem_u32(&ctrl->acc_full_bar[group * 2 + acc]), (count >> 1) & 1, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE,
+                               p.wait_cycles);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < S::ROWS / 16; ++c) {
-          if (c * 16 < t.rows) {
-            uint32_t v[16];
-            tmem_ld_32x16(taddr + acc * S::ROWS + c * 16, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 s = *reinterpret_cast<const float4*>(&scale[acc][c * 16 + j]);
-              sum[c * 16 + j] = fmaf(__uint_as_float(v[j]), s.x, sum[c * 16 + j]);
-              sum[c * 16 + j + 1] = fmaf(__uint_as_float(v[j + 1]), s.y, sum[c * 16 + j + 1]);
-              sum[c * 16 + j + 2] = fmaf(__uint_as_float(v[j + 2]), s.z, sum[c * 16 + j + 2]);
-              sum[c * 16 + j + 3] = fmaf(__uint_as_float(v[j + 3]), s.w, sum[c * 16 + j + 3]);
-            }
-          }
+        const float* scale = ctrl->scale[slot];
+        const float w = scale[S::ROWS];
+        if (t.rows <= 16) {
+          add_rows<16>(taddr + acc * S::ROWS, scale, w, sum);
+        } else if (t.rows <= 32) {
+          add_rows<32>(taddr + acc * S::ROWS, scale, w, sum);
+        } else {
+          add_rows<64>(taddr + acc * S::ROWS, scale, w, sum);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ctrl->acc_empty_bar[acc]));
-        if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&ctrl->acc_empty_bar[group * 2 + acc]));
+          mbar_arrive(smem_u32(&ctrl->scale_empty_bar[slot]));
+        }
       }
       if (!ok) break;
       const int feature = quarter * 32 + lane, n = t.across * A_ROWS + feature;
-      if constexpr (SPLIT) {
+      if constexpr (ONE) {
+        const uint32_t at = part + (group * S::ROWS * A_ROWS + feature) * 4;
 #pragma unroll
         for (int j = 0; j < S::ROWS; ++j) {
-          if (j < t.rows) asm volatile("st.shared.f32 [%0], %1;" ::"r"(part + (j * A_ROWS + feature) * 4), "f"(sum[j]) : "memory");
+          if (j < t.rows) asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + j * (A_ROWS * 4)), "f"(sum[j]) : "memory");
         }
-      } else {
+      } else if (n < p.N) {
         const long long out = static_cast<long long>(t.row0) * p.N + n;
-#pragma unroll
-        for (int j = 0; j < S::ROWS; ++j) {
-          if (j < t.rows && n < p.N) store1_as(p.out, p.out_type, out + static_cast<long long>(j) * p.N, sum[j]);
+        if (p.out_type == FFM_TYPE_BF16) {
+          store_rows(static_cast<bf16*>(p.out) + out, p.N, t.rows, sum);
+        } else if (p.out_type == FFM_TYPE_FP16) {
+          store_rows(static_cast<fp16*>(p.out) + out, p.N, t.rows, sum);
+        } else {
+          store_rows(static_cast<float*>(p.out) + out, p.N, t.rows, sum);
         }
       }
     }
   }
-
-  if constexpr (SPLIT) {
+  if constexpr (ONE) {
     __syncwarp();
     cluster_sync_all();
     BlockWalker again(&ctrl->groups, p, S::ROWS, blockIdx.x / split, total);
-    if (warp >= 2 && again.next(t)) {
-      // every rank adds up and stores every split-th row
-      const int feature = threadIdx.x - 64, n = t.across * A_ROWS + feature;
-      for (int j = rank; j < t.rows; j += split) {
-        float v = 0.0f;
-        for (int r = 0; r < split; ++r) v += ld_shared_cluster(map_to_cta(part + (j * A_ROWS + feature) * 4, r));
-        if (n < p.N) store1_as(p.out, p.out_type, static_cast<long long>(t.row0 + j) * p.N + n, v);
+    if (warp >= 4 && again.next(t)) {
+      // a warp has a row, a lane four features of it
+      const int n = t.across * A_ROWS + lane * 4;
+      for (int j = rank + (warp - 4) * split; j < t.rows; j += 8 * split) {
+        float4 v[2 * MAX_SPLIT];
+#pragma unroll
+        for (int r = 0; r < MAX_SPLIT; ++r) {
+          if (r < split) {
+            const uint32_t at = map_to_cta(part + (j * A_ROWS + lane * 4) * 4, r);
+            v[2 * r] = ld_shared_cluster(at);
+            v[2 * r + 1] = ld_shared_cluster(at + S::ROWS * A_ROWS * 4);
+          }
+        }
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int r = 0; r < 2 * MAX_SPLIT; ++r) {
+          if (r < 2 * split) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+        }
+        const long long out = static_cast<long long>(t.row0 + j) * p.N + n;
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          if (n + i < p.N) store1_as(p.out, p.out_type, out + i, i == 0 ? f[0] : i == 1 ? f[1] : i == 2 ? f[2] : f[3]);
+        }
       }
     }
     __syncwarp();
@@ -753,7 +831,7 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 2 * S::ROWS);
+    tmem_dealloc(tmem_base, 4 * S::ROWS);
   }
 }
 
@@ -795,23 +873,42 @@ int launch_many(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const CUtensor
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
 
-template <bool SPLIT>
-int launch_few(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const BlockParams& p, long long tiles, int split, cudaStream_t stream) {
+template <bool ONE>
+bool few_config(cudaLaunchConfig_t& config, cudaLaunchAttribute& attribute, int split) {
   static PerDevice room;
-  auto kernel = block_gemm_few_kernel<SPLIT>;
-  if (!allow_smem(kernel, FewRows::SMEM_BYTES, room)) return FFM_ERR_LAUNCH;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(SPLIT ? tiles * split : (tiles < num_sms() ? tiles : num_sms())));
+  if (!allow_smem(block_gemm_few_kernel<ONE>, FewRows<ONE>::SMEM_BYTES, room)) return false;
   config.blockDim = dim3(FEW_THREADS);
-  config.dynamicSmemBytes = FewRows::SMEM_BYTES;
-  config.stream = stream;
-  cudaLaunchAttribute attribute = {};
+  config.dynamicSmemBytes = FewRows<ONE>::SMEM_BYTES;
   attribute.id = cudaLaunchAttributeClusterDimension;
   attribute.val.clusterDim.x = static_cast<unsigned>(split);
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
-  config.numAttrs = SPLIT ? 1 : 0;
-  const cudaError_t rc = cudaLaunchKernelEx(&config, kernel, tm_x, tm_w, p, split);
+  config.numAttrs = ONE ? 1 : 0;
+  return true;
+}
+
+// Clusters of `split` CTAs that run at once: fewer than their SMs (148 give 74 of 2, 33 of 4, 22 of 6, 15 of 8).
+int clusters_at_once(int split) {
+  static PerDevice found[MAX_SPLIT + 1];
+  return found[split].get([&] {
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attribute = {};
+    int n = 0;
+    if (!few_config<true>(config, attribute, split)) return 0;
+    config.gridDim = dim3(split);
+    if (cudaOccupancyMaxActiveClusters(&n, block_gemm_few_kernel<true>, &config) != cudaSuccess) cudaGetLastError();
+    return n;
+  });
+}
+
+template <bool ONE>
+int launch_few(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const BlockParams& p, long long tiles, int split, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attribute = {};
+  if (!few_config<ONE>(config, attribute, split)) return FFM_ERR_LAUNCH;
+  config.gridDim = dim3(static_cast<unsigned>(ONE ? tiles * split : (tiles < num_sms() ? tiles : num_sms())));
+  config.stream = stream;
+  const cudaError_t rc = cudaLaunchKernelEx(&config, block_gemm_few_kernel<ONE>, tm_x, tm_w, p, split);
   if (rc != cudaSuccess) cudaGetLastError();
   return rc == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
@@ -874,16 +971,32 @@ extern "C" int ffm_linear_blocks_e4m3(const ffm_linear_blocks_args* args, ffm_st
   p.status = a.status;
   p.status_host = a.status_host;
   p.wait_cycles = gemm_wait_cycles();
+  const bool grouped = a.ends != nullptr;
   const int64_t average = a.rows / a.experts;
-  const bool few = average <= FewRows::ROWS;
-  // tiles at most: every expert may end inside of one, and so may the rows behind the last
+  // Tiles at most: every expert may end inside of one, and so may the rows behind the last. And about: half of the experts' ends cost one.
   auto tiles = [&](int64_t tile_rows, int64_t width) {
-    const int64_t parts = a.ends != nullptr ? (a.experts < a.rows ? a.experts : a.rows) + 1 : 0;
-    return (a.rows / tile_rows + (a.ends != nullptr ? parts : (a.rows % tile_rows != 0))) * ((a.N + width - 1) / width);
+    const int64_t ends = grouped ? (a.experts < a.rows ? a.experts : a.rows) + 1 : (a.rows % tile_rows != 0);
+    return (a.rows / tile_rows + ends) * ((a.N + width - 1) / width);
   };
-  const int64_t wide = tiles(A_ROWS, 256);
-  const int box_n = few ? A_ROWS : (wide >= 2 * num_sms() ? 256 : 128), box_m = few ? 16 : A_ROWS;
-  const int64_t most = tiles(few ? FewRows::ROWS : A_ROWS, box_n);
+  auto rounds = [&](int64_t width) {
+    const int64_t down = a.rows / A_ROWS + (grouped ? (a.experts + 1) / 2 : (a.rows % A_ROWS != 0));
+    return (down * ((a.N + width - 1) / width) + num_sms() - 1) / num_sms();
+  };
+  // One tile a cluster, where all fit at once: its contraction is split over as many CTAs as that leaves.
+  const int64_t few_tiles = tiles(FEW_ROWS, A_ROWS);
+  int split = 1;
+  for (int s = MAX_SPLIT; s > 1 && split == 1; --s) {
+    if (p.k_blocks >= 2 * s && few_tiles * s <= num_sms() && few_tiles <= clusters_at_once(s)) split = s;
+  }
+  // The weights' stream bounds few rows. us, few against many rows a tile: 64 experts of 2816 x 2048, rows each 4: 62 / 67, 16: 65 / 70, 32: 73 / 71, 64:
+  // 123 / 72; dense 4096 x 4096, 16 rows 8 / 13, 64 rows 10.5 / 13, 128 rows 17 / 13; where the contraction is not split, 32 x 14336 x 4096 18 / 14;
+  // 64 x 1024 x 1024 7.6 / 6.1.
+  const bool few = grouped ? average <= 24 : a.rows <= 16 || (a.rows <= FEW_ROWS && split > 1 && p.k_blocks >= 16);
+  // an expert's rows in one load of x for the most part
+  p.box_rows = average <= (grouped ? 8 : 16) ? 16 : (average <= (grouped ? 24 : 32) ? 32 : FEW_ROWS);
+  // A tile of 256 features takes 1.65 times as long as one of 128 (1024 x 4096 x 4096: one round of it 23 us, two of 128 27; 512 x 4096 x 4096: 21 and 15).
+  const int box_n = few || rounds(256) * 165 > rounds(128) * 100 ? A_ROWS : 256, box_m = few ? p.box_rows : A_ROWS;
+  const int64_t most = few ? few_tiles : tiles(A_ROWS, box_n);
   if (most > 0x3fffffff) return FFM_ERR_UNSUPPORTED;
   CUtensorMap tm_x, tm_w;
   int rc = make_byte_map(&tm_x, a.x, 0, a.rows, a.K, a.rows > 1 ? a.x_stride : a.K, box_m);
@@ -891,11 +1004,7 @@ extern "C" int ffm_linear_blocks_e4m3(const ffm_linear_blocks_args* args, ffm_st
   if (rc != FFM_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool four = p.out_type == FFM_TYPE_FP32;
-  if (few) {
-    int split = 1;
-    while (split < MAX_SPLIT && most * split * 2 <= num_sms() && p.k_blocks >= split * 4) split *= 2;
-    return split > 1 ? launch_few<true>(tm_x, tm_w, p, most, split, st) : launch_few<false>(tm_x, tm_w, p, most, 1, st);
-  }
+  if (few) return most <= num_sms() ? launch_few<true>(tm_x, tm_w, p, most, split, st) : launch_few<false>(tm_x, tm_w, p, most, 1, st);
   CUtensorMap tm_out = {};  // read only where rows lie on 16 bytes
   if (p.out_wide) {
     rc = make_box_map(&tm_out, a.out, 1, a.rows, a.N, a.N, type_bytes(p.out_type));
