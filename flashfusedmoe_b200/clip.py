@@ -19,12 +19,6 @@ def _arguments(max_norm, norm_type):
     return max_norm, _KINDS[norm_type]
 
 
-def _no_sparse(grads):
-    for g in grads:
-        if g.is_sparse:
-            raise RuntimeError("gradient clipping does not take sparse gradients")
-
-
 def _norm(grads, sharded, like, max_norm, largest, group):
     capturing = like.is_cuda and torch.cuda.is_current_stream_capturing()
     native, other = _lib.native(), None
@@ -49,14 +43,12 @@ def clip_coefficient(grads, max_norm, norm_type=2.0, *, sharded=(), group=None):
     captured."""
     grads, sharded = list(grads), list(sharded)
     max_norm, largest = _arguments(max_norm, norm_type)
-    _no_sparse(grads + sharded)
     if not grads and not sharded:
         raise ValueError("there are no gradients")
     return _norm(grads, sharded, (grads + sharded)[0], max_norm, largest, group)
 
 
 @torch.compiler.disable
-@torch.no_grad()
 def clip_grad_norm(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, *, sharded=(), group=None):
     """Scales the gradients of `parameters` (a tensor or an iterable of them) in place so that their norm together is at most `max_norm`,
     as torch.nn.utils.clip_grad_norm_ does, and returns the norm before (float32 on the device): every gradient is multiplied by the
@@ -67,19 +59,20 @@ def clip_grad_norm(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False
     gradient are passed over; without any gradient the norm is 0."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm, largest = _arguments(max_norm, norm_type)
+    if group is None and not error_if_nonfinite:
+        capturing = bool(parameters) and parameters[0].is_cuda and torch.cuda.is_current_stream_capturing()
+        norm = _lib.native().clip_grad_norm(parameters, max_norm, largest, capturing)
+        return torch.zeros((), device=parameters[0].device if parameters else None) if norm is None else norm
     apart = {id(p) for p in sharded}
+    if not apart <= {id(p) for p in parameters}:
+        raise ValueError("sharded must be some of the parameters")
     with_grad = [p for p in parameters if p.grad is not None]
     grads = [p.grad for p in with_grad if id(p) not in apart]
     local = [p.grad for p in with_grad if id(p) in apart]
-    if len(apart - {id(p) for p in parameters}) > 0:
-        raise ValueError("sharded must be some of the parameters")
-    if not grads and not local and (group is None or not parameters):
-        return torch.zeros((), device=parameters[0].device if parameters else None)
-    _no_sparse(grads + local)
     every = [*grads, *local]
-    like = (every or parameters)[0]
-    _lib.native().check_separate(every)
-    norm, coefficient = _norm(grads, local, like, max_norm, largest, group)
+    if not every and (group is None or not parameters):
+        return torch.zeros((), device=parameters[0].device if parameters else None)
+    norm, coefficient = _norm(grads, local, (every or parameters)[0], max_norm, largest, group)
     if error_if_nonfinite and not bool(torch.isfinite(norm)):
         raise RuntimeError("The norm of the gradients is not finite, so they cannot be clipped by it")
     _lib.native().scale_gradients(every, coefficient)

@@ -7,8 +7,7 @@
 // and the last block to come adds them in the order of the blocks.
 #include "ffm_device.h"
 #include "ffm_internal.h"
-#include "ffm_gemm_common.cuh"
-#include "ffm_types.cuh"
+#include "ffm_norm_common.cuh"
 
 namespace ffm {
 
@@ -34,7 +33,6 @@ struct ClipJob {
 };
 
 struct NormEnd {
-  int kind;
   int parts;     // of all launches
   int first;     // of this launch's
   int last;      // this is the last launch
@@ -46,16 +44,6 @@ struct NormEnd {
   float* coefficient;
   unsigned int* ticket;
 };
-
-// eight values of a tensor from element e on; zeros past its end
-__device__ __forceinline__ void read8(const ClipTensor& a, long long e, float (&v)[8]) {
-  if (a.wide && e + 8 <= a.n) {
-    load8_as(a.x, a.type, e, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = e + j < a.n ? load1_as(a.x, a.type, e + j) : 0.0f;
-  }
-}
 
 // magnitudes as bits compare as numbers do, and NaN is above all
 __device__ __forceinline__ unsigned int magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -93,7 +81,35 @@ __device__ __forceinline__ double join_block(int kind, double v, double* shared)
   return v;
 }
 
-template <int MAX>
+// What a thread's groups of eight add to the block's value
+template <int KIND>
+__device__ __forceinline__ void take(const float (&v)[8], double& sum, unsigned int& top) {
+  if (KIND == 0) {
+    sum += squares(v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, magnitude(v[j]));
+  }
+}
+
+// A whole chunk on 16 bytes: all loads before the first value is used (behind a switch over the types for every eight they followed one another:
+// 208 M bf16 values took 124 us, so 67)
+template <typename T, int KIND>
+__device__ __forceinline__ void take_chunk(const T* x, double& sum, unsigned int& top) {
+  constexpr int V = VALUES<T>, STEPS = CLIP_CHUNK / V / CLIP_THREADS;
+  uint4 raw[STEPS];
+#pragma unroll
+  for (int u = 0; u < STEPS; ++u) raw[u] = __ldcs(reinterpret_cast<const uint4*>(x) + u * CLIP_THREADS + threadIdx.x);
+#pragma unroll
+  for (int u = 0; u < STEPS; u += 8 / V) {
+    float v[8];
+    unpack<T>(raw[u], reinterpret_cast<float(&)[V]>(v));
+    if constexpr (V == 4) unpack<T>(raw[u + 1], reinterpret_cast<float(&)[V]>(v[4]));
+    take<KIND>(v, sum, top);
+  }
+}
+
+template <int MAX, int KIND>
 __global__ void __launch_bounds__(CLIP_THREADS)
 grad_norm_kernel(const __grid_constant__ ClipJob<MAX> job, const __grid_constant__ NormEnd end) {
   __shared__ double shared[CLIP_THREADS / 32];
@@ -105,22 +121,31 @@ grad_norm_kernel(const __grid_constant__ ClipJob<MAX> job, const __grid_constant
   for (long long chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     while (chunk >= job.tensor[i].chunks_end) ++i;  // the chunk's tensor, for the whole block alike
     const ClipTensor& a = job.tensor[i];
-    const long long c0 = (chunk - (i > 0 ? job.tensor[i - 1].chunks_end : 0)) * CLIP_CHUNK + threadIdx.x * 8;
-    float v[CLIP_UNROLL][8];
-#pragma unroll
-    for (int u = 0; u < CLIP_UNROLL; ++u) read8(a, c0 + u * CLIP_THREADS * 8, v[u]);
-#pragma unroll
-    for (int u = 0; u < CLIP_UNROLL; ++u) {
-      if (end.kind == 0) {
-        sum += squares(v[u]);
+    const long long c0 = (chunk - (i > 0 ? job.tensor[i - 1].chunks_end : 0)) * CLIP_CHUNK;
+    if (a.wide && c0 + CLIP_CHUNK <= a.n) {
+      if (a.type == FFM_TYPE_BF16) {
+        take_chunk<bf16, KIND>(static_cast<const bf16*>(a.x) + c0, sum, top);
+      } else if (a.type == FFM_TYPE_FP16) {
+        take_chunk<fp16, KIND>(static_cast<const fp16*>(a.x) + c0, sum, top);
       } else {
+        take_chunk<float, KIND>(static_cast<const float*>(a.x) + c0, sum, top);
+      }
+    } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude(v[u][j]));
+      for (int u = 0; u < CLIP_UNROLL; ++u) {
+        // neighbours in neighbouring threads; zeros past the tensor's end
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const long long e = c0 + (u * 8 + j) * CLIP_THREADS + threadIdx.x;
+          v[j] = e < a.n ? load1_as(a.x, a.type, e) : 0.0f;
+        }
+        take<KIND>(v, sum, top);
       }
     }
   }
-  if (end.kind != 0) sum = __uint_as_float(top);
-  sum = join_block(end.kind, sum, shared);
+  if (KIND != 0) sum = __uint_as_float(top);
+  sum = join_block(KIND, sum, shared);
   if (threadIdx.x == 0) {
     end.part[end.first + blockIdx.x] = sum;
     if (end.last) {
@@ -134,17 +159,34 @@ grad_norm_kernel(const __grid_constant__ ClipJob<MAX> job, const __grid_constant
   __syncthreads();
   if (!last) return;
   double v = 0.0;
-  for (int k = threadIdx.x; k < end.parts; k += CLIP_THREADS) v = join(end.kind, v, __ldcg(end.part + k));
-  v = join_block(end.kind, v, shared);
+  for (int k = threadIdx.x; k < end.parts; k += CLIP_THREADS) v = join(KIND, v, __ldcg(end.part + k));
+  v = join_block(KIND, v, shared);
   if (threadIdx.x == 0) {
-    if (end.other != nullptr) v = join(end.kind, v, *end.other);
+    if (end.other != nullptr) v = join(KIND, v, *end.other);
     if (end.total != nullptr) *end.total = v;
-    const double norm = end.kind == 0 ? sqrt(v) : v;
+    const double norm = KIND == 0 ? sqrt(v) : v;
     if (end.norm != nullptr) *end.norm = static_cast<float>(norm);
     if (end.coefficient != nullptr) {
       const double c = end.max_norm / (norm + 1e-6);
       *end.coefficient = c >= 1.0 ? 1.0f : static_cast<float>(c);
     }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(T* x, float f) {
+  constexpr int V = VALUES<T>, STEPS = CLIP_CHUNK / V / CLIP_THREADS;
+  uint4* at = reinterpret_cast<uint4*>(x) + threadIdx.x;
+  uint4 raw[STEPS];
+#pragma unroll
+  for (int u = 0; u < STEPS; ++u) raw[u] = at[u * CLIP_THREADS];
+#pragma unroll
+  for (int u = 0; u < STEPS; ++u) {
+    float2 v[V / 2];
+    unpack2<T>(raw[u], v);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) v[j] = mul2(v[j], both(f));
+    store2<T>(reinterpret_cast<T*>(at + u * CLIP_THREADS), v);
   }
 }
 
@@ -159,22 +201,19 @@ scale_tensors_kernel(const __grid_constant__ ClipJob<MAX> job, const float* __re
   for (long long chunk = chunks - 1 - blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
     while (i > 0 && chunk < job.tensor[i - 1].chunks_end) --i;
     const ClipTensor& a = job.tensor[i];
-    const long long c0 = (chunk - (i > 0 ? job.tensor[i - 1].chunks_end : 0)) * CLIP_CHUNK + threadIdx.x * 8;
-    float v[CLIP_UNROLL][8];
-#pragma unroll
-    for (int u = 0; u < CLIP_UNROLL; ++u) read8(a, c0 + u * CLIP_THREADS * 8, v[u]);
-#pragma unroll
-    for (int u = 0; u < CLIP_UNROLL; ++u) {
-      const long long e = c0 + u * CLIP_THREADS * 8;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[u][j] *= f;
-      if (a.wide && e + 8 <= a.n) {
-        store8_as(a.x, a.type, e, v[u]);
+    const long long c0 = (chunk - (i > 0 ? job.tensor[i - 1].chunks_end : 0)) * CLIP_CHUNK;
+    if (a.wide && c0 + CLIP_CHUNK <= a.n) {
+      if (a.type == FFM_TYPE_BF16) {
+        scale_chunk(static_cast<bf16*>(a.x) + c0, f);
+      } else if (a.type == FFM_TYPE_FP16) {
+        scale_chunk(static_cast<fp16*>(a.x) + c0, f);
       } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (e + j < a.n) store1_as(a.x, a.type, e + j, v[u][j]);
-        }
+        scale_chunk(static_cast<float*>(a.x) + c0, f);
+      }
+    } else {
+      // neighbours in neighbouring threads
+      for (long long e = c0 + threadIdx.x; e < a.n && e < c0 + CLIP_CHUNK; e += CLIP_THREADS) {
+        store1_as(a.x, a.type, e, load1_as(a.x, a.type, e) * f);
       }
     }
   }
@@ -201,12 +240,12 @@ int fill_job(ClipJob<MAX>& job, const ffm_clip_tensor* t, int count) {
   return static_cast<int>(chunks < clip_blocks() ? (chunks > 0 ? chunks : 1) : clip_blocks());
 }
 
-template <int MAX>
+template <int MAX, int KIND>
 int launch_norm(const ffm_clip_tensor* t, int count, NormEnd& end, cudaStream_t stream) {
   ClipJob<MAX> job;
   const int blocks = fill_job(job, t, count);
   end.parts = end.first + blocks;
-  grad_norm_kernel<MAX><<<blocks, CLIP_THREADS, 0, stream>>>(job, end);
+  grad_norm_kernel<MAX, KIND><<<blocks, CLIP_THREADS, 0, stream>>>(job, end);
   end.first += blocks;
   return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
 }
@@ -245,7 +284,6 @@ extern "C" int ffm_grad_norm(const ffm_clip_tensor* tensors, int count, const ff
   if (!(args->max_norm >= 0.0)) return FFM_ERR_BAD_ARG;
   if (!args->workspace || static_cast<size_t>(args->workspace_bytes) < ffm_grad_norm_workspace_bytes(count)) return FFM_ERR_WORKSPACE;
   NormEnd end = {};
-  end.kind = static_cast<int>(args->kind);
   end.max_norm = args->max_norm;
   end.other = args->other;
   end.part = static_cast<double*>(args->workspace);
@@ -256,8 +294,11 @@ extern "C" int ffm_grad_norm(const ffm_clip_tensor* tensors, int count, const ff
   for (int from = 0; from == 0 || from < count; from += FFM_CLIP_MAX) {
     const int n = count - from < FFM_CLIP_MAX ? count - from : FFM_CLIP_MAX;
     end.last = from + n == count;
-    const int rc = n <= CLIP_FEW ? launch_norm<CLIP_FEW>(tensors + from, n, end, static_cast<cudaStream_t>(stream))
-                                 : launch_norm<FFM_CLIP_MAX>(tensors + from, n, end, static_cast<cudaStream_t>(stream));
+    auto launch = [&](auto most) {
+      return args->kind == 0 ? launch_norm<decltype(most)::value, 0>(tensors + from, n, end, static_cast<cudaStream_t>(stream))
+                             : launch_norm<decltype(most)::value, 1>(tensors + from, n, end, static_cast<cudaStream_t>(stream));
+    };
+    const int rc = n <= CLIP_FEW ? launch(std::integral_constant<int, CLIP_FEW>{}) : launch(std::integral_constant<int, FFM_CLIP_MAX>{});
     if (rc != FFM_OK) return rc;
     if (args->launched != nullptr) ++*args->launched;
   }

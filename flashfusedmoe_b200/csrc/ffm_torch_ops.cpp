@@ -984,50 +984,61 @@ struct ClipTable {
   }
 };
 
-// The norm of `grads` and of what `other` (float64 [1], a sum of squares or a magnitude) stands for: (total float64 [1], norm, coefficient).
-py::tuple gradient_norm(const Tensors& grads, const Tensor& like, double max_norm, bool largest, const OptTensor& other, bool capturing) {
-  not_traced("the gradient norm");
-  on_gpu(like, "grad");
-  if (!(max_norm >= 0.0)) throw py::value_error("max_norm must not be negative, got " + std::to_string(max_norm));
-  for (const Tensor& t : grads) on_gpu(t, "grad");
-  const On device(like);
-  ClipTable table;
-  for (const Tensor& t : grads) table.add(t, like, "grad");
+struct ClipNorm {
+  Tensor norm, coefficient, workspace;  // the workspace begins with the sum of squares (the magnitude), float64
+};
+
+// The norm of `grads` and of what `other` (float64 [1], a sum of squares or a magnitude) stands for
+ClipNorm norm_of(const ClipTable& table, const Tensor& like, const On& device, double max_norm, bool largest, const Tensor& other, bool capturing) {
   ffm_grad_norm_args a = {};
   a.kind = largest ? 1 : 0;
   a.max_norm = max_norm;
-  Tensor more;
-  if (other.has_value()) {
-    same_device(*other, like, "other");
-    if (other->numel() != 1 || other->scalar_type() != at::kDouble) throw py::type_error("other must be one float64 value");
-    more = other->resolve_neg();
-    a.other = more.data_ptr<double>();
-  }
-  const auto options = like.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
-  const Tensor total = at::empty({1}, options.dtype(at::kDouble)), both = at::empty({2}, options.dtype(at::kFloat));
-  a.total = total.data_ptr<double>();
-  a.norm = both.data_ptr<float>();
-  a.coefficient = both.data_ptr<float>() + 1;
-  a.workspace_bytes = static_cast<int64_t>(grad_norm_workspace(table.count()));
-  const Tensor workspace = at::empty({a.workspace_bytes}, options.dtype(at::kByte));
-  a.workspace = workspace.data_ptr();
+  a.other = static_cast<const double*>(address(other));
+  const auto options = at::TensorOptions().device(like.device()).dtype(at::kFloat);
+  ClipNorm out;
+  out.norm = at::empty({}, options);
+  out.coefficient = at::empty({}, options);
+  const int64_t doubles = static_cast<int64_t>(grad_norm_workspace(table.count())) / 8;
+  out.workspace = at::empty({1 + doubles}, options.dtype(at::kDouble));
+  a.total = out.workspace.data_ptr<double>();
+  a.norm = out.norm.data_ptr<float>();
+  a.coefficient = out.coefficient.data_ptr<float>();
+  a.workspace = a.total + 1;
+  a.workspace_bytes = doubles * 8;
   const Tensor ticket = ticket_for(like, device.stream(), capturing);
   a.ticket = ticket.data_ptr();
   int64_t launched = 0;
   a.launched = &launched;
   check(grad_norm(table.entries.data(), table.count(), &a, device.stream()), "ffm_grad_norm");
   launches += launched;
-  return py::make_tuple(total, both.select(0, 0), both.select(0, 1));
+  return out;
+}
+
+void check_norm(const Tensors& grads, const Tensor& like, double max_norm) {
+  not_traced("gradient clipping");
+  on_gpu(like, "grad");
+  if (!(max_norm >= 0.0)) throw py::value_error("max_norm must not be negative, got " + std::to_string(max_norm));
+  for (const Tensor& t : grads) on_gpu(t, "grad");
+}
+
+// (total float64 [1], norm, coefficient)
+py::tuple gradient_norm(const Tensors& grads, const Tensor& like, double max_norm, bool largest, const OptTensor& other, bool capturing) {
+  check_norm(grads, like, max_norm);
+  const On device(like);
+  ClipTable table;
+  for (const Tensor& t : grads) table.add(t, like, "grad");
+  Tensor more;
+  if (other.has_value()) {
+    same_device(*other, like, "other");
+    if (other->numel() != 1 || other->scalar_type() != at::kDouble) throw py::type_error("other must be one float64 value");
+    more = other->resolve_neg();
+  }
+  const ClipNorm r = norm_of(table, like, device, max_norm, largest, more, capturing);
+  return py::make_tuple(r.workspace.narrow(0, 0, 1), r.norm, r.coefficient);
 }
 
 // grads *= factor (one float32 on the device), in place
-void scale_gradients_by(const Tensors& grads, const Tensor& factor) {
-  not_traced("clipping");
-  on_gpu(factor, "factor");
-  if (factor.numel() != 1 || factor.scalar_type() != at::kFloat) throw py::type_error("factor must be one float32 value");
-  const On device(factor);
-  ClipTable table;
-  for (const Tensor& t : grads) table.add(t, factor, "grad");
+void scale_by(const Tensors& grads, const ClipTable& table, const Tensor& factor, const On& device) {
   int64_t launched = 0;
   check(scale_tensors(table.entries.data(), table.count(), factor.data_ptr<float>(), &launched, device.stream()), "ffm_scale_tensors");
   launches += launched;
@@ -1063,6 +1074,35 @@ void check_separate(const Tensors& grads) {
   }
 }
 
+void scale_gradients_by(const Tensors& grads, const Tensor& factor) {
+  not_traced("gradient clipping");
+  on_gpu(factor, "factor");
+  if (factor.numel() != 1 || factor.scalar_type() != at::kFloat) throw py::type_error("factor must be one float32 value");
+  check_separate(grads);
+  const On device(factor);
+  ClipTable table;
+  for (const Tensor& t : grads) table.add(t, factor, "grad");
+  scale_by(grads, table, factor, device);
+}
+
+// The gradients of `parameters` scaled in place to a norm of max_norm at most: their norm, or nothing where there is no gradient
+OptTensor clip_grad_norm(const Tensors& parameters, double max_norm, bool largest, bool capturing) {
+  Tensors grads;
+  grads.reserve(parameters.size());
+  for (const Tensor& p : parameters) {
+    if (p.grad().defined()) grads.push_back(p.grad());
+  }
+  if (grads.empty()) return std::nullopt;
+  check_norm(grads, grads[0], max_norm);
+  check_separate(grads);
+  const On device(grads[0]);
+  ClipTable table;
+  for (const Tensor& t : grads) table.add(t, grads[0], "grad");
+  const ClipNorm r = norm_of(table, grads[0], device, max_norm, largest, Tensor(), capturing);
+  scale_by(grads, table, r.coefficient, device);
+  return r.norm;
+}
+
 }  // namespace
 
 void define_ops(py::module_& m) {
@@ -1078,6 +1118,6 @@ void define_ops(py::module_& m) {
     return linear_e4m3(x, x_scale, weight, weight_scale, ends, torch::python::detail::py_object_to_dtype(out_type), status, status_host);
   });
   m.def("gradient_norm", &gradient_norm);
-  m.def("check_separate", &check_separate);
+  m.def("clip_grad_norm", &clip_grad_norm);
   m.def("scale_gradients", &scale_gradients_by);
 }

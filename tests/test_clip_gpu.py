@@ -143,7 +143,7 @@ def test_refusals():
         clip_coefficient([g.double()], 1.0)
     with pytest.raises(RuntimeError, match="no CPU path"):
         clip_coefficient([g, g.cpu()], 1.0)
-    with pytest.raises(RuntimeError, match="sparse"):
+    with pytest.raises(ValueError, match="dense"):
         clip_coefficient([g.to_sparse()], 1.0)
 
 
