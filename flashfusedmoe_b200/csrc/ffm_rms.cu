@@ -52,6 +52,27 @@ __device__ __forceinline__ void store_packed(T* p, const Place<T, VEC>& at, int 
   }
 }
 
+// y of a chunk as e4m3, and the scale of the block of 128 columns that 16 (fp32: 32) neighbouring lanes hold; `has` is not the same for all of them
+// where the row ends inside
+template <typename T>
+__device__ __forceinline__ void store_e4m3(const float (&v)[VALUES<T>], bool has, int col, uint8_t* y, float* y_scale) {
+  constexpr int V = VALUES<T>;
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) top = fmaxf(top, has ? fabsf(v[j]) : 0.0f);
+#pragma unroll
+  for (int o = E4M3_BLOCK / V / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float scale = e4m3_scale(top), inverse = 1.0f / scale;
+  if (!has) return;
+  const uint32_t low = pack_e4m3x4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
+  if constexpr (V == 8) {
+    *reinterpret_cast<uint2*>(y + col) = make_uint2(low, pack_e4m3x4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
+  } else {
+    *reinterpret_cast<uint32_t*>(y + col) = low;
+  }
+  if (col % E4M3_BLOCK == 0) y_scale[col / E4M3_BLOCK] = scale;
+}
+
 // A team of threads for every row, each holding CH chunks of 16 bytes in registers. E4M3: y and y_scale [rows, ceil(D / 128)] instead of y in T;
 // the 16 (fp32: 32) neighbours that hold a block's columns meet in a butterfly.
 template <typename T, int CH, bool VEC, bool E4M3>
@@ -97,23 +118,8 @@ rms_norm_forward_kernel(const T* __restrict__ x, long long x_stride, const T* __
     if constexpr (!E4M3) {
       store_chunk(static_cast<T*>(y) + row * D, at, c, v);
     } else {
-      float top = 0.0f;
-#pragma unroll
-      for (int j = 0; j < V; ++j) top = fmaxf(top, at.has(c, 0) ? fabsf(v[j]) : 0.0f);
-#pragma unroll
-      for (int o = E4M3_BLOCK / V / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float scale = e4m3_scale(top), inverse = 1.0f / scale;
-      if (at.has(c, 0)) {
-        const int col = at.column(c, 0);
-        uint8_t* to = static_cast<uint8_t*>(y) + row * D + col;
-        const uint32_t low = pack_e4m3x4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
-        if constexpr (V == 8) {
-          *reinterpret_cast<uint2*>(to) = make_uint2(low, pack_e4m3x4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
-        } else {
-          *reinterpret_cast<uint32_t*>(to) = low;
-        }
-        if (col % E4M3_BLOCK == 0) y_scale[row * ((D + E4M3_BLOCK - 1) / E4M3_BLOCK) + col / E4M3_BLOCK] = scale;
-      }
+      const int across = (D + E4M3_BLOCK - 1) / E4M3_BLOCK;
+      store_e4m3<T>(v, at.has(c, 0), at.column(c, 0), static_cast<uint8_t*>(y) + row * D, y_scale + row * across);
     }
   }
 }
@@ -202,8 +208,123 @@ rms_norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ dh, con
   }
 }
 
+// The weight (and offset) in shared memory in fp32, four neighbours of every thread side by side: threads read 16 bytes each without a bank in
+// common. Filled by the whole block.
+template <typename T>
+__device__ __forceinline__ void fill_weight(float* to, const void* weight, int type, float offset, int D, int team) {
+  constexpr int V = VALUES<T>, PARTS = V / 4;
+  for (int i = threadIdx.x; i < team * RMS_CHUNKS_MAX * V; i += blockDim.x) {
+    const int j = i & 3, quad = i >> 2, t = quad % team, p = quad / team;
+    const int col = (p / PARTS * team + t) * V + p % PARTS * 4 + j;
+    to[i] = offset + (weight != nullptr && col < D ? load1_as(weight, type, col) : 1.0f);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void read_weight(uint32_t thread_base, int c, int team, float2 (&w)[VALUES<T> / 2]) {
+  constexpr int PARTS = VALUES<T> / 4;
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    const uint4 u = read_shared_16(thread_base + (c * PARTS + p) * team * 16);
+    w[2 * p] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    w[2 * p + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+}
+
+// Rows of a team: its own, and how often its loop runs (teams of less than a warp go in step with their warp's first).
+struct RmsTrips {
+  long long first, step;
+  int mine, all;
+  __device__ __forceinline__ RmsTrips(long long rows, int team) {
+    const int teams = blockDim.x / team;
+    first = static_cast<long long>(blockIdx.x) * teams + threadIdx.x / team;
+    step = static_cast<long long>(gridDim.x) * teams;
+    auto count = [&](long long from) { return from < rows ? static_cast<int>((rows - from + step - 1) / step) : 0; };
+    mine = count(first);
+    all = team < 32 ? count(first - (threadIdx.x & 31) / team) : mine;
+  }
+};
+
 // Many rows of 16-byte boundaries: every thread copies its chunks of the next rows to shared memory (S rows ahead; it reads back what it copied
-// itself), the weight lies there in fp32, and teams of one block go their own way. A block leaves one row of partial sums of dw.
+// itself), the weight lies there in fp32, and teams of one block go their own way. A row waits for the next ones' copies to be on their way, not
+// for its own sum (8192 x 7168 bf16 in 8 bits with a team a row and nothing ahead: 98 us).
+template <typename T, int S, bool RESIDUAL, bool E4M3>
+__global__ void __launch_bounds__(RMS_STREAM_THREADS, 1)
+rms_norm_forward_stream_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ residual, long long residual_stride,
+                               const void* __restrict__ weight, int w_type, float offset, long long rows, int D, float eps, int team,
+                               T* __restrict__ h, void* __restrict__ y, float* __restrict__ y_scale, float* __restrict__ rstd) {
+  extern __shared__ __align__(16) float scale[];  // weight, ring
+  __shared__ float part[2][1][32];
+  constexpr int V = VALUES<T>, CH = RMS_CHUNKS_MAX, IN = RESIDUAL ? 2 : 1;
+  const Place<T, true> at(team, D);
+  const uint32_t my_scale = smem_u32(scale) + at.t * 16;
+  const uint32_t ring = smem_u32(scale + team * CH * V) + threadIdx.x * 16, slot = blockDim.x * 16, row_bytes = IN * CH * slot;
+  const float inv = 1.0f / static_cast<float>(D);
+  const int across = (D + E4M3_BLOCK - 1) / E4M3_BLOCK;
+  const RmsTrips trips(rows, team);
+  const T *source = x + trips.first * x_stride + at.t * V, *source_r = RESIDUAL ? residual + trips.first * residual_stride + at.t * V : nullptr;
+  auto fetch = [&](int k, uint32_t to) {
+    const int chunks = k < trips.mine ? at.count : 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      copy_async_16(to + c * slot, source + c * team * V, c < chunks, x);
+      if (RESIDUAL) copy_async_16(to + (CH + c) * slot, source_r + c * team * V, c < chunks, x);
+    }
+    copy_async_commit();
+    source += trips.step * x_stride;
+    if (RESIDUAL) source_r += trips.step * residual_stride;
+  };
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(s, ring + s * row_bytes);
+  fill_weight<T>(scale, weight, w_type, offset, D, team);
+  __syncthreads();
+  int parity = 0;
+  uint32_t here = ring;  // the row's stage
+  for (int k = 0; k < trips.all; ++k, parity ^= 1) {
+    const long long row = trips.first + k * trips.step;
+    const int chunks = k < trips.mine ? at.count : 0;  // to write
+    copy_async_wait<S - 1>();
+    uint4 raw[CH];
+    float2 s2 = both(0.0f);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      raw[c] = read_shared_16(here + c * slot);
+      if (RESIDUAL) {
+        raw[c] = add_packed<T>(raw[c], read_shared_16(here + (CH + c) * slot));
+        if (c < chunks) *reinterpret_cast<uint4*>(h + row * D + at.column(c, 0)) = raw[c];
+      }
+      float2 v[V / 2];
+      unpack2<T>(raw[c], v);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) s2 = fma2(v[j], v[j], s2);
+    }
+    fetch(k + S, here);  // this thread's chunks have been read
+    here = here == ring + (S - 1) * row_bytes ? ring : here + row_bytes;
+    float s[1] = {s2.x + s2.y};
+    own_team_sum<1>(s, team, part[parity]);
+    const float r = rsqrtf(fmaf(s[0], inv, eps));
+    if (rstd != nullptr && at.t == 0 && chunks > 0) rstd[row] = r;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float2 v[V / 2], w[V / 2];
+      unpack2<T>(raw[c], v);
+      read_weight<T>(my_scale, c, team, w);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) v[j] = mul2(mul2(v[j], both(r)), w[j]);
+      if constexpr (E4M3) {
+        float f[V];
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) f[2 * j] = v[j].x, f[2 * j + 1] = v[j].y;
+        store_e4m3<T>(f, c < chunks, at.column(c, 0), static_cast<uint8_t*>(y) + row * D, y_scale + row * across);
+      } else {
+        if (c < chunks) store2<T>(static_cast<T*>(y) + row * D + at.column(c, 0), v);
+      }
+    }
+  }
+  copy_async_wait<0>();
+}
+
+// The backward pass in the same way. A block leaves one row of partial sums of dw.
 template <typename T, int S, bool DH>
 __global__ void __launch_bounds__(RMS_STREAM_THREADS, 1)
 rms_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict__ dh, const T* __restrict__ h, long long h_stride,
@@ -217,10 +338,9 @@ rms_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict__ 
   const uint32_t ring = smem_u32(scale + team * CH * V) + threadIdx.x * 16, slot = blockDim.x * 16;
   const int teams = blockDim.x / team;
   const float inv = 1.0f / static_cast<float>(D);
-  const long long first = static_cast<long long>(blockIdx.x) * teams + threadIdx.x / team, step = static_cast<long long>(gridDim.x) * teams;
-  // rows of this team; those of a warp or less go in step with their warp's first
-  auto count = [&](long long from) { return from < rows ? static_cast<int>((rows - from + step - 1) / step) : 0; };
-  const int mine = count(first), all = team < 32 ? count(first - (threadIdx.x & 31) / team) : mine;
+  const RmsTrips trips(rows, team);
+  const long long first = trips.first, step = trips.step;
+  const int mine = trips.mine, all = trips.all;
   const T *source = h + first * h_stride + at.t * V, *source_dy = dy + first * D + at.t * V, *source_dh = DH ? dh + first * D + at.t * V : nullptr;
   auto fetch = [&](int k, uint32_t to) {
     const int chunks = k < mine ? at.count : 0;
@@ -238,21 +358,8 @@ rms_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict__ 
   const uint32_t row_bytes = IN * CH * slot;
 #pragma unroll
   for (int s = 0; s < S; ++s) fetch(s, ring + s * row_bytes);
-  // the weight, four neighbours of every thread side by side: threads read 16 bytes each without a bank in common
-  for (int i = threadIdx.x; i < team * CH * V; i += blockDim.x) {
-    const int j = i & 3, quad = i >> 2, t = quad % team, p = quad / team;
-    const int col = (p / PARTS * team + t) * V + p % PARTS * 4 + j;
-    scale[i] = offset + (weight != nullptr && col < D ? load1_as(weight, w_type, col) : 1.0f);
-  }
+  fill_weight<T>(scale, weight, w_type, offset, D, team);
   __syncthreads();
-  auto read_weight = [&](int c, float2(&w)[V / 2]) {
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-      const uint4 u = read_shared_16(my_scale + (c * PARTS + p) * team * 16);
-      w[2 * p] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
-      w[2 * p + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
-    }
-  };
   float2 aw[CH][V / 2];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -276,7 +383,7 @@ rms_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict__ 
       float2 v[V / 2], g[V / 2], w[V / 2];
       unpack2<T>(read_shared_16(here + c * slot), v);
       unpack2<T>(read_shared_16(here + (CH + c) * slot), g);
-      read_weight(c, w);
+      read_weight<T>(my_scale, c, team, w);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) {
         const float2 xh = mul2(v[j], both(r));
@@ -293,7 +400,7 @@ rms_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict__ 
       float2 v[V / 2], g[V / 2], w[V / 2];
       unpack2<T>(read_shared_16(here + c * slot), v);
       unpack2<T>(read_shared_16(here + (CH + c) * slot), g);
-      read_weight(c, w);
+      read_weight<T>(my_scale, c, team, w);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) v[j] = fma2(v[j], c2, mul2(mul2(g[j], w[j]), both(r)));
       if (DH) {
@@ -400,15 +507,15 @@ struct RmsStream {
   int stages, smem;
 };
 
-// The ring as deep as shared memory allows, over as many teams as go into a block; shape.teams == 0: it does not fit.
-RmsStream rms_stream(int D, int type, bool dh) {
+// The ring of so many inputs as deep as shared memory allows, over as many teams as go into a block; shape.teams == 0: it does not fit.
+RmsStream rms_stream(int D, int type, int inputs, int least) {
   const int row_values = 16 / type_bytes(type);
   RmsStream r;
   for (int threads = RMS_STREAM_THREADS; threads >= 128; threads /= 2) {
-    RmsShape s = rms_shape(D, type, RMS_CHUNKS_MAX, 1, threads);
+    RmsShape s = rms_shape(D, type, RMS_CHUNKS_MAX, least, threads);
     if (s.threads > threads) break;
     for (r.stages = 3; r.stages >= 2; --r.stages) {
-      const int ring = r.stages * (dh ? 3 : 2) * RMS_CHUNKS_MAX * s.threads * 16, sums = s.threads * RMS_CHUNKS_MAX * row_values * 4;
+      const int ring = r.stages * inputs * RMS_CHUNKS_MAX * s.threads * 16, sums = s.threads * RMS_CHUNKS_MAX * row_values * 4;
       r.smem = s.team * RMS_CHUNKS_MAX * row_values * 4 + (ring > sums ? ring : sums);
       r.shape = s;
       if (r.smem <= RMS_STREAM_SMEM) return r;
@@ -429,19 +536,37 @@ bool rms_vectors(int type, int D, int64_t stride_a, int64_t stride_b) {
   return static_cast<int64_t>(D) * type_bytes(type) % 16 == 0 && (stride_a * type_bytes(type)) % 16 == 0 && (stride_b * type_bytes(type)) % 16 == 0;
 }
 
+// A ring pays where a team has several rows to go through.
+bool rms_streams(int64_t rows, const RmsStream& r) { return r.shape.teams > 0 && rows > 2ll * num_sms() * r.shape.teams && rows < 1ll << 31; }
+
+template <typename K>
+bool rms_room(K kernel, PerDevice& room) {
+  return room.get([&] {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RMS_STREAM_SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    return 1;
+  }) > 0;
+}
+
+template <typename T, int S, bool RESIDUAL, bool E4M3>
+int launch_rms_forward_stream(const ffm_rms_norm_args& a, const RmsStream& r, cudaStream_t stream) {
+  auto kernel = rms_norm_forward_stream_kernel<T, S, RESIDUAL, E4M3>;
+  static PerDevice room;
+  if (!rms_room(kernel, room)) return FFM_ERR_LAUNCH;
+  kernel<<<num_sms(), r.shape.threads, r.smem, stream>>>(static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.residual), a.residual_stride,
+                                                        a.weight, static_cast<int>(a.w_type), static_cast<float>(a.offset), a.rows,
+                                                        static_cast<int>(a.D), static_cast<float>(a.eps), r.shape.team, static_cast<T*>(a.h), a.y,
+                                                        a.y_scale, a.rstd);
+  return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
+}
+
 template <typename T, int S, bool DH>
 int launch_rms_stream(const ffm_rms_norm_args& a, const RmsStream& r, float* parts, cudaStream_t stream) {
   auto kernel = rms_norm_backward_stream_kernel<T, S, DH>;
   static PerDevice room;
-  if (room.get([&] {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RMS_STREAM_SMEM) != cudaSuccess) {
-          cudaGetLastError();
-          return 0;
-        }
-        return 1;
-      }) <= 0) {
-    return FFM_ERR_LAUNCH;
-  }
+  if (!rms_room(kernel, room)) return FFM_ERR_LAUNCH;
   kernel<<<num_sms(), r.shape.threads, r.smem, stream>>>(static_cast<const T*>(a.dy), static_cast<const T*>(a.dh), static_cast<const T*>(a.x), a.x_stride,
                                                         a.weight, static_cast<int>(a.w_type), static_cast<float>(a.offset), a.rstd, a.rows,
                                                         static_cast<int>(a.D), r.shape.team, static_cast<T*>(a.dx), parts);
@@ -472,6 +597,20 @@ extern "C" int ffm_rms_norm_forward(const ffm_rms_norm_args* args, ffm_stream_t 
   const bool vec = rms_vectors(type, D, a.x_stride, a.residual != nullptr ? a.residual_stride : 0) && !off_16_bytes(a.x, a.residual, a.h, a.weight) &&
                    (e4m3 || !off_16_bytes(a.y));
   if (e4m3 && (!vec || (reinterpret_cast<uintptr_t>(a.y) & 7u) != 0)) return FFM_ERR_UNSUPPORTED;
+  const RmsStream ring = rms_stream(D, type, a.residual != nullptr ? 2 : 1, e4m3 ? 32 : 1);
+  if (vec && rms_streams(a.rows, ring)) {
+    return rms_with_type(type, [&](auto tag) {
+      using T = decltype(tag);
+      cudaStream_t st = static_cast<cudaStream_t>(stream);
+      auto launch = [&](auto stages, auto residual) {
+        constexpr int S = decltype(stages)::value;
+        constexpr bool R = decltype(residual)::value;
+        return e4m3 ? launch_rms_forward_stream<T, S, R, true>(a, ring, st) : launch_rms_forward_stream<T, S, R, false>(a, ring, st);
+      };
+      auto with = [&](auto stages) { return a.residual != nullptr ? launch(stages, std::true_type{}) : launch(stages, std::false_type{}); };
+      return ring.stages == 3 ? with(std::integral_constant<int, 3>{}) : with(std::integral_constant<int, 2>{});
+    });
+  }
   const RmsShape s = rms_forward_shape(a.rows, D, type, e4m3);
   const int64_t blocks = (a.rows + s.teams - 1) / s.teams;
   if (blocks > 0x7fffffffll) return FFM_ERR_UNSUPPORTED;
@@ -508,10 +647,9 @@ extern "C" int ffm_rms_norm_backward(const ffm_rms_norm_args* args, ffm_stream_t
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* parts = a.dweight != nullptr ? static_cast<float*>(a.workspace) : nullptr;
   const bool vec = rms_vectors(type, D, a.x_stride, 0) && !off_16_bytes(a.x, a.dy, a.dh, a.dx);
-  const RmsStream r = rms_stream(D, type, a.dh != nullptr);
+  const RmsStream r = rms_stream(D, type, a.dh != nullptr ? 3 : 2, 1);
   int count, rc;
-  // a ring pays where a team has several rows to go through
-  if (vec && r.shape.teams > 0 && a.rows > 2ll * num_sms() * r.shape.teams && a.rows < 1ll << 31) {
+  if (vec && rms_streams(a.rows, r)) {
     count = num_sms();
     rc = rms_with_type(type, [&](auto tag) {
       using T = decltype(tag);
