@@ -69,7 +69,7 @@ quantize_row_blocks_kernel(const T* __restrict__ x, long long stride, long long 
     const float s = e4m3_scale(top);
     const long long b = first + i * TEAMS;
     if (b < blocks && col[i] < K) {
-      store_e4m3<T>(q + row[i] * K + col[i], raw[i], 1.0f / s);
+      store_e4m3<T>(q + row[i] * K + col[i], raw[i], reciprocal(s));
       if (t == 0) scale[b] = s;
     }
   }
@@ -77,7 +77,7 @@ quantize_row_blocks_kernel(const T* __restrict__ x, long long stride, long long 
 
 // A scale for 128 x 128 values of a matrix: one thread block for each, its values in registers in between. blockIdx.y: the matrix.
 template <typename T>
-__global__ void __launch_bounds__(QB_THREADS)
+__global__ void __launch_bounds__(QB_THREADS, sizeof(T) == 2 ? 4 : 2)
 quantize_tiles_kernel(const T* __restrict__ x, int N, int K, int down, int across, uint8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int V = VALUES<T>, LANES = E4M3_BLOCK / V, TEAMS = QB_THREADS / LANES, STEPS = E4M3_BLOCK / TEAMS;
   __shared__ float part[QB_THREADS / 32];
@@ -100,7 +100,7 @@ quantize_tiles_kernel(const T* __restrict__ x, int N, int K, int down, int acros
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < QB_THREADS / 32; ++w) top = fmaxf(top, part[w]);
-  const float s = e4m3_scale(top), inverse = 1.0f / s;
+  const float s = e4m3_scale(top), inverse = reciprocal(s);
   if (threadIdx.x == 0) scale[tile] = s;
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {

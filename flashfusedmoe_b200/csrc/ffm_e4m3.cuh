@@ -20,4 +20,14 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
 // for a block of zeros. An infinity makes the scale infinite, and the block's numbers 0 and NaN.
 __device__ __forceinline__ float e4m3_scale(float amax) { return amax > 0.0f ? fmaxf(amax / 448.0f, 1.17549435e-38f) : 1.0f; }
 
+// The same within two roundings, without a division
+__device__ __forceinline__ float e4m3_scale_near(float amax) { return amax > 0.0f ? fmaxf(amax * (1.0f / 448.0f), 1.17549435e-38f) : 1.0f; }
+
+// 1 / x within a rounding or so, for what is then rounded to 8 bits; x is 2^-126 at least
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 }  // namespace ffm

@@ -24,20 +24,19 @@ constexpr int RMS_CHUNKS_MAX = 4;   // chunks of 16 bytes of a row that a thread
 constexpr int RMS_BACK_TEAM = 512, RMS_BACK_SM_THREADS = 768, RMS_STREAM_THREADS = 512;
 constexpr int RMS_STREAM_SMEM = 226 << 10;
 
-// h, packed as the row lies in memory
+// h, packed as the row lies in memory. Two 16-bit values at a time: the sum in fp32 rounded to 16 bits is the sum rounded once (24 bits hold twice 11 and 2).
 template <typename T>
 __device__ __forceinline__ uint4 add_packed(const uint4& a, const uint4& b) {
-  float u[VALUES<T>], v[VALUES<T>];
-  unpack<T>(a, u);
-  unpack<T>(b, v);
-#pragma unroll
-  for (int j = 0; j < VALUES<T>; ++j) u[j] += v[j];
   if constexpr (sizeof(T) == 4) {
-    return make_uint4(__float_as_uint(u[0]), __float_as_uint(u[1]), __float_as_uint(u[2]), __float_as_uint(u[3]));
+    return make_uint4(__float_as_uint(__uint_as_float(a.x) + __uint_as_float(b.x)), __float_as_uint(__uint_as_float(a.y) + __uint_as_float(b.y)),
+                      __float_as_uint(__uint_as_float(a.z) + __uint_as_float(b.z)), __float_as_uint(__uint_as_float(a.w) + __uint_as_float(b.w)));
   } else {
-    uint4 out;
-    store8(reinterpret_cast<T*>(&out), u);
-    return out;
+    using T2 = std::conditional_t<std::is_same<T, bf16>::value, __nv_bfloat162, __half2>;
+    auto add = [](uint32_t u, uint32_t v) {
+      const T2 sum = __hadd2(*reinterpret_cast<const T2*>(&u), *reinterpret_cast<const T2*>(&v));
+      return *reinterpret_cast<const uint32_t*>(&sum);
+    };
+    return make_uint4(add(a.x, b.x), add(a.y, b.y), add(a.z, b.z), add(a.w, b.w));
   }
 }
 
@@ -62,7 +61,7 @@ __device__ __forceinline__ void store_e4m3(const float (&v)[VALUES<T>], bool has
   for (int j = 0; j < V; ++j) top = fmaxf(top, has ? fabsf(v[j]) : 0.0f);
 #pragma unroll
   for (int o = E4M3_BLOCK / V / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float scale = e4m3_scale(top), inverse = 1.0f / scale;
+  const float scale = e4m3_scale_near(top), inverse = reciprocal(scale);
   if (!has) return;
   const uint32_t low = pack_e4m3x4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
   if constexpr (V == 8) {
@@ -483,21 +482,25 @@ RmsShape rms_shape(int D, int type, int chunks, int least, int threads) {
 
 // Few rows leave SMs idle, and a row then takes as many threads as it has chunks; many rows take few threads each, up to a warp, which
 // needs no barrier.
-RmsShape rms_forward_shape(int64_t rows, int D, int type, bool e4m3) {
+RmsShape rms_forward_shape(int64_t rows, int D, int type, bool e4m3, bool vec) {
   const int pieces = (D + 16 / type_bytes(type) - 1) / (16 / type_bytes(type));
   const int least = e4m3 ? 32 : 1;
   if (rows <= num_sms() && pieces <= RMS_TEAM) return rms_shape(D, type, 1, least, RMS_THREADS);
+  // single values: with four chunks (32 loads) a thread's registers spill
+  if (!vec && pieces <= 2 * RMS_TEAM) return rms_shape(D, type, 2, least, RMS_THREADS);
   return rms_shape(D, type, RMS_CHUNKS_MAX, least, RMS_THREADS);
 }
 
-RmsShape rms_backward_shape(int D, int type) {
-  const RmsShape s = rms_shape(D, type, 2, 1, RMS_THREADS);
-  return s.team <= RMS_BACK_TEAM ? s : rms_shape(D, type, RMS_CHUNKS_MAX, 1, RMS_THREADS);
+// Single values: one chunk (two of 16 bits spilled, 4093 x 2051 fp16 took 64 us)
+RmsShape rms_backward_shape(int D, int type, bool vec) {
+  const RmsShape s = rms_shape(D, type, vec ? 2 : 1, 1, RMS_THREADS);
+  return s.team <= (vec ? RMS_BACK_TEAM : RMS_TEAM) ? s : rms_shape(D, type, RMS_CHUNKS_MAX, 1, RMS_THREADS);
 }
 
 // Blocks of the backward kernel for any rows, and its rows of partial sums
 int rms_backward_blocks(int64_t rows, const RmsShape& s) {
-  const int64_t want = (rows + s.teams - 1) / s.teams, most = static_cast<int64_t>(num_sms()) * (s.chunks == 2 ? RMS_BACK_SM_THREADS / s.threads : 1);
+  const int on_sm = s.chunks == 1 ? RMS_TEAM / s.threads : (s.chunks == 2 ? RMS_BACK_SM_THREADS / s.threads : 1);
+  const int64_t want = (rows + s.teams - 1) / s.teams, most = static_cast<int64_t>(num_sms()) * on_sm;
   return static_cast<int>(want < most ? (want > 0 ? want : 1) : most);
 }
 int rms_backward_parts(int blocks, const RmsShape& s) { return blocks * (s.threads / (s.team < 32 ? 32 : s.team)); }
@@ -611,7 +614,7 @@ extern "C" int ffm_rms_norm_forward(const ffm_rms_norm_args* args, ffm_stream_t 
       return ring.stages == 3 ? with(std::integral_constant<int, 3>{}) : with(std::integral_constant<int, 2>{});
     });
   }
-  const RmsShape s = rms_forward_shape(a.rows, D, type, e4m3);
+  const RmsShape s = rms_forward_shape(a.rows, D, type, e4m3, vec);
   const int64_t blocks = (a.rows + s.teams - 1) / s.teams;
   if (blocks > 0x7fffffffll) return FFM_ERR_UNSUPPORTED;
   return rms_with_type(type, [&](auto tag) {
@@ -624,15 +627,21 @@ extern "C" int ffm_rms_norm_forward(const ffm_rms_norm_args* args, ffm_stream_t 
     };
     if (e4m3) return s.chunks == 1 ? launch(rms_norm_forward_kernel<T, 1, true, true>) : launch(rms_norm_forward_kernel<T, RMS_CHUNKS_MAX, true, true>);
     if (vec) return s.chunks == 1 ? launch(rms_norm_forward_kernel<T, 1, true, false>) : launch(rms_norm_forward_kernel<T, RMS_CHUNKS_MAX, true, false>);
-    return s.chunks == 1 ? launch(rms_norm_forward_kernel<T, 1, false, false>) : launch(rms_norm_forward_kernel<T, RMS_CHUNKS_MAX, false, false>);
+    return s.chunks == 1   ? launch(rms_norm_forward_kernel<T, 1, false, false>)
+           : s.chunks == 2 ? launch(rms_norm_forward_kernel<T, 2, false, false>)
+                           : launch(rms_norm_forward_kernel<T, RMS_CHUNKS_MAX, false, false>);
   });
 }
 
 extern "C" size_t ffm_rms_norm_workspace_bytes(int64_t rows, int D, int x_type) {
   if (rows < 0 || !is_type(x_type) || D <= 0 || D > rms_columns(x_type)) return 0;
-  const RmsShape s = rms_backward_shape(D, x_type);
-  const int parts = rms_backward_parts(rms_backward_blocks(rows, s), s);
-  return sizeof(float) * static_cast<size_t>(D) * (parts > num_sms() ? parts : num_sms());
+  int most = num_sms();  // a streaming kernel's
+  for (const bool vec : {false, true}) {
+    const RmsShape s = rms_backward_shape(D, x_type, vec);
+    const int parts = rms_backward_parts(rms_backward_blocks(rows, s), s);
+    most = parts > most ? parts : most;
+  }
+  return sizeof(float) * static_cast<size_t>(D) * most;
 }
 
 extern "C" int ffm_rms_norm_backward(const ffm_rms_norm_args* args, ffm_stream_t stream) {
@@ -657,10 +666,10 @@ extern "C" int ffm_rms_norm_backward(const ffm_rms_norm_args* args, ffm_stream_t
       return r.stages == 3 ? launch_rms_stream<T, 3, false>(a, r, parts, st) : launch_rms_stream<T, 2, false>(a, r, parts, st);
     });
   } else {
-    const RmsShape s = rms_backward_shape(D, type);
+    const bool wide = vec && !off_16_bytes(a.weight);
+    const RmsShape s = rms_backward_shape(D, type, wide);
     const int blocks = rms_backward_blocks(a.rows, s);
     count = rms_backward_parts(blocks, s);
-    const bool wide = vec && !off_16_bytes(a.weight);
     rc = rms_with_type(type, [&](auto tag) {
       using T = decltype(tag);
       auto launch = [&](auto kernel) {
@@ -669,9 +678,8 @@ extern "C" int ffm_rms_norm_backward(const ffm_rms_norm_args* args, ffm_stream_t
                                              parts);
         return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
       };
-      if (s.chunks == 2) {
-        return wide ? launch(rms_norm_backward_kernel<T, 2, true, RMS_BACK_SM_THREADS>) : launch(rms_norm_backward_kernel<T, 2, false, RMS_BACK_SM_THREADS>);
-      }
+      if (s.chunks == 1) return launch(rms_norm_backward_kernel<T, 1, false, RMS_TEAM>);
+      if (s.chunks == 2) return launch(rms_norm_backward_kernel<T, 2, true, RMS_BACK_SM_THREADS>);
       return wide ? launch(rms_norm_backward_kernel<T, RMS_CHUNKS_MAX, true, RMS_TEAM>) : launch(rms_norm_backward_kernel<T, RMS_CHUNKS_MAX, false, RMS_TEAM>);
     });
   }
