@@ -23,7 +23,7 @@ def _norm(grads, sharded, like, max_norm, largest, group):
     capturing = like.is_cuda and torch.cuda.is_current_stream_capturing()
     native, other = _lib.native(), None
     if group is not None:
-        other = native.gradient_norm(sharded, like, 0.0, largest, None, capturing)[0]
+        other = native.gradient_norm(sharded, like, 0.0, largest, None, capturing)[0][:1]
         dist.all_reduce(other, dist.ReduceOp.MAX if largest else dist.ReduceOp.SUM, group=group)
     else:
         grads = [*grads, *sharded]

@@ -19,7 +19,7 @@ namespace {
 // ---- quantising -------------------------------------------------------------------------------------------------
 
 constexpr int QB_THREADS = 256;
-constexpr int QB_GROUPS = 4;  // blocks of a row that a thread works on at once
+constexpr int QB_GROUPS = 2;  // blocks of a row that a thread works on at once
 
 template <typename T>
 __device__ __forceinline__ void store_e4m3(uint8_t* to, const uint4& raw, float inverse) {
@@ -50,16 +50,20 @@ quantize_row_blocks_kernel(const T* __restrict__ x, long long stride, long long 
   constexpr int V = VALUES<T>, LANES = E4M3_BLOCK / V, TEAMS = QB_THREADS / LANES;
   const int t = threadIdx.x % LANES;
   const long long first = static_cast<long long>(blockIdx.x) * (TEAMS * QB_GROUPS) + threadIdx.x / LANES;
+  const int rows_on = TEAMS / across, blocks_on = TEAMS % across;  // from one of a thread's blocks to the next
+  long long row = (first >> 32) == 0 ? static_cast<uint32_t>(first) / static_cast<uint32_t>(across) : first / across;
+  int block = static_cast<int>(first - row * across);
   uint4 raw[QB_GROUPS];
-  long long row[QB_GROUPS];
-  int col[QB_GROUPS];
+  long long out[QB_GROUPS];  // -1: past the row's end, or the last row
 #pragma unroll
   for (int i = 0; i < QB_GROUPS; ++i) {
-    const long long b = first + i * TEAMS;
-    row[i] = (b >> 32) == 0 ? static_cast<uint32_t>(b) / static_cast<uint32_t>(across) : b / across;
-    col[i] = static_cast<int>(b - row[i] * across) * E4M3_BLOCK + t * V;
-    const bool has = b < blocks && col[i] < K;
-    raw[i] = has ? *reinterpret_cast<const uint4*>(x + row[i] * stride + col[i]) : make_uint4(0, 0, 0, 0);
+    const int col = block * E4M3_BLOCK + t * V;
+    const bool has = first + i * TEAMS < blocks && col < K;
+    raw[i] = has ? *reinterpret_cast<const uint4*>(x + row * stride + col) : make_uint4(0, 0, 0, 0);
+    out[i] = has ? row * K + col : -1;
+    row += rows_on;
+    block += blocks_on;
+    if (block >= across) block -= across, ++row;
   }
 #pragma unroll
   for (int i = 0; i < QB_GROUPS; ++i) {
@@ -67,30 +71,28 @@ quantize_row_blocks_kernel(const T* __restrict__ x, long long stride, long long 
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float s = e4m3_scale(top);
-    const long long b = first + i * TEAMS;
-    if (b < blocks && col[i] < K) {
-      store_e4m3<T>(q + row[i] * K + col[i], raw[i], reciprocal(s));
-      if (t == 0) scale[b] = s;
+    if (out[i] >= 0) {
+      store_e4m3<T>(q + out[i], raw[i], reciprocal(s));
+      if (t == 0) scale[first + i * TEAMS] = s;
     }
   }
 }
 
-// A scale for 128 x 128 values of a matrix: one thread block for each, its values in registers in between. blockIdx.y: the matrix.
+// A scale for 128 x 128 values of a matrix: one thread block for each, its values in registers in between. Three blocks of 16-bit values on an SM: with
+// two 8 x 14336 x 4096 bf16 took 261 us, with four, which spill, 226; three 214 (6.6 TB/s).
 template <typename T>
-__global__ void __launch_bounds__(QB_THREADS, sizeof(T) == 2 ? 4 : 2)
+__global__ void __launch_bounds__(QB_THREADS, sizeof(T) == 2 ? 3 : 2)
 quantize_tiles_kernel(const T* __restrict__ x, int N, int K, int down, int across, uint8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int V = VALUES<T>, LANES = E4M3_BLOCK / V, TEAMS = QB_THREADS / LANES, STEPS = E4M3_BLOCK / TEAMS;
   __shared__ float part[QB_THREADS / 32];
   const long long tile = blockIdx.x;
   const int bn = static_cast<int>(tile / across % down), bk = static_cast<int>(tile % across);
-  const long long base = tile / (static_cast<long long>(down) * across) * N * K;
   const int col = bk * E4M3_BLOCK + threadIdx.x % LANES * V, n0 = bn * E4M3_BLOCK + threadIdx.x / LANES;
+  const int left = col < K ? N - n0 : 0;  // rows from this thread's first on
+  const long long first = tile / (static_cast<long long>(down) * across) * N * K + static_cast<long long>(n0) * K + col, step = static_cast<long long>(TEAMS) * K;
   uint4 raw[STEPS];
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int n = n0 + i * TEAMS;
-    raw[i] = n < N && col < K ? *reinterpret_cast<const uint4*>(x + base + static_cast<long long>(n) * K + col) : make_uint4(0, 0, 0, 0);
-  }
+  for (int i = 0; i < STEPS; ++i) raw[i] = i * TEAMS < left ? *reinterpret_cast<const uint4*>(x + first + i * step) : make_uint4(0, 0, 0, 0);
   float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) top = fmaxf(top, largest<T>(raw[i]));
@@ -104,8 +106,7 @@ quantize_tiles_kernel(const T* __restrict__ x, int N, int K, int down, int acros
   if (threadIdx.x == 0) scale[tile] = s;
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    const int n = n0 + i * TEAMS;
-    if (n < N && col < K) store_e4m3<T>(q + base + static_cast<long long>(n) * K + col, raw[i], inverse);
+    if (i * TEAMS < left) store_e4m3<T>(q + first + i * step, raw[i], inverse);
   }
 }
 
@@ -545,13 +546,13 @@ struct FewRows {
   static constexpr int STAGE_BYTES = (A_ROWS + ROWS) * 128;
   static constexpr int STAGES = ONE ? 6 : 8;
   static constexpr int PART = ONE ? 2 * ROWS * A_ROWS * 4 : 0;  // the two groups' sums
-  static constexpr int SLOTS = 8;                 // blocks whose scales are there or on their way
+  static constexpr int SLOTS = 8;  // blocks of a group whose scales are there or on their way
   struct Ctrl {
-    unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[4], acc_empty_bar[4], scale_full_bar[SLOTS], scale_empty_bar[SLOTS], drain_bar;
+    unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[4], acc_empty_bar[4], scale_full_bar[2 * SLOTS], scale_empty_bar[2 * SLOTS], drain_bar;
     uint32_t tmem_base;
     int abort_flag;
     int filled;
-    alignas(16) float scale[SLOTS][ROWS + 4];  // of the rows, and of the features
+    alignas(16) float scale[2 * SLOTS][ROWS + 4];  // of the rows, and of the features; a ring for each group
     Groups groups;
   };
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PART + static_cast<int>(sizeof(Ctrl)) + 1024;
@@ -621,7 +622,7 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
       mbar_init(smem_u32(&ctrl->acc_full_bar[a]), 1);
       mbar_init(smem_u32(&ctrl->acc_empty_bar[a]), 4);
     }
-    for (int i = 0; i < S::SLOTS; ++i) {
+    for (int i = 0; i < 2 * S::SLOTS; ++i) {
       mbar_init(smem_u32(&ctrl->scale_full_bar[i]), 32);
       mbar_init(smem_u32(&ctrl->scale_empty_bar[i]), 4);
     }
@@ -702,16 +703,20 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
       }
     }
   } else if (warp == 2) {
-    // the scales of the tile's rows and features, block by block, ahead of the sums that they belong to
-    int slot = 0;
-    uint32_t phase = 0;
+    // the scales of the tile's rows and features, block by block, ahead of the sums that they belong to. Each group has a ring of its own and so
+    // waits for every round of it: on a ring of both, one that has skipped the other's tile would take the round before for its own.
+    int group = 0;
+    uint32_t count[2] = {0, 0};  // blocks that a group was given so far
     bool ok = true;
-    while (ok && walker.next(t)) {
+    for (; ok && walker.next(t); group ^= 1) {
       const float* ws = p.w_scale + (static_cast<long long>(t.group) * scale_rows + t.across) * p.k_blocks;
       const float* xs0 = p.x_scale + static_cast<long long>(t.row0 + min(lane, t.rows - 1)) * p.k_blocks;
       const float* xs1 = p.x_scale + static_cast<long long>(t.row0 + min(lane + 32, t.rows - 1)) * p.k_blocks;
       for (int kb = from(); kb < to(); ++kb) {
-        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_empty_bar[slot]), phase ^ 1u, abort_flag, p.status, FFM_STATUS_WAIT_PRODUCER, p.wait_cycles);
+        if (ONE) group = (kb - from()) & 1;
+        const uint32_t slot = group * S::SLOTS + count[group] % S::SLOTS;
+        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_empty_bar[slot]), ((count[group] / S::SLOTS) & 1) ^ 1u, abort_flag, p.status,
+                               FFM_STATUS_WAIT_PRODUCER, p.wait_cycles);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t dst = smem_u32(ctrl->scale[slot]);
@@ -719,27 +724,23 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
         if (t.rows > 32) copy_async_4(dst + (lane + 32) * 4, xs1 + kb);
         if (lane == 0) copy_async_4(dst + S::ROWS * 4, ws + kb);
         copy_async_arrive(smem_u32(&ctrl->scale_full_bar[slot]));
-        if (++slot == S::SLOTS) slot = 0, phase ^= 1u;
+        ++count[group];
       }
     }
     copy_async_wait<0>();
   } else if (warp >= 4) {
     const int quarter = warp & 3, group = (warp - 4) >> 2;
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + group * 2 * S::ROWS;
-    uint32_t count = 0, blocks = 0;  // accumulators that this group was given so far, and blocks of all tiles so far
+    uint32_t count = 0;  // blocks that this group was given so far
     bool ok = true;
     for (int turn = 0; ok && walker.next(t); turn ^= 1) {
-      if (!ONE && turn != group) {
-        blocks += to() - from();
-        continue;
-      }
+      if (!ONE && turn != group) continue;
       float sum[S::ROWS];
 #pragma unroll
       for (int j = 0; j < S::ROWS; ++j) sum[j] = 0.0f;
-      for (int kb = from() + (ONE ? group : 0); kb < to(); kb += ONE ? 2 : 1, ++count, ++blocks) {
-        if (ONE) blocks = kb - from();
-        const uint32_t acc = count & 1, slot = blocks % S::SLOTS;
-        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_full_bar[slot]), (blocks / S::SLOTS) & 1, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE,
+      for (int kb = from() + (ONE ? group : 0); kb < to(); kb += ONE ? 2 : 1, ++count) {
+        const uint32_t acc = count & 1, slot = group * S::SLOTS + count % S::SLOTS;
+        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_full_bar[slot]), (count / S::SLOTS) & 1, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE,
                                p.wait_cycles) &&
              mbar_wait_bounded(smem_u32(&ctrl->acc_full_bar[group * 2 + acc]), (count >> 1) & 1, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE,
                                p.wait_cycles);

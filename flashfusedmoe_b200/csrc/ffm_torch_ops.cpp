@@ -1021,7 +1021,7 @@ void check_norm(const Tensors& grads, const Tensor& like, double max_norm) {
   for (const Tensor& t : grads) on_gpu(t, "grad");
 }
 
-// (total float64 [1], norm, coefficient)
+// (float64 [n] that begins with the total, norm, coefficient)
 py::tuple gradient_norm(const Tensors& grads, const Tensor& like, double max_norm, bool largest, const OptTensor& other, bool capturing) {
   check_norm(grads, like, max_norm);
   const On device(like);
@@ -1034,7 +1034,7 @@ py::tuple gradient_norm(const Tensors& grads, const Tensor& like, double max_nor
     more = other->resolve_neg();
   }
   const ClipNorm r = norm_of(table, like, device, max_norm, largest, more, capturing);
-  return py::make_tuple(r.workspace.narrow(0, 0, 1), r.norm, r.coefficient);
+  return py::make_tuple(r.workspace, r.norm, r.coefficient);
 }
 
 // grads *= factor (one float32 on the device), in place

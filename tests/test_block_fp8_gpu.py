@@ -119,6 +119,20 @@ def test_grouped(sizes, spare, N, K, dtype):
     ops.check_status()
 
 
+@pytest.mark.parametrize("rows,N,K,experts", [(288, 2816, 2048, 64), (100, 4096, 1024, 8), (700, 1000, 2064, 40), (6000, 1400, 528, 48)])
+def test_many_tiles_a_block_of_threads(rows, N, K, experts):
+    """Tiles follow one another on an SM: every one of them, and the same bits each time."""
+    x, xs, w, ws = _operands(rows, N, K, experts)
+    sizes = torch.bincount(torch.randint(0, experts, (rows,), generator=torch.Generator().manual_seed(1)), minlength=experts)
+    ends = sizes.cumsum(0).int().cuda()
+    outs = [linear_e4m3(x, xs, w, ws, ends=ends) for _ in range(8)]
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    begin = 0
+    for e, n in enumerate(sizes.tolist()):
+        _check(outs[0][begin:begin + n], x[begin:begin + n], xs[begin:begin + n], w[e], ws[e])
+        begin += n
+
+
 def test_groups_do_not_reach_into_one_another():
     """NaN rows and weights of one expert stay in its rows, and those behind the last in none."""
     for sizes, spare in (([5, 7, 3], 4), ([200, 130, 300], 40)):
