@@ -255,20 +255,21 @@ __device__ __forceinline__ void copy_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+__device__ __forceinline__ void st_shared_v2(uint32_t addr, float2 v) {
+  asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
+}
+
 __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 
-// byte b of row r in a warp's boxes
-__device__ __forceinline__ uint32_t in_boxes(int r, int b) { return (b >> 7) * 4096 + box_offset(r, (b >> 4) & 7) + (b & 15); }
-
 // A value in front of the first whole word of a row of 16-bit values
 __device__ __forceinline__ int head_of(const uint8_t* row) { return (reinterpret_cast<uintptr_t>(row) >> 1) & 1; }
 
-// The launch's 168 registers a thread go from the four warps of the first group to the eight that hold sums: 128 x 56 + 256 x 224 = 384 x 168.
-constexpr int ISSUE_REGISTERS = 56, SUM_REGISTERS = 224;
+// The launch's 168 registers a thread go from the four warps of the first group to the eight that hold sums: 128 x 72 + 256 x 216 = 384 x 168.
+constexpr int ISSUE_REGISTERS = 72, SUM_REGISTERS = 216;
 static_assert(128 * ISSUE_REGISTERS + 256 * SUM_REGISTERS <= BLOCK_THREADS * 168, "more registers than the launch has");
 
 //   warp 0      TMA producer          warp 1   MMA issuer, TMEM owner          warp 2   row ranges, scales          warp 3   nothing
@@ -394,16 +395,16 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * S::COLS;
     const uint32_t mine = staging + (warp - 4) * S::STORE_WARP;  // this warp's rows on their way out
-    int acc = 0, slot = 0;
-    uint32_t acc_phase = 0, slot_phase = 0;
+    uint32_t blocks = 0;  // so far
     bool ok = true;
     while (ok && walker.next(t)) {
       float2 sum[S::COLS / 2];
 #pragma unroll
       for (int j = 0; j < S::COLS / 2; ++j) sum[j] = both(0.0f);
       uint32_t v[2][32];
-      for (int kb = 0; kb < t.k_blocks; ++kb) {
-        ok = mbar_wait_bounded(smem_u32(&ctrl->acc_full_bar[acc]), acc_phase, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
+      for (int kb = 0; kb < t.k_blocks; ++kb, ++blocks) {
+        const uint32_t acc = blocks & 1, slot = blocks % S::SLOTS;
+        ok = mbar_wait_bounded(smem_u32(&ctrl->acc_full_bar[acc]), (blocks >> 1) & 1, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -411,12 +412,11 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
         // the stores: 137 us, so 122)
         tmem_ld_32x32(taddr + acc * BN, v[0]);
         tmem_ld_32x32(taddr + acc * BN + 32, v[1]);
-        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_full_bar[slot]), slot_phase, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
+        ok = mbar_wait_bounded(smem_u32(&ctrl->scale_full_bar[slot]), (blocks / S::SLOTS) & 1, abort_flag, p.status, FFM_STATUS_WAIT_EPILOGUE, p.wait_cycles);
         ok = __all_sync(0xffffffffu, ok);
         const float2 s = both(ctrl->scale[slot][quarter * 32 + lane] * ctrl->scale[slot][A_ROWS + half]);
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctrl->scale_empty_bar[slot]));
-        if (++slot == S::SLOTS) slot = 0, slot_phase ^= 1u;
 #pragma unroll
         for (int c = 0; c < S::COLS / 64; ++c) {
           tmem_ld_wait();
@@ -434,25 +434,25 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
           }
         }
         if (!ok) break;
-        if (++acc == 2) acc = 0, acc_phase ^= 1u;
       }
       if (!ok) break;
-      // Up to 256 bytes of every row at a time through shared memory. 32 whole rows on 16 bytes go out by themselves, while the next tile's sums
-      // begin; others are stored from here.
-      constexpr int STEP = S::COLS * OUT_BYTES > 256 ? 256 / OUT_BYTES : S::COLS;
+      // 128 bytes of every row at a time through one of two boxes in shared memory. 32 whole rows on 16 bytes go out by themselves, while the next
+      // tile's sums begin; others are stored from here.
+      constexpr int STEP = 128 / OUT_BYTES;
       const int limit = min(t.rows - quarter * 32, 32);  // of this warp's rows
+      const long long pitch = static_cast<long long>(p.N) * OUT_BYTES;
 #pragma unroll
       for (int c = 0; c < S::COLS / STEP; ++c) {
         const int first = t.across * BN + half * S::COLS + c * STEP, count = min(STEP, p.N - first);
-        if (lane == 0) bulk_wait_read<0>();  // what was sent before has been read
+        const uint32_t box = mine + (c & 1) * 4096;
+        if (lane == 0) bulk_wait_read<S::COLS / STEP % 2 == 0 ? 1 : 0>();  // what was sent from this box has been read
         __syncwarp();
-        const long long pitch = static_cast<long long>(p.N) * OUT_BYTES;
-        uint8_t* out = static_cast<uint8_t*>(p.out) + (t.row0 + quarter * 32) * pitch + first * OUT_BYTES;
+        uint8_t* out = static_cast<uint8_t*>(p.out) + (t.row0 + quarter * 32) * pitch + static_cast<long long>(first) * OUT_BYTES;
         // 16-bit rows off 16 bytes are staged as the words that memory has them in, without the value in front of the first
         const bool shift = OUT_BYTES == 2 && !p.out_wide && head_of(out + lane * pitch);
 #pragma unroll
-        for (int q = 0; q < STEP * OUT_BYTES / 16; ++q) {
-          const uint32_t at = mine + in_boxes(lane, q * 16);
+        for (int q = 0; q < 8; ++q) {
+          const uint32_t at = box + box_offset(lane, q);
           if constexpr (OUT_BYTES == 2) {
             uint32_t u[4];
 #pragma unroll
@@ -464,51 +464,47 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
             st_shared_v4(at, u[0], u[1], u[2], u[3]);
           } else {
             const float2* f = sum + c * (STEP / 2) + q * 2;
-            st_shared_v4(at, __float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+            // by pairs, as the sums lie: stored by fours they would be moved in every block of the contraction (8192 x 4096 x 4096: 162 us, so 143)
+            st_shared_v2(at, f[0]);
+            st_shared_v2(at + 8, f[1]);
           }
         }
-        if (count <= 0 || limit <= 0) continue;
-        if (p.out_wide && limit == 32) {
+        if (count > 0 && limit == 32 && p.out_wide) {
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) {
-            for (int b = 0; b < count * OUT_BYTES; b += 128) tma_store_3d(&tm_out, mine + b * 32, first + b / OUT_BYTES, t.row0 + quarter * 32, 0);
-            bulk_commit();
-          }
-        } else if (p.out_wide) {
+          if (lane == 0) tma_store_3d(&tm_out, box, first, t.row0 + quarter * 32, 0);
+        } else if (count > 0 && limit > 0 && p.out_wide) {
           __syncwarp();
-          for (int i = lane; i < limit * 16; i += 32) {  // 16 bytes each
-            const int r = i >> 4, at = (i & 15) * 16;
+          for (int i = lane; i < limit * 8; i += 32) {  // 16 bytes each
+            const int r = i >> 3, q = i & 7;
             uint4 u;
-            ld_shared_v4(mine + in_boxes(r, at), u);
-            if (at < count * OUT_BYTES) *reinterpret_cast<uint4*>(out + r * pitch + at) = u;
+            ld_shared_v4(box + box_offset(r, q), u);
+            if (q * (16 / OUT_BYTES) < count) *reinterpret_cast<uint4*>(out + r * pitch + q * 16) = u;
           }
-        } else {
+        } else if (count > 0 && limit > 0) {
           if constexpr (OUT_BYTES == 2) {
             // what is not in a whole word: the first value, and the last
-            uint8_t* row = out + lane * pitch;
-            const int last = (count - (shift ? 1 : 0)) & 1;
-            if (lane < limit && shift) *reinterpret_cast<uint16_t*>(row) = static_cast<uint16_t>(pack_out(p.out_type, sum[c * (STEP / 2)].x, 0.0f));
-            if (lane < limit && last) {
-              const int word = (count - (shift ? 1 : 0)) >> 1;
-              reinterpret_cast<uint16_t*>(row)[count - 1] = static_cast<uint16_t>(ld_shared_u32(mine + in_boxes(lane, word * 4)));
+            uint16_t* row = reinterpret_cast<uint16_t*>(out + lane * pitch);
+            const int left = count - (shift ? 1 : 0);
+            if (lane < limit && shift) row[0] = static_cast<uint16_t>(pack_out(p.out_type, sum[c * (STEP / 2)].x, 0.0f));
+            if (lane < limit && (left & 1)) {
+              row[count - 1] = static_cast<uint16_t>(ld_shared_u32(box + box_offset(lane, left >> 3) + (left >> 1 & 3) * 4));
             }
           }
           __syncwarp();
-          // words of a row: a warp's 32 at a time
+          // a row's words, one a lane
           for (int r0 = 0; r0 < limit; r0 += 8) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = r0 + i;
               uint8_t* row = out + r * pitch;
               const int head = OUT_BYTES == 2 ? head_of(row) : 0, words = r < limit ? (OUT_BYTES == 2 ? (count - head) >> 1 : count) : 0;
-              const uint32_t from = mine + r * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4;
-              uint32_t* to = reinterpret_cast<uint32_t*>(row + head * 2) + lane;
-              if (lane < words) to[0] = ld_shared_u32(from);
-              if (STEP * OUT_BYTES > 128 && lane + 32 < words) to[32] = ld_shared_u32(from + 4096);
+              const uint32_t from = box + r * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4;
+              if (lane < words) reinterpret_cast<uint32_t*>(row + head * 2)[lane] = ld_shared_u32(from);
             }
           }
         }
+        if (lane == 0) bulk_commit();  // empty where nothing was sent
       }
     }
     bulk_wait0();  // its stores have landed before the CTA's shared memory goes away
