@@ -565,12 +565,14 @@ struct RmsGradients {
 RmsGradients rms_backward_of(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& weight, const Tensor& rstd, const RmsCall& call,
                              bool want_x, bool want_weight) {
   const On device(h);
+  on_gpu(h, "x");
   ffm_rms_norm_args a = {};
   a.x_type = element_type(h, "x");
   const int64_t D = h.size(-1);
   const Rows r = as_rows(h);
   // saved-tensor hooks may have handed back other tensors than were saved
-  if (rstd.numel() != r.rows || rstd.scalar_type() != at::kFloat || !rstd.is_cuda()) throw py::value_error("saved statistics do not belong to x");
+  if (rstd.numel() != r.rows || rstd.scalar_type() != at::kFloat || rstd.device() != h.device()) throw py::value_error("saved statistics do not belong to x");
+  check_vector(weight, h, "weight");
   const Tensor s = plain(rstd), w = weight.defined() ? plain(weight) : Tensor();
   auto gradient = [&](const Tensor& t, const char* name) {
     if (!t.defined()) return Tensor();
