@@ -32,7 +32,7 @@ def _norm(grads, sharded, like, max_norm, largest, group):
 
 @torch.compiler.disable
 def clip_coefficient(grads, max_norm, norm_type=2.0, *, sharded=(), group=None):
-    """(norm, coefficient) of the tensors in `grads` together: the root of the sum of all squares (norm_type 2) or the largest
+    """(norm, coefficient) of the tensors in `grads` (or of the one tensor) together: the root of the sum of all squares (norm_type 2) or the largest
     magnitude (inf), and min(1, max_norm / (norm + 1e-6)); NaN where the norm is NaN. Both are float32 on the device, and the coefficient is
     what AdamW.step(grad_scale=...) and adamw_step() take: gradients are then clipped without a pass of their own.
 
@@ -41,7 +41,7 @@ def clip_coefficient(grads, max_norm, norm_type=2.0, *, sharded=(), group=None):
     (MoELayer.expert_params); their part of the norm is all-reduced over `group`, so every rank calls with as many tensors of its own as it
     has, and gets the same norm. Without a group they count as the others. Everything runs on the current stream without a host wait and can be
     captured."""
-    grads, sharded = list(grads), list(sharded)
+    grads, sharded = [grads] if isinstance(grads, torch.Tensor) else list(grads), list(sharded)
     max_norm, largest = _arguments(max_norm, norm_type)
     if not grads and not sharded:
         raise ValueError("there are no gradients")

