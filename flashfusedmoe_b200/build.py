@@ -49,7 +49,7 @@ def _native_command(source, target):
 def _native_link_command(objs, target):
     import torch
     return (["g++", "-shared"] + objs + ["-o", target, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch",
-                                         "-ltorch_cpu", "-ltorch_python", "-lc10"])
+                                         "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10"])
 
 
 def build(force=False, verbose=False):
