@@ -90,7 +90,8 @@ def _check(out, x, xs, w, ws):
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("rows,N,K", [(1, 1, 16), (1, 128, 128), (1, 4096, 7168), (3, 130, 144), (16, 64, 272), (17, 129, 256), (64, 500, 1040), (65, 256, 128),
-                                      (128, 128, 128), (129, 127, 400), (300, 1000, 2064), (1000, 3001, 512), (4096, 2048, 1024), (200, 40000, 64)])
+                                      (128, 128, 128), (129, 127, 400), (300, 1000, 2064), (1000, 3001, 512), (4096, 2048, 1024), (200, 40000, 64),
+                                      (1, 3001, 2064), (1, 40000, 272), (1, 200000, 64), (1, 130, 16384), (1, 130, 16400), (1, 257, 528)])
 def test_dense(rows, N, K, dtype):
     x, xs, w, ws = _operands(rows, N, K)
     out = linear_e4m3(x, xs, w, ws, out_dtype=DTYPES[dtype])
@@ -199,6 +200,32 @@ def test_same_bits_in_graphs_with_other_ends():
     torch.cuda.synchronize()
     assert all(torch.equal(o, want_other) for o in outs)
     ops.check_status()
+
+
+@pytest.mark.parametrize("rows,N,K,experts", [(1, 1000, 1040, None), (2, 4096, 1024, None), (60, 700, 2048, None), (3, 300, 512, 4), (100, 4096, 512, 16)])
+def test_calls_of_few_rows_in_graphs(rows, N, K, experts):
+    x, xs, w, ws = _operands(rows, N, K, experts)
+    ends = None if experts is None else torch.linspace(0, rows, experts + 1)[1:].int().cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = linear_e4m3(x, xs, w, ws, ends=ends)
+    for seed in range(3):
+        other = _operands(rows, N, K, experts, seed)
+        for a, b in zip((x, xs, w, ws), other):
+            a.copy_(b)
+        graph.replay()
+        assert torch.equal(out, linear_e4m3(*other, ends=ends))
+
+
+def test_one_row_with_values_that_are_not_finite():
+    x, xs, w, ws = _operands(1, 400, 384)
+    want = linear_e4m3(x, xs, w, ws)
+    w.view(torch.uint8)[7, 300] = 0x7f
+    ws[2, 1] = float("inf")
+    out = linear_e4m3(x, xs, w, ws)[0]
+    bad = torch.zeros(400, dtype=torch.bool, device="cuda")
+    bad[7] = bad[256:384] = True
+    assert torch.equal(out[~bad], want[0, ~bad]) and not bool(out[bad].isfinite().any())
 
 
 def test_outputs_beyond_32_bits():
