@@ -80,51 +80,65 @@ __global__ void __launch_bounds__(RMS_TEAM)
 rms_norm_forward_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ residual, long long residual_stride,
                         const void* __restrict__ weight, int w_type, float offset, long long rows, int D, float eps, int team,
                         T* __restrict__ h, void* __restrict__ y, float* __restrict__ y_scale, float* __restrict__ rstd) {
-  __shared__ float part[1][32];
+  __shared__ float part[2][1][32];
   constexpr int V = VALUES<T>;
-  Place<T, VEC> at(team, D);
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / team) + threadIdx.x / team;
-  if (row >= rows) at.count = 0;  // goes along for the sums
-  uint4 raw[CH];
-  load_row(x + (row < rows ? row : 0) * x_stride, at, raw);
-  if (residual != nullptr) {
-    uint4 more[CH];
-    load_row(residual + (row < rows ? row : 0) * residual_stride, at, more);
+  const Place<T, VEC> all(team, D);
+  const int teams = blockDim.x / team;
+  // single values: the weight's stay in registers for all rows of a thread, or they would be fetched one by one
+  constexpr bool HELD = !VEC && CH == 1;
+  float held[V];
+  if (HELD) load_vector<T, VEC>(weight, w_type, all, 0, 1.0f, held);
+  int parity = 0;
+  for (long long base = static_cast<long long>(blockIdx.x) * teams; base < rows; base += static_cast<long long>(gridDim.x) * teams, parity ^= 1) {
+    const long long row = base + threadIdx.x / team;
+    Place<T, VEC> at = all;
+    if (row >= rows) at.count = 0;  // goes along for the sums
+    uint4 raw[CH];
+    load_row(x + (row < rows ? row : 0) * x_stride, at, raw);
+    if (residual != nullptr) {
+      uint4 more[CH];
+      load_row(residual + (row < rows ? row : 0) * residual_stride, at, more);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        raw[c] = add_packed<T>(raw[c], more[c]);
+        store_packed(h + row * D, at, c, raw[c]);
+      }
+    }
+    float s[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      raw[c] = add_packed<T>(raw[c], more[c]);
-      store_packed(h + row * D, at, c, raw[c]);
+      float v[V];
+      unpack<T>(raw[c], v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[0] = fmaf(v[j], v[j], s[0]);
     }
-  }
-  float s[1] = {0.0f};
+    team_sum(s, team, part[parity]);
+    stay_packed(raw);
+    const float r = rsqrtf(s[0] / static_cast<float>(D) + eps);
+    if (rstd != nullptr && at.t == 0 && row < rows) rstd[row] = r;
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    float v[V];
-    unpack<T>(raw[c], v);
+    for (int c = 0; c < CH; ++c) {
+      float v[V], w[V];
+      unpack<T>(raw[c], v);
+      if constexpr (HELD) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[0] = fmaf(v[j], v[j], s[0]);
-  }
-  team_sum(s, team, part);
-  stay_packed(raw);
-  const float r = rsqrtf(s[0] / static_cast<float>(D) + eps);
-  if (rstd != nullptr && at.t == 0 && row < rows) rstd[row] = r;
+        for (int j = 0; j < V; ++j) w[j] = held[j];
+      } else {
+        load_vector<T, VEC>(weight, w_type, at, c, 1.0f, w);
+      }
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    float v[V], w[V];
-    unpack<T>(raw[c], v);
-    load_vector<T, VEC>(weight, w_type, at, c, 1.0f, w);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = v[j] * r * (w[j] + offset);
-    if constexpr (!E4M3) {
-      store_chunk(static_cast<T*>(y) + row * D, at, c, v);
-    } else {
-      const int across = (D + E4M3_BLOCK - 1) / E4M3_BLOCK;
-      store_e4m3<T>(v, at.has(c, 0), at.column(c, 0), static_cast<uint8_t*>(y) + row * D, y_scale + row * across);
+      for (int j = 0; j < V; ++j) v[j] = v[j] * r * (w[j] + offset);
+      if constexpr (!E4M3) {
+        store_chunk(static_cast<T*>(y) + row * D, at, c, v);
+      } else {
+        const int across = (D + E4M3_BLOCK - 1) / E4M3_BLOCK;
+        store_e4m3<T>(v, at.has(c, 0), at.column(c, 0), static_cast<uint8_t*>(y) + row * D, y_scale + row * across);
+      }
     }
   }
 }
 
-// dx (skipped where null), and for every team (of a warp or more; the teams of a warp are added up) one row of partial sums of dw. dh: null
+// dx (skipped where null), and for every block one row of partial sums of dw. dh: null
 // where no residual stream was handed on. Any rows.
 template <typename T, int CH, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -142,6 +156,18 @@ rms_norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ dh, con
 #pragma unroll
     for (int j = 0; j < V; ++j) aw[c][j] = 0.0f;
   }
+  // single values: the weight's stay in registers (8 of 85), or they would be fetched one by one twice a row
+  constexpr bool HELD = !VEC && CH == 1;
+  float held[V];
+  if (HELD) load_vector<T, VEC>(weight, w_type, at, 0, 1.0f, held);
+  auto weights = [&](int c, const Place<T, VEC>& here, float(&w)[V]) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = held[j];
+    } else {
+      load_vector<T, VEC>(weight, w_type, here, c, 1.0f, w);
+    }
+  };
   int parity = 0;
   // all teams of a block go through their rows in step
   for (long long base = static_cast<long long>(blockIdx.x) * teams; base < rows; base += step, parity ^= 1) {
@@ -159,7 +185,7 @@ rms_norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ dh, con
       float v[V], g[V], w[V];
       unpack<T>(v_raw[c], v);
       unpack<T>(g_raw[c], g);
-      load_vector<T, VEC>(weight, w_type, here, c, 1.0f, w);
+      weights(c, here, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float xh = here.has(c, VEC ? 0 : j) ? v[j] * r : 0.0f;
@@ -179,7 +205,7 @@ rms_norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ dh, con
       float v[V], g[V], w[V], m[V];
       unpack<T>(v_raw[c], v);
       unpack<T>(g_raw[c], g);
-      load_vector<T, VEC>(weight, w_type, here, c, 1.0f, w);
+      weights(c, here, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) m[j] = 0.0f;
       if (dh != nullptr) unpack<T>(more[c], m);
@@ -196,15 +222,28 @@ rms_norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ dh, con
       for (int j = 0; j < V; ++j) aw[c][j] += __shfl_xor_sync(0xffffffffu, aw[c][j], o);
     }
   }
-  const int wide = team < 32 ? 32 : team;
-  if (threadIdx.x % wide >= team) return;
-  float* to = parts + (static_cast<long long>(blockIdx.x) * (blockDim.x / wide) + threadIdx.x / wide) * D;
+  // one row of sums a block: its teams (of a warp or more) add theirs one after the other
+  extern __shared__ float sums[];
+  const int wide = team < 32 ? 32 : team, groups = blockDim.x / wide;
+  float* to = parts + static_cast<long long>(blockIdx.x) * D;
+  for (int g = 0; g < groups; ++g) {
+    if (threadIdx.x / wide == g && threadIdx.x % wide < team) {
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
+      for (int c = 0; c < CH; ++c) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (at.has(c, VEC ? 0 : j)) to[at.column(c, j)] = aw[c][j];
+        for (int j = 0; j < V; ++j) {
+          if (!at.has(c, VEC ? 0 : j)) continue;
+          const int col = at.column(c, j);
+          const float total = g > 0 ? sums[col] + aw[c][j] : aw[c][j];
+          if (g + 1 < groups) {
+            sums[col] = total;
+          } else {
+            to[col] = total;
+          }
+        }
+      }
     }
+    if (g + 1 < groups) __syncthreads();
   }
 }
 
@@ -487,25 +526,24 @@ RmsShape rms_forward_shape(int64_t rows, int D, int type, bool e4m3, bool vec) {
   const int pieces = (D + 16 / type_bytes(type) - 1) / (16 / type_bytes(type));
   const int least = e4m3 ? 32 : 1;
   if (rows <= num_sms() && pieces <= RMS_TEAM) return rms_shape(D, type, 1, least, RMS_THREADS);
-  // single values: with four chunks (32 loads) a thread's registers spill
-  if (!vec && pieces <= 2 * RMS_TEAM) return rms_shape(D, type, 2, least, RMS_THREADS);
+  // Single values: with four chunks (32 loads) a thread's registers spill; with one of 16-bit values the weight's stay in them (4093 x 2051 bf16 with a
+  // residual: 30 us, with two chunks 49; fp32 61 and 41).
+  if (!vec && pieces <= 2 * RMS_TEAM) return rms_shape(D, type, type != FFM_TYPE_FP32 && pieces <= RMS_TEAM ? 1 : 2, least, RMS_THREADS);
   return rms_shape(D, type, RMS_CHUNKS_MAX, least, RMS_THREADS);
 }
 
-// Single values: one chunk (two of 16 bits spilled, 4093 x 2051 fp16 took 64 us)
+// Single values: one chunk, whose weights stay in registers (4093 x 2051 fp16: 27 us; fetched for every row 50, with two chunks, which spill, 64)
 RmsShape rms_backward_shape(int D, int type, bool vec) {
   const RmsShape s = rms_shape(D, type, vec ? 2 : 1, 1, RMS_THREADS);
   return s.team <= (vec ? RMS_BACK_TEAM : RMS_TEAM) ? s : rms_shape(D, type, RMS_CHUNKS_MAX, 1, RMS_THREADS);
 }
 
-// Blocks of the backward kernel for any rows, and its rows of partial sums
+// Blocks of the backward kernel for any rows, each with a row of partial sums
 int rms_backward_blocks(int64_t rows, const RmsShape& s) {
-  const int on_sm = s.chunks == 1 ? RMS_TEAM / s.threads : (s.chunks == 2 ? RMS_BACK_SM_THREADS / s.threads : 1);
+  const int on_sm = s.chunks <= 2 && s.threads <= RMS_BACK_SM_THREADS ? RMS_BACK_SM_THREADS / s.threads : 1;
   const int64_t want = (rows + s.teams - 1) / s.teams, most = static_cast<int64_t>(num_sms()) * on_sm;
   return static_cast<int>(want < most ? (want > 0 ? want : 1) : most);
 }
-int rms_backward_parts(int blocks, const RmsShape& s) { return blocks * (s.threads / (s.team < 32 ? 32 : s.team)); }
-
 struct RmsStream {
   RmsShape shape;
   int stages, smem;
@@ -616,7 +654,8 @@ extern "C" int ffm_rms_norm_forward(const ffm_rms_norm_args* args, ffm_stream_t 
     });
   }
   const RmsShape s = rms_forward_shape(a.rows, D, type, e4m3, vec);
-  const int64_t blocks = (a.rows + s.teams - 1) / s.teams;
+  const int64_t each = (a.rows + s.teams - 1) / s.teams, resident = static_cast<int64_t>(num_sms()) * (RMS_TEAM / s.threads);
+  const int64_t blocks = !vec && s.chunks == 1 && each > resident ? resident : each;
   if (blocks > 0x7fffffffll) return FFM_ERR_UNSUPPORTED;
   return rms_with_type(type, [&](auto tag) {
     using T = decltype(tag);
@@ -639,8 +678,8 @@ extern "C" size_t ffm_rms_norm_workspace_bytes(int64_t rows, int D, int x_type) 
   int most = num_sms();  // a streaming kernel's
   for (const bool vec : {false, true}) {
     const RmsShape s = rms_backward_shape(D, x_type, vec);
-    const int parts = rms_backward_parts(rms_backward_blocks(rows, s), s);
-    most = parts > most ? parts : most;
+    const int blocks = rms_backward_blocks(rows, s);
+    most = blocks > most ? blocks : most;
   }
   return sizeof(float) * static_cast<size_t>(D) * most;
 }
@@ -669,17 +708,19 @@ extern "C" int ffm_rms_norm_backward(const ffm_rms_norm_args* args, ffm_stream_t
   } else {
     const bool wide = vec && !off_16_bytes(a.weight);
     const RmsShape s = rms_backward_shape(D, type, wide);
-    const int blocks = rms_backward_blocks(a.rows, s);
-    count = rms_backward_parts(blocks, s);
+    const int blocks = count = rms_backward_blocks(a.rows, s);
+    // for the teams' sums; several teams have rows of up to 2048 (fp32: 1024) values
+    const size_t smem = s.threads > (s.team < 32 ? 32 : s.team) ? D * sizeof(float) : 0;
     rc = rms_with_type(type, [&](auto tag) {
       using T = decltype(tag);
       auto launch = [&](auto kernel) {
-        kernel<<<blocks, s.threads, 0, st>>>(static_cast<const T*>(a.dy), static_cast<const T*>(a.dh), static_cast<const T*>(a.x), a.x_stride, a.weight,
+        kernel<<<blocks, s.threads, smem, st>>>(static_cast<const T*>(a.dy), static_cast<const T*>(a.dh), static_cast<const T*>(a.x), a.x_stride, a.weight,
                                              static_cast<int>(a.w_type), static_cast<float>(a.offset), a.rstd, a.rows, D, s.team, static_cast<T*>(a.dx),
                                              parts);
         return cudaGetLastError() == cudaSuccess ? FFM_OK : FFM_ERR_LAUNCH;
       };
-      if (s.chunks == 1) return launch(rms_norm_backward_kernel<T, 1, false, RMS_TEAM>);
+      if (s.chunks == 1 && s.threads > RMS_BACK_SM_THREADS) return launch(rms_norm_backward_kernel<T, 1, false, RMS_TEAM>);
+      if (s.chunks == 1) return launch(rms_norm_backward_kernel<T, 1, false, RMS_BACK_SM_THREADS>);
       if (s.chunks == 2) return launch(rms_norm_backward_kernel<T, 2, true, RMS_BACK_SM_THREADS>);
       return wide ? launch(rms_norm_backward_kernel<T, RMS_CHUNKS_MAX, true, RMS_TEAM>) : launch(rms_norm_backward_kernel<T, RMS_CHUNKS_MAX, false, RMS_TEAM>);
     });
