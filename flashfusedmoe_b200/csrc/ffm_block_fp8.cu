@@ -844,7 +844,7 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
 // The products of one row on the CUDA cores: a stream of the weights, without the way through TMA, MMA, TMEM and a cluster's meeting that a tile takes.
 // Bound by its instructions (eight conversions of two values to fp16 and sixteen on to fp32 for 16 weights): 4096 x 4096 6.9 us, a call of no size 2.6. A block has `features` of them and its warps equal shares of their 512-byte chunks; every share of a feature leaves one sum, added in their order.
 constexpr int ROW_THREADS = 512, ROW_WARPS = ROW_THREADS / 32;
-constexpr int ROW_AHEAD = 3;        // chunks that a warp has on their way: instructions bound it, with eight it is slower
+constexpr int ROW_AHEAD = 2;        // chunks that a warp works on, with as many on their way: instructions bound it, with more it is slower
 constexpr int ROW_K_MAX = 16384;    // the row lies in shared memory in fp32, and two blocks on an SM
 constexpr int ROW_FEATURES = 256;   // of a block at most: they lie in up to three blocks of weights' scales
 
@@ -862,12 +862,27 @@ block_row_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w, i
   __shared__ float parts[ROW_FEATURES][ROW_WARPS + 1], scale[3][ROW_K_MAX / E4M3_BLOCK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pieces = K / 16, chunks = (pieces + 31) / 32, first = blockIdx.x * features, count = min(features, p.N - first);
+  // this warp's chunks of all features' together; the first of them are on their way while the row is laid out
+  const int all = count * chunks, begin = all * warp / ROW_WARPS, end = all * (warp + 1) / ROW_WARPS;
+  int feature = begin / chunks, chunk = begin % chunks, next_chunk = chunk, ahead = begin;
+  const uint8_t* next_row = w + static_cast<long long>(first + feature) * K;
+  auto fetch = [&](uint4 (&u)[ROW_AHEAD]) {
+#pragma unroll
+    for (int i = 0; i < ROW_AHEAD; ++i) {
+      const int piece = next_chunk * 32 + lane;
+      u[i] = ahead < end && piece < pieces ? *reinterpret_cast<const uint4*>(next_row + piece * 16) : make_uint4(0, 0, 0, 0);
+      ++ahead;
+      if (++next_chunk == chunks) next_chunk = 0, next_row += K;
+    }
+  };
+  uint4 u[ROW_AHEAD];
+  fetch(u);
   for (int i = threadIdx.x; i < pieces; i += ROW_THREADS) {
-    const uint4 u = *reinterpret_cast<const uint4*>(x + i * 16);
-    row[i] = unpack_e4m3x4(u.x);
-    row[pieces + i] = unpack_e4m3x4(u.y);
-    row[2 * pieces + i] = unpack_e4m3x4(u.z);
-    row[3 * pieces + i] = unpack_e4m3x4(u.w);
+    const uint4 v = *reinterpret_cast<const uint4*>(x + i * 16);
+    row[i] = unpack_e4m3x4(v.x);
+    row[pieces + i] = unpack_e4m3x4(v.y);
+    row[2 * pieces + i] = unpack_e4m3x4(v.z);
+    row[3 * pieces + i] = unpack_e4m3x4(v.w);
   }
   const int band = first / E4M3_BLOCK, bands = (first + count - 1) / E4M3_BLOCK - band + 1;
   for (int i = threadIdx.x; i < bands * p.k_blocks; i += ROW_THREADS) {
@@ -876,9 +891,6 @@ block_row_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w, i
   }
   for (int i = threadIdx.x; i < count * ROW_WARPS; i += ROW_THREADS) parts[i / ROW_WARPS][i % ROW_WARPS] = 0.0f;
   __syncthreads();
-  // this warp's chunks of all features' together
-  const int all = count * chunks, begin = all * warp / ROW_WARPS, end = all * (warp + 1) / ROW_WARPS;
-  int feature = begin / chunks, chunk = begin % chunks;
   float sum = 0.0f;
   auto leave = [&](int f) {
     const float total = warp_sum(sum);
@@ -886,21 +898,16 @@ block_row_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w, i
     sum = 0.0f;
   };
   for (int at = begin; at < end; at += ROW_AHEAD) {
-    uint4 u[ROW_AHEAD];
-    int f = feature, c = chunk;
+    uint4 now[ROW_AHEAD];
 #pragma unroll
-    for (int i = 0; i < ROW_AHEAD; ++i) {
-      const int piece = c * 32 + lane;
-      const bool has = at + i < end && piece < pieces;
-      u[i] = has ? *reinterpret_cast<const uint4*>(w + static_cast<long long>(first + f) * K + piece * 16) : make_uint4(0, 0, 0, 0);
-      if (++c == chunks) c = 0, ++f;
-    }
+    for (int i = 0; i < ROW_AHEAD; ++i) now[i] = u[i];
+    fetch(u);
 #pragma unroll
     for (int i = 0; i < ROW_AHEAD; ++i) {
       if (at + i >= end) break;
       const int piece = chunk * 32 + lane;
       if (piece < pieces) {
-        const uint32_t word[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        const uint32_t word[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
         float2 a = both(0.0f), b = both(0.0f);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -1074,8 +1081,9 @@ extern "C" int ffm_linear_blocks_e4m3(const ffm_linear_blocks_args* args, ffm_st
   p.status_host = a.status_host;
   p.wait_cycles = gemm_wait_cycles();
   const bool grouped = a.ends != nullptr;
-  // One row: us, against a cluster a tile: 256 x 512 2.6 / 5.4, 2048 x 2048 3.6 / 5.9, 4096 x 4096 6.8 / 7.6, 5632 x 4096 8.4 / 8.4, 4096 x 7168 9.9 / 9.4.
-  if (!grouped && a.rows == 1 && a.K <= ROW_K_MAX && a.N * a.K <= 24ll << 20) {
+  // One row: us, against a cluster a tile: 256 x 512 2.9 / 5.4, 2048 x 2048 4.1 / 5.9, 4096 x 4096 6.9 / 7.6, 4096 x 7168 9.6 / 9.4 (weights not in L2: 11.2
+  // / 12.7), 14336 x 4096 15.7 / 14.0.
+  if (!grouped && a.rows == 1 && a.K <= ROW_K_MAX && a.N * a.K <= 32ll << 20) {
     if (off_16_bytes(a.x, a.w)) return FFM_ERR_UNSUPPORTED;
     return launch_row(a, p, static_cast<cudaStream_t>(stream));
   }

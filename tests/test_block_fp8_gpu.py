@@ -91,7 +91,7 @@ def _check(out, x, xs, w, ws):
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("rows,N,K", [(1, 1, 16), (1, 128, 128), (1, 4096, 7168), (3, 130, 144), (16, 64, 272), (17, 129, 256), (64, 500, 1040), (65, 256, 128),
                                       (128, 128, 128), (129, 127, 400), (300, 1000, 2064), (1000, 3001, 512), (4096, 2048, 1024), (200, 40000, 64),
-                                      (1, 3001, 2064), (1, 40000, 272), (1, 200000, 64), (1, 130, 16384), (1, 130, 16400), (1, 257, 528)])
+                                      (1, 3001, 2064), (1, 40000, 272), (1, 200000, 64), (1, 130, 16384), (1, 130, 16400), (1, 257, 528), (1, 14000, 4096), (2, 4096, 7168)])
 def test_dense(rows, N, K, dtype):
     x, xs, w, ws = _operands(rows, N, K)
     out = linear_e4m3(x, xs, w, ws, out_dtype=DTYPES[dtype])
