@@ -20,14 +20,13 @@ def _arguments(max_norm, norm_type):
 
 
 def _norm(grads, sharded, like, max_norm, largest, group):
-    capturing = like.is_cuda and torch.cuda.is_current_stream_capturing()
     native, other = _lib.native(), None
     if group is not None:
-        other = native.gradient_norm(sharded, like, 0.0, largest, None, capturing)[0][:1]
+        other = native.gradient_norm(sharded, like, 0.0, largest, None)[0][:1]
         dist.all_reduce(other, dist.ReduceOp.MAX if largest else dist.ReduceOp.SUM, group=group)
     else:
         grads = [*grads, *sharded]
-    return native.gradient_norm(grads, like, max_norm, largest, other, capturing)[1:]
+    return native.gradient_norm(grads, like, max_norm, largest, other)[1:]
 
 
 @torch.compiler.disable
@@ -60,8 +59,7 @@ def clip_grad_norm(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm, largest = _arguments(max_norm, norm_type)
     if group is None and not error_if_nonfinite:
-        capturing = bool(parameters) and parameters[0].is_cuda and torch.cuda.is_current_stream_capturing()
-        norm = _lib.native().clip_grad_norm(parameters, max_norm, largest, capturing)
+        norm = _lib.native().clip_grad_norm(parameters, max_norm, largest)
         return torch.zeros((), device=parameters[0].device if parameters else None) if norm is None else norm
     apart = {id(p) for p in sharded}
     if not apart <= {id(p) for p in parameters}:

@@ -996,7 +996,7 @@ struct ClipNorm {
 };
 
 // The norm of `grads` and of what `other` (float64 [1], a sum of squares or a magnitude) stands for
-ClipNorm norm_of(const ClipTable& table, const Tensor& like, const On& device, double max_norm, bool largest, const Tensor& other, bool capturing) {
+ClipNorm norm_of(const ClipTable& table, const Tensor& like, const On& device, double max_norm, bool largest, const Tensor& other) {
   ffm_grad_norm_args a = {};
   a.kind = largest ? 1 : 0;
   a.max_norm = max_norm;
@@ -1011,7 +1011,7 @@ ClipNorm norm_of(const ClipTable& table, const Tensor& like, const On& device, d
   a.coefficient = out.coefficient.data_ptr<float>();
   a.workspace = a.total + 1;
   a.workspace_bytes = doubles * 8;
-  const Tensor ticket = ticket_for(like, device.stream(), capturing);
+  const Tensor ticket = ticket_for(like, device.stream(), capture_id(device.stream()) != 0);
   a.ticket = ticket.data_ptr();
   int64_t launched = 0;
   a.launched = &launched;
@@ -1028,7 +1028,7 @@ void check_norm(const Tensors& grads, const Tensor& like, double max_norm) {
 }
 
 // (float64 [n] that begins with the total, norm, coefficient)
-py::tuple gradient_norm(const Tensors& grads, const Tensor& like, double max_norm, bool largest, const OptTensor& other, bool capturing) {
+py::tuple gradient_norm(const Tensors& grads, const Tensor& like, double max_norm, bool largest, const OptTensor& other) {
   check_norm(grads, like, max_norm);
   const On device(like);
   ClipTable table;
@@ -1039,7 +1039,7 @@ py::tuple gradient_norm(const Tensors& grads, const Tensor& like, double max_nor
     if (other->numel() != 1 || other->scalar_type() != at::kDouble) throw py::type_error("other must be one float64 value");
     more = other->resolve_neg();
   }
-  const ClipNorm r = norm_of(table, like, device, max_norm, largest, more, capturing);
+  const ClipNorm r = norm_of(table, like, device, max_norm, largest, more);
   return py::make_tuple(r.workspace, r.norm, r.coefficient);
 }
 
@@ -1059,18 +1059,18 @@ void scale_by(const Tensors& grads, const ClipTable& table, const Tensor& factor
   }
 }
 
-// Whether two of the tensors, or two elements of one, share memory: scaling in place would multiply twice.
+// Refuses tensors of which one, or two of which, share memory: scaling in place would multiply twice. What does not lie dense is scaled as a copy, made
+// before anything is, and so only once.
 void check_separate(const Tensors& grads) {
   std::vector<std::pair<const char*, const char*>> ranges;
   for (const Tensor& t : grads) {
     if (t.numel() == 0) continue;
-    int64_t last = 0;
     for (int64_t d = 0; d < t.dim(); ++d) {
       if (t.size(d) > 1 && t.stride(d) == 0) throw py::value_error("a gradient that was expanded cannot be scaled in place");
-      last += (t.size(d) - 1) * t.stride(d);
     }
+    if (!dense(t)) continue;
     const char* from = static_cast<const char*>(t.data_ptr());
-    ranges.emplace_back(from, from + (last + 1) * t.element_size());
+    ranges.emplace_back(from, from + t.numel() * t.element_size());
   }
   std::sort(ranges.begin(), ranges.end());
   const char* end = nullptr;
@@ -1092,7 +1092,7 @@ void scale_gradients_by(const Tensors& grads, const Tensor& factor) {
 }
 
 // The gradients of `parameters` scaled in place to a norm of max_norm at most: their norm, or nothing where there is no gradient
-OptTensor clip_grad_norm(const Tensors& parameters, double max_norm, bool largest, bool capturing) {
+OptTensor clip_grad_norm(const Tensors& parameters, double max_norm, bool largest) {
   Tensors grads;
   grads.reserve(parameters.size());
   for (const Tensor& p : parameters) {
@@ -1104,7 +1104,7 @@ OptTensor clip_grad_norm(const Tensors& parameters, double max_norm, bool larges
   const On device(grads[0]);
   ClipTable table;
   for (const Tensor& t : grads) table.add(t, grads[0], "grad");
-  const ClipNorm r = norm_of(table, grads[0], device, max_norm, largest, Tensor(), capturing);
+  const ClipNorm r = norm_of(table, grads[0], device, max_norm, largest, Tensor());
   scale_by(grads, table, r.coefficient, device);
   return r.norm;
 }

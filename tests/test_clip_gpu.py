@@ -84,6 +84,15 @@ def test_mixed_types_shapes_and_orders():
     assert torch.equal(base[:, 50:], untouched)
 
 
+def test_columns_of_one_buffer():
+    base = torch.randn(64, 96, device="cuda")
+    before, params = base.clone(), _params([base[:, :50], base[:, 50:]])
+    norm, coefficient = clip_coefficient([p.grad for p in params], 1.0)
+    _near(norm, _norm([before]), 5)
+    clip_grad_norm(params, 1.0)
+    assert torch.equal(base, before * coefficient)
+
+
 @pytest.mark.parametrize("dtype,scale", [("fp32", 1e25), ("bf16", 1e30), ("fp32", 1e-25), ("bf16", 1e-38), ("fp16", 6e-8), ("fp32", 1e-42)])
 def test_values_whose_squares_leave_fp32(dtype, scale):
     grads = [(torch.randn(5000, device="cuda").double() * scale).to(DTYPES[dtype])]

@@ -193,7 +193,7 @@ def test_calls_without_a_device_return_an_error(monkeypatch):
 class _OneRank:
     """A stand-in for the library's norm of a rank's own gradients, on host tensors: what a group adds up is tested without a GPU."""
 
-    def gradient_norm(self, grads, like, max_norm, largest, other, capturing):
+    def gradient_norm(self, grads, like, max_norm, largest, other):
         if largest:
             total = torch.stack([g.abs().max() for g in grads]).max().double() if grads else torch.zeros((), dtype=torch.float64)
             total = total if other is None else torch.maximum(total, other[0])

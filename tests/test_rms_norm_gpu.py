@@ -166,6 +166,17 @@ def test_gradients_of_some_inputs():
     x.requires_grad_()
     y = rms_norm(x)
     assert torch.equal(torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(rms_norm(x, torch.ones_like(w).detach()), x, dy)[0])
+    # without a weight, with a residual of which alone a gradient is asked for; the same tensor as both
+    x.requires_grad_(False), more.requires_grad_()
+    dy, dh, _ = _inputs(50, 384, torch.bfloat16, seed=2)
+    alone = torch.autograd.grad(rms_norm(x, residual=more), more, [dy, dh])[0]
+    ones = torch.ones_like(w).detach()
+    assert torch.equal(alone, torch.autograd.grad(rms_norm(x, ones, residual=more), more, [dy, dh])[0])
+    x.requires_grad_()
+    twice, = torch.autograd.grad(rms_norm(x, w.detach(), residual=x), x, [dy, dh])
+    again = x.detach().clone().requires_grad_()
+    once, = torch.autograd.grad(rms_norm(x, w.detach(), residual=again), x, [dy, dh])
+    assert torch.equal(twice, once + once)
     # an expanded gradient, and one that is not contiguous
     a = torch.autograd.grad(rms_norm(x, w).sum(), x)[0]
     assert torch.equal(a, torch.autograd.grad(rms_norm(x, w), x, torch.ones_like(x))[0])
