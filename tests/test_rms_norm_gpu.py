@@ -123,9 +123,11 @@ def test_8_bit_output_of_extreme_rows():
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("rows,dim", [(1, 1), (1, 4096), (3, 7), (5, 64), (2, 8192), (7, 1000), (700, 1024), (149, 2051), (3, 16384), (700, 127),
-                                      (1200, 520), (5000, 64), (600, 7168)])
+                                      (1200, 520), (5000, 64), (600, 7168), (400, 16384), (400, 9216), (5, 32768), (40, 12001)])
 @pytest.mark.parametrize("residual", [True, False])
 def test_gradients(rows, dim, dtype, residual):
+    if dtype == "fp32" and dim > 16384:
+        pytest.skip("fp32 rows end at 16384")
     x, more, w = _inputs(rows, dim, DTYPES[dtype], residual)
     dy, dh, _ = _inputs(rows, dim, DTYPES[dtype], seed=1)
     leaves = [t.requires_grad_() for t in (x, more, w) if t is not None]
