@@ -539,7 +539,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
 
 // The weights are streamed once and everything else should cost nothing: a tile loads and computes the boxes (of 16, 32 or 64 rows) that hold rows.
 // Bound by the weights' stream: 288 rows on 64 experts of 2816 x 2048 63 us (369 MB, 5.9 TB/s). A call of no size takes 5.4 us (launch, set-up, a
-// block's way through TMA, MMA and TMEM, the cluster's meeting), one row against 4096 x 7168 9.5.
+// block's way through TMA, MMA and TMEM, the cluster's meeting), two rows against 4096 x 7168 9.3.
 constexpr int FEW_ROWS = 64;
 
 // ONE: a cluster's CTAs share one tile's contraction, and so do the two groups of warps of each; else a CTA goes through tiles.
