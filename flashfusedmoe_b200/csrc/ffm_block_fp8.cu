@@ -19,19 +19,7 @@ namespace {
 // ---- quantising -------------------------------------------------------------------------------------------------
 
 constexpr int QB_THREADS = 256;
-constexpr int QB_GROUPS = 2;  // blocks of a row that a thread works on at once
-
-template <typename T>
-__device__ __forceinline__ void store_e4m3(uint8_t* to, const uint4& raw, float inverse) {
-  float v[VALUES<T>];
-  unpack<T>(raw, v);
-  const uint32_t low = pack_e4m3x4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
-  if constexpr (VALUES<T> == 8) {
-    *reinterpret_cast<uint2*>(to) = make_uint2(low, pack_e4m3x4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
-  } else {
-    *reinterpret_cast<uint32_t*>(to) = low;
-  }
-}
+constexpr int QB_CHUNKS = 2;  // of 16 bytes, of a block of a row, that a thread holds
 
 template <typename T>
 __device__ __forceinline__ float largest(const uint4& raw) {
@@ -42,45 +30,44 @@ __device__ __forceinline__ float largest(const uint4& raw) {
   return top;
 }
 
-// A scale for 128 values of a row: 16 (fp32: 32) neighbouring lanes hold a block, 16 bytes each. HBM-bound: 32768 x 7168 bf16 125 us (5.6 TB/s); with
-// two more blocks a thread 136, with a division for each of them 140.
+// A scale for 128 values of a row: eight (fp32: 16) neighbouring lanes hold a block, two chunks of 16 bytes each, which share what the scale costs.
+// HBM-bound: 32768 x 7168 bf16 125 us (5.7 TB/s), with 16 lanes a block and a chunk each 150; 61 x 7168 1.5 us in a graph.
 template <typename T>
 __global__ void __launch_bounds__(QB_THREADS)
 quantize_row_blocks_kernel(const T* __restrict__ x, long long stride, long long blocks, int across, int K, uint8_t* __restrict__ q,
                            float* __restrict__ scale) {
-  constexpr int V = VALUES<T>, LANES = E4M3_BLOCK / V, TEAMS = QB_THREADS / LANES;
+  constexpr int V = VALUES<T>, LANES = E4M3_BLOCK / V / QB_CHUNKS, TEAMS = QB_THREADS / LANES;
   const int t = threadIdx.x % LANES;
-  const long long first = static_cast<long long>(blockIdx.x) * (TEAMS * QB_GROUPS) + threadIdx.x / LANES;
-  const int rows_on = TEAMS / across, blocks_on = TEAMS % across;  // from one of a thread's blocks to the next
-  long long row = (first >> 32) == 0 ? static_cast<uint32_t>(first) / static_cast<uint32_t>(across) : first / across;
-  int block = static_cast<int>(first - row * across);
-  uint4 raw[QB_GROUPS];
-  long long out[QB_GROUPS];  // -1: past the row's end, or the last row
+  const long long at = static_cast<long long>(blockIdx.x) * TEAMS + threadIdx.x / LANES;
+  const long long row = (at >> 32) == 0 ? static_cast<uint32_t>(at) / static_cast<uint32_t>(across) : at / across;
+  const int first = static_cast<int>(at - row * across) * E4M3_BLOCK + t * V;
+  bool has[QB_CHUNKS];  // in the row, and the row there
+  uint4 raw[QB_CHUNKS];
 #pragma unroll
-  for (int i = 0; i < QB_GROUPS; ++i) {
-    const int col = block * E4M3_BLOCK + t * V;
-    const bool has = first + i * TEAMS < blocks && col < K;
-    raw[i] = has ? *reinterpret_cast<const uint4*>(x + row * stride + col) : make_uint4(0, 0, 0, 0);
-    out[i] = has ? row * K + col : -1;
-    row += rows_on;
-    block += blocks_on;
-    if (block >= across) block -= across, ++row;
+  for (int c = 0; c < QB_CHUNKS; ++c) {
+    const int col = first + c * LANES * V;
+    has[c] = at < blocks && col < K;
+    raw[c] = has[c] ? *reinterpret_cast<const uint4*>(x + row * stride + col) : make_uint4(0, 0, 0, 0);
   }
+  float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < QB_GROUPS; ++i) {
-    float top = largest<T>(raw[i]);
+  for (int c = 0; c < QB_CHUNKS; ++c) top = fmaxf(top, largest<T>(raw[c]));
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float s = e4m3_scale(top);
-    if (out[i] >= 0) {
-      store_e4m3<T>(q + out[i], raw[i], reciprocal(s));
-      if (t == 0) scale[first + i * TEAMS] = s;
+  for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float2 v[1][QB_CHUNKS * V / 2];
+#pragma unroll
+  for (int c = 0; c < QB_CHUNKS; ++c) unpack2<T>(raw[c], reinterpret_cast<float2(&)[V / 2]>(v[0][c * V / 2]));
+  quantize_chunks(v, {top}, [&](int, const uint32_t(&word)[QB_CHUNKS * V / 4], float s) {
+#pragma unroll
+    for (int c = 0; c < QB_CHUNKS; ++c) {
+      if (has[c]) store_words(q + row * K + first + c * LANES * V, reinterpret_cast<const uint32_t(&)[V / 4]>(word[c * V / 4]));
     }
-  }
+    if (t == 0 && has[0]) scale[at] = s;
+  });
 }
 
-// A scale for 128 x 128 values of a matrix: one thread block for each, its values in registers in between. Three blocks of 16-bit values on an SM: with
-// two 8 x 14336 x 4096 bf16 took 261 us, with four, which spill, 226; three 214 (6.6 TB/s).
+// A scale for 128 x 128 values of a matrix: one thread block for each, its values in registers in between. Three blocks of 16-bit values on an SM:
+// 8 x 14336 x 4096 bf16 219 us (6.4 TB/s); with products in place of quotients three took 214, two 261, and four, which spill, 226.
 template <typename T>
 __global__ void __launch_bounds__(QB_THREADS, sizeof(T) == 2 ? 3 : 2)
 quantize_tiles_kernel(const T* __restrict__ x, int N, int K, int down, int across, uint8_t* __restrict__ q, float* __restrict__ scale) {
@@ -103,11 +90,28 @@ quantize_tiles_kernel(const T* __restrict__ x, int N, int K, int down, int acros
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < QB_THREADS / 32; ++w) top = fmaxf(top, part[w]);
-  const float s = e4m3_scale(top), inverse = reciprocal(s);
-  if (threadIdx.x == 0) scale[tile] = s;
+  auto store = [&](int i, const uint4& u, auto&& pack) {
+    float2 v[V / 2];
+    unpack2<T>(u, v);
+    uint32_t word[V / 4];
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    if (i * TEAMS < left) store_e4m3<T>(q + first + i * step, raw[i], inverse);
+    for (int j = 0; j < V / 4; ++j) word[j] = pack(v[2 * j], v[2 * j + 1]);
+    store_words(q + first + i * step, word);
+  };
+  if (e4m3_by_division(top)) {
+    const float s = e4m3_scale_divided(top);
+    if (threadIdx.x == 0) scale[tile] = s;
+#pragma unroll 1
+    for (int i = 0; i < STEPS && i * TEAMS < left; ++i) {  // rare: read again, so that it takes no registers from the other way
+      store(i, *reinterpret_cast<const uint4*>(x + first + i * step), [&](float2 a, float2 b) { return pack_divided(a, b, s); });
+    }
+  } else {
+    const float s = e4m3_scale(top), y = -reciprocal(s);
+    if (threadIdx.x == 0) scale[tile] = s;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (i * TEAMS < left) store(i, raw[i], [&](float2 a, float2 b) { return pack_quotients(a, b, s, y); });
+    }
   }
 }
 
@@ -1038,7 +1042,7 @@ extern "C" int ffm_quantize_blocks_e4m3(const void* x, int x_type, int64_t matri
   if (off_16_bytes(x) || (row_stride * type_bytes(x_type)) % 16 != 0 || (reinterpret_cast<uintptr_t>(q) & 7u) != 0) return FFM_ERR_UNSUPPORTED;
   const int across = (K + E4M3_BLOCK - 1) / E4M3_BLOCK, down = static_cast<int>((rows + block_rows - 1) / block_rows);
   const long long blocks = block_rows == 1 ? rows * across : matrices * down * across;
-  const int per = block_rows == 1 ? QB_GROUPS * QB_THREADS / (x_type == FFM_TYPE_FP32 ? 32 : 16) : 1;
+  const int per = block_rows == 1 ? QB_CHUNKS * QB_THREADS / (x_type == FFM_TYPE_FP32 ? 32 : 16) : 1;
   const long long grid = (blocks + per - 1) / per;
   if (grid > 0x7fffffffll) return FFM_ERR_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -52,25 +52,26 @@ __device__ __forceinline__ void store_packed(T* p, const Place<T, VEC>& at, int 
   }
 }
 
-// y of a chunk as e4m3, and the scale of the block of 128 columns that 16 (fp32: 32) neighbouring lanes hold; `has` is not the same for all of them
-// where the row ends inside
-template <typename T>
-__device__ __forceinline__ void store_e4m3(const float (&v)[VALUES<T>], bool has, int col, uint8_t* y, float* y_scale) {
+// y of a thread's chunks as e4m3, and the scales of the blocks of 128 columns that 16 (fp32: 32) neighbouring lanes hold; chunks from `chunks` on are past
+// the row's end, which may lie inside a block
+template <typename T, int CH>
+__device__ __forceinline__ void store_e4m3(const float2 (&v)[CH][VALUES<T> / 2], int chunks, const Place<T, true>& at, uint8_t* y, float* y_scale) {
   constexpr int V = VALUES<T>;
-  float top = 0.0f;
+  float top[CH];
 #pragma unroll
-  for (int j = 0; j < V; ++j) top = fmaxf(top, has ? fabsf(v[j]) : 0.0f);
+  for (int c = 0; c < CH; ++c) {
+    top[c] = 0.0f;
 #pragma unroll
-  for (int o = E4M3_BLOCK / V / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float scale = e4m3_scale_near(top), inverse = reciprocal(scale);
-  if (!has) return;
-  const uint32_t low = pack_e4m3x4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse);
-  if constexpr (V == 8) {
-    *reinterpret_cast<uint2*>(y + col) = make_uint2(low, pack_e4m3x4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
-  } else {
-    *reinterpret_cast<uint32_t*>(y + col) = low;
+    for (int j = 0; j < V / 2; ++j) top[c] = fmaxf(top[c], c < chunks ? fmaxf(fabsf(v[c][j].x), fabsf(v[c][j].y)) : 0.0f);
+#pragma unroll
+    for (int o = E4M3_BLOCK / V / 2; o > 0; o >>= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
   }
-  if (col % E4M3_BLOCK == 0) y_scale[col / E4M3_BLOCK] = scale;
+  quantize_chunks(v, top, [&](int c, const uint32_t(&word)[V / 4], float s) {
+    if (c >= chunks) return;
+    const int col = at.column(c, 0);
+    store_words(y + col, word);
+    if (col % E4M3_BLOCK == 0) y_scale[col / E4M3_BLOCK] = s;
+  });
 }
 
 // A team of threads for every row, each holding CH chunks of 16 bytes in registers. E4M3: y and y_scale [rows, ceil(D / 128)] instead of y in T;
@@ -116,6 +117,7 @@ rms_norm_forward_kernel(const T* __restrict__ x, long long x_stride, const T* __
     stay_packed(raw);
     const float r = rsqrtf(s[0] / static_cast<float>(D) + eps);
     if (rstd != nullptr && at.t == 0 && row < rows) rstd[row] = r;
+    [[maybe_unused]] float2 pairs[E4M3 ? CH : 1][V / 2];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       float v[V], w[V];
@@ -131,10 +133,11 @@ rms_norm_forward_kernel(const T* __restrict__ x, long long x_stride, const T* __
       if constexpr (!E4M3) {
         store_chunk(static_cast<T*>(y) + row * D, at, c, v);
       } else {
-        const int across = (D + E4M3_BLOCK - 1) / E4M3_BLOCK;
-        store_e4m3<T>(v, at.has(c, 0), at.column(c, 0), static_cast<uint8_t*>(y) + row * D, y_scale + row * across);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) pairs[c][j] = make_float2(v[2 * j], v[2 * j + 1]);
       }
     }
+    if constexpr (E4M3) store_e4m3<T, CH>(pairs, at.count, at, static_cast<uint8_t*>(y) + row * D, y_scale + row * ((D + E4M3_BLOCK - 1) / E4M3_BLOCK));
   }
 }
 
@@ -343,6 +346,7 @@ rms_norm_forward_stream_kernel(const T* __restrict__ x, long long x_stride, cons
     own_team_sum<1>(s, team, part[parity]);
     const float r = rsqrtf(fmaf(s[0], inv, eps));
     if (rstd != nullptr && at.t == 0 && chunks > 0) rstd[row] = r;
+    [[maybe_unused]] float2 pairs[E4M3 ? CH : 1][V / 2];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       float2 v[V / 2], w[V / 2];
@@ -351,14 +355,13 @@ rms_norm_forward_stream_kernel(const T* __restrict__ x, long long x_stride, cons
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) v[j] = mul2(mul2(v[j], both(r)), w[j]);
       if constexpr (E4M3) {
-        float f[V];
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j) f[2 * j] = v[j].x, f[2 * j + 1] = v[j].y;
-        store_e4m3<T>(f, c < chunks, at.column(c, 0), static_cast<uint8_t*>(y) + row * D, y_scale + row * across);
+        for (int j = 0; j < V / 2; ++j) pairs[c][j] = v[j];
       } else {
         if (c < chunks) store2<T>(static_cast<T*>(y) + row * D + at.column(c, 0), v);
       }
     }
+    if constexpr (E4M3) store_e4m3<T, CH>(pairs, chunks, at, static_cast<uint8_t*>(y) + row * D, y_scale + row * across);
   }
   copy_async_wait<0>();
 }

@@ -11,7 +11,8 @@ def quantize_e4m3(x, block_rows=1):
 
     block_rows = 1 (activations): a scale for 128 values of a row, scales [*, ceil(K / 128)]. block_rows = 128 (weights): x is [*, N, K] and
     a scale serves 128 x 128 values, scales [*, ceil(N / 128), ceil(K / 128)]. Blocks at the ends may be smaller. The scale is the block's
-    largest magnitude / 448, at least 2^-126, and 1 for a block of zeros. NaN values stay NaN and do not count for the scale; a block with an
+    largest magnitude / 448, at least 2^-126, and 1 for a block of zeros, and the values are (x / scale).to(torch.float8_e4m3fn), both quotients
+    rounded as fp32 division rounds them. NaN values stay NaN and do not count for the scale; a block with an
     infinity has an infinite scale and stands for NaN throughout.
 
     x: a CUDA tensor in bfloat16, float16 or float32, K a multiple of 16; what is not contiguous (block_rows = 1: whose rows are not) is

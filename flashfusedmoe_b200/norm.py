@@ -25,8 +25,8 @@ def rms_norm(x, weight=None, eps=1e-6, *, residual=None, weight_offset=0.0, quan
     Without a residual h is x, and the result is y. With one (of x's shape and type) the sum is rounded to x's type, and the result is
     (y, h): h is the residual stream to hand on. weight_offset = 1 is for weights that are stored less 1.
 
-    quantize=True makes y the operand of linear_e4m3(): float8_e4m3fn values and a float32 scale for every 128 columns, rounded once from fp32;
-    the result is (values, scales) or (values, scales, h). D is a multiple of 16 then, and the call is not differentiable.
+    quantize=True makes y the operand of linear_e4m3(): float8_e4m3fn values and a float32 scale for every 128 columns, those of
+    quantize_e4m3() for y in fp32; the result is (values, scales) or (values, scales, h). D is a multiple of 16 then, and the call is not differentiable.
 
     x, residual and weight [D] (None: 1) are CUDA tensors in bfloat16, float16 or float32, the weight in its own; y and h have x's type and
     shape and are contiguous. Everything between is fp32. D is any number up to 32768 (float32: 16384). The rows of x and residual may be further

@@ -616,7 +616,7 @@ int ffm_scale_many(int count, void* const* x, const int64_t* types, const int64_
  *
  * ffm_rms_norm_forward reads x, residual, weight and writes h (with a residual), rstd (f32 [rows], null: not wanted: 1 / sqrt(...)) and y; with
  *   y_scale (f32 [rows, ceil(D / 128)]) y is e4m3 [rows, D]: y over the scale of its 128 columns, which is their largest magnitude / 448,
- *   at least 2^-126 (1 where all are zero). D % 16 == 0 and addresses and rows on 16 bytes then.
+ *   at least 2^-126 (1 where all are zero); both quotients are rounded as fp32 division rounds them. D % 16 == 0 and addresses and rows on 16 bytes then.
  * ffm_rms_norm_backward reads dy, dh (null: none), x (the forward pass's h, rows x_stride apart), rstd and weight, and writes dx (null: not
  *   wanted; the gradient of x and of residual, dh added) and dweight (null: not wanted; summed in fp32 in a fixed order).
  *   workspace: ffm_rms_norm_workspace_bytes, needed with dweight. rows == 0 gives zero sums.
@@ -655,6 +655,7 @@ int ffm_rms_norm_backward(const ffm_rms_norm_args* args, ffm_stream_t stream);
  * ffm_quantize_blocks_e4m3: x [matrices, rows, K] (FFM_TYPE_*) to q and scale. block_rows = 1: a scale for 128 values of a row, [rows,
  *   ceil(K / 128)], matrices = 1, rows row_stride elements apart; block_rows = 128: one for 128 x 128 values, [matrices, ceil(rows / 128),
  *   ceil(K / 128)], x contiguous. The scale is the largest magnitude / 448, at least 2^-126 (1 where all are zero); NaN values do not count.
+ *   q is x / scale; both quotients are rounded as fp32 division rounds them.
  * ffm_linear_blocks_e4m3: out [rows, N] (out_type) = x [rows, K] w[e] [N, K]^T with x_scale [rows, ceil(K / 128)] and w_scale [experts,
  *   ceil(N / 128), ceil(K / 128)]; e is the expert with ends[e - 1] <= row < ends[e], rows from the last end on are 0. ends null: experts
  *   = 1 takes all rows. ends (int32 on the device) must not decrease nor pass rows: such ends are moved into place and set

@@ -67,6 +67,26 @@ def test_quantize_extremes_and_strides():
         assert values.shape == shape and scale.numel() == 0
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("block_rows,rows,K", [(1, 61, 7168), (1, 3000, 272), (128, 300, 2064)])
+def test_codes_are_the_rounded_quotients(block_rows, rows, K, dtype):
+    """Values halfway between two e4m3 numbers, which 16-bit inputs often are, go to the even one: the codes are those of the quotient in fp32."""
+    x = torch.randn(rows, K).to(DTYPES[dtype])
+    # k m with k halfway between two e4m3 numbers, against a scale of m: a rounded 1 / m puts some of them on the other side
+    halfway = torch.tensor([17.0 + 2 * i for i in range(8)] + [34.0 + 4 * i for i in range(8)] + [0.5 + i for i in range(8)])
+    for i, m in enumerate((7.0, 13.0, 15.0, 61.0, 63.0)):
+        at = slice(128 * (i % 2), 128 * (i % 2) + 128)
+        where = i // 2 * block_rows
+        x[where:where + block_rows, at] = 0
+        x[where, at.start:at.start + 24] = (halfway * m).to(x.dtype)
+        x[where, at.start + 24:at.start + 48] = (-halfway * m).to(x.dtype)
+        x[where, at.start + 127] = 448 * m
+    values, scale = quantize_e4m3(x.cuda(), block_rows)
+    spread = _spread(scale.cpu(), block_rows, x.shape).float()
+    assert [float(scale[i // 2, i % 2]) for i in range(5)] == [7.0, 13.0, 15.0, 61.0, 63.0]
+    assert torch.equal(values.cpu().view(torch.uint8), (x.float() / spread).to(torch.float8_e4m3fn).view(torch.uint8))
+
+
 def _operands(rows, N, K, experts=None, seed=0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     x = torch.randn(rows, K, device="cuda", generator=g) * (0.2 + 3 * torch.rand(rows, 1, device="cuda", generator=g))
@@ -86,6 +106,51 @@ def _check(out, x, xs, w, ws):
     bound = bound * (1 + half) + half * want.abs() + torch.finfo(out.dtype).tiny * torch.finfo(out.dtype).eps
     off = (out.double() - want).abs()
     assert out.shape == want.shape and bool((off <= bound).all()), float((off / bound).nan_to_num(0).max())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("block_rows,rows,K", [(1, 61, 7168), (1, 3000, 272), (128, 300, 2064)])
+def test_codes_are_the_rounded_quotients(block_rows, rows, K, dtype):
+    """Values halfway between two e4m3 numbers, which 16-bit inputs often are, go to the even one: the codes are those of the quotient in fp32."""
+    x = torch.randn(rows, K).to(DTYPES[dtype])
+    # k m with k halfway between two e4m3 numbers, against a scale of m: a rounded 1 / m puts some of them on the other side
+    halfway = torch.tensor([17.0 + 2 * i for i in range(8)] + [34.0 + 4 * i for i in range(8)] + [0.5 + i for i in range(8)])
+    for i, m in enumerate((7.0, 13.0, 15.0, 61.0)):
+        row, col = i // 2 * block_rows, i % 2 * 128
+        x[row:row + block_rows, col:col + 128] = 0
+        x[row, col:col + 24] = (halfway * m).to(x.dtype)
+        x[row, col + 24:col + 48] = (-halfway * m).to(x.dtype)
+        x[row, col + 127] = 448 * m
+    values, scale = quantize_e4m3(x.cuda(), block_rows)
+    spread = _spread(scale.cpu(), block_rows, x.shape).float()
+    assert spread[0, 0] == 7.0 and spread[0, 128] == 13.0 and spread[block_rows, 0] == 15.0
+    assert torch.equal(values.cpu().view(torch.uint8), (x.float() / spread).to(torch.float8_e4m3fn).view(torch.uint8))
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_codes_beside_borders_at_all_scales(block_rows):
+    """Values at, one step above and one below the borders between e4m3 numbers, for scales of every size: the codes of a division all the same."""
+    g = torch.Generator().manual_seed(0)
+    rows = 20000 if block_rows == 1 else 300
+    scale = (1 + torch.rand(rows, generator=g)) * torch.exp2(torch.randint(-126, 119, (rows,), generator=g).float())
+    # mantissas at which quotients come closest to the middle between two fp32 numbers
+    near = torch.arange(8, 16).repeat_interleave(33) * 2 ** 20 + torch.arange(-16, 17).repeat(8)
+    near = near[near >= 2 ** 23].float()
+    scale[:near.numel()] = (near * torch.exp2(torch.randint(-80, 80, (near.numel(),), generator=g).float()))[:rows]
+    scale[-8:] = torch.tensor([2.0 ** -126, 1e-38, 2.0 ** -80, 2.0 ** -79, 2.0 ** -79 * 1.5, 7e35, 2.0 ** -149, 0.0])
+    top = (448 * scale).clamp(max=3.4e38)
+    scale = torch.where(top > 0, (top / 448).clamp(min=2.0 ** -126), 1.0)
+    border = torch.arange(16, 32).float() / 16 * torch.exp2(torch.randint(-10, 8, (rows, 16), generator=g).float()) * scale[:, None]
+    x = torch.cat([border, torch.nextafter(border, border * 2), torch.nextafter(border, border * 0)], 1)
+    x = torch.cat([x, -x, torch.zeros(rows, 1), -torch.zeros(rows, 1), torch.rand(rows, 29, generator=g) * top[:, None], top[:, None]], 1)
+    x = torch.minimum(torch.maximum(x, -top[:, None]), top[:, None])
+    if block_rows == 128:   # a block for each
+        x, where = torch.zeros(rows * 128, 128), x
+        x[torch.arange(rows) * 128 + torch.arange(rows) % 128] = where
+        scale = scale.repeat_interleave(128)
+    values, got = quantize_e4m3(x.cuda(), block_rows)
+    assert torch.equal(got.cpu().view(-1), scale[::block_rows])
+    assert torch.equal(values.cpu().view(torch.uint8), (x / scale[:, None]).to(torch.float8_e4m3fn).view(torch.uint8))
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))

@@ -107,6 +107,23 @@ def test_8_bit_output(rows, dim, dtype):
     assert bool((off <= torch.maximum(2.0 ** -4 * y.abs(), 2.0 ** -10 * over) * (1 + 2.0 ** -10) + C * y.abs()).all())
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows", [5, 6000])
+def test_8_bit_codes_are_the_rounded_quotients(rows, dtype):
+    """h = k / 256 with whole k, and eps such that the root is 1: y = k m / 256 and the scale m / 256 are exact. k halfway between two e4m3 numbers
+    goes to the even one, and a scale or a reciprocal that is a rounding off would put some of them on the other side."""
+    half = [17 + 2 * i for i in range(8)] + [34 + 4 * i for i in range(8)] + [68 + 8 * i for i in range(8)] + [136 + 16 * i for i in range(8)]
+    half = torch.tensor(half + [448] + [3] * 95, dtype=torch.float32)
+    g = torch.Generator().manual_seed(0)
+    k = torch.stack([half[torch.rand(rows, 128, generator=g).argsort(1)] for _ in range(2)], 1).view(rows, 256)
+    k *= torch.where(torch.rand(rows, 256, generator=g) < 0.5, -1.0, 1.0)
+    eps = 1.0 - float(2 * half.double().square().sum()) * 2.0 ** -24
+    for m in (7.0, 13.0, 15.0, 61.0):
+        values, scale = rms_norm((k / 256).to(DTYPES[dtype]).cuda(), torch.full((256,), m, device="cuda"), eps, quantize=True)
+        assert bool((scale == m / 256).all())
+        assert torch.equal(values.cpu().view(torch.uint8), k.to(torch.float8_e4m3fn).view(torch.uint8))
+
+
 def test_8_bit_output_of_extreme_rows():
     w = torch.ones(256, device="cuda")
     x = torch.randn(4, 256, device="cuda")
