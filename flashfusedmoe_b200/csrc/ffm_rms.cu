@@ -436,7 +436,7 @@ rms_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict__ 
     float s[1] = {s2.x + s2.y};
     own_team_sum<1>(s, team, part[parity]);
     const int chunks = dx != nullptr && k < mine ? at.count : 0;  // to write
-    const float2 c2 = both(-r * r * (s[0] * inv));
+    const float2 c2 = both(-r * (s[0] * inv));  // times v r: r^2 leaves fp32 where rows are below 2^-64 and eps is 0
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       float2 v[V / 2], g[V / 2], w[V / 2];
@@ -444,7 +444,7 @@ rms_norm_backward_stream_kernel(const T* __restrict__ dy, const T* __restrict__ 
       unpack2<T>(read_shared_16(here + (CH + c) * slot), g);
       read_weight<T>(my_scale, c, team, w);
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) v[j] = fma2(v[j], c2, mul2(mul2(g[j], w[j]), both(r)));
+      for (int j = 0; j < V / 2; ++j) v[j] = fma2(mul2(v[j], both(r)), c2, mul2(mul2(g[j], w[j]), both(r)));
       if (DH) {
         unpack2<T>(read_shared_16(here + (2 * CH + c) * slot), g);
 #pragma unroll

@@ -165,6 +165,29 @@ def test_gradients(rows, dim, dtype, residual):
         _close(got[-1], each.sum(0), each.abs().sum(0) * (rows + 128) / 128)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [6, 25000])
+@pytest.mark.parametrize("residual", [True, False])
+def test_gradients_of_tiny_rows(rows, dtype, residual):
+    """Rows of whole multiples of 2^-66, whose squares are exact sums in fp32, without eps: the root's inverse is about 2^66, its square is infinite."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = (torch.randint(-2, 3, (rows, 256), device="cuda", generator=g) * 2.0 ** -66).to(DTYPES[dtype])
+    more = torch.zeros_like(x) if residual else None
+    _, _, w = _inputs(1, 256, DTYPES[dtype])
+    dy, _, _ = _inputs(rows, 256, DTYPES[dtype], seed=1)
+    x.requires_grad_(), w.requires_grad_()
+    out = rms_norm(x, w, 0.0, residual=more)
+    got = torch.autograd.grad(out, [x, w], [dy, torch.zeros_like(dy)] if residual else dy)
+    with torch.no_grad():
+        _, xh, y, r = _formula(x, None, w, 0.0)
+        _close(out[0] if residual else out, y)
+        g = dy.double() * w.double()
+        dx = r * (g - xh * (g * xh).mean(-1, keepdim=True))
+        _close(got[0], dx, r * (g.abs() + xh.abs() * (g * xh).abs().mean(-1, keepdim=True)))
+        each = dy.double() * xh
+        _close(got[1], each.sum(0), each.abs().sum(0) * (rows + 128) / 128)
+
+
 def test_gradients_of_some_inputs():
     x, more, w = _inputs(50, 384, torch.bfloat16)
     dy, dh, _ = _inputs(50, 384, torch.bfloat16, seed=1)
