@@ -23,7 +23,13 @@ def _norm(grads, sharded, like, max_norm, largest, group):
     native, other = _lib.native(), None
     if group is not None:
         other = native.gradient_norm(sharded, like, 0.0, largest, None)[0][:1]
-        dist.all_reduce(other, dist.ReduceOp.MAX if largest else dist.ReduceOp.SUM, group=group)
+        if largest:
+            # MAX of numbers drops a NaN of another rank. As whole numbers the bits of magnitudes compare as those do, and NaN is above all.
+            bits = other.view(torch.int64) & 0x7fffffffffffffff
+            dist.all_reduce(bits, dist.ReduceOp.MAX, group=group)
+            other = bits.view(torch.float64)
+        else:
+            dist.all_reduce(other, dist.ReduceOp.SUM, group=group)
     else:
         grads = [*grads, *sharded]
     return native.gradient_norm(grads, like, max_norm, largest, other)[1:]

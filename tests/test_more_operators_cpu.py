@@ -237,3 +237,40 @@ def test_sharded_gradients_are_added_up_over_the_group():
     for r in ranks:
         r.join(120)
     assert [r.exitcode for r in ranks] == [0, 0] and sorted(out.get() for _ in ranks) == [0, 1]
+
+
+def _rank_with_nan(rank, port, out):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.distributed.init_process_group("gloo", rank=rank, world_size=2)
+    _lib._native = _OneRank()
+    _lib.native = lambda: _lib._native
+    group = torch.distributed.group.WORLD
+    for kind in (2.0, float("inf")):
+        for bad in (0, 1):
+            for value in (float("nan"), float("inf")):
+                dense = torch.tensor([1.0])
+                expert = torch.tensor([3.0, -value if rank == bad else 2.0])   # a negative NaN, where there is a sign
+                norm, coefficient = clip_coefficient([dense], 1.0, kind, sharded=[expert], group=group)
+                assert bool(norm.isnan() if value != value else norm.isinf()), (kind, bad, value, norm)
+                assert bool(coefficient.isnan()) if value != value else float(coefficient) == 0.0
+                p, q = torch.nn.Parameter(torch.zeros(1)), torch.nn.Parameter(torch.zeros(2))
+                p.grad, q.grad = dense, expert
+                try:
+                    clip_grad_norm([p, q], 1.0, kind, error_if_nonfinite=True, sharded=[q], group=group)
+                except RuntimeError as e:
+                    assert "not finite" in str(e)
+                else:
+                    raise AssertionError("no error")
+    out.put(rank)
+    torch.distributed.destroy_process_group()
+
+
+def test_a_nan_of_one_rank_reaches_all():
+    context = multiprocessing.get_context("spawn")
+    out, port = context.Queue(), 29900 + os.getpid() % 90
+    ranks = [context.Process(target=_rank_with_nan, args=(r, port, out)) for r in range(2)]
+    for r in ranks:
+        r.start()
+    for r in ranks:
+        r.join(120)
+    assert [r.exitcode for r in ranks] == [0, 0] and sorted(out.get() for _ in ranks) == [0, 1]
