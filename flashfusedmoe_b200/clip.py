@@ -19,6 +19,11 @@ def _arguments(max_norm, norm_type):
     return max_norm, _KINDS[norm_type]
 
 
+def _nothing():
+    """Stands for the gradients of a rank that has none, on its current device."""
+    return torch.empty(0, device="cuda")
+
+
 def _norm(grads, sharded, like, max_norm, largest, group):
     native, other = _lib.native(), None
     if group is not None:
@@ -44,13 +49,13 @@ def clip_coefficient(grads, max_norm, norm_type=2.0, *, sharded=(), group=None):
     CUDA tensors of one device in bfloat16, float16 or float32, in any order of their dimensions (others are copied). Sums are in
     64 bits and in a fixed order. sharded: gradients of which every rank of `group` has others, as of experts under expert parallelism
     (MoELayer.expert_params); their part of the norm is all-reduced over `group`, so every rank calls with as many tensors of its own as it
-    has, and gets the same norm. Without a group they count as the others. Everything runs on the current stream without a host wait and can be
+    has, none included, and gets the same norm. Without a group they count as the others. Everything runs on the current stream without a host wait and can be
     captured."""
     grads, sharded = [grads] if isinstance(grads, torch.Tensor) else list(grads), list(sharded)
     max_norm, largest = _arguments(max_norm, norm_type)
-    if not grads and not sharded:
+    if not grads and not sharded and group is None:
         raise ValueError("there are no gradients")
-    return _norm(grads, sharded, (grads + sharded)[0], max_norm, largest, group)
+    return _norm(grads, sharded, (grads + sharded or [_nothing()])[0], max_norm, largest, group)
 
 
 @torch.compiler.disable
@@ -74,9 +79,9 @@ def clip_grad_norm(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False
     grads = [p.grad for p in with_grad if id(p) not in apart]
     local = [p.grad for p in with_grad if id(p) in apart]
     every = [*grads, *local]
-    if not every and (group is None or not parameters):
+    if not every and group is None:
         return torch.zeros((), device=parameters[0].device if parameters else None)
-    norm, coefficient = _norm(grads, local, (every or parameters)[0], max_norm, largest, group)
+    norm, coefficient = _norm(grads, local, (every or parameters or [_nothing()])[0], max_norm, largest, group)
     if error_if_nonfinite and not bool(torch.isfinite(norm)):
         raise RuntimeError("The norm of the gradients is not finite, so they cannot be clipped by it")
     _lib.native().scale_gradients(every, coefficient)

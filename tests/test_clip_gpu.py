@@ -204,6 +204,26 @@ def test_sharded_gradients_over_a_group_of_one():
         dist.destroy_process_group()
 
 
+def test_a_group_of_one_without_gradients_and_with_a_nan():
+    import torch.distributed as dist
+    if dist.is_initialized():
+        pytest.skip("a process group is there")
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT="29543")
+    dist.init_process_group("nccl", rank=0, world_size=1, device_id=torch.device("cuda", 0))
+    try:
+        group = dist.group.WORLD
+        for kind in (2.0, INF):
+            norm, coefficient = clip_coefficient([], 1.0, kind, group=group)
+            assert float(norm) == 0.0 and float(coefficient) == 1.0
+            assert float(clip_grad_norm([], 1.0, kind, group=group)) == 0.0
+            bad = torch.ones(3000, device="cuda")
+            bad[1234] = float("nan")
+            norm, coefficient = clip_coefficient([torch.ones(5, device="cuda")], 1.0, kind, sharded=[-bad], group=group)
+            assert bool(norm.isnan()) and bool(coefficient.isnan())
+    finally:
+        dist.destroy_process_group()
+
+
 def test_a_training_step():
     """Norm, layer, loss, clipping and the optimizer's step as a user runs them: the coefficient handed to AdamW is clipping in place."""
     def build():

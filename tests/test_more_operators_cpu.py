@@ -2,13 +2,14 @@
 host, arguments of the C entry points."""
 
 import ctypes
+import datetime
 import multiprocessing
 import os
 
 import pytest
 import torch
 
-from flashfusedmoe_b200 import MoELayer, RMSNorm, _lib, clip_coefficient, clip_grad_norm, linear_e4m3, quantize_e4m3, rms_norm
+from flashfusedmoe_b200 import MoELayer, RMSNorm, _lib, clip, clip_coefficient, clip_grad_norm, linear_e4m3, quantize_e4m3, rms_norm
 
 BAD, UNSUPPORTED, WORKSPACE = -1, -2, -4
 BF16, FP16, FP32 = 0, 1, 2
@@ -269,6 +270,35 @@ def test_a_nan_of_one_rank_reaches_all():
     context = multiprocessing.get_context("spawn")
     out, port = context.Queue(), 29900 + os.getpid() % 90
     ranks = [context.Process(target=_rank_with_nan, args=(r, port, out)) for r in range(2)]
+    for r in ranks:
+        r.start()
+    for r in ranks:
+        r.join(120)
+    assert [r.exitcode for r in ranks] == [0, 0] and sorted(out.get() for _ in ranks) == [0, 1]
+
+
+def _rank_without_any(rank, port, out):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.distributed.init_process_group("gloo", rank=rank, world_size=2, timeout=datetime.timedelta(seconds=30))
+    _lib._native = _OneRank()
+    _lib.native = lambda: _lib._native
+    clip._nothing = lambda: torch.empty(0)   # the device's
+    group = torch.distributed.group.WORLD
+    p = torch.nn.Parameter(torch.zeros(2))
+    p.grad = torch.tensor([3.0, 4.0])
+    mine = [p] if rank == 0 else []
+    for kind, want in ((2.0, 5.0), (float("inf"), 4.0)):
+        norm, coefficient = clip_coefficient([], 1.0, kind, sharded=[q.grad for q in mine], group=group)
+        assert abs(float(norm) - want) < 1e-5 and abs(float(coefficient) - 1 / want) < 1e-5
+    assert abs(float(clip_grad_norm(mine, 10.0, sharded=mine, group=group)) - 5.0) < 1e-5
+    out.put(rank)
+    torch.distributed.destroy_process_group()
+
+
+def test_a_rank_without_gradients_takes_part():
+    context = multiprocessing.get_context("spawn")
+    out, port = context.Queue(), 29990 + os.getpid() % 90
+    ranks = [context.Process(target=_rank_without_any, args=(r, port, out)) for r in range(2)]
     for r in ranks:
         r.start()
     for r in ranks:
