@@ -19,6 +19,10 @@ def _arguments(max_norm, norm_type):
     return max_norm, _KINDS[norm_type]
 
 
+def _tensors(given):
+    return [given] if isinstance(given, torch.Tensor) else list(given)
+
+
 def _nothing():
     """Stands for the gradients of a rank that has none, on its current device."""
     return torch.empty(0, device="cuda")
@@ -51,7 +55,7 @@ def clip_coefficient(grads, max_norm, norm_type=2.0, *, sharded=(), group=None):
     (MoELayer.expert_params); their part of the norm is all-reduced over `group`, so every rank calls with as many tensors of its own as it
     has, none included, and gets the same norm. Without a group they count as the others. Everything runs on the current stream without a host wait and can be
     captured."""
-    grads, sharded = [grads] if isinstance(grads, torch.Tensor) else list(grads), list(sharded)
+    grads, sharded = _tensors(grads), _tensors(sharded)
     max_norm, largest = _arguments(max_norm, norm_type)
     if not grads and not sharded and group is None:
         raise ValueError("there are no gradients")
@@ -67,14 +71,14 @@ def clip_grad_norm(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False
     sharded: those of `parameters` of which every rank of `group` has others (see clip_coefficient()). error_if_nonfinite raises
     where the norm is not finite, which waits for the device and cannot be captured. No two gradients may share memory. Parameters without a
     gradient are passed over; without any gradient the norm is 0."""
-    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    parameters = _tensors(parameters)
     max_norm, largest = _arguments(max_norm, norm_type)
+    apart = {id(p) for p in _tensors(sharded)}
+    if apart and not apart <= {id(p) for p in parameters}:
+        raise ValueError("sharded must be some of the parameters")
     if group is None and not error_if_nonfinite:
         norm = _lib.native().clip_grad_norm(parameters, max_norm, largest)
         return torch.zeros((), device=parameters[0].device if parameters else None) if norm is None else norm
-    apart = {id(p) for p in sharded}
-    if not apart <= {id(p) for p in parameters}:
-        raise ValueError("sharded must be some of the parameters")
     with_grad = [p for p in parameters if p.grad is not None]
     grads = [p.grad for p in with_grad if id(p) not in apart]
     local = [p.grad for p in with_grad if id(p) in apart]

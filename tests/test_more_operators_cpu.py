@@ -64,6 +64,17 @@ def test_clipping_arguments():
         clip_grad_norm([p], 1.0, sharded=[torch.nn.Parameter(torch.ones(2))], group=object())
 
 
+def test_sharded_parameters_are_checked_without_a_group_too(monkeypatch):
+    p, other = (torch.nn.Parameter(torch.ones(2)) for _ in range(2))
+    for error_if_nonfinite in (False, True):
+        with pytest.raises(ValueError, match="sharded"):
+            clip_grad_norm([p], 1.0, error_if_nonfinite=error_if_nonfinite, sharded=[other])
+    assert float(clip_grad_norm([p], 1.0, sharded=p)) == 0.0   # one tensor stands for a list of it
+    monkeypatch.setattr(_lib, "native", _OneRank)
+    norm, _ = clip_coefficient([torch.tensor([3.0])], 1.0, sharded=torch.tensor(4.0))
+    assert float(norm) == 5.0
+
+
 class RmsArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int64) for n in ("rows", "D", "x_type", "w_type", "x_stride", "residual_stride")] + \
         [(n, ctypes.c_double) for n in ("eps", "offset")] + \
