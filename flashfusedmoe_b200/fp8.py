@@ -36,7 +36,7 @@ def linear_e4m3(x, x_scale, weight, weight_scale, *, ends=None, out_dtype=torch.
     for t, name in ((x, "x"), (x_scale, "x_scale"), (weight, "weight"), (weight_scale, "weight_scale")):
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be a CUDA tensor: flashfusedmoe_b200 has no CPU path")
-    if not ops.has_status(x.device) and torch.cuda.is_current_stream_capturing():
+    if ops.first_call(x.device) and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("the first call on a device cannot be captured: make one before")
     ops.raise_reported(x.device)
     return _lib.native().linear_e4m3(x, x_scale, weight, weight_scale, ends, out_dtype, ops.status_tensor(x.device).data_ptr(),

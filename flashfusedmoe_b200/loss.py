@@ -49,7 +49,7 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index=-100, reduction
         raise TypeError(f"target must be int64, got {target.dtype}")
     if not z_loss_coeff >= 0.0:
         raise ValueError(f"z_loss_coeff must not be negative, got {z_loss_coeff}")
-    if not ops.has_status(hidden.device) and torch.cuda.is_current_stream_capturing():
+    if ops.first_call(hidden.device) and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("the first call on a device cannot be captured: make one before")
     ops.raise_reported(hidden.device)
     return _lib.native().linear_cross_entropy(hidden, weight, target, ignore_index, _REDUCTIONS[reduction], z_loss_coeff, _piece_rows,

@@ -138,6 +138,12 @@ def has_status(device):
     return device.index in _status
 
 
+def first_call(device):
+    """Whether `device` still lacks its status word or the host word that failures are reported to: neither can be made in a capture, and a graph
+    without the second would never report."""
+    return not has_status(device) or device.index not in _reported
+
+
 def check_status(device=None):
     """Synchronise and raise if any kernel reported a device-side failure since the last check."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)

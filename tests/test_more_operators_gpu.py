@@ -195,6 +195,36 @@ def test_a_first_call_cannot_be_captured(monkeypatch):
             linear_e4m3(x, s, x, s[:1])
 
 
+def test_a_call_that_could_not_report_cannot_be_captured(monkeypatch):
+    """The status word alone, as other calls make it, is not enough: without the host word bad ends in a replay would never be reported."""
+    q, s = torch.zeros(4, 128, device=DEV).to(torch.float8_e4m3fn), torch.ones(4, 1, device=DEV)
+    hidden, target = torch.randn(4, 64, device=DEV).bfloat16(), torch.zeros(4, dtype=torch.int64, device=DEV)
+
+    def calls():
+        return (lambda: linear_e4m3(q, s, q, s[:1])), (lambda: linear_cross_entropy(hidden, hidden, target))
+
+    for call in calls():
+        call()
+    ops.check_status()
+    monkeypatch.setattr(ops, "_reported", {})
+    for call in calls():
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            with pytest.raises(RuntimeError, match="first call"):
+                call()
+    x, xs = torch.zeros(50, 128, device=DEV).to(torch.float8_e4m3fn), torch.ones(50, 1, device=DEV)
+    w, ws, ends = torch.stack([x, x]), torch.ones(2, 1, 1, device=DEV), torch.tensor([20, 50], dtype=torch.int32, device=DEV)
+    linear_e4m3(x, xs, w, ws, ends=ends)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        linear_e4m3(x, xs, w, ws, ends=ends)
+    ends.fill_(51)   # past the rows: moved into place, and reported
+    graph.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="104"):
+        linear_e4m3(x, xs, w, ws)
+    ops.check_status()
+
+
 def test_compiled_functions_call_them_eagerly():
     x, w = torch.randn(40, 128, device=DEV).bfloat16().requires_grad_(), torch.ones(128, device=DEV).requires_grad_()
     wq, ws = quantize_e4m3(torch.randn(64, 128, device=DEV), 128)
