@@ -5,6 +5,8 @@ import ctypes
 import datetime
 import multiprocessing
 import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -315,3 +317,40 @@ def test_a_rank_without_gradients_takes_part():
     for r in ranks:
         r.join(120)
     assert [r.exitcode for r in ranks] == [0, 0] and sorted(out.get() for _ in ranks) == [0, 1]
+
+
+_FIRST_CALLS = r"""
+#include <atomic>
+#include <chrono>
+#include <cstdio>
+#include <thread>
+#include <vector>
+#include "ffm_gemm_common.cuh"
+
+// in place of the runtime's: slow, as a first call is
+extern "C" cudaError_t cudaGetDriverEntryPoint(const char*, void** f, unsigned long long, cudaDriverEntryPointQueryResult* result) {
+  std::this_thread::sleep_for(std::chrono::milliseconds(200));
+  *f = reinterpret_cast<void*>(64);
+  *result = cudaDriverEntryPointSuccess;
+  return cudaSuccess;
+}
+
+int main() {
+  std::atomic<int> missing{0};
+  std::vector<std::thread> threads;
+  for (int i = 0; i < 8; ++i) threads.emplace_back([&] { missing += ffm::get_encode_fn() == nullptr; });
+  for (auto& t : threads) t.join();
+  std::printf("%d", missing.load());
+  return 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("nvcc") is None, reason="needs nvcc")
+def test_first_calls_of_several_threads_find_the_driver(tmp_path):
+    source, program = tmp_path / "first.cu", tmp_path / "first"
+    source.write_text(_FIRST_CALLS)
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    subprocess.run(["nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-cudart", "shared", "-I", csrc, str(source), "-o", str(program),
+                    "-lpthread"], check=True, capture_output=True)
+    assert subprocess.run([str(program)], check=True, capture_output=True, text=True).stdout == "0"
