@@ -71,7 +71,7 @@ class MoELayer(nn.Module):
 
         # only where asked for: a subclass may have a `norm` or `pre_norm` of its own
         self._pre_norm = pre_norm
-        if isinstance(pre_norm, str) and pre_norm not in ("layer", "rms"):
+        if pre_norm and isinstance(pre_norm, str) and pre_norm not in ("layer", "rms"):
             raise ValueError(f"Unknown norm: {pre_norm}")
         if pre_norm:
             self.norm = (RMSNorm if pre_norm == "rms" else LayerNorm)(d_model, eps=norm_eps)

@@ -51,6 +51,12 @@ def test_layers_have_the_norm_that_was_asked_for():
         MoELayer(32, 64, 4, pre_norm="batch")
 
 
+def test_what_stands_for_no_norm():
+    for none in (False, None, 0, ""):
+        assert not any(n.startswith("norm") for n, _ in MoELayer(32, 64, 4, pre_norm=none).named_parameters())
+    assert [n for n, _ in MoELayer(32, 64, 4, pre_norm=1).named_parameters() if n.startswith("norm")] == ["norm.weight", "norm.bias"]
+
+
 def test_clipping_arguments():
     p = torch.nn.Parameter(torch.ones(2))
     for call in (clip_coefficient, clip_grad_norm):
