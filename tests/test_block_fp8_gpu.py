@@ -165,6 +165,12 @@ def test_dense(rows, N, K, dtype):
     ops.check_status()
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,N,K", [(33, 700, 2048), (64, 4096, 2064), (20, 1000, 2048), (17, 130, 4096), (64, 129, 16400), (48, 257, 2064)])
+def test_dense_rows_of_a_tile_whose_contraction_is_shared(rows, N, K, dtype):
+    test_dense(rows, N, K, dtype)
+
+
 # rows of each expert, and rows behind the last
 GROUPS = [([1], 0), ([0], 3), ([5, 0, 1, 64, 0, 65], 2), ([0, 0, 0, 0], 7), ([128, 0, 129, 1, 300, 127], 0), ([1000, 3, 0, 0, 700], 130),
           ([3] * 40, 5), ([0] * 33 + [200] + [0] * 31 + [1], 1), ([400, 300, 500, 2], 0)]

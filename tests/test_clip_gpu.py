@@ -259,3 +259,28 @@ def test_a_training_step():
     # most lr (1 + a little) each, which Adam's sign-like first steps take for tiny gradients too
     for a, b in zip(*results):
         assert float((a.float() - b.float()).abs().max()) <= 2 * 3 * 1.1e-2
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("in_place", [True, False])
+def test_the_optimizer_gets_the_clipped_gradients(dtype, in_place):
+    """One step from nothing leaves (1 - beta) times the clipped gradient and its square in the moments. In place the gradient is rounded to its type
+    first; then come roundings of fp32: the coefficient's product, 1 - beta, and the moment's product (for the square twice the first, and one more)."""
+    grads = _grads([5000, 33, 128 * 70], DTYPES[dtype])
+    params, limit = _params([g.clone() for g in grads]), 0.3 * _norm(grads)
+    opt = AdamW(params, lr=1e-2)
+    _, coefficient = clip_coefficient(grads, limit)
+    assert abs(float(coefficient) - 0.3) < 1e-5
+    if in_place:
+        clip_grad_norm(params, limit)
+        opt.step()
+    else:
+        opt.step(grad_scale=coefficient)
+    info = torch.finfo(DTYPES[dtype])
+    half, least = (info.eps / 2, info.tiny * info.eps) if in_place else (2.0 ** -24, 0.0)
+    for p, g in zip(params, grads):
+        want = g.double() * coefficient.double()
+        m, v = (opt.state[p][name].double() for name in ("exp_avg", "exp_avg_sq"))
+        off = (half + 3 * 2.0 ** -24) * (1 + 2.0 ** -10) * want.abs() + least
+        assert bool(((m - 0.1 * want).abs() <= 0.1 * off).all())
+        assert bool(((v - 0.001 * want.square()).abs() <= 0.001 * (2 * want.abs() * off + off * off + 5 * 2.0 ** -24 * want.square()) + 1e-44).all())

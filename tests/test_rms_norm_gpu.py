@@ -311,3 +311,55 @@ def test_module_and_layer():
     assert torch.equal(out, want)
     out.sum().backward()
     assert layer.norm.weight.grad is not None
+
+
+# Rows enough for the kernels that go through them in a ring, with teams of 1 to 512 threads a row on 148 SMs; widths that end inside a chunk of a
+# thread's, or inside a block of 128
+MANY = [(5000, 1024), (4800, 520), (600, 7168), (80000, 64), (1600, 2056), (700, 8192), (25000, 200)]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,dim", MANY + [(160000, 8)])
+@pytest.mark.parametrize("residual", [True, False])
+def test_forward_of_many_rows(rows, dim, dtype, residual):
+    test_forward(rows, dim, dtype, residual)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,dim", [(5000, 1024), (5000, 144), (700, 7168), (1600, 2064), (5000, 16), (700, 8192)])
+def test_8_bit_output_of_many_rows(rows, dim, dtype):
+    test_8_bit_output(rows, dim, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,dim", MANY)
+@pytest.mark.parametrize("residual", [True, False])
+def test_gradients_of_many_rows(rows, dim, dtype, residual):
+    test_gradients(rows, dim, dtype, residual)
+
+
+def test_options_of_many_rows():
+    rows, dim = 5000, 1024
+    x, more, w = _inputs(rows, dim, torch.bfloat16)
+    y, h = rms_norm(x, None, 0.5, residual=more)
+    want, _, out, _ = _formula(x, more, None, 0.5)
+    assert torch.equal(h.double(), want)
+    _close(y, out)
+    _close(rms_norm(x, w.float(), weight_offset=1.0), _formula(x, None, w, 1e-6, 1.0)[2])
+    wide = torch.zeros(rows, 2 * dim, dtype=x.dtype, device="cuda")   # rows further apart
+    wide[:, 8:8 + dim], wide[:, dim + 8:] = x, 0
+    y, h = rms_norm(wide[:, 8:8 + dim], w, residual=more)
+    assert torch.equal(h.double(), _formula(x, more, w, 1e-6)[0])
+    _close(y, _formula(x, more, w, 1e-6)[2])
+    values, scale = rms_norm(wide[:, 8:8 + dim], w, quantize=True)
+    again = rms_norm(x, w, quantize=True)
+    assert torch.equal(values.view(torch.uint8), again[0].view(torch.uint8)) and torch.equal(scale, again[1])
+    x[17, 5], x[4999, 1000] = float("nan"), float("inf")     # stay in their rows
+    y = rms_norm(x, w)
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[17] = rest[4999] = False
+    assert bool(y[17].isnan().all()) and bool(y[4999, 1000].isnan()) and not bool(y[4999, :1000].any())
+    _close(y[rest], _formula(x[rest], None, w, 1e-6)[2])
+    dy = _inputs(rows, dim, torch.bfloat16, seed=1)[0]
+    dx, = torch.autograd.grad(rms_norm(x.requires_grad_(), w), x, dy)
+    assert bool(dx[17].isnan().all()) and bool(dx[rest].isfinite().all())
