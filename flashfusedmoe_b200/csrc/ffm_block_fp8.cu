@@ -1085,8 +1085,9 @@ extern "C" int ffm_linear_blocks_e4m3(const ffm_linear_blocks_args* args, ffm_st
   p.status_host = a.status_host;
   p.wait_cycles = gemm_wait_cycles();
   const bool grouped = a.ends != nullptr;
-  // One row: us, against a cluster a tile: 256 x 512 2.9 / 5.4, 2048 x 2048 4.1 / 5.9, 4096 x 4096 6.9 / 7.6, 4096 x 7168 9.6 / 9.4 (weights not in L2: 11.2
-  // / 12.7), 14336 x 4096 15.7 / 14.0.
+  // One row: us against a cluster a tile, weights in L2 (from memory): 256 x 512 2.6 / 5.1, 2048 x 2048 3.9 / 5.8 (4.3 / 6.7), 4096 x 4096 6.5 / 7.3
+  // (7.3 / 8.8), 24 M weights 8.0 / 9.4 (9.0 / 10.9), 28 M 9.1 / 9.2 (10.1 / 10.8), 32 M 9.7 / 9.6 (10.7 / 11.5), 40 M 10240 x 4096 11.5 / 13.9 (12.7 / 15.0),
+  // but 2560 x 16384 11.9 / 11.2 (13.2 / 12.9), 44 M 13.3 / 11.2 (14.7 / 13.1), 56 M 14.8 / 13.9 (16.4 / 15.7).
   if (!grouped && a.rows == 1 && a.K <= ROW_K_MAX && a.N * a.K <= 32ll << 20) {
     if (off_16_bytes(a.x, a.w)) return FFM_ERR_UNSUPPORTED;
     return launch_row(a, p, static_cast<cudaStream_t>(stream));

@@ -8,7 +8,7 @@
 //
 // HBM-bound: forward reads x and the residual and writes h and y, backward reads dy, dh and h and writes dx, the gradient of both
 // inputs. One sum over a row is all that stands between reading and writing it. bf16 with a residual: 16384 x 1024 forward 23 us, backward 27 + 3 (4.5 to
-// 5.9 TB/s; 7 rows a team), 8192 x 7168 with 8 bits out 75 us (5.5 TB/s; instructions for a scale and a rounding a value, issue slots 45 %).
+// 5.9 TB/s; 7 rows a team), 8192 x 7168 with 8 bits out 76 us (5.4 TB/s; instructions for a scale, a quotient and a rounding a value).
 #include "ffm_device.h"
 #include "ffm_e4m3.cuh"
 #include "ffm_internal.h"
@@ -553,7 +553,7 @@ struct RmsStream {
 };
 
 // The ring of so many inputs as deep as shared memory allows, over as many teams as go into a block; shape.teams == 0: it does not fit. Rows that fit
-// once only are fetched when the one before has been read: 4096 x 16384 bf16 backward 113 us, held in registers, which spill, 307.
+// once only are fetched when the one before has been read: 4096 x 16384 bf16 backward 116 us, held in registers, which spill, 307.
 RmsStream rms_stream(int D, int type, int inputs, int least) {
   const int row_values = 16 / type_bytes(type);
   RmsStream r;

@@ -25,7 +25,8 @@ def linear_e4m3(x, x_scale, weight, weight_scale, *, ends=None, out_dtype=torch.
     """x weight^T of e4m3 operands with a scale for every block of 128, as quantize_e4m3() and rms_norm(quantize=True) make them.
 
     x [*, K] with x_scale [*, ceil(K / 128)], weight [N, K] with weight_scale [ceil(N / 128), ceil(K / 128)]: the result is [*, N] in
-    `out_dtype` (bfloat16, float16 or float32), summed in fp32 and rounded once. K is a multiple of 16, N and the number of rows any.
+    `out_dtype` (bfloat16, float16 or float32), summed in fp32 and rounded once; x_scale * weight_scale is formed in fp32 and has to be a normal
+    number or infinite there. K is a multiple of 16, N and the number of rows any.
 
     Grouped by expert: x [rows, K], weight [experts, N, K], weight_scale [experts, ceil(N / 128), ceil(K / 128)] and ends [experts]
     (int32, on the device): rows ends[e - 1] to ends[e] - 1 of x are multiplied by weight[e]. Experts may have no rows, and rows from the

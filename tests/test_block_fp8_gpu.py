@@ -334,3 +334,38 @@ def test_norm_quantised_into_the_experts_products():
         want = torch.nn.functional.rms_norm(h[at].double(), (D,), eps=1e-6) @ _wide(w[e], ws[e], 128).t()
         assert n == 0 or float((up[at].double() - want).norm() / want.norm()) < 2.0 ** -4
         begin += n
+
+
+def test_experts_of_a_layer_by_their_products():
+    """Router, rows by expert, gated activation and weighted sum as the documentation has them: `ends` from the sorted experts, each product as above."""
+    T, D, H, experts, k = 150, 256, 320, 6, 2
+    g = torch.Generator(device="cuda").manual_seed(0)
+    y, stream = (torch.randn(T, D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    up, up_scale = quantize_e4m3(torch.randn(experts, 2 * H, D, device="cuda", generator=g) * D ** -0.5, block_rows=128)
+    down, down_scale = quantize_e4m3(torch.randn(experts, D, H, device="cuda", generator=g) * H ** -0.5, block_rows=128)
+    logits = torch.randn(T, experts, device="cuda", generator=g)
+    logits[:, 3] -= 100   # an expert without rows
+    share, chosen = torch.topk(logits.softmax(-1), k)
+    x, x_scale, stream = rms_norm(y, torch.ones(D, device="cuda"), residual=stream, quantize=True)
+    expert, order = chosen.flatten().sort(stable=True)
+    ends = torch.searchsorted(expert, torch.arange(experts, device="cuda"), right=True).int()
+    token = order // k
+    both = linear_e4m3(x[token], x_scale[token], up, up_scale, ends=ends)
+    gate, value = both.chunk(2, -1)
+    hidden = quantize_e4m3(torch.nn.functional.silu(gate) * value)
+    out = linear_e4m3(*hidden, down, down_scale, ends=ends, out_dtype=torch.float32)
+    result = torch.zeros(T, D, device="cuda").index_add_(0, token, out * share.flatten()[order, None])
+    want = torch.zeros(T, D, dtype=torch.float64, device="cuda")
+    begin = 0
+    for e, end in enumerate(ends.tolist()):
+        at = slice(begin, end)
+        rows = torch.nonzero((chosen == e).any(1))[:, 0]
+        assert torch.equal(token[at], rows) and (e != 3 or begin == end)
+        _check(both[at], x[rows], x_scale[rows], up[e], up_scale[e])
+        _check(out[at], hidden[0][at], hidden[1][at], down[e], down_scale[e])
+        want[rows] += out[at].double() * share.double()[chosen == e][:, None]
+        begin = end
+    assert begin == T * k
+    # a product and a sum in fp32 for each of two experts
+    size = torch.zeros(T, D, dtype=torch.float64, device="cuda").index_add_(0, token, (out.double() * share.double().flatten()[order, None]).abs())
+    assert bool(((result.double() - want).abs() <= 4 * 2.0 ** -24 * size).all())
