@@ -87,6 +87,28 @@ def test_codes_are_the_rounded_quotients(block_rows, rows, K, dtype):
     assert torch.equal(values.cpu().view(torch.uint8), (x.float() / spread).to(torch.float8_e4m3fn).view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_extreme_values_of_all_types(block_rows, dtype):
+    """The type's smallest numbers, NaN in either half of a word and in whole words, zeros of both signs: codes and scales of a division on the host."""
+    x = torch.randn(4 * block_rows, 256).to(DTYPES[dtype])
+    tiny = torch.finfo(DTYPES[dtype]).tiny * torch.finfo(DTYPES[dtype]).eps
+    x[:block_rows, :128] = (torch.randint(-7, 8, (block_rows, 128)) * tiny).to(x.dtype)
+    x[block_rows, [0, 3, 10, 11, 127]] = float("nan")
+    x[2 * block_rows, 128:] = -0.0
+    x[2 * block_rows + 1 if block_rows > 1 else 2, 5] = 448.0
+    x[3 * block_rows, 7] = float("-inf")
+    values, scale = quantize_e4m3(x.cuda(), block_rows)
+    # NaN counts as 0 for the scale
+    top = torch.nn.functional.max_pool2d(x.float().nan_to_num(0.0, float("inf"), -float("inf")).abs()[None, None], (block_rows, 128))[0, 0]
+    want = torch.where(top > 0, (top / 448).clamp(min=2.0 ** -126), 1.0)
+    assert torch.equal(scale.cpu(), want)
+    codes = (x.float() / _spread(want, block_rows, x.shape).float()).to(torch.float8_e4m3fn)
+    nan = codes.float().isnan()
+    assert torch.equal(values.cpu().float().isnan(), nan) and int(nan.sum()) == 6
+    assert torch.equal(values.cpu().view(torch.uint8)[~nan], codes.view(torch.uint8)[~nan])
+
+
 def _operands(rows, N, K, experts=None, seed=0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     x = torch.randn(rows, K, device="cuda", generator=g) * (0.2 + 3 * torch.rand(rows, 1, device="cuda", generator=g))
